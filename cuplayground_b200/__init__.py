@@ -13,7 +13,8 @@ __all__ = ["AristosConfig", "AristosError", "baseline_config", "_lib"]
 def __getattr__(name):
     # torch-dependent pieces are imported on first use so that config parsing works without importing torch
     if name in ("MoELayer", "layer", "gate_topk", "gate_topk_screened", "dispatch", "permute", "expert_ffn", "combine",
-                "fill_normal", "nccl_unique_id"):
+                "fill_normal", "nccl_unique_id", "quantize_fp4", "dequantize_fp4", "expert_product_fp4", "expert_ffn_fp4",
+                "moe_few_tokens"):
         import importlib
 
         _layer = importlib.import_module(".layer", __name__)   # `from . import layer` would re-enter __getattr__

@@ -16,7 +16,7 @@ STATUS_NAMES = {0: "ARISTOS_OK", 1: "ARISTOS_ERR_INVALID_ARG", 2: "ARISTOS_ERR_C
                 7: "ARISTOS_ERR_WORKSPACE", 8: "ARISTOS_ERR_DEVICE_TIMEOUT", 9: "ARISTOS_ERR_DEVICE_BOUNDS",
                 10: "ARISTOS_ERR_NOMEM", 11: "ARISTOS_ERR_GATE_SCREEN", 12: "ARISTOS_ERR_NONFINITE"}
 
-DTYPE_F32, DTYPE_TF32, DTYPE_BF16, DTYPE_F16, DTYPE_FP8_E4M3 = 0, 1, 2, 3, 4
+DTYPE_F32, DTYPE_TF32, DTYPE_BF16, DTYPE_F16, DTYPE_FP8_E4M3, DTYPE_FP4_E2M1 = 0, 1, 2, 3, 4, 5
 ACT_RELU, ACT_GELU, ACT_SWIGLU, ACT_IDENTITY = 0, 1, 2, 3
 GATE_SOFTMAX, GATE_SIGMOID = 0, 1
 
@@ -97,6 +97,14 @@ PROTOTYPES = {
     "aristos_quantize_fp8": (_st, [_vp, C.c_int64, C.c_int64, _i, _i, _i, _vp, _vp, _vp]),
     "aristos_expert_ffn_fp8": (_st, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i,
                                      _i, _i, _i, _i, _vp, _vp]),
+    "aristos_fp4_scale_bytes": (_sz, [C.c_int64, C.c_int64, _i]),
+    "aristos_quantize_fp4": (_st, [_vp, C.c_int64, C.c_int64, _i, _i, _vp, _vp, _vp]),
+    "aristos_dequantize_fp4": (_st, [_vp, _vp, C.c_int64, C.c_int64, _i, _i, _vp, _vp]),
+    "aristos_expert_product_fp4": (_st, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "aristos_expert_ffn_fp4": (_st, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i,
+                                     _i, _vp, _vp]),
+    "aristos_moe_few_tokens_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "aristos_moe_few_tokens": (_st, [_vp] * 12 + [_i] * 10 + [_vp, _vp, _vp, _vp, _sz, _vp, _vp]),
     "aristos_combine": (_st, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
     "aristos_selftest_bounded_wait": (_st, [_i, C.POINTER(_i), _vp]),
     "aristos_selftest_bounded_flag_wait": (_st, [_i, C.POINTER(_i), _vp]),

@@ -1,0 +1,494 @@
+// Grouped products and the expert FFN on microscaled 4-bit operands (MXFP4, fp4_format.cuh) with the block-scaled
+// tensor-core instruction of sm_100a.
+//
+//   y[g, r, n] = act( sum_k A[g, r, k] * B[g % experts, n, k] ),  A and B: e2m1 elements times 2^(s - 127) per 32 of K.
+//
+// tcgen05.mma kind::mxf4 multiplies 64 elements of K per instruction and applies both operands' scales itself (two scale
+// bytes per row and instruction, taken from TMEM), accumulating in fp32: no promotion pass, no unpacking, unlike the fp8
+// path, whose fp32 scales per 128 elements have to be applied outside. What is left to the other warps is loading and
+// the epilogue.
+//
+// Tile 128 x 256 (SwiGLU: 128 gate and 128 up columns in one instruction), K in stages of 256 elements = one 128-byte
+// swizzled row, four stages of 51 KB. Per stage the producer loads the codes by TMA and the scales by untiled bulk copies
+// (they lie in global memory in the very tiles that tcgen05.cp takes to TMEM); the issuing thread copies the scales to
+// one of two TMEM buffers and issues up to four MMAs. Only whole 64-element steps that exist are issued, so nothing of a
+// row's padding is ever read.
+//
+// TMEM holds 512 columns; two accumulators of 256 would leave none for the scales. They overlap instead: columns
+// [0, 256) and [192, 448), scales from 448. The epilogue reads the 64 shared columns of a finished tile first and then
+// lets the issuer start the next one, which fills the other buffer while the rest is drained.
+//
+// Roles (320 threads): warp 0 TMA, warp 1 TMEM + MMA, warps 2-9 epilogue, two warps per lane quarter that take the
+// 32-column chunks in turn. Every wait is bounded.
+//
+// The up projection of the FFN writes its output as MXFP4 again: a thread holds 32 adjacent columns of its row, i.e. a
+// whole block, so scale and codes come out of its registers, rounded once from fp32. Only valid rows are written.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "fp4_format.cuh"
+#include "ptx_sm100.cuh"
+#include "tensor_map.cuh"
+
+namespace aristos {
+
+namespace {
+
+constexpr int F4_BM = 128;
+constexpr int F4_BN = 256;
+constexpr int F4_KB = 256;                               // elements of K per stage: 128 bytes
+constexpr int F4_STAGES = 4;
+constexpr int F4_A_BYTES = F4_BM * F4_KB / 2;            // 16 KB
+constexpr int F4_B_BYTES = F4_BN * F4_KB / 2;            // 32 KB: two boxes of 128 weight rows
+constexpr int F4_SF_BYTES = 2 * FP4_TILE_BYTES;          // scales of 128 rows and one stage of K
+constexpr int F4_STAGE_BYTES = F4_A_BYTES + F4_B_BYTES + 3 * F4_SF_BYTES;
+static_assert(F4_STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
+constexpr int F4_EPI_WARPS = 8;
+constexpr int F4_THREADS = 32 * (2 + F4_EPI_WARPS);
+constexpr int F4_MAX_GROUPS = 1024;
+constexpr int F4_AUX_BYTES = (256 + (F4_MAX_GROUPS + 1) * 4 + 127) & ~127;
+constexpr int F4_SMEM_BYTES = 1024 + F4_STAGES * F4_STAGE_BYTES + F4_AUX_BYTES;
+static_assert(F4_SMEM_BYTES <= 227 * 1024, "fp4 GEMM: shared memory");
+constexpr int F4_TMEM_COLS = 512;
+constexpr int F4_ACC1 = 192;                             // first column of the second accumulator
+constexpr int F4_SF_COL = 448, F4_SF_COLS = 32;          // two scale buffers: A 2 x 4 columns, B 2 x 8 columns
+
+struct Fp4GemmParams {
+    const int32_t* count;
+    int groups, experts, rows_per_group;
+    int N, K;
+    int gated, act;
+    const uint8_t* sa;       // scale tiles of A: [groups][row tiles][K tiles][512]
+    const uint8_t* sb0;      // of B: [experts][N tiles][K tiles][512]
+    const uint8_t* sb1;      // SwiGLU: of the up projection's weights
+    void* out;               // [groups * rows_per_group][N], bf16 / fp16 / fp32; or (quantised) codes, two per byte
+    uint8_t* out_scales;     // quantised: scale tiles of the output
+    int32_t* dev_status;
+};
+
+// D[tmem] (+)= A[smem] * B[smem]^T with block scales from TMEM; K = 64 elements, issued by ONE thread.
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                          uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+        "}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+        : "memory");
+}
+
+// e2m1 x e2m1 -> fp32, ue8m0 scales, both operands K-major, tile M x N; sf: which 16-bit half of the scale words.
+__host__ __device__ constexpr uint32_t umma_idesc_mxf4(int M, int N, uint32_t sf) {
+    return (sf << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
+           (static_cast<uint32_t>(M >> 7) << 27) | (sf << 29);
+}
+
+// 32 rows x 16 bytes of shared memory (512 contiguous bytes) to 4 TMEM columns of every lane quarter.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(128 >> 4) << 32;          // 8-row groups are 128 bytes apart, no swizzle
+    d |= static_cast<uint64_t>(1) << 46;
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ float activate(float v, int act) {
+    if (act == ARISTOS_ACT_RELU) return act_relu(v);
+    if (act == ARISTOS_ACT_GELU) return act_gelu(v);
+    return v;
+}
+
+// 32 fp32 values of one row to memory.
+template <typename T> __device__ __forceinline__ void store_row32(T* dst, const float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = v[8 * i + j];
+        store8(dst + 8 * i, w);
+    }
+}
+
+enum { OUT_F32 = ARISTOS_DTYPE_F32, OUT_BF16 = ARISTOS_DTYPE_BF16, OUT_F16 = ARISTOS_DTYPE_F16, OUT_FP4 = 5 };
+
+template <int OUT>
+__global__ void __launch_bounds__(F4_THREADS, 1)
+ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
+                            const __grid_constant__ CUtensorMap tmB1, const Fp4GemmParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* aux = smem + F4_STAGES * F4_STAGE_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(aux);     // full[S], empty[S], tfull[2], tempty
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 192);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(aux + 196);
+    int* prefix = reinterpret_cast<int*>(aux + 256);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t bar_full = ptx::smem_u32(bars);
+    const uint32_t bar_empty = bar_full + 8 * F4_STAGES;
+    const uint32_t bar_tfull = bar_empty + 8 * F4_STAGES;
+    const uint32_t bar_tempty = bar_tfull + 16;
+    const uint32_t smem_base = ptx::smem_u32(smem);
+
+    const int out_w = p.gated ? 128 : 256;
+    const int n_tiles = (p.N + out_w - 1) / out_w;
+    const int kblocks = (p.K + F4_KB - 1) / F4_KB;
+    const int ktiles = fp4_col_tiles(p.K);                 // scale tiles along K (128 elements each)
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < F4_STAGES; ++s) {
+            ptx::mbar_init(bar_full + 8 * s, 1);
+            ptx::mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) ptx::mbar_init(bar_tfull + 8 * b, 1);
+        ptx::mbar_init(bar_tempty, F4_EPI_WARPS);
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 0) {
+        // tiles before row group `v` of the expert-major order
+        int running = 0;
+        if (lane == 0) prefix[0] = 0;
+        for (int g0 = 0; g0 < p.groups; g0 += 32) {
+            const int g = g0 + lane;
+            int v = 0;
+            if (g < p.groups) {
+                const int rows = max(0, min(p.count[ordered_group(g, p.groups, p.experts)], p.rows_per_group));
+                v = ((rows + F4_BM - 1) / F4_BM) * n_tiles;
+            }
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, v, d);
+                if (lane >= d) v += o;
+            }
+            if (g < p.groups) prefix[g + 1] = running + v;
+            running += __shfl_sync(0xffffffffu, v, 31);
+        }
+    } else if (warp == 1) {
+        ptx::tmem_alloc(ptx::smem_u32(tmem_slot), F4_TMEM_COLS);
+    }
+    ptx::tcgen05_fence_before();
+    __syncthreads();
+    ptx::tcgen05_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total_tiles = prefix[p.groups];
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ producer
+        if (ptx::elect_one()) {
+            ptx::prefetch_tensormap(&tmA);
+            ptx::prefetch_tensormap(&tmB0);
+            ptx::prefetch_tensormap(&tmB1);
+            const int a_row_tiles = fp4_row_tiles(p.rows_per_group), b_row_tiles = fp4_row_tiles(p.N);
+            int stage = 0;
+            uint32_t phase = 0;
+            int vg = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+                while (tile >= prefix[vg + 1]) ++vg;
+                const int g = ordered_group(vg, p.groups, p.experts);
+                const int local = tile - prefix[vg];
+                const int mt = (prefix[vg + 1] - prefix[vg]) / n_tiles;
+                const int m0 = (local % mt) * F4_BM;
+                const int n0 = (local / mt) * out_w;
+                const int e = g % p.experts;
+                const int n1 = p.gated ? n0 : n0 + 128;     // second 128-row box of B
+                const bool second = n1 < p.N;               // its scale tiles exist (its codes read as zeros otherwise)
+                const uint8_t* sfa = p.sa + ((size_t)g * a_row_tiles + m0 / 128) * ktiles * FP4_TILE_BYTES;
+                const uint8_t* sfb0 = p.sb0 + ((size_t)e * b_row_tiles + n0 / 128) * ktiles * FP4_TILE_BYTES;
+                const uint8_t* sfb1 = p.sb1 + ((size_t)e * b_row_tiles + n1 / 128) * ktiles * FP4_TILE_BYTES;
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    ok = ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.dev_status);
+                    if (!ok) break;
+                    const uint32_t full = bar_full + 8 * stage;
+                    const uint32_t sa = smem_base + stage * F4_STAGE_BYTES;
+                    const uint32_t sf = sa + F4_A_BYTES + F4_B_BYTES;
+                    const uint32_t sf_bytes = min(2, ktiles - 2 * kb) * FP4_TILE_BYTES;
+                    const size_t sf_off = (size_t)kb * F4_SF_BYTES;
+                    ptx::mbar_arrive_expect_tx(full, F4_A_BYTES + F4_B_BYTES + (second ? 3 : 2) * sf_bytes);
+                    ptx::tma_load_3d(sa, &tmA, kb * (F4_KB / 2), m0, g, full);
+                    ptx::tma_load_3d(sa + F4_A_BYTES, &tmB0, kb * (F4_KB / 2), n0, e, full);
+                    ptx::tma_load_3d(sa + F4_A_BYTES + F4_B_BYTES / 2, &tmB1, kb * (F4_KB / 2), n1, e, full);
+                    bulk_load(sf, sfa + sf_off, sf_bytes, full);
+                    bulk_load(sf + F4_SF_BYTES, sfb0 + sf_off, sf_bytes, full);
+                    if (second) bulk_load(sf + 2 * F4_SF_BYTES, sfb1 + sf_off, sf_bytes, full);
+                    if (++stage == F4_STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA issuer
+        if (ptx::elect_one()) {
+            int it = 0, t = 0;                             // stages and tiles issued so far
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x, ++t) {
+                const uint32_t tmem_d = tmem_base + (t & 1) * F4_ACC1;
+                if (t > 0) {
+                    // the columns that this accumulator shares with the previous tile's have been read (and all of
+                    // the tile before that, whose accumulator this is)
+                    ok = ptx::mbar_wait_bounded(bar_tempty, (t - 1) & 1, abort_flag, p.dev_status);
+                    if (!ok) break;
+                    ptx::tcgen05_fence_after();
+                }
+                for (int kb = 0; kb < kblocks; ++kb, ++it) {
+                    const int stage = it % F4_STAGES;
+                    ok = ptx::mbar_wait_bounded(bar_full + 8 * stage, (it / F4_STAGES) & 1, abort_flag, p.dev_status);
+                    if (!ok) break;
+                    // the scale buffer of this stage was read by the MMAs of two stages ago
+                    if (it >= 2) {
+                        ok = ptx::mbar_wait_bounded(bar_empty + 8 * ((it - 2) % F4_STAGES), ((it - 2) / F4_STAGES) & 1,
+                                                    abort_flag, p.dev_status);
+                        if (!ok) break;
+                    }
+                    ptx::tcgen05_fence_after();
+                    const uint32_t sa = smem_base + stage * F4_STAGE_BYTES;
+                    const uint32_t sf = sa + F4_A_BYTES + F4_B_BYTES;
+                    const uint32_t tsf = tmem_base + F4_SF_COL + (it & 1) * F4_SF_COLS;
+                    const int steps = min(4, (p.K - kb * F4_KB) / 64);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (2 * h < steps) {
+                            tmem_copy_scales(tsf + 4 * h, sf + h * FP4_TILE_BYTES);
+                            tmem_copy_scales(tsf + 8 + 8 * h, sf + F4_SF_BYTES + h * FP4_TILE_BYTES);
+                            tmem_copy_scales(tsf + 8 + 8 * h + 4, sf + 2 * F4_SF_BYTES + h * FP4_TILE_BYTES);
+                        }
+                    }
+                    const uint64_t da = ptx::umma_desc_k_sw128(sa);
+                    const uint64_t db = ptx::umma_desc_k_sw128(sa + F4_A_BYTES);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)            // K = 64 elements = 32 bytes per instruction
+                        if (k < steps)
+                            umma_mxf4(tmem_d, da + 2 * k, db + 2 * k, umma_idesc_mxf4(F4_BM, F4_BN, (k & 1) * 2),
+                                      tsf + 4 * (k >> 1), tsf + 8 + 8 * (k >> 1), (kb | k) != 0 ? 1u : 0u);
+                    ptx::umma_commit(bar_empty + 8 * stage);
+                }
+                if (!ok) break;
+                ptx::umma_commit(bar_tfull + 8 * (t & 1));
+            }
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------------ epilogue
+        const int quarter = warp & 3;                       // TMEM lanes this warp may read
+        const int sub = (warp - 2) >> 2;                    // 0 / 1: even or odd 32-column chunks
+        const int row_in_tile = quarter * 32 + lane;
+        int vg = 0, t = 0;
+        for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++t) {
+            while (tile >= prefix[vg + 1]) ++vg;
+            const int g = ordered_group(vg, p.groups, p.experts);
+            const int local = tile - prefix[vg];
+            const int mt = (prefix[vg + 1] - prefix[vg]) / n_tiles;
+            const int m0 = (local % mt) * F4_BM;
+            const int n0 = (local / mt) * out_w;
+            const int row = m0 + row_in_tile;
+            const bool row_ok = row < min(p.count[g], p.rows_per_group);
+            const size_t grow = (size_t)g * p.rows_per_group + row;
+            bool ok = ptx::mbar_wait_bounded(bar_tfull + 8 * (t & 1), (t >> 1) & 1, abort_flag, p.dev_status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            ptx::tcgen05_fence_after();
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (t & 1) * F4_ACC1;
+            const int chunks = p.gated ? 2 : 4;             // of this warp: sub, sub + 2, ...
+            for (int c = 0; c < chunks; ++c) {
+                // first the chunk whose columns the next tile needs: the last one in the first accumulator (columns
+                // 192-255; SwiGLU: with its gate columns), the first one in the second
+                const int j = (t & 1) ? c : (c == 0 ? chunks - 1 : c - 1);
+                const int col = (sub + 2 * j) * 32;
+                uint32_t a[32], b[32];
+                ptx::tmem_ld_32x32b_x32(taddr + col, a);
+                if (p.gated) ptx::tmem_ld_32x32b_x32(taddr + 128 + col, b);
+                ptx::tmem_ld_wait();
+                if (c == 0) {
+                    ptx::tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(bar_tempty);
+                }
+                if (!row_ok || n0 + col >= p.N) continue;
+                float v[32];
+                if (p.gated) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = act_silu(__uint_as_float(a[i])) * __uint_as_float(b[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = activate(__uint_as_float(a[i]), p.act);
+                }
+                if constexpr (OUT == OUT_FP4) {
+                    float m = 0.0f;                         // the bits of |NaN| are above infinity's: NaN is kept
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(v[i]) & 0x7FFFFFFFu));
+                    const uint32_t s = fp4_scale_of(m);
+                    const float inv = fp4_inverse_scale(s);
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        w[i] = 0;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            w[i] |= fp4_pack2(v[8 * i + 2 * q] * inv, v[8 * i + 2 * q + 1] * inv) << (8 * q);
+                        if (s == 255u) w[i] = 0;
+                    }
+                    uint8_t* codes = static_cast<uint8_t*>(p.out) + grow * (p.N / 2) + (n0 + col) / 2;
+                    *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
+                    const size_t tile_at = ((size_t)g * fp4_row_tiles(p.rows_per_group) + row / 128) * fp4_col_tiles(p.N) +
+                                           (n0 + col) / 128;
+                    p.out_scales[tile_at * FP4_TILE_BYTES + fp4_tile_word(row) + (col / 32) % 4] = (uint8_t)s;
+                } else if constexpr (OUT == OUT_F32) {
+                    store_row32(static_cast<float*>(p.out) + grow * p.N + n0 + col, v);
+                } else if constexpr (OUT == OUT_BF16) {
+                    store_row32(static_cast<__nv_bfloat16*>(p.out) + grow * p.N + n0 + col, v);
+                } else {
+                    store_row32(static_cast<__half*>(p.out) + grow * p.N + n0 + col, v);
+                }
+            }
+        }
+    }
+
+    ptx::tcgen05_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tcgen05_fence_after();
+        ptx::tmem_dealloc(tmem_base, F4_TMEM_COLS);
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, const Fp4GemmParams& p, int out,
+                                 cudaStream_t st) {
+    CUtensorMap tmA, tmB0, tmB1;
+    ARISTOS_TRY(encode_map_3d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A, p.K / 2, p.rows_per_group, p.groups, 128));
+    ARISTOS_TRY(encode_map_3d(&tmB0, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B0, p.K / 2, p.N, p.experts, 128));
+    ARISTOS_TRY(encode_map_3d(&tmB1, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B1, p.K / 2, p.N, p.experts, 128));
+    const int sms = device_sm_count();
+    if (sms <= 0) { set_last_error("no CUDA device"); return ARISTOS_ERR_CUDA; }
+    const int64_t bound = (int64_t)p.groups * ceil_div(p.rows_per_group, F4_BM) * ceil_div(p.N, p.gated ? 128 : 256);
+    const int grid = (int)(bound < sms ? bound : sms);
+    auto run = [&](auto kernel) -> aristos_status_t {
+        ARISTOS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F4_SMEM_BYTES));
+        kernel<<<grid, F4_THREADS, F4_SMEM_BYTES, st>>>(tmA, tmB0, tmB1, p);
+        ARISTOS_COUNT_LAUNCH();
+        ARISTOS_CUDA_TRY(cudaGetLastError());
+        return ARISTOS_OK;
+    };
+    switch (out) {
+        case OUT_F32: return run(ffn_fp4_grouped_gemm_kernel<OUT_F32>);
+        case OUT_BF16: return run(ffn_fp4_grouped_gemm_kernel<OUT_BF16>);
+        case OUT_F16: return run(ffn_fp4_grouped_gemm_kernel<OUT_F16>);
+        default: return run(ffn_fp4_grouped_gemm_kernel<OUT_FP4>);
+    }
+}
+
+aristos_status_t check_fp4_product(const char* what, int groups, int rows_per_group, int experts, int N, int K,
+                                   int out_dtype) {
+    if (groups < 0 || rows_per_group < 0 || experts <= 0 || N <= 0 || K <= 0) {
+        set_last_error("%s: bad size", what);
+        return ARISTOS_ERR_INVALID_ARG;
+    }
+    if (N % 64 != 0 || K % 64 != 0) {
+        set_last_error("%s: the feature sizes must be multiples of 64", what);
+        return ARISTOS_ERR_CONFIG;
+    }
+    if (groups > F4_MAX_GROUPS) {
+        set_last_error("%s: more than %d row groups", what, F4_MAX_GROUPS);
+        return ARISTOS_ERR_CONFIG;
+    }
+    // the tiles of all row groups are numbered in 31 bits
+    if ((int64_t)groups * ceil_div(rows_per_group, F4_BM) * ceil_div(N, 128) >= (int64_t)1 << 30) {
+        set_last_error("%s: too many tiles", what);
+        return ARISTOS_ERR_CONFIG;
+    }
+    if (out_dtype != ARISTOS_DTYPE_F32 && out_dtype != ARISTOS_DTYPE_BF16 && out_dtype != ARISTOS_DTYPE_F16) {
+        set_last_error("%s: the output dtype must be f32, bf16 or f16", what);
+        return ARISTOS_ERR_UNSUPPORTED;
+    }
+    return ARISTOS_OK;
+}
+
+}  // namespace
+}  // namespace aristos
+
+using namespace aristos;
+
+extern "C" aristos_status_t aristos_expert_product_fp4(const void* aq, const void* sa, const int32_t* count, int groups,
+                                                       int rows_per_group, int experts, const void* bq, const void* sb,
+                                                       int N, int K, int out_dtype, void* y, int32_t* dev_status,
+                                                       void* stream) {
+    ARISTOS_TRY(check_fp4_product("expert_product_fp4", groups, rows_per_group, experts, N, K, out_dtype));
+    if (groups == 0 || rows_per_group == 0) return ARISTOS_OK;
+    if (!aq || !sa || !count || !bq || !sb || !y) {
+        set_last_error("expert_product_fp4: NULL pointer");
+        return ARISTOS_ERR_INVALID_ARG;
+    }
+    if (!aligned16(aq) || !aligned16(sa) || !aligned16(bq) || !aligned16(sb) || !aligned16(y)) {
+        set_last_error("expert_product_fp4: pointers must be 16-byte aligned");
+        return ARISTOS_ERR_INVALID_ARG;
+    }
+    Fp4GemmParams p{};
+    p.count = count;
+    p.groups = groups;
+    p.experts = experts;
+    p.rows_per_group = rows_per_group;
+    p.N = N; p.K = K;
+    p.act = ARISTOS_ACT_IDENTITY;
+    p.sa = static_cast<const uint8_t*>(sa);
+    p.sb0 = p.sb1 = static_cast<const uint8_t*>(sb);
+    p.out = y;
+    p.dev_status = dev_status;
+    return launch_fp4_gemm(aq, bq, bq, p, out_dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" aristos_status_t aristos_expert_ffn_fp4(const void* xq, const void* sx, const int32_t* count, int groups,
+                                                   int rows_per_group, int experts, const void* w1q, const void* s1,
+                                                   const void* w3q, const void* s3, const void* w2q, const void* s2,
+                                                   void* hq_scratch, void* sh_scratch, void* y, int H, int I,
+                                                   int hidden_act, int out_dtype, int32_t* dev_status, void* stream) {
+    if (hidden_act < 0 || hidden_act > 2) { set_last_error("expert_ffn_fp4: hidden_act must be 0, 1 or 2"); return ARISTOS_ERR_INVALID_ARG; }
+    ARISTOS_TRY(check_fp4_product("expert_ffn_fp4", groups, rows_per_group, experts, H, I, out_dtype));
+    ARISTOS_TRY(check_fp4_product("expert_ffn_fp4", groups, rows_per_group, experts, I, H, out_dtype));
+    if (groups == 0 || rows_per_group == 0) return ARISTOS_OK;
+    const bool gated = hidden_act == ARISTOS_ACT_SWIGLU;
+    if (!xq || !sx || !count || !w1q || !s1 || !w2q || !s2 || !hq_scratch || !sh_scratch || !y) {
+        set_last_error("expert_ffn_fp4: NULL pointer");
+        return ARISTOS_ERR_INVALID_ARG;
+    }
+    if (gated && (!w3q || !s3)) { set_last_error("expert_ffn_fp4: SwiGLU needs w3 and its scales"); return ARISTOS_ERR_INVALID_ARG; }
+    for (const void* q : {xq, sx, w1q, s1, w2q, s2, (const void*)hq_scratch, (const void*)sh_scratch, (const void*)y,
+                          gated ? w3q : w1q, gated ? s3 : s1}) {
+        if (!aligned16(q)) {
+            set_last_error("expert_ffn_fp4: pointers must be 16-byte aligned");
+            return ARISTOS_ERR_INVALID_ARG;
+        }
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    Fp4GemmParams p{};
+    p.count = count;
+    p.groups = groups;
+    p.experts = experts;
+    p.rows_per_group = rows_per_group;
+    p.dev_status = dev_status;
+    p.N = I; p.K = H;
+    p.gated = gated ? 1 : 0;
+    p.act = hidden_act;
+    p.sa = static_cast<const uint8_t*>(sx);
+    p.sb0 = static_cast<const uint8_t*>(s1);
+    p.sb1 = static_cast<const uint8_t*>(gated ? s3 : s1);
+    p.out = hq_scratch;
+    p.out_scales = static_cast<uint8_t*>(sh_scratch);
+    ARISTOS_TRY(launch_fp4_gemm(xq, w1q, gated ? w3q : w1q, p, OUT_FP4, st));
+    p.N = H; p.K = I;
+    p.gated = 0;
+    p.act = ARISTOS_ACT_IDENTITY;
+    p.sa = static_cast<const uint8_t*>(sh_scratch);
+    p.sb0 = p.sb1 = static_cast<const uint8_t*>(s2);
+    p.out = y;
+    p.out_scales = nullptr;
+    return launch_fp4_gemm(hq_scratch, w2q, w2q, p, out_dtype, st);
+}

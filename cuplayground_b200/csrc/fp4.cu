@@ -1,0 +1,259 @@
+// Quantisation to the microscaled 4-bit format and back (aristos_quantize_fp4 / aristos_dequantize_fp4).
+//
+// For a block of 32 columns with largest magnitude m: s = floor(log2 m) + 125 (clamped at 0), codes = e2m1(v * 2^(127 - s))
+// rounded to nearest even and saturated at 6. Multiplying by a power of two is exact, so the only rounding is the one to
+// e2m1 and the codes do not depend on how the work is cut up.
+//
+// Both directions are bound by HBM. A unit of work is one row's 128 columns = one 4-byte scale word: a half warp takes it,
+// 8 columns (16 bytes of a 16-bit tensor) per lane, so loads and stores of a warp are contiguous; four lanes share a
+// block and find its maximum with two shuffles. UNITS units are in flight per half warp.
+#include "common.cuh"
+#include "fp4_format.cuh"
+
+namespace aristos {
+
+namespace {
+
+constexpr int Q4_THREADS = 256;
+constexpr int Q4_HALVES = Q4_THREADS / 16;
+constexpr int Q4_UNITS = 4;
+
+// Division by a constant found at launch: u / d for u < 2^31.
+struct Divider {
+    uint32_t d, magic, shift;
+};
+Divider make_divider(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return Divider{d, (uint32_t)((1ull << (31 + s)) / d + 1), 31 + s};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t u, const Divider& v) {
+    return (uint32_t)(((uint64_t)u * v.magic) >> v.shift);
+}
+
+template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ void load_raw(const T* p, Raw8<T>& r) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+}
+template <typename T>
+__device__ __forceinline__ void raw_to_float(const Raw8<T>& r, float (&v)[8]) {
+    load8(reinterpret_cast<const T*>(&r.v[0]), v);
+}
+
+// The largest magnitude as an fp32 number, except that a NaN stays one (the bits of NaN are above those of infinity).
+__device__ __forceinline__ float magnitude_max(float a, float b) {
+    return __uint_as_float(max(__float_as_uint(a) & 0x7FFFFFFFu, __float_as_uint(b) & 0x7FFFFFFFu));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(Q4_THREADS)
+quantize_fp4_kernel(const T* __restrict__ src, int64_t mats, int rows, int cols, uint32_t units, Divider tiles,
+                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    const int l = threadIdx.x & 15;
+    const uint32_t half = blockIdx.x * Q4_HALVES + (threadIdx.x >> 4);
+    const uint32_t stride = gridDim.x * Q4_HALVES;
+    const size_t mat_scales = fp4_matrix_scale_bytes(rows, cols);
+    for (int64_t mat = blockIdx.y; mat < mats; mat += gridDim.y) {
+        const T* s = src + (size_t)mat * rows * cols;
+        uint8_t* c = codes + (size_t)mat * rows * (cols / 2);
+        uint8_t* sc = scales + (size_t)mat * mat_scales;
+        // the loop bound is the same for both halves of a warp, so that the shuffles below are reached together
+        for (uint32_t u0 = 0; u0 < units; u0 += stride * Q4_UNITS) {
+            Raw8<T> raw[Q4_UNITS];
+            uint32_t row[Q4_UNITS], tile[Q4_UNITS];
+            bool in[Q4_UNITS];
+#pragma unroll
+            for (int i = 0; i < Q4_UNITS; ++i) {
+                const uint32_t u = u0 + i * stride + half;
+                row[i] = divide(u, tiles);
+                tile[i] = u - row[i] * tiles.d;
+                in[i] = u < units && row[i] < (uint32_t)rows && tile[i] * 128 + l * 8 < (uint32_t)cols;
+                if (in[i]) {
+                    load_raw(s + (size_t)row[i] * cols + tile[i] * 128 + l * 8, raw[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) raw[i].v[j] = make_uint4(0, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < Q4_UNITS; ++i) {
+                float v[8];
+                raw_to_float(raw[i], v);
+                float m = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = magnitude_max(m, v[j]);
+                m = magnitude_max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = magnitude_max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const uint32_t sb = fp4_scale_of(m);
+                const float inv = fp4_inverse_scale(sb);
+                uint32_t packed = 0;
+                if (sb != 255u) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) packed |= fp4_pack2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
+                }
+                uint32_t word = sb << (8 * (l >> 2));
+                word |= __shfl_xor_sync(0xffffffffu, word, 4);
+                word |= __shfl_xor_sync(0xffffffffu, word, 8);
+                if (in[i])
+                    *reinterpret_cast<uint32_t*>(c + (size_t)row[i] * (cols / 2) + tile[i] * 64 + l * 4) = packed;
+                // rows that only fill up a tile of 128 get scale 0, as the missing blocks of a row do
+                if (l == 0 && u0 + i * stride + half < units)
+                    *reinterpret_cast<uint32_t*>(sc + ((size_t)(row[i] >> 7) * tiles.d + tile[i]) * FP4_TILE_BYTES +
+                                                 fp4_tile_word(row[i])) = word;
+            }
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(Q4_THREADS)
+dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t mats, int rows,
+                      int cols, uint32_t units, Divider tiles, T* __restrict__ dst) {
+    const int l = threadIdx.x & 15;
+    const uint32_t half = blockIdx.x * Q4_HALVES + (threadIdx.x >> 4);
+    const uint32_t stride = gridDim.x * Q4_HALVES;
+    const size_t mat_scales = fp4_matrix_scale_bytes(rows, cols);
+    for (int64_t mat = blockIdx.y; mat < mats; mat += gridDim.y) {
+        T* d = dst + (size_t)mat * rows * cols;
+        const uint8_t* c = codes + (size_t)mat * rows * (cols / 2);
+        const uint8_t* sc = scales + (size_t)mat * mat_scales;
+        for (uint32_t u0 = half; u0 < units; u0 += stride * Q4_UNITS) {
+            uint32_t word[Q4_UNITS], sword[Q4_UNITS];
+            size_t at[Q4_UNITS];
+            bool in[Q4_UNITS];
+#pragma unroll
+            for (int i = 0; i < Q4_UNITS; ++i) {
+                const uint32_t u = u0 + i * stride;
+                const uint32_t row = divide(u, tiles), tile = u - row * tiles.d;
+                in[i] = u < units && tile * 128 + l * 8 < (uint32_t)cols;
+                at[i] = (size_t)row * cols + tile * 128 + l * 8;
+                word[i] = sword[i] = 0;
+                if (in[i]) {
+                    word[i] = __ldcs(reinterpret_cast<const uint32_t*>(c + at[i] / 2));
+                    sword[i] = __ldg(reinterpret_cast<const uint32_t*>(
+                        sc + ((size_t)(row >> 7) * tiles.d + tile) * FP4_TILE_BYTES + fp4_tile_word(row)));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < Q4_UNITS; ++i) {
+                if (!in[i]) continue;
+                const float f = fp4_scale_value((sword[i] >> (8 * (l >> 2))) & 255u);
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 p = __half22float2(fp4_unpack2((word[i] >> (8 * j)) & 255u));
+                    v[2 * j] = p.x * f;
+                    v[2 * j + 1] = p.y * f;
+                }
+                store8(d + at[i], v);
+            }
+        }
+    }
+}
+
+aristos_status_t check_fp4_shape(const char* what, int64_t mats, int64_t rows, int cols) {
+    if (mats < 0 || rows < 0 || cols <= 0 || cols % 64 != 0) {
+        set_last_error("%s: sizes must not be negative and cols must be a multiple of 64", what);
+        return ARISTOS_ERR_INVALID_ARG;
+    }
+    // a matrix's units (row, 128 columns) are numbered in 31 bits
+    if (rows > (1 << 30) || (rows + 127) / 128 * 128 * (int64_t)fp4_col_tiles(cols) > (int64_t)1 << 30) {
+        set_last_error("%s: a matrix of more than 2^37 elements", what);
+        return ARISTOS_ERR_CONFIG;
+    }
+    return ARISTOS_OK;
+}
+
+dim3 unit_grid(uint32_t units, int64_t mats) {
+    // enough CTAs to fill the device, no more than the units of a matrix ask for
+    const uint32_t need = (units + Q4_HALVES - 1) / Q4_HALVES;
+    const int64_t fill = (int64_t)device_sm_count() * 8;
+    const uint32_t y = (uint32_t)(mats < 65535 ? mats : 65535);
+    int64_t x = (fill + y - 1) / y;
+    if (x < 1) x = 1;
+    return dim3(x < need ? (uint32_t)x : need, y);
+}
+
+}  // namespace
+}  // namespace aristos
+
+using namespace aristos;
+
+extern "C" size_t aristos_fp4_scale_bytes(int64_t mats, int64_t rows, int cols) {
+    if (mats < 0 || rows < 0 || cols <= 0 || rows > (1 << 30)) return 0;
+    return (size_t)mats * fp4_matrix_scale_bytes((int)rows, cols);
+}
+
+extern "C" aristos_status_t aristos_quantize_fp4(const void* src, int64_t mats, int64_t rows, int cols, int src_dtype,
+                                                 void* codes, void* scales, void* stream) {
+    ARISTOS_TRY(check_fp4_shape("quantize_fp4", mats, rows, cols));
+    if (mats == 0 || rows == 0) return ARISTOS_OK;
+    if (!src || !codes || !scales) { set_last_error("quantize_fp4: NULL pointer"); return ARISTOS_ERR_INVALID_ARG; }
+    if (!aligned16(src) || !aligned16(codes) || !aligned16(scales)) {
+        set_last_error("quantize_fp4: pointers must be 16-byte aligned");
+        return ARISTOS_ERR_INVALID_ARG;
+    }
+    const Divider tiles = make_divider((uint32_t)fp4_col_tiles(cols));
+    const uint32_t units = (uint32_t)fp4_row_tiles((int)rows) * FP4_TILE_ROWS * tiles.d;
+    const dim3 grid = unit_grid(units, mats);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    uint8_t *c = static_cast<uint8_t*>(codes), *s = static_cast<uint8_t*>(scales);
+    switch (src_dtype) {
+        case ARISTOS_DTYPE_F32:
+            quantize_fp4_kernel<float><<<grid, Q4_THREADS, 0, st>>>(static_cast<const float*>(src), mats, (int)rows, cols,
+                                                                    units, tiles, c, s);
+            break;
+        case ARISTOS_DTYPE_BF16:
+            quantize_fp4_kernel<__nv_bfloat16><<<grid, Q4_THREADS, 0, st>>>(static_cast<const __nv_bfloat16*>(src), mats,
+                                                                            (int)rows, cols, units, tiles, c, s);
+            break;
+        case ARISTOS_DTYPE_F16:
+            quantize_fp4_kernel<__half><<<grid, Q4_THREADS, 0, st>>>(static_cast<const __half*>(src), mats, (int)rows,
+                                                                     cols, units, tiles, c, s);
+            break;
+        default:
+            set_last_error("quantize_fp4: source dtype must be f32, bf16 or f16");
+            return ARISTOS_ERR_UNSUPPORTED;
+    }
+    ARISTOS_COUNT_LAUNCH();
+    ARISTOS_CUDA_TRY(cudaGetLastError());
+    return ARISTOS_OK;
+}
+
+extern "C" aristos_status_t aristos_dequantize_fp4(const void* codes, const void* scales, int64_t mats, int64_t rows,
+                                                   int cols, int dst_dtype, void* dst, void* stream) {
+    ARISTOS_TRY(check_fp4_shape("dequantize_fp4", mats, rows, cols));
+    if (mats == 0 || rows == 0) return ARISTOS_OK;
+    if (!dst || !codes || !scales) { set_last_error("dequantize_fp4: NULL pointer"); return ARISTOS_ERR_INVALID_ARG; }
+    if (!aligned16(dst) || !aligned16(codes) || !aligned16(scales)) {
+        set_last_error("dequantize_fp4: pointers must be 16-byte aligned");
+        return ARISTOS_ERR_INVALID_ARG;
+    }
+    const Divider tiles = make_divider((uint32_t)fp4_col_tiles(cols));
+    const uint32_t units = (uint32_t)rows * tiles.d;
+    const dim3 grid = unit_grid(units, mats);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const uint8_t *c = static_cast<const uint8_t*>(codes), *s = static_cast<const uint8_t*>(scales);
+    switch (dst_dtype) {
+        case ARISTOS_DTYPE_F32:
+            dequantize_fp4_kernel<float><<<grid, Q4_THREADS, 0, st>>>(c, s, mats, (int)rows, cols, units, tiles,
+                                                                      static_cast<float*>(dst));
+            break;
+        case ARISTOS_DTYPE_BF16:
+            dequantize_fp4_kernel<__nv_bfloat16><<<grid, Q4_THREADS, 0, st>>>(c, s, mats, (int)rows, cols, units, tiles,
+                                                                              static_cast<__nv_bfloat16*>(dst));
+            break;
+        case ARISTOS_DTYPE_F16:
+            dequantize_fp4_kernel<__half><<<grid, Q4_THREADS, 0, st>>>(c, s, mats, (int)rows, cols, units, tiles,
+                                                                       static_cast<__half*>(dst));
+            break;
+        default:
+            set_last_error("dequantize_fp4: destination dtype must be f32, bf16 or f16");
+            return ARISTOS_ERR_UNSUPPORTED;
+    }
+    ARISTOS_COUNT_LAUNCH();
+    ARISTOS_CUDA_TRY(cudaGetLastError());
+    return ARISTOS_OK;
+}

@@ -231,6 +231,163 @@ def expert_ffn_fp8(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, hidden_act: int, de
     return y
 
 
+# ---- microscaled 4-bit operands -------------------------------------------------------------------------------------
+def _one_device(*tensors) -> torch.device:
+    """The CUDA device that all the given tensors (None: not given) are on."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1 or next(iter(devices)).type != "cuda":
+        raise ValueError(f"tensors must all be on one CUDA device, got {sorted(map(str, devices))}")
+    return next(iter(devices))
+
+
+def _fp4_scale_shape(lead, rows: int, cols: int):
+    return (*lead, (rows + 127) // 128, (cols + 127) // 128, 32, 4, 4)
+
+
+def _expect(name: str, t: torch.Tensor, shape, dtype: torch.dtype) -> None:
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def quantize_fp4(src: torch.Tensor):
+    """MXFP4 codes and scales of a (..., rows, cols) tensor in f32, bf16 or f16, cols a multiple of 64: codes uint8
+    (..., rows, cols / 2), two e2m1 elements to a byte, the even column in the low half; scales uint8
+    (..., ceil(rows / 128), ceil(cols / 128), 32, 4, 4): the byte 2^(s - 127) of row r and columns 32 b .. 32 b + 31 is
+    [..., r / 128, b / 4, r % 32, r / 32 % 4, b % 4]. See aristos_quantize_fp4."""
+    rows, cols = src.shape[-2], src.shape[-1]
+    lead = src.shape[:-2]
+    with torch.cuda.device(_one_device(src)):
+        q = torch.empty((*lead, rows, cols // 2), dtype=torch.uint8, device=src.device)
+        scales = torch.empty(_fp4_scale_shape(lead, rows, cols), dtype=torch.uint8, device=src.device)
+        _lib.check(_lib.load().aristos_quantize_fp4(_ptr(src), lead.numel(), rows, cols, _dt(src), _ptr(q), _ptr(scales),
+                                                    _stream_ptr()))
+    return q, scales
+
+
+def dequantize_fp4(q: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that MXFP4 codes and scales (as quantize_fp4 gives them) stand for, in f32, bf16 or f16."""
+    rows, cols = q.shape[-2], 2 * q.shape[-1]
+    lead = q.shape[:-2]
+    _expect("q", q, q.shape, torch.uint8)
+    _expect("scales", scales, _fp4_scale_shape(lead, rows, cols), torch.uint8)
+    with torch.cuda.device(_one_device(q, scales)):
+        out = torch.empty((*lead, rows, cols), dtype=dtype, device=q.device)
+        _lib.check(_lib.load().aristos_dequantize_fp4(_ptr(q), _ptr(scales), lead.numel(), rows, cols, _dt(out),
+                                                      _ptr(out), _stream_ptr()))
+    return out
+
+
+def _fp4_output(y, shape, dtype, device):
+    if y is None:
+        return torch.zeros(shape, dtype=dtype or torch.bfloat16, device=device)
+    _expect("y", y, shape, dtype or y.dtype)
+    return y
+
+
+def expert_product_fp4(aq, sa, count, bq, sb, y=None, dtype: Optional[torch.dtype] = None, dev_status=None):
+    """y[g, r] = A[g, r] . B[g % experts]^T for r < count[g], both operands in MXFP4: aq (groups, rows, K / 2) with sa,
+    bq (experts, N, K / 2) with sb, count (groups) int32 -> y (groups, rows, N) in `dtype` (bf16 unless given; f32 and
+    f16). Rows past count[g] keep what y holds (zeros in a y made here)."""
+    groups, rows, half = aq.shape
+    experts, N = bq.shape[:2]
+    for name, t, shape in (("aq", aq, (groups, rows, half)), ("sa", sa, _fp4_scale_shape((groups,), rows, 2 * half)),
+                           ("bq", bq, (experts, N, half)), ("sb", sb, _fp4_scale_shape((experts,), N, 2 * half))):
+        _expect(name, t, shape, torch.uint8)
+    _expect("count", count, (groups,), torch.int32)
+    with torch.cuda.device(_one_device(aq, sa, count, bq, sb, y, dev_status)):
+        y = _fp4_output(y, (groups, rows, N), dtype, aq.device)
+        _lib.check(_lib.load().aristos_expert_product_fp4(_ptr(aq), _ptr(sa), _ptr(count), groups, rows, experts, _ptr(bq),
+                                                          _ptr(sb), N, 2 * half, _dt(y), _ptr(y), _ptr(dev_status),
+                                                          _stream_ptr()))
+    return y
+
+
+def expert_ffn_fp4(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, hidden_act: int, y=None,
+                   dtype: Optional[torch.dtype] = None, dev_status=None):
+    """Expert FFN on MXFP4 operands: xq (groups, rows, H / 2) with sx; w1q / w3q (experts, I, H / 2) and w2q
+    (experts, H, I / 2) with their scales (w3q, s3: SwiGLU only, else None) -> y (groups, rows, H) in `dtype` (bf16 unless
+    given). The hidden activations are rounded to MXFP4 between the projections. Rows past count[g] keep what y holds."""
+    groups, rows, half = xq.shape
+    experts, I = w1q.shape[:2]
+    H = 2 * half
+    checks = [("xq", xq, (groups, rows, half)), ("sx", sx, _fp4_scale_shape((groups,), rows, H)),
+              ("w1q", w1q, (experts, I, half)), ("s1", s1, _fp4_scale_shape((experts,), I, H)),
+              ("w2q", w2q, (experts, H, I // 2)), ("s2", s2, _fp4_scale_shape((experts,), H, I))]
+    if hidden_act == _lib.ACT_SWIGLU:
+        if w3q is None or s3 is None:
+            raise ValueError("SwiGLU needs w3q and s3")
+        checks += [("w3q", w3q, (experts, I, half)), ("s3", s3, _fp4_scale_shape((experts,), I, H))]
+    else:
+        w3q = s3 = None
+    for name, t, shape in checks:
+        _expect(name, t, shape, torch.uint8)
+    _expect("count", count, (groups,), torch.int32)
+    with torch.cuda.device(_one_device(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, y, dev_status)):
+        y = _fp4_output(y, (groups, rows, H), dtype, xq.device)
+        hq = torch.empty((groups, rows, I // 2), dtype=torch.uint8, device=xq.device)
+        sh = torch.empty(_fp4_scale_shape((groups,), rows, I), dtype=torch.uint8, device=xq.device)
+        _lib.check(_lib.load().aristos_expert_ffn_fp4(_ptr(xq), _ptr(sx), _ptr(count), groups, rows, experts, _ptr(w1q),
+                                                      _ptr(s1), _ptr(w3q), _ptr(s3), _ptr(w2q), _ptr(s2), _ptr(hq),
+                                                      _ptr(sh), _ptr(y), H, I, hidden_act, _dt(y), _ptr(dev_status),
+                                                      _stream_ptr()))
+    return y
+
+
+# ---- the layer for a few tokens ---------------------------------------------------------------------------------------
+def moe_few_tokens(x, w_gate, w1, w3, w2, k: int, hidden_act: int, *, gate_fn: int = 0, renorm: int = 0, gate_bias=None,
+                   scales=None, b1=None, b3=None, b2=None, out=None, dev_status=None):
+    """The whole layer for up to 64 tokens in two kernels: x (tokens, H) bf16 or f16; w_gate (E, H); w1 / w3 (E, I, H) and
+    w2 (E, H, I) in x's dtype, or quantised (uint8) with scales = (s1, s3, s2): e4m3 codes as quantize_fp8(w, 128) gives
+    them (bf16 tokens only) or MXFP4 codes (E, I, H / 2), (E, H, I / 2) as quantize_fp4 gives them. Optional biases
+    b1 / b3 (E, I), b2 (E, H) in x's dtype, gate_bias (E) fp32. w3, s3 and b3 are SwiGLU's. Nothing is dropped.
+    Returns (out (tokens, H), topk_idx (tokens, k) int32, topk_w (tokens, k) fp32). See aristos_moe_few_tokens."""
+    n, H = x.shape
+    E, I = w1.shape[:2]
+    gated = hidden_act == _lib.ACT_SWIGLU
+    if gated and w3 is None:
+        raise ValueError("SwiGLU needs w3")
+    w3, b3 = (w3, b3) if gated else (None, None)
+    dt = _dt(x)
+    _expect("w_gate", w_gate, (E, H), x.dtype)
+    if w1.dtype == torch.uint8:
+        if scales is None:
+            raise ValueError("quantised weights need scales = (s1, s3, s2)")
+        s1, s3, s2 = scales
+        s3 = s3 if gated else None
+        fp4 = w1.shape[2] * 2 == H
+        wdt, per, code = (_lib.DTYPE_FP4_E2M1, 2, torch.uint8) if fp4 else (_lib.DTYPE_FP8_E4M3, 1, torch.uint8)
+        shape = ((lambda r, c: _fp4_scale_shape((E,), r, c)) if fp4 else (lambda r, c: (E, (r + 127) // 128, c // 128)))
+        for name, t, r, c in (("s1", s1, I, H), ("s3", s3, I, H), ("s2", s2, H, I)):
+            if t is not None or name != "s3" or gated:
+                if t is None:
+                    raise ValueError(f"{name} is missing")
+                _expect(name, t, shape(r, c), torch.uint8 if fp4 else torch.float32)
+    else:
+        s1 = s3 = s2 = None
+        wdt, per, code = dt, 1, x.dtype
+    _expect("w1", w1, (E, I, H // per), code)
+    _expect("w2", w2, (E, H, I // per), code)
+    if gated:
+        _expect("w3", w3, (E, I, H // per), code)
+    for name, t, shape, d in (("gate_bias", gate_bias, (E,), torch.float32), ("b1", b1, (E, I), x.dtype),
+                              ("b3", b3, (E, I), x.dtype), ("b2", b2, (E, H), x.dtype), ("out", out, (n, H), x.dtype)):
+        if t is not None:
+            _expect(name, t, shape, d)
+    lib = _lib.load()
+    with torch.cuda.device(_one_device(x, w_gate, w1, w3, w2, s1, s3, s2, gate_bias, b1, b3, b2, out, dev_status)):
+        if out is None:
+            out = torch.empty_like(x)
+        idx = torch.empty((n, k), dtype=torch.int32, device=x.device)
+        w = torch.empty((n, k), dtype=torch.float32, device=x.device)
+        nbytes = lib.aristos_moe_few_tokens_workspace_bytes(n, H, I, E, k)
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.aristos_moe_few_tokens(_ptr(x), _ptr(w_gate), _ptr(gate_bias), _ptr(w1), _ptr(w3), _ptr(w2),
+                                              _ptr(s1), _ptr(s3), _ptr(s2), _ptr(b1), _ptr(b3), _ptr(b2), n, H, I, E, k,
+                                              gate_fn, renorm, hidden_act, dt, wdt, _ptr(out), _ptr(idx), _ptr(w),
+                                              _ptr(ws), nbytes, _ptr(dev_status), _stream_ptr()))
+    return out, idx, w
+
+
 def combine(y, slot_of, topk_w):
     S, k = slot_of.shape
     H = y.shape[-1]

@@ -54,7 +54,8 @@ typedef enum aristos_status {
 
 /* torch_dtype (aristos_config.schema.json:54-58) and hidden_act (:24-28), with the extension values. */
 enum { ARISTOS_DTYPE_F32 = 0, ARISTOS_DTYPE_TF32 = 1, ARISTOS_DTYPE_BF16 = 2, ARISTOS_DTYPE_F16 = 3,
-       ARISTOS_DTYPE_FP8_E4M3 = 4 /* extension */ };
+       ARISTOS_DTYPE_FP8_E4M3 = 4 /* extension */,
+       ARISTOS_DTYPE_FP4_E2M1 = 5 /* extension: weights of aristos_moe_few_tokens */ };
 enum { ARISTOS_ACT_RELU = 0, ARISTOS_ACT_GELU = 1, ARISTOS_ACT_SWIGLU = 2 /* extension */,
        ARISTOS_ACT_IDENTITY = 3 /* extension, second projection */ };
 enum { ARISTOS_GATE_SOFTMAX = 0, ARISTOS_GATE_SIGMOID = 1 };
@@ -342,6 +343,59 @@ ARISTOS_API aristos_status_t aristos_expert_ffn_fp8(const void* xq, const float*
                                                     void* hq_scratch, float* sh_scratch, void* y, int H, int I,
                                                     int hidden_act, int row_begin, int row_end, int sm_limit,
                                                     int32_t* dev_status, void* stream);
+/*
+ * Microscaled 4-bit operands (MXFP4, extension): e2m1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign), two to a byte,
+ * the even column in the low half; 32 consecutive columns of a row share the scale 2^(s - 127), one byte s (255: NaN).
+ * Scales are stored in tiles of 128 rows x 4 blocks = 512 bytes, in the order the tensor cores take them: the byte of
+ * (row, block) of a matrix is [row / 128][block / 4][row % 32][row / 32 % 4][block % 4]; a matrix has
+ * ceil(rows / 128) * ceil(cols / 128) tiles (aristos_fp4_scale_bytes for `mats` matrices).
+ * aristos_quantize_fp4: src (mats, rows, cols) in f32, bf16 or f16 -> codes (mats, rows, cols / 2) and scales:
+ *   s = floor(log2 of the block's largest magnitude) + 125, at least 0; elements round to nearest even and saturate at
+ *   6 * 2^(s - 127). A block with an infinity or NaN gets scale 255 and comes back as NaN. Scale bytes of rows and
+ *   blocks that only fill up a tile are 0. aristos_dequantize_fp4 is the way back (bf16 and f32: exact but for
+ *   overflow).
+ * aristos_expert_product_fp4: y[g, r] = A[g, r] . B[g % experts]^T for r < count[g] (count on the device; clamped to
+ *   [0, rows_per_group]); A (groups, rows_per_group, K), B (experts, N, K), y (groups, rows_per_group, N) in out_dtype
+ *   (f32, bf16, f16), fp32 accumulation. Rows past count[g] are not touched.
+ * aristos_expert_ffn_fp4: the expert FFN on such operands, as aristos_expert_ffn_fp8: xq (groups, rows, H), w1q / w3q
+ *   (experts, I, H), w2q (experts, H, I); the hidden activations are rounded once, from fp32 to MXFP4, for the down
+ *   projection: hq_scratch (groups * rows * I / 2 bytes), sh_scratch (aristos_fp4_scale_bytes(groups, rows, I)).
+ * All pointers 16-byte aligned, feature sizes multiples of 64, at most 1024 row groups; dev_status as above, may be NULL.
+ */
+ARISTOS_API size_t aristos_fp4_scale_bytes(int64_t mats, int64_t rows, int cols);
+ARISTOS_API aristos_status_t aristos_quantize_fp4(const void* src, int64_t mats, int64_t rows, int cols, int src_dtype,
+                                                  void* codes, void* scales, void* stream);
+ARISTOS_API aristos_status_t aristos_dequantize_fp4(const void* codes, const void* scales, int64_t mats, int64_t rows,
+                                                    int cols, int dst_dtype, void* dst, void* stream);
+ARISTOS_API aristos_status_t aristos_expert_product_fp4(const void* aq, const void* sa, const int32_t* count, int groups,
+                                                        int rows_per_group, int experts, const void* bq, const void* sb,
+                                                        int N, int K, int out_dtype, void* y, int32_t* dev_status,
+                                                        void* stream);
+ARISTOS_API aristos_status_t aristos_expert_ffn_fp4(const void* xq, const void* sx, const int32_t* count, int groups,
+                                                    int rows_per_group, int experts, const void* w1q, const void* s1,
+                                                    const void* w3q, const void* s3, const void* w2q, const void* s2,
+                                                    void* hq_scratch, void* sh_scratch, void* y, int H, int I,
+                                                    int hidden_act, int out_dtype, int32_t* dev_status, void* stream);
+/*
+ * The whole layer for a few tokens (a serving step): gate, top-k, the chosen experts, weighted sum, in two kernels that
+ * read every chosen expert's weights once. x, out (tokens, H) in bf16 or f16 (`dtype`), 0 <= tokens <=
+ * ARISTOS_FEW_TOKENS_MAX; w_gate (E, H) and the optional biases b1 / b3 (E, I), b2 (E, H) in the same dtype; gate_bias
+ * (E) fp32 or NULL. weights_dtype: `dtype` itself, ARISTOS_DTYPE_FP8_E4M3 (bf16 activations only; s1 / s3 / s2 fp32 as
+ * aristos_quantize_fp8(block_rows = 128) writes them; H and I multiples of 128) or ARISTOS_DTYPE_FP4_E2M1 (codes and
+ * scale tiles of aristos_quantize_fp4). Activations are not quantised. The routing is aristos_gate_topk's, bit for bit;
+ * no token is dropped. topk_idx / topk_w (tokens, k) receive it, or NULL. workspace:
+ * aristos_moe_few_tokens_workspace_bytes (0: sizes out of range) on the device, owned by the caller; it needs no
+ * initialisation, and calls that may overlap on the GPU need one each.
+ */
+enum { ARISTOS_FEW_TOKENS_MAX = 64 };
+ARISTOS_API size_t aristos_moe_few_tokens_workspace_bytes(int tokens, int H, int I, int E, int k);
+ARISTOS_API aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_gate, const float* gate_bias,
+                                                    const void* w1, const void* w3, const void* w2, const void* s1,
+                                                    const void* s3, const void* s2, const void* b1, const void* b3,
+                                                    const void* b2, int tokens, int H, int I, int E, int k, int gate_fn,
+                                                    int renorm, int hidden_act, int dtype, int weights_dtype, void* out,
+                                                    int32_t* topk_idx, float* topk_w, void* workspace,
+                                                    size_t workspace_bytes, int32_t* dev_status, void* stream);
 /* Combine: out[t] = sum_j topk_w[t,j] * y[slot_of[t,j]] in increasing j (fp32), dropped assignments add
  * nothing. Replaces Combine / VAA / deviceCombine (auditorium/combine.cuh:19-205). */
 ARISTOS_API aristos_status_t aristos_combine(const void* y, const int32_t* slot_of, const float* topk_w, int S,

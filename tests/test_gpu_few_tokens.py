@@ -1,0 +1,232 @@
+"""The layer for few tokens (moe_few_tokens): routing bit for bit as the gate's, outputs against 64 bits, at the sizes where
+tiles, steps and lists end, for every weight format; graphs, streams and overlapping calls."""
+import math
+
+import pytest
+
+import fp4_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def _mods():
+    import torch
+    import cuplayground_b200 as cp
+    import cuplayground_b200.layer as layer
+    return torch, cp, layer
+
+
+class Case:
+    def __init__(self, n, E, k, H, I, act, weights="16", dtype="bfloat16", gate_fn=0, renorm=0, bias=False, seed=1, std=0.05):
+        torch, cp, layer = _mods()
+        self.torch, self.layer = torch, layer
+        self.dt = getattr(torch, dtype)
+        self.act, self.k, self.weights = act, k, weights
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        mk = lambda shape, s: (torch.randn(shape, device="cuda", generator=g) * s).to(self.dt)
+        self.x, self.wg = mk((n, H), 1.0), mk((E, H), 0.1)
+        names = ["1", "3", "2"] if act == 2 else ["1", "2"]
+        self.w, self.s, self.mats, self.b = {}, {}, {}, {}
+        for m in names:
+            w = mk((E, H, I) if m == "2" else (E, I, H), std)
+            if weights == "16":
+                self.w[m], self.s[m], self.mats[m] = w, None, (lambda e, w=w: w[e].double())
+            elif weights == "8":
+                q, s = layer.quantize_fp8(w, 128)
+                self.w[m], self.s[m], self.mats[m] = q, s, (lambda e, q=q, s=s: R.decode_fp8(q[e], s[e]))
+            else:
+                q, s = layer.quantize_fp4(w)
+                self.w[m], self.s[m], self.mats[m] = q, s, (lambda e, q=q, s=s: R.decode(q[e], s[e]))
+            self.b[m] = mk((E, H if m == "2" else I), 0.3) if bias else None
+        self.gate_bias = torch.randn(E, device="cuda", generator=g) * 0.2 if bias else None
+        self.kw = dict(gate_fn=gate_fn, renorm=renorm)
+
+    def run(self, x=None, **more):
+        s = None if self.weights == "16" else (self.s["1"], self.s.get("3"), self.s["2"])
+        return self.layer.moe_few_tokens(self.x if x is None else x, self.wg, self.w["1"], self.w.get("3"), self.w["2"],
+                                         self.k, self.act, gate_bias=self.gate_bias, scales=s, b1=self.b["1"],
+                                         b3=self.b.get("3"), b2=self.b["2"], **self.kw, **more)
+
+    def check(self, got, x=None):
+        torch = self.torch
+        x = self.x if x is None else x
+        out, idx, w = got
+        want_idx, want_w = self.layer.gate_topk(x, self.wg, self.k, gate_bias=self.gate_bias, **self.kw)
+        assert torch.equal(idx, want_idx), "the routing is the gate's"
+        assert torch.equal(w, want_w), "the combine weights are the gate's, bit for bit"
+        # value and remainder of a 16-bit type: two half steps
+        ref, bound = R.moe_few(x, idx, w, self.mats, self.b, self.act, R.half_step(self.dt) ** 2)
+        R.assert_within(out, ref, bound + R.half_step(self.dt) * (ref.abs() + bound) * 1.01 + 2.0 ** -25)
+
+
+FORMATS = [("16", "bfloat16"), ("16", "float16"), ("8", "bfloat16"), ("4", "bfloat16"), ("4", "float16")]
+
+
+@pytest.mark.parametrize("weights,dtype", FORMATS)
+@pytest.mark.parametrize("n,E,k,H,I,act", [
+    (1, 8, 2, 256, 512, 2),
+    (1, 1, 1, 128, 128, 0),             # one expert, the smallest sizes: most warps have no step
+    (3, 8, 1, 384, 256, 1),
+    (8, 4, 4, 640, 384, 2),             # every expert, one full token tile
+    (9, 5, 2, 256, 640, 0),             # two token tiles
+    (17, 40, 8, 512, 256, 2),
+    (33, 3, 2, 384, 384, 1),            # long lists, four tiles in use of eight
+    (64, 2, 1, 256, 256, 2),
+    (64, 300, 16, 128, 128, 1),         # more experts than one word of lanes covers, the largest k
+])
+def test_layer(n, E, k, H, I, act, weights, dtype):
+    c = Case(n, E, k, H, I, act, weights, dtype, gate_fn=n % 2, renorm=(n + E) % 2, bias=n % 3 == 0, seed=n)
+    got = c.run()
+    c.check(got)
+    again = c.run()
+    assert all(c.torch.equal(a, b) for a, b in zip(got, again)), "the same call gives the same bits"
+
+
+@pytest.mark.parametrize("weights,dtype", [f for f in FORMATS if f[0] != "8"])
+@pytest.mark.parametrize("H,I", [(64, 64), (192, 320), (1088, 192)])
+def test_feature_sizes_of_64(H, I, weights, dtype):
+    """Sizes at which the last step of a 4-bit row is cut in the middle and units of 64 rows end inside a scale tile."""
+    for n, act in ((2, 2), (11, 0)):
+        c = Case(n, 6, 2, H, I, act, weights, dtype, bias=True, seed=H + I)
+        c.check(c.run())
+
+
+@pytest.mark.parametrize("weights", ["16", "8", "4"])
+def test_wide_layer(weights):
+    c = Case(2, 8, 2, 4096, 1536, 2, weights, std=0.02, renorm=1)
+    c.check(c.run())
+
+
+def test_every_number_of_tokens():
+    c = Case(64, 7, 3, 128, 192, 2, "16")
+    for n in range(1, 65):
+        x = c.x[:n]
+        c.check(c.run(x), x)
+
+
+def test_all_tokens_on_one_expert_and_none_on_the_others():
+    torch, cp, layer = _mods()
+    c = Case(64, 16, 2, 256, 256, 2, "4")
+    c.gate_bias = torch.full((16,), -1000.0, device="cuda")
+    c.gate_bias[5], c.gate_bias[11] = 1000.0, 900.0
+    got = c.run()
+    assert (got[1] == torch.tensor([5, 11], device="cuda", dtype=torch.int32)).all()
+    c.check(got)
+
+
+def test_equal_logits_go_to_the_lower_expert():
+    torch, cp, layer = _mods()
+    c = Case(5, 12, 3, 128, 128, 0)
+    c.wg = c.wg[:1].expand(12, -1).contiguous()
+    got = c.run()
+    assert (got[1] == torch.arange(3, device="cuda", dtype=torch.int32)).all()
+    c.check(got)
+
+
+@pytest.mark.parametrize("weights", ["16", "8", "4"])
+def test_infinities_and_nan_stay_in_their_token(weights):
+    torch, cp, layer = _mods()
+    c = Case(6, 4, 2, 256, 256, 2, weights)
+    clean = c.run()[0]
+    x = c.x.clone()
+    x[2, 7], x[4, 100] = math.nan, math.inf
+    out = c.run(x)[0]
+    keep = [0, 1, 3, 5]
+    assert torch.equal(out[keep], clean[keep])
+    assert not torch.isfinite(out[[2, 4]]).any()
+
+
+def test_nan_in_an_expert_that_nobody_chose_does_not_show():
+    torch, cp, layer = _mods()
+    c = Case(4, 8, 1, 128, 128, 2)
+    c.gate_bias = torch.zeros(8, device="cuda")
+    c.gate_bias[3] = -1000.0
+    for m in ("1", "3", "2"):
+        c.w[m][3] = math.nan
+    assert torch.isfinite(c.run()[0]).all()
+
+
+def test_4_bit_weights_with_scales_far_from_one():
+    torch, cp, layer = _mods()
+    c = Case(3, 4, 2, 256, 256, 0, "4")
+    for m in ("1", "2"):
+        w = R.decode(c.w[m], c.s[m]).float()
+        shift = torch.randint(-50, 30, (*w.shape[:2], w.shape[2] // 32), device="cuda").float()
+        w = w * torch.exp2(shift).repeat_interleave(32, -1)
+        q, s = layer.quantize_fp4(w)
+        c.w[m], c.s[m], c.mats[m] = q, s, (lambda e, q=q, s=s: R.decode(q[e], s[e]))
+    c.check(c.run())
+
+
+def test_in_graphs_with_new_inputs():
+    torch, cp, layer = _mods()
+    a, b = Case(3, 8, 2, 256, 256, 2, "16", seed=1), Case(20, 8, 2, 256, 256, 2, "4", seed=2)
+    graphs, held = [], []
+    for c in (a, b):
+        c.run()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(c.run())
+        graphs.append(g)
+    for seed in range(3):
+        for c, g, h in zip((a, b), graphs, held):
+            c.x.copy_(torch.randn(c.x.shape, device="cuda"))
+            g.replay()
+        torch.cuda.synchronize()
+        for c, h in zip((a, b), held):
+            c.check(h)
+
+
+def test_calls_that_overlap_on_two_streams():
+    torch, cp, layer = _mods()
+    cases = [Case(4, 16, 2, 1024, 1024, 2, "16", seed=1), Case(9, 16, 2, 1024, 1024, 1, "4", seed=2)]
+    want = [c.run() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    results = [[], []]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, (c, st) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(st):
+                results[i].append(c.run(dev_status=status))
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    for r, w in zip(results, want):
+        for got in r:
+            assert all(torch.equal(p, q) for p, q in zip(got, w))
+
+
+def test_no_tokens():
+    torch, cp, layer = _mods()
+    c = Case(4, 4, 2, 128, 128, 0)
+    out, idx, w = c.run(c.x[:0])
+    assert out.shape == (0, 128) and idx.shape == (0, 2) and w.shape == (0, 2)
+
+
+def test_refusals():
+    torch, cp, layer = _mods()
+    c = Case(4, 4, 2, 128, 128, 2)
+    with pytest.raises(cp.AristosError) as e:
+        c.run(torch.zeros(65, 128, device="cuda", dtype=torch.bfloat16))
+    assert e.value.status == 2 and "64" in str(e.value)
+    c.k = 5
+    with pytest.raises(cp.AristosError):
+        c.run()
+    c.k = 2
+    with pytest.raises(ValueError):
+        c.run(c.x.float())
+    with pytest.raises(ValueError):
+        layer.moe_few_tokens(c.x, c.wg, c.w["1"], None, c.w["2"], 2, 2)
+    with pytest.raises(ValueError):
+        layer.moe_few_tokens(c.x, c.wg, c.w["1"], c.w["3"][:2], c.w["2"], 2, 2)
+    with pytest.raises(ValueError):
+        layer.moe_few_tokens(c.x, c.wg[:, :64], c.w["1"], c.w["3"], c.w["2"], 2, 2)
+    with pytest.raises(ValueError):
+        layer.moe_few_tokens(c.x, c.wg, c.w["1"].view(torch.uint8), c.w["3"], c.w["2"], 2, 2)
+    f = Case(4, 4, 2, 128, 128, 0, "8")
+    f.dt, f.x, f.wg = torch.float16, f.x.half(), f.wg.half()
+    with pytest.raises(cp.AristosError) as e:                          # 8-bit weights go with bf16 tokens
+        f.run()
+    assert e.value.status == 6
