@@ -7,27 +7,30 @@
 //
 // With few tokens every weight is used a handful of times, so the layer is bound by reading the chosen experts' weights
 // once: 2, 1 or 0.53 bytes each. Everything else is arranged around that stream:
-//  * few_gate_kernel: a warp per expert and four tokens computes the logits and clears the counters.
+//  * few_gate_kernel: a warp per expert and four tokens computes the logits; it also clears the counters.
 //  * few_ffn_kernel: one CTA per SM, launched while the gate still runs. Every CTA does the (small) top-k and the
 //    expert lists for itself, so no further kernel or grid barrier is needed. The work is a list of items (chosen expert,
-//    8 * RG weight rows): all of the up projection, then all of the down projection, dealt out to groups of W warps.
-//    The warps of a group cut K among themselves (64-byte pieces in turn, so together they read a row's bytes in order),
-//    add their sums through shared memory in a fixed order and one item is done.
-//  * Weights go straight from HBM to registers (each byte is used by one warp only), D steps ahead. The position of the
-//    loads runs ahead of that of the arithmetic across item boundaries and from the up into the down projection, so the
-//    stream does not stop for reductions or for the wait below.
+//    8 * RG weight rows, part of K): all of the up projection, then all of the down projection, dealt out in turn to
+//    groups of W warps. The warps of a group cut K among themselves (64-byte pieces in turn, so together they read a
+//    row's bytes in order) and leave their sums in shared memory; a helper warp per group adds them in a fixed order and
+//    does the epilogue, the stores and the bookkeeping, so that the streaming warps never wait for any of it.
+//  * Weights travel by cp.async into a ring that every lane has for itself, D steps ahead of the arithmetic and across
+//    item boundaries, from the up into the down projection: the stream does not stop for reductions or for the wait below.
 //  * An item of the down projection waits until all of its expert's up items are done (a counter per expert; the wait is
 //    bounded). Up items never wait and come first in every group's list, so the wait ends.
 //  * The products run on the warp-level matrix instruction m16n8k16: 16 weight rows (gate and up rows of the same
-//    columns for SwiGLU) x 8 tokens x 16 of K. The order of K inside a step does not matter to the sum, so a lane keeps
-//    the 16 adjacent bytes it loaded and the tokens are read in the same order. The 5th-generation tensor cores would
-//    need 128 weight rows per instruction and the operands in shared memory, for a rate that this stream cannot use.
-//  * Expert outputs are summed per block of rows by the group that finishes the block last, in the order of j.
-// 8-bit weights (e4m3, one scale per 128 x 128) are widened to bf16 exactly and their scale multiplies the fp32 sum of a
-// step; 4-bit weights (MXFP4) are widened with their scale applied (a power of two: exact). Activations meet them in
-// bf16: fp16 tokens as two bf16 numbers (value and remainder, exact). The hidden activations are kept as two 16-bit
-// numbers as well (the second holds what the first rounds off), so that they lose nothing that the output type would
-// show: a single rounding of h to bf16 would by itself be as large as that of the output.
+//    columns for SwiGLU) x 8 tokens x 16 of K. The order of K inside a step does not matter to the sum, so a lane uses
+//    the bytes as they lie and the tokens are read in the same order. The 5th-generation tensor cores would need 128
+//    weight rows per instruction and both operands in shared memory, for a rate that this stream cannot use.
+//  * Expert outputs are summed per block of rows by the helper that finishes the block last, in the order of j.
+//
+// Operand types. The instruction multiplies 16-bit numbers. bf16 weights meet tokens in bf16 (as they are) and hidden
+// activations as two bf16 numbers, value and remainder: a single rounding of h to bf16 would by itself be as large as
+// that of the output. fp16, e4m3 and e2m1 weights meet fp16 numbers, in which all three are exact; bf16 tokens and the
+// hidden activations are brought into fp16's range by a power of two per token (the largest magnitude to [2^14, 2^15)),
+// which is undone on the fp32 sums: bf16 tokens lose nothing that is not 2^-40 of the token's largest element, hidden
+// activations are rounded once to 11 bits. h itself is kept in fp32. Scales of quantised weights multiply fp32 sums:
+// e4m3's per step (half of its 128 columns), e2m1's per block of 32.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -42,19 +45,26 @@ namespace {
 constexpr int FEW_MAX_TOKENS = ARISTOS_FEW_TOKENS_MAX;
 constexpr int FEW_MAX_EXPERTS = 1024;
 constexpr int FEW_MAX_SLOTS = FEW_MAX_TOKENS * MAX_TOPK;
-constexpr int FEW_THREADS = 512;
 static_assert(FEW_MAX_TOKENS <= 64, "the expert lists keep the tokens of an expert in 64 bits");
+
+constexpr int FEW_W = 7;                                  // warps that share an item (7 + a helper, twice: 128 registers each)
+constexpr int FEW_GROUPS = 2;                             // groups per CTA
+constexpr int FEW_STREAM_WARPS = FEW_W * FEW_GROUPS;
+constexpr int FEW_WARPS = FEW_STREAM_WARPS + FEW_GROUPS;  // and a helper per group
+constexpr int FEW_THREADS = 32 * FEW_WARPS;
 
 enum { FEW_BF16 = 0, FEW_F16 = 1, FEW_FP8 = 2, FEW_FP4 = 3 };      // weight formats
 
 struct FewParams {
     const float* logits;
-    const void* x;                 // (planes, n, H) 16-bit
+    const uint16_t* x;             // (n, H) in the operand type
+    const float* x_scale;          // (n) what the sums of a token are multiplied with, or NULL: 1
     const uint8_t *w1, *w3, *w2;
-    const void *s1, *s3, *s2;      // fp8: fp32 per 128 x 128; fp4: scale tiles
+    const uint8_t *s1, *s3, *s2;   // fp8: fp32 per 128 x 128; fp4: scale tiles
     const void *b1, *b3, *b2;      // activations' dtype, or NULL
-    void* h;                       // (2, slots, I) 16-bit: value, remainder
-    float* partial;                // (slots, H)
+    float* h;                      // (slots, I)
+    uint32_t* h_max;               // (slots) bits of the largest |h| of a row
+    float* partial;                // (parts, slots, H)
     int32_t* done;                 // up items finished, per chosen expert
     int32_t* ticket;               // down items finished, per block of rows
     void* out;
@@ -63,9 +73,17 @@ struct FewParams {
     int32_t* dev_status;
     int n, H, I, E, k;
     int gate_fn, renorm, act;
-    int x_planes;
+    int parts;                     // K of the down projection is cut into so many items
     int f16;                       // dtype of out and of the biases: fp16, else bf16
 };
+
+// The power of two that brings a largest magnitude (its bits) to [2^14, 2^15) and the one that undoes it. Zero, and what
+// is not finite, stays as it is; the exponent is bounded so that both are normal numbers.
+__device__ __forceinline__ float few_norm(uint32_t max_bits, bool undo) {
+    const int field = (int)(max_bits >> 23);
+    const int e = (max_bits == 0 || field == 255) ? 0 : max(min(127 + 14 - field, 120), -120);
+    return __uint_as_float((uint32_t)(127 + (undo ? -e : e)) << 23);
+}
 
 // ---- gate --------------------------------------------------------------------------------------------------------------
 constexpr int FEW_GATE_WARPS = 8, FEW_GATE_TOK = 4;
@@ -73,22 +91,39 @@ constexpr int FEW_GATE_WARPS = 8, FEW_GATE_TOK = 4;
 template <typename T>
 __global__ void __launch_bounds__(FEW_GATE_WARPS * 32)
 few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* __restrict__ bias, int n, int H, int E,
-                float* __restrict__ logits, int32_t* __restrict__ counters, int ncounters,
-                __nv_bfloat16* __restrict__ x_planes) {
+                float* __restrict__ logits, int32_t* __restrict__ counters, int ncounters, __half* __restrict__ x_norm,
+                float* __restrict__ x_scale) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int gt = blockIdx.x * blockDim.x + threadIdx.x, threads = gridDim.x * blockDim.x;
     for (int i = gt; i < ncounters; i += threads) counters[i] = 0;
-    if (x_planes) {
-        const size_t total = (size_t)n * H;
-        for (size_t i = gt; i < total; i += threads) {
-            const float v = static_cast<float>(x[i]);
-            const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-            x_planes[i] = hi;
-            // an infinite value has no remainder (inf - inf would be NaN)
-            x_planes[total + i] = __float2bfloat16_rn(isinf(v) ? 0.0f : v - __bfloat162float(hi));
+    const int lane = gt & 31;
+    int warp = gt >> 5;
+    const int nchunk = H >> 3;
+    if (x_norm) {
+        // the first n warps: a token in fp16, scaled by a power of two
+        if (warp < n) {
+            const T* row = x + (size_t)warp * H;
+            uint32_t m = 0;
+            for (int q = lane; q < nchunk; q += 32) {
+                float v[8];
+                load8(row + q * 8, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+            }
+            m = __reduce_max_sync(0xffffffffu, m);
+            const float f = few_norm(m, false);
+            for (int q = lane; q < nchunk; q += 32) {
+                float v[8];
+                load8(row + q * 8, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= f;
+                store8(x_norm + (size_t)warp * H + q * 8, v);
+            }
+            if (lane == 0) x_scale[warp] = few_norm(m, true);
         }
+        warp -= n;
+        if (warp < 0) return;
     }
-    const int warp = gt >> 5, lane = gt & 31;
     const int tgroups = (n + FEW_GATE_TOK - 1) / FEW_GATE_TOK;
     if (warp >= E * tgroups) return;
     const int e = warp / tgroups, t0 = (warp - e * tgroups) * FEW_GATE_TOK;
@@ -99,7 +134,6 @@ few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* 
     float2 acc[FEW_GATE_TOK];
 #pragma unroll
     for (int i = 0; i < FEW_GATE_TOK; ++i) acc[i] = make_float2(0.0f, 0.0f);
-    const int nchunk = H >> 3;
 #pragma unroll 4
     for (int q = lane; q < nchunk; q += 32) {
         GateChunk<T> wc;
@@ -112,19 +146,19 @@ few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* 
             for (int j = 0; j < 4; ++j) fma_pair(acc[i], xc, wc, j);
         }
     }
-    const float b = bias ? bias[e] : 0.0f;
 #pragma unroll
     for (int i = 0; i < FEW_GATE_TOK; ++i) {
         float s = acc[i].x + acc[i].y;
 #pragma unroll
         for (int m = 16; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-        if (bias) s = s + b;
+        if (bias) s = s + bias[e];
         if (lane == 0 && t0 + i < n) logits[(size_t)(t0 + i) * E + e] = s;
     }
 }
 
 // ---- the experts ---------------------------------------------------------------------------------------------------------
 struct FewLists {
+    uint64_t bars[FEW_GROUPS * 4];             // per group: sums written (2 buffers), buffer free (2)
     float w[FEW_MAX_SLOTS];                    // combine weights (t, j)
     uint32_t mask[FEW_MAX_EXPERTS][2];         // tokens that chose an expert
     uint16_t idx[FEW_MAX_SLOTS];               // chosen experts (t, j)
@@ -133,7 +167,7 @@ struct FewLists {
     uint16_t active[FEW_MAX_EXPERTS];          // chosen experts, increasing
     uint8_t token[FEW_MAX_SLOTS];              // token of a row
     int actives;
-    int last[FEW_THREADS / 32];                // per group: this item finished its block of rows
+    int abort;
 };
 
 // Top-k of one token by one warp: the selection and the weights of the gate kernels, bit for bit (gate.cu).
@@ -200,14 +234,22 @@ __device__ __forceinline__ void few_topk(const float* __restrict__ l, const FewP
         if (j < p.k && lane == j) s.w[t * p.k + j] = w_sel[j];
 }
 
-__device__ __forceinline__ uint4 load_stream(const uint8_t* ptr) {       // weights: read once, kept out of L1
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
+
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
-// Activations: through L1 (every warp of the CTA reads the same rows). Not the read-only path: h is written in this
-// kernel, and read only after the acquire that follows its expert's counter.
+// Activations. Not the read-only path: h is written in this kernel, and read only after the acquire that follows its
+// expert's counter.
 __device__ __forceinline__ uint4 load_act(const void* ptr) {
     uint4 v;
     asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
@@ -225,34 +267,15 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+    const __half2 t = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
     const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&t);
 }
-
-// The 8 adjacent elements number `sub` of a lane's 16 bytes of weights as four 16-bit pairs. scale: fp4 only, 2^(s-127).
-template <int WF>
-__device__ __forceinline__ void widen(const uint4& raw, int sub, float scale, uint32_t (&v)[4]) {
-    if constexpr (WF == FEW_BF16 || WF == FEW_F16) {
-        v[0] = raw.x; v[1] = raw.y; v[2] = raw.z; v[3] = raw.w;
-    } else if constexpr (WF == FEW_FP8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t two = (word_of(raw, 2 * sub + (i >> 1)) >> (16 * (i & 1))) & 0xFFFFu;
-            const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
-            v[i] = bf16_pair(f.x, f.y);
-        }
-    } else {
-        const uint32_t w = word_of(raw, sub);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(fp4_unpack2((w >> (8 * i)) & 255u));
-            v[i] = bf16_pair(f.x * scale, f.y * scale);
-        }
-    }
-}
+__device__ __forceinline__ uint32_t half_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
 template <int WF> struct FewFormat;
 template <> struct FewFormat<FEW_BF16> { static constexpr int SUBS = 1; };
@@ -260,31 +283,41 @@ template <> struct FewFormat<FEW_F16> { static constexpr int SUBS = 1; };
 template <> struct FewFormat<FEW_FP8> { static constexpr int SUBS = 2; };
 template <> struct FewFormat<FEW_FP4> { static constexpr int SUBS = 4; };
 
-// NT: token tiles of 8 (at least ceil(n / 8)); RG: groups of 8 weight rows per item; W: warps per item; D: steps in flight.
-template <int WF, int NT, int RG, int W, int D>
+// NT: token tiles of 8 (at least ceil(n / 8)); RG: groups of 8 weight rows per item; D: steps in flight; BUFS: buffers for
+// the sums of an item.
+template <int WF, int NT, int RG_, int D_, int BUFS_>
+struct FewShape {
+    static constexpr int RG = RG_, D = D_, BUFS = BUFS_;
+    static constexpr int SUBS = FewFormat<WF>::SUBS;
+    static constexpr int STEP_K = 32 * SUBS;            // elements of K per step: 64 bytes of a row
+    static constexpr int TILES = RG / 2;                // m16 tiles: row groups (2 t, 2 t + 1)
+    static constexpr int SCALE_BYTES = WF == FEW_FP4 ? 32 * RG : (WF == FEW_FP8 ? 16 : 0);
+    static constexpr int SLOT = RG * 512 + SCALE_BYTES;
+    static constexpr int RED = TILES * NT * 128;        // floats per warp of one buffer
+    static constexpr size_t SMEM = (size_t)FEW_STREAM_WARPS * (D * SLOT + BUFS * RED * 4);
+    static_assert(RG == 2 || RG == 4, "a lane of a quad copies the scale word of one row group");
+};
+
+template <int WF, int NT, class S>
 __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_constant__ FewParams p) {
-    constexpr bool F16 = WF == FEW_F16;
-    constexpr int SUBS = FewFormat<WF>::SUBS;
-    constexpr int LANE_K = 8 * SUBS;                    // elements of K that a lane loads per step
-    constexpr int STEP_K = 4 * LANE_K;
-    constexpr int TILES = RG / 2;                       // m16 tiles: row groups (2 t, 2 t + 1)
-    constexpr int GROUPS = FEW_THREADS / 32 / W;
-    constexpr int RED = TILES * NT * 128;               // floats per warp of one reduction buffer
+    constexpr bool F16 = WF != FEW_BF16;                // operand type
+    constexpr int RG = S::RG, TILES = S::TILES, SUBS = S::SUBS, STEP_K = S::STEP_K, RED = S::RED;
     __shared__ FewLists s;
-    extern __shared__ float red_all[];
+    extern __shared__ __align__(16) uint8_t few_smem[];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = lane >> 2, q = lane & 3;
-    const int wk = warp % W, grp = warp / W;
-    const int tid = wk * 32 + lane;                     // inside the group
-    float* red = red_all + grp * 2 * W * RED;
     const bool gated = p.act == ARISTOS_ACT_SWIGLU;
 
     for (int i = threadIdx.x; i < 2 * p.E; i += FEW_THREADS) s.mask[i >> 1][i & 1] = 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < FEW_GROUPS * 4; ++i) ptx::mbar_init(ptx::smem_u32(&s.bars[i]), (i & 2) ? 1 : FEW_W);
+        s.abort = 0;
+        ptx::fence_mbar_init();
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     // ---- routing and expert lists (every CTA for itself) ------------------------------------------------------------------
-    for (int t = warp; t < p.n; t += FEW_THREADS / 32) few_topk(p.logits + (size_t)t * p.E, p, t, lane, s);
+    for (int t = warp; t < p.n; t += FEW_WARPS) few_topk(p.logits + (size_t)t * p.E, p, t, lane, s);
     __syncthreads();
     const int slots = p.n * p.k;
     for (int i = threadIdx.x; i < slots; i += FEW_THREADS) {
@@ -332,298 +365,412 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     const int actives = s.actives;
     const int up_rows = gated ? 4 * RG : 8 * RG, down_rows = 8 * RG;
     const int up_blocks = p.I / up_rows, down_blocks = p.H / down_rows;
-    const int up_items = actives * up_blocks, items = up_items + actives * down_blocks;
+    const int up_items = actives * up_blocks, items = up_items + actives * down_blocks * p.parts;
     const int up_steps = (p.H + STEP_K - 1) / STEP_K, down_steps = (p.I + STEP_K - 1) / STEP_K;
-    const int stride = gridDim.x * GROUPS, first = blockIdx.x * GROUPS + grp;
+    const int part_steps = (down_steps + p.parts - 1) / p.parts;
+    const int grp = warp < FEW_STREAM_WARPS ? warp / FEW_W : warp - FEW_STREAM_WARPS;
+    const int stride = gridDim.x * FEW_GROUPS, first = blockIdx.x * FEW_GROUPS + grp;
 
-    // Row of row group i of an item that starts at weight row r0. The two row groups of a tile are 32 rows apart (or gate
-    // and up rows of the same number), so that the 4-bit scale words of both lie side by side.
-    auto block_row = [&](bool pairs, int rb) {
-        // rows are cut into units of 64; a unit holds 32 / (8 * TILES) blocks (gated with one tile: 8)
-        if (!pairs && TILES == 1) return rb * 8;
-        constexpr int PER = TILES == 1 ? 4 : (TILES == 2 ? 2 : 1);
-        return pairs ? (rb / PER) * 64 + (rb % PER) * 8 * TILES : (rb / 4) * 64 + (rb % 4) * 8;
+    struct Item {
+        bool up;
+        int a, row, part;          // chosen expert, first weight row, part of K
+        int begin, end;            // steps
     };
-    static_assert(RG == 2 || RG == 4, "row groups per item");
+    auto item_at = [&](int it) {
+        Item i;
+        i.up = it < up_items;
+        if (i.up) {
+            i.a = it / up_blocks;
+            i.row = (it - i.a * up_blocks) * up_rows;
+            i.part = 0;
+            i.begin = 0;
+            i.end = up_steps;
+        } else {
+            const int local = it - up_items, per = down_blocks * p.parts;
+            i.a = local / per;
+            const int r = local - i.a * per;
+            const int rb = r / p.parts;
+            i.row = rb * down_rows;
+            i.part = r - rb * p.parts;
+            i.begin = i.part * part_steps;
+            i.end = min(i.begin + part_steps, down_steps);
+        }
+        return i;
+    };
+    auto tokens_of = [&](int e) { return __popc(s.mask[e][0]) + __popc(s.mask[e][1]); };
+    const uint32_t bar_full = ptx::smem_u32(&s.bars[grp * 4]), bar_free = bar_full + 16;
+    float* red = reinterpret_cast<float*>(few_smem + FEW_STREAM_WARPS * S::D * S::SLOT) + grp * FEW_W * S::BUFS * RED;
 
-    // position of the loads: item, step, one pointer per row group
-    int l_it = first - stride, l_s = 0, l_steps = 0;
+    if (warp >= FEW_STREAM_WARPS) {
+        // ============================================================ helper: sums, epilogue, bookkeeping
+        int nth = 0;
+        for (int it = first; it < items; it += stride, ++nth) {
+            const Item item = item_at(it);
+            const int e = s.active[item.a], base = s.base[e], m = tokens_of(e);
+            const int b = nth % S::BUFS;
+            const float* buf = red + b * FEW_W * RED;
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_full + 8 * b, (nth / S::BUFS) & 1, &s.abort, p.dev_status)))
+                return;
+            // the sum of row `j` of the item (in the order of its row groups) for token `tok` of the expert
+            auto total = [&](int j, int tok) {
+                const int at = (((j >> 4) * NT + (tok >> 3)) * 4 + ((j >> 3) & 1) * 2 + (tok & 1)) * 32 + (j & 7) * 4 + ((tok & 7) >> 1);
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < FEW_W; ++w) v += buf[w * RED + at];
+                return v;
+            };
+            auto bias_at = [&](const void* bias, size_t i) {
+                if (!bias) return 0.0f;
+                return p.f16 ? __half2float(static_cast<const __half*>(bias)[i])
+                             : __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[i]);
+            };
+            if (item.up) {
+                const int rows = up_rows;                  // 8, 16 or 32: a power of two that a warp holds evenly
+                const int span = min(rows, 32);
+                for (int i0 = 0; i0 < rows * m; i0 += 32) {
+                    const int i = i0 + lane;
+                    const int tok = i / rows, j = i - tok * rows;
+                    uint32_t mag = 0;
+                    if (tok < m) {
+                        const int slot = base + tok;
+                        const float f = p.x_scale ? __ldg(p.x_scale + s.token[slot]) : 1.0f;
+                        const size_t col = (size_t)e * p.I + item.row + j;
+                        float v;
+                        if (gated) {
+                            // row groups alternate between gate and up rows
+                            const int jg = (j >> 3) * 16 + (j & 7);
+                            const float gate = total(jg, tok) * f + bias_at(p.b1, col);
+                            const float lin = total(jg + 8, tok) * f + bias_at(p.b3, col);
+                            v = act_silu(gate) * lin;
+                        } else {
+                            v = total(j, tok) * f + bias_at(p.b1, col);
+                            v = p.act == ARISTOS_ACT_RELU ? act_relu(v) : act_gelu(v);
+                        }
+                        p.h[(size_t)slot * p.I + item.row + j] = v;
+                        mag = __float_as_uint(v) & 0x7FFFFFFFu;
+                    }
+                    if constexpr (F16) {
+                        for (int d = span >> 1; d >= 1; d >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, d));
+                        if (tok < m && (lane & (span - 1)) == 0) atomicMax(p.h_max + base + tok, mag);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(bar_free + 8 * b);
+                    __threadfence();
+                    atomicAdd(p.done + item.a, 1);
+                }
+            } else {
+                for (int i = lane; i < down_rows * m; i += 32) {
+                    const int tok = i / down_rows, j = i - tok * down_rows;
+                    const int slot = base + tok;
+                    float v = total(j, tok);
+                    if constexpr (F16) v *= few_norm(__ldcg(p.h_max + slot), true);
+                    if (item.part == 0) v += bias_at(p.b2, (size_t)e * p.H + item.row + j);
+                    p.partial[((size_t)item.part * slots + slot) * p.H + item.row + j] = v;
+                }
+                __syncwarp();
+                int last = 0;
+                if (lane == 0) {
+                    ptx::mbar_arrive(bar_free + 8 * b);
+                    __threadfence();
+                    last = atomicAdd(p.ticket + item.row / down_rows, 1) == actives * p.parts - 1;
+                    __threadfence();
+                }
+                if (__shfl_sync(0xffffffffu, last, 0)) {
+                    // every chosen expert has delivered these rows: the weighted sum of each token, in the order of j
+                    for (int i = lane; i < down_rows * p.n; i += 32) {
+                        const int tok = i / down_rows, j = i - tok * down_rows;
+                        float v = 0.0f;
+                        for (int c = 0; c < p.k; ++c) {
+                            const float* src = p.partial + (size_t)s.slot[tok * p.k + c] * p.H + item.row + j;
+                            float y = __ldcg(src);
+                            for (int q = 1; q < p.parts; ++q) y += __ldcg(src + (size_t)q * slots * p.H);
+                            v = fmaf(s.w[tok * p.k + c], y, v);
+                        }
+                        const size_t at = (size_t)tok * p.H + item.row + j;
+                        if (p.f16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+                        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+                    }
+                }
+            }
+        }
+        return;
+    }
+
+    // ================================================================ streaming warps
+    const int g = lane >> 2, q = lane & 3;
+    const int wk = warp % FEW_W;
+    const uint32_t ring = ptx::smem_u32(few_smem) + warp * (S::D * S::SLOT);
+    // where this lane's 16 bytes of a row group go: as they lie, but 4-bit rows block by block (32 elements = 16 bytes),
+    // so that the 8 codes a lane takes of every block can be read without bank conflicts
+    const uint32_t put = WF == FEW_FP4 ? (q * 8 + g) * 16 : lane * 16;
+
+    // ---- position of the loads
+    int l_it = first - stride, l_s = 0, l_end = 0, l_K = 0, l_slot = 0;
     const uint8_t* l_ptr[RG];
-    const uint8_t* l_scale[RG];                         // fp4: scale words of the row; fp8: of its 128 x 128 blocks
+    const uint8_t* l_scale = nullptr;                   // fp4: the words of this lane's row in row group q; fp8: group `lane`
     auto next_load_item = [&]() {
+        Item i;
         do {
             l_it += stride;
             if (l_it >= items) return;
-            l_steps = l_it < up_items ? up_steps : down_steps;
-        } while (wk >= l_steps);
-        l_s = wk;
-        const bool up = l_it < up_items;
-        const int local = up ? l_it : l_it - up_items;
-        const int blocks = up ? up_blocks : down_blocks;
-        const int a = local / blocks, rb = local - a * blocks;
-        const int e = s.active[a];
-        const int rows = up ? p.I : p.H, K = up ? p.H : p.I;
+            i = item_at(l_it);
+            l_s = i.begin + wk;
+        } while (l_s >= i.end);
+        l_end = i.end;
+        const int e = s.active[i.a];
+        const int rows = i.up ? p.I : p.H, K = i.up ? p.H : p.I;
+        l_K = K;
         const size_t row_bytes = (size_t)K * 2 / SUBS;
-        const bool pairs = !(up && gated);
-        const int r0 = block_row(pairs, rb);
+        const bool alternate = i.up && gated;
+        // weight row 8 * group of the item: SwiGLU alternates between gate and up rows
+        auto row_of = [&](int group) { return i.row + 8 * (alternate ? group >> 1 : group); };
 #pragma unroll
-        for (int i = 0; i < RG; ++i) {
-            const bool third = !pairs && (i & 1);
-            const int row = r0 + (pairs ? 8 * (i >> 1) + 32 * (i & 1) : 32 * (i >> 1)) + g;
-            const uint8_t* w = up ? (third ? p.w3 : p.w1) : p.w2;
-            l_ptr[i] = w + ((size_t)e * rows + row) * row_bytes + q * 16;
-            const uint8_t* sc = static_cast<const uint8_t*>(up ? (third ? p.s3 : p.s1) : p.s2);
-            if constexpr (WF == FEW_FP4)
-                l_scale[i] = sc + ((size_t)e * fp4_row_tiles(rows) + (row >> 7)) * fp4_col_tiles(K) * FP4_TILE_BYTES + fp4_tile_word(row);
-            else if constexpr (WF == FEW_FP8)
-                l_scale[i] = sc + ((size_t)e * ((rows + 127) / 128) + (row >> 7)) * (K / 128) * 4;
+        for (int r = 0; r < RG; ++r) {
+            const uint8_t* w = i.up ? (alternate && (r & 1) ? p.w3 : p.w1) : p.w2;
+            l_ptr[r] = w + ((size_t)e * rows + row_of(r) + g) * row_bytes + q * 16;
+        }
+        if constexpr (WF == FEW_FP4) {
+            const int group = min(q, RG - 1), row = row_of(group) + g;
+            const uint8_t* sc = i.up ? (alternate && (group & 1) ? p.s3 : p.s1) : p.s2;
+            l_scale = sc + ((size_t)e * fp4_row_tiles(rows) + (row >> 7)) * fp4_col_tiles(K) * FP4_TILE_BYTES + fp4_tile_word(row);
+        } else if constexpr (WF == FEW_FP8) {
+            const int group = min(lane, RG - 1);
+            const uint8_t* sc = i.up ? (alternate && (group & 1) ? p.s3 : p.s1) : p.s2;
+            l_scale = sc + ((size_t)e * ((rows + 127) / 128) + (row_of(group) >> 7)) * (K / 128) * 4;
         }
     };
-    uint4 ring[D][RG];
-    uint32_t ring_scale[D][RG];
-    auto issue = [&](uint4 (&r)[RG], uint32_t (&rs)[RG]) {
-        if (l_it >= items) return;
-        // a lane whose part of the last step lies past K (4-bit weights, K an odd multiple of 64) loads zeros
-        const bool in = WF != FEW_FP4 || l_s * STEP_K + q * LANE_K < (l_it < up_items ? p.H : p.I);
+    auto issue = [&]() {
+        if (l_it < items) {
+            const uint32_t to = ring + l_slot * S::SLOT;
+            // a lane whose part of the last step lies past K (4-bit weights, K an odd multiple of 64) gets zeros
+            const int bytes = WF != FEW_FP4 || l_s * STEP_K + q * 32 < l_K ? 16 : 0;
 #pragma unroll
-        for (int i = 0; i < RG; ++i) {
-            r[i] = in ? load_stream(l_ptr[i] + (size_t)l_s * 64) : make_uint4(0, 0, 0, 0);
-            if constexpr (WF == FEW_FP4)
-                rs[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(l_scale[i] + (size_t)l_s * FP4_TILE_BYTES)) : 0u;
-            else if constexpr (WF == FEW_FP8)
-                rs[i] = __ldg(reinterpret_cast<const uint32_t*>(l_scale[i]) + (l_s >> 1));
+            for (int r = 0; r < RG; ++r) copy_async16(to + r * 512 + put, l_ptr[r] + (bytes ? (size_t)l_s * 64 : 0), bytes);
+            if constexpr (WF == FEW_FP4) {
+                if (q < RG) copy_async4(to + RG * 512 + (g * RG + q) * 4, l_scale + (size_t)l_s * FP4_TILE_BYTES);
+            } else if constexpr (WF == FEW_FP8) {
+                if (lane < RG) copy_async4(to + RG * 512 + lane * 4, l_scale + (l_s >> 1) * 4);
+            }
+            if (++l_slot == S::D) l_slot = 0;
+            l_s += FEW_W;
+            if (l_s >= l_end) next_load_item();
         }
-        l_s += W;
-        if (l_s >= l_steps) next_load_item();
+        copy_commit();                                  // one group per step, empty ones at the end
     };
 
-    // position of the arithmetic
-    int c_it = first, c_s = wk, c_steps = 0, c_a = 0, c_m = 0, c_row = 0;
-    bool c_up = true;
-    int parity = 0, ready = -1;
-    const uint16_t* rows_at[NT];                        // plane 0 of this lane's token row in tile nt, at its part of step 0
-    size_t plane = 0;
-    int planes = 1;
-    float acc[TILES][NT][4];
-    auto start_item = [&]() {
-        c_up = c_it < up_items;
-        const int local = c_up ? c_it : c_it - up_items;
-        const int blocks = c_up ? up_blocks : down_blocks;
-        c_a = local / blocks;
-        c_row = block_row(!(c_up && gated), local - c_a * blocks);
-        c_steps = c_up ? up_steps : down_steps;
-        c_s = wk;
-        const int e = s.active[c_a], base = s.base[e];
-        c_m = __popc(s.mask[e][0]) + __popc(s.mask[e][1]);
-        planes = c_up ? p.x_planes : 2;
-        plane = c_up ? (size_t)p.n * p.H : (size_t)slots * p.I;
+    if (first >= items) return;
+    next_load_item();
+#pragma unroll 1
+    for (int d = 0; d < S::D - 1; ++d) issue();
+
+    int c_slot = 0, nth = 0, ready = -1;
+    for (int it = first; it < items; it += stride, ++nth) {
+        const Item item = item_at(it);
+        const int e = s.active[item.a], base = s.base[e], m = tokens_of(e);
+        const int K = item.up ? p.H : p.I;
+        if (!item.up && ready < item.a) {
+            // all of this expert's hidden activations must be there (the list is in expert order)
+            bool ok = true;
+            if (lane == 0) {
+                uint64_t t0 = 0;
+                for (uint32_t i = 0;; ++i) {
+                    int32_t v;
+                    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.done + item.a) : "memory");
+                    if (v >= up_blocks) break;
+                    if (i == 0) t0 = ptx::globaltimer_ns();
+                    if ((i & 63u) == 63u) {
+                        ok = !*static_cast<volatile int*>(&s.abort);
+                        if (ok && ptx::globaltimer_ns() - t0 > ptx::WAIT_LIMIT_NS) {
+                            s.abort = 1;
+                            if (p.dev_status) atomicOr(p.dev_status, DEV_FAULT_TIMEOUT);
+                            ok = false;
+                        }
+                        if (!ok) break;
+                    }
+                }
+            }
+            if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+            ready = item.a;
+        }
+        // this lane's token row in every tile; rows past the expert's last one repeat it, their sums are not used
+        uint32_t row_at[NT];
+        float norm[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            // rows past the expert's last one repeat it; their sums are not used
-            const int slot = base + min(nt * 8 + g, c_m - 1);
-            rows_at[nt] = (c_up ? static_cast<const uint16_t*>(p.x) + (size_t)s.token[slot] * p.H
-                                : static_cast<const uint16_t*>(p.h) + (size_t)slot * p.I) + q * LANE_K;
+            const int slot = base + min(nt * 8 + g, m - 1);
+            row_at[nt] = item.up ? s.token[slot] : slot;
+            norm[nt] = F16 && !item.up ? few_norm(__ldcg(p.h_max + slot), false) : 1.0f;
         }
+        float acc[TILES][NT][4];
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[t][nt][i] = 0.0f;
-        if (!c_up && ready < c_a) {
-            // all of this expert's hidden activations must be there (lists are in expert order: earlier ones are too)
-            if (lane == 0) {
-                const int32_t* flag = p.done + c_a;
-                uint64_t t0 = 0;
-                for (uint32_t i = 0;; ++i) {
-                    int32_t v;
-                    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
-                    if (v >= up_blocks) break;
-                    if (i == 0) t0 = ptx::globaltimer_ns();
-                    if ((i & 63u) == 63u && ptx::globaltimer_ns() - t0 > ptx::WAIT_LIMIT_NS) {
-                        if (p.dev_status) atomicOr(p.dev_status, DEV_FAULT_TIMEOUT);
-                        break;
+
+        for (int st = item.begin + wk; st < item.end; st += FEW_W) {
+            const int k0 = st * STEP_K;
+            // elements k0 + sub_at(sub) .. + 7 of the token row are this lane's share of sub-step `sub`
+            auto sub_at = [&](int sub) { return WF == FEW_FP4 ? sub * 32 + q * 8 : q * 8 * SUBS + sub * 8; };
+            const int subs = WF == FEW_FP4 ? min(SUBS, (K - k0) >> 5) : SUBS;
+            // operand of token tile nt, sub-step sub: value, and (bf16 hidden activations) remainder
+            auto load_tokens = [&](int nt, int sub, uint4& hi, uint4& lo) {
+                if (item.up) {
+                    hi = load_act(p.x + (size_t)row_at[nt] * p.H + k0 + sub_at(sub));
+                } else {
+                    const float* src = p.h + (size_t)row_at[nt] * p.I + k0 + sub_at(sub);
+                    hi = load_act(src);
+                    lo = load_act(src + 4);
+                }
+            };
+            auto convert_tokens = [&](int nt, uint4& hi, uint4& lo) {
+                if (item.up) return;
+                const float v[8] = {__uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w),
+                                    __uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w)};
+                uint32_t a[4], b[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (F16) {
+                        a[i] = half_pair(v[2 * i] * norm[nt], v[2 * i + 1] * norm[nt]);
+                        b[i] = 0;
+                    } else {
+                        a[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
+                        const float r0 = v[2 * i] - __uint_as_float(a[i] << 16), r1 = v[2 * i + 1] - __uint_as_float(a[i] & 0xFFFF0000u);
+                        // a value that rounds to infinity has no remainder
+                        b[i] = bf16_pair((a[i] & 0x7F80u) == 0x7F80u ? 0.0f : r0, (a[i] & 0x7F800000u) == 0x7F800000u ? 0.0f : r1);
                     }
                 }
-            }
-            __syncwarp();
-            ready = c_a;
-        }
-    };
+                hi = make_uint4(a[0], a[1], a[2], a[3]);
+                lo = make_uint4(b[0], b[1], b[2], b[3]);
+            };
+            // the first tile's tokens are asked for before the wait for the weights
+            uint4 hi0[SUBS], lo0[SUBS];
+#pragma unroll
+            for (int sub = 0; sub < SUBS; ++sub)
+                if (sub < subs) load_tokens(0, sub, hi0[sub], lo0[sub]);
 
-    auto compute = [&](const uint4 (&r)[RG], const uint32_t (&rs)[RG]) {
-        const size_t k0 = (size_t)c_s * STEP_K;
-        const bool in = WF != FEW_FP4 || (int)k0 + q * LANE_K < (c_up ? p.H : p.I);
-        float scale[RG];
-        if constexpr (WF == FEW_FP4) {
+            copy_wait<S::D - 2>();
+            __syncwarp();
+            const uint32_t from = ring + c_slot * S::SLOT;
+            if (++c_slot == S::D) c_slot = 0;
+
+            uint4 raw[RG];
+            if constexpr (WF != FEW_FP4) {
 #pragma unroll
-            for (int i = 0; i < RG; ++i) scale[i] = fp4_scale_value((rs[i] >> (8 * q)) & 255u);
-        }
-        float part[TILES][NT][4];                       // fp8: the sums of this step, to be scaled
-        if constexpr (WF == FEW_FP8) {
+                for (int r = 0; r < RG; ++r) raw[r] = ptx::ld_shared_v4(from + r * 512 + lane * 16);
+            }
+            uint32_t scale[RG];
+            if constexpr (WF == FEW_FP4) {
 #pragma unroll
-            for (int t = 0; t < TILES; ++t)
+                for (int r = 0; r < RG; ++r) scale[r] = ld_shared(from + RG * 512 + (g * RG + r) * 4);
+            } else if constexpr (WF == FEW_FP8) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int r = 0; r < RG; ++r) scale[r] = ld_shared(from + RG * 512 + r * 4);
+            }
+            float part[TILES][NT][4];                   // quantised weights: sums that still need their scale
+            if constexpr (WF == FEW_FP8) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) part[t][nt][i] = 0.0f;
-        }
+                for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int sub = 0; sub < SUBS; ++sub) {
-            uint32_t a[RG][4];
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < RG; ++i) widen<WF>(r[i], sub, WF == FEW_FP4 ? scale[i] : 1.0f, a[i]);
+                        for (int i = 0; i < 4; ++i) part[t][nt][i] = 0.0f;
+            }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                if (nt * 8 >= c_m) break;
-                for (int pl = 0; pl < planes; ++pl) {
-                    const uint4 b = in ? load_act(rows_at[nt] + pl * plane + k0 + sub * 8) : make_uint4(0, 0, 0, 0);
+            for (int sub = 0; sub < SUBS; ++sub) {
+                if (sub >= subs) break;
+                uint32_t a[RG][4];
+#pragma unroll
+                for (int r = 0; r < RG; ++r) {
+                    if constexpr (WF == FEW_FP4) {
+                        const uint32_t w = ld_shared(from + r * 512 + (sub * 8 + g) * 16 + q * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) a[r][i] = half_bits(fp4_unpack2((w >> (8 * i)) & 255u));
+                    } else if constexpr (WF == FEW_FP8) {
+                        const uint32_t w[2] = {sub == 0 ? raw[r].x : raw[r].z, sub == 0 ? raw[r].y : raw[r].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu), __NV_E4M3);
+                            a[r][i] = half_bits(*reinterpret_cast<const __half2*>(&hr));
+                        }
+                    } else {
+                        a[r][0] = raw[r].x; a[r][1] = raw[r].y; a[r][2] = raw[r].z; a[r][3] = raw[r].w;
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    if (nt * 8 >= m) break;
+                    uint4 hi, lo;
+                    if (nt == 0) { hi = hi0[sub]; lo = lo0[sub]; }
+                    else load_tokens(nt, sub, hi, lo);
+                    convert_tokens(nt, hi, lo);
 #pragma unroll
                     for (int t = 0; t < TILES; ++t) {
-                        float (&c)[4] = WF == FEW_FP8 ? part[t][nt] : acc[t][nt];
-                        mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], b.x, b.y);
-                        mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], b.z, b.w);
+                        float fresh[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        float (&c)[4] = WF == FEW_FP4 ? fresh : (WF == FEW_FP8 ? part[t][nt] : acc[t][nt]);
+                        mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], hi.x, hi.y);
+                        mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], hi.z, hi.w);
+                        if (!F16 && !item.up) {
+                            mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], lo.x, lo.y);
+                            mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], lo.z, lo.w);
+                        }
+                        if constexpr (WF == FEW_FP4) {
+                            // scale byte `sub` as the exponent of an fp32 number: 0 (2^-127) counts as zero, 255 (NaN) as
+                            // infinity
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t sw = scale[2 * t + (i >> 1)];
+                                const uint32_t f = (sub < 3 ? sw << (23 - 8 * sub) : sw >> 1) & 0x7F800000u;
+                                acc[t][nt][i] = fmaf(fresh[i], __uint_as_float(f), acc[t][nt][i]);
+                            }
+                        }
                     }
                 }
             }
+            if constexpr (WF == FEW_FP8) {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            acc[t][nt][i] = fmaf(part[t][nt][i], __uint_as_float(scale[2 * t + (i >> 1)]), acc[t][nt][i]);
+            }
+            __syncwarp();                               // every lane has read the slot that the next issue may refill
+            issue();
         }
-        if constexpr (WF == FEW_FP8) {
-#pragma unroll
-            for (int t = 0; t < TILES; ++t)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[t][nt][i] = fmaf(part[t][nt][i], __uint_as_float(rs[2 * t + (i >> 1)]), acc[t][nt][i]);
-        }
-    };
-
-    // Sum over the W warps, epilogue, bookkeeping.
-    auto finish_item = [&]() {
-        float* buf = red + parity * W * RED;
-        parity ^= 1;
+        // ---- leave the sums to the helper
+        const int b = nth % S::BUFS;
+        if (nth >= S::BUFS &&
+            !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_free + 8 * b, (nth / S::BUFS - 1) & 1, &s.abort, p.dev_status)))
+            break;
+        float* buf = red + (b * FEW_W + wk) * RED;
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-                if (nt * 8 < c_m)
+                if (nt * 8 < m)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) buf[wk * RED + ((t * NT + nt) * 4 + i) * 32 + lane] = acc[t][nt][i];
-        ptx::named_barrier_sync(1 + grp, 32 * W);
-        auto total = [&](int t, int half, int row8, int tok) {
-            const int at = ((t * NT + (tok >> 3)) * 4 + half * 2 + (tok & 1)) * 32 + row8 * 4 + ((tok & 7) >> 1);
-            float v = 0.0f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) v += buf[w * RED + at];
-            return v;
-        };
-        auto bias_at = [&](const void* b, size_t i) {
-            if (!b) return 0.0f;
-            return p.f16 ? __half2float(static_cast<const __half*>(b)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(b)[i]);
-        };
-        const int e = s.active[c_a], base = s.base[e];
-        if (c_up) {
-            const int rows = gated ? 8 * TILES : 16 * TILES;
-            for (int i = tid; i < rows * c_m; i += 32 * W) {
-                const int tok = i / rows, j = i - tok * rows;
-                float v;
-                int row;
-                if (gated) {
-                    row = c_row + 32 * (j >> 3) + (j & 7);
-                    const float gate = total(j >> 3, 0, j & 7, tok) + bias_at(p.b1, (size_t)e * p.I + row);
-                    const float lin = total(j >> 3, 1, j & 7, tok) + bias_at(p.b3, (size_t)e * p.I + row);
-                    v = act_silu(gate) * lin;
-                } else {
-                    row = c_row + 8 * (j >> 4) + 32 * ((j >> 3) & 1) + (j & 7);
-                    v = total(j >> 4, (j >> 3) & 1, j & 7, tok) + bias_at(p.b1, (size_t)e * p.I + row);
-                    v = p.act == ARISTOS_ACT_RELU ? act_relu(v) : act_gelu(v);
-                }
-                const size_t at = (size_t)(base + tok) * p.I + row;
-                if constexpr (F16) {
-                    __half* h = static_cast<__half*>(p.h);
-                    const __half hi = __float2half_rn(v);
-                    h[at] = hi;
-                    const float rest = v - __half2float(hi);
-                    h[(size_t)slots * p.I + at] = __float2half_rn(isinf(__half2float(hi)) ? 0.0f : rest);
-                } else {
-                    __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p.h);
-                    const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-                    h[at] = hi;
-                    const float rest = v - __bfloat162float(hi);
-                    h[(size_t)slots * p.I + at] = __float2bfloat16_rn(isinf(__bfloat162float(hi)) ? 0.0f : rest);
-                }
-            }
-            ptx::named_barrier_sync(1 + grp, 32 * W);
-            if (tid == 0) {
-                __threadfence();
-                atomicAdd(p.done + c_a, 1);
-            }
-        } else {
-            constexpr int rows = 16 * TILES;
-            for (int i = tid; i < rows * c_m; i += 32 * W) {
-                const int tok = i / rows, j = i - tok * rows;
-                const int row = c_row + 8 * (j >> 4) + 32 * ((j >> 3) & 1) + (j & 7);
-                p.partial[(size_t)(base + tok) * p.H + row] =
-                    total(j >> 4, (j >> 3) & 1, j & 7, tok) + bias_at(p.b2, (size_t)e * p.H + row);
-            }
-            ptx::named_barrier_sync(1 + grp, 32 * W);
-            if (tid == 0) {
-                __threadfence();
-                const int rb = (c_it - up_items) % down_blocks;
-                s.last[grp] = atomicAdd(p.ticket + rb, 1) == actives - 1;
-                __threadfence();
-            }
-            ptx::named_barrier_sync(1 + grp, 32 * W);
-            if (s.last[grp]) {
-                // every chosen expert has delivered these rows: the weighted sum of each token, in the order of j
-                for (int i = tid; i < rows * p.n; i += 32 * W) {
-                    const int tok = i / rows, j = i - tok * rows;
-                    const int row = c_row + 8 * (j >> 4) + 32 * ((j >> 3) & 1) + (j & 7);
-                    float v = 0.0f;
-                    for (int c = 0; c < p.k; ++c)
-                        v = fmaf(s.w[tok * p.k + c], __ldcg(p.partial + (size_t)s.slot[tok * p.k + c] * p.H + row), v);
-                    const size_t at = (size_t)tok * p.H + row;
-                    if (p.f16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
-                    else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-                }
-            }
-        }
-    };
-
-    if (first >= items) return;
-    next_load_item();
-#pragma unroll
-    for (int d = 0; d < D; ++d) issue(ring[d], ring_scale[d]);
-    // the next item; items of which this warp has no step are finished at once
-    auto settle = [&]() {
-        while (c_it < items) {
-            start_item();
-            if (wk < c_steps) return;
-            finish_item();
-            c_it += stride;
-        }
-    };
-    settle();
-    while (c_it < items) {
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-            if (c_it < items) {
-                compute(ring[d], ring_scale[d]);
-                issue(ring[d], ring_scale[d]);
-                c_s += W;
-                if (c_s >= c_steps) {
-                    finish_item();
-                    c_it += stride;
-                    settle();
-                }
-            }
-        }
+                    for (int i = 0; i < 4; ++i) buf[((t * NT + nt) * 4 + i) * 32 + lane] = acc[t][nt][i];
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar_full + 8 * b);
     }
+    copy_wait<0>();
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
+// Parts of K of the down projection: so many that its items are about as long as those of the up projection. A group's
+// share of a small call is only a few items, and the call ends with the longest of them.
+int few_parts(int H, int I) {
+    const int parts = (I + H / 2) / H;
+    return parts < 1 ? 1 : (parts > 8 ? 8 : parts);
+}
+
 struct FewPlan {
-    size_t logits, counters, x_planes, h, partial, total;
+    size_t logits, counters, x_norm, x_scale, h, partial, total;
     int ncounters;
 };
 FewPlan few_plan(int n, int H, int I, int E, int k) {
@@ -632,28 +779,27 @@ FewPlan few_plan(int n, int H, int I, int E, int k) {
     auto take = [&](size_t bytes) { const size_t here = at; at = align_up(at + bytes, 256); return here; };
     const size_t slots = (size_t)n * k;
     f.logits = take((size_t)n * E * 4);
-    f.ncounters = FEW_MAX_EXPERTS + H / 16;
+    f.ncounters = FEW_MAX_EXPERTS + FEW_MAX_SLOTS + H / 16;
     f.counters = take((size_t)f.ncounters * 4);
-    f.x_planes = take((size_t)n * H * 4);
+    f.x_norm = take((size_t)n * H * 2);
+    f.x_scale = take((size_t)n * 4);
     f.h = take(slots * I * 4);
-    f.partial = take(slots * H * 4);
+    f.partial = take(slots * H * 4 * few_parts(H, I));
     f.total = at;
     return f;
 }
 
-template <int WF, int NT>
+template <int WF, int NT, class S>
 aristos_status_t launch_few(const FewParams& p, cudaStream_t st) {
-    constexpr int RG = 2, W = 8, D = NT <= 2 ? 6 : (NT == 4 ? 4 : 3);
-    constexpr int RED = RG / 2 * NT * 128;
-    constexpr size_t smem = (size_t)2 * (FEW_THREADS / 32) * RED * sizeof(float);
-    auto kernel = few_ffn_kernel<WF, NT, RG, W, D>;
-    ARISTOS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    auto kernel = few_ffn_kernel<WF, NT, S>;
+    static_assert(S::SMEM + sizeof(FewLists) <= 227 * 1024, "few tokens: shared memory");
+    ARISTOS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
     const int sms = device_sm_count();
     if (sms <= 0) { set_last_error("no CUDA device"); return ARISTOS_ERR_CUDA; }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(sms);
     cfg.blockDim = dim3(FEW_THREADS);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
     // Cooperative: all CTAs are resident together, so that two calls on two streams cannot each hold a part of the SMs
     // while their down projections wait for up items of CTAs that found no place. Programmatic serialisation: the CTAs
@@ -672,10 +818,10 @@ aristos_status_t launch_few(const FewParams& p, cudaStream_t st) {
 
 template <int WF>
 aristos_status_t launch_few_tokens(const FewParams& p, cudaStream_t st) {
-    if (p.n <= 8) return launch_few<WF, 1>(p, st);
-    if (p.n <= 16) return launch_few<WF, 2>(p, st);
-    if (p.n <= 32) return launch_few<WF, 4>(p, st);
-    return launch_few<WF, 8>(p, st);
+    if (p.n <= 8) return launch_few<WF, 1, FewShape<WF, 1, 4, 5, 2>>(p, st);
+    if (p.n <= 16) return launch_few<WF, 2, FewShape<WF, 2, 4, 4, 2>>(p, st);
+    if (p.n <= 32) return launch_few<WF, 4, FewShape<WF, 4, 4, 4, 1>>(p, st);
+    return launch_few<WF, 8, FewShape<WF, 8, 2, 6, 1>>(p, st);
 }
 
 aristos_status_t few_check(int tokens, int H, int I, int E, int k, int weights_dtype) {
@@ -694,7 +840,7 @@ aristos_status_t few_check(int tokens, int H, int I, int E, int k, int weights_d
         return ARISTOS_ERR_CONFIG;
     }
     // items are numbered in 31 bits
-    if ((int64_t)E * ((int64_t)H + I) / 8 >= (int64_t)1 << 30) { set_last_error("moe_few_tokens: too many weight rows"); return ARISTOS_ERR_CONFIG; }
+    if ((int64_t)E * ((int64_t)H * few_parts(H, I) + I) / 8 >= (int64_t)1 << 30) { set_last_error("moe_few_tokens: too many weight rows"); return ARISTOS_ERR_CONFIG; }
     return ARISTOS_OK;
 }
 
@@ -742,39 +888,45 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
     }
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool f16 = dtype == ARISTOS_DTYPE_F16, split = f16 && fp4;     // fp16 tokens as two bf16 planes
+    const bool f16 = dtype == ARISTOS_DTYPE_F16;
+    const bool norm = !f16 && (fp8 || fp4);                 // bf16 tokens meet quantised weights as scaled fp16 numbers
     FewParams p{};
     p.logits = reinterpret_cast<float*>(ws + f.logits);
-    p.x = split ? static_cast<const void*>(ws + f.x_planes) : x;
-    p.x_planes = split ? 2 : 1;
+    p.x = static_cast<const uint16_t*>(norm ? static_cast<const void*>(ws + f.x_norm) : x);
+    p.x_scale = norm ? reinterpret_cast<const float*>(ws + f.x_scale) : nullptr;
     p.w1 = static_cast<const uint8_t*>(w1);
     p.w3 = static_cast<const uint8_t*>(gated ? w3 : nullptr);
     p.w2 = static_cast<const uint8_t*>(w2);
-    p.s1 = s1; p.s3 = s3; p.s2 = s2;
+    p.s1 = static_cast<const uint8_t*>(s1);
+    p.s3 = static_cast<const uint8_t*>(s3);
+    p.s2 = static_cast<const uint8_t*>(s2);
     p.b1 = b1; p.b3 = gated ? b3 : nullptr; p.b2 = b2;
-    p.h = ws + f.h;
+    p.h = reinterpret_cast<float*>(ws + f.h);
     p.partial = reinterpret_cast<float*>(ws + f.partial);
     p.done = reinterpret_cast<int32_t*>(ws + f.counters);
-    p.ticket = p.done + FEW_MAX_EXPERTS;
+    p.h_max = reinterpret_cast<uint32_t*>(p.done + FEW_MAX_EXPERTS);
+    p.ticket = p.done + FEW_MAX_EXPERTS + FEW_MAX_SLOTS;
     p.out = out;
     p.topk_idx = topk_idx;
     p.topk_w = topk_w;
     p.dev_status = dev_status;
     p.n = tokens; p.H = H; p.I = I; p.E = E; p.k = k;
     p.gate_fn = gate_fn; p.renorm = renorm; p.act = hidden_act;
+    p.parts = few_parts(H, I);
     p.f16 = f16 ? 1 : 0;
 
-    const int gate_warps = E * ceil_div(tokens, FEW_GATE_TOK);
-    int gate_grid = ceil_div(gate_warps, FEW_GATE_WARPS);
+    const int gate_warps = E * ceil_div(tokens, FEW_GATE_TOK) + (norm ? tokens : 0);
+    const int gate_grid = ceil_div(gate_warps, FEW_GATE_WARPS);
+    __half* x_norm = norm ? reinterpret_cast<__half*>(ws + f.x_norm) : nullptr;
+    float* x_scale = norm ? reinterpret_cast<float*>(ws + f.x_scale) : nullptr;
     if (f16)
         few_gate_kernel<__half><<<gate_grid, FEW_GATE_WARPS * 32, 0, st>>>(
             static_cast<const __half*>(x), static_cast<const __half*>(w_gate), gate_bias, tokens, H, E,
-            const_cast<float*>(p.logits), p.done, f.ncounters,
-            split ? reinterpret_cast<__nv_bfloat16*>(ws + f.x_planes) : nullptr);
+            const_cast<float*>(p.logits), p.done, f.ncounters, x_norm, x_scale);
     else
         few_gate_kernel<__nv_bfloat16><<<gate_grid, FEW_GATE_WARPS * 32, 0, st>>>(
             static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(w_gate), gate_bias, tokens, H, E,
-            const_cast<float*>(p.logits), p.done, f.ncounters, nullptr);
+            const_cast<float*>(p.logits), p.done, f.ncounters, x_norm, x_scale);
     ARISTOS_COUNT_LAUNCH();
     ARISTOS_CUDA_TRY(cudaGetLastError());
     if (fp4) return launch_few_tokens<FEW_FP4>(p, st);

@@ -103,7 +103,9 @@ def ffn_fp4(x, w1, w3, w2, act):
 
 def moe_few(x, idx, w, mats, biases, act, h_step):
     """out (n, H) and its bound for given routing; mats: {"1", "3", "2"} -> (E, ...) float64 (or a function of e);
-    biases the same or None; h_step: relative step of the stored hidden activations (value and remainder)."""
+    biases the same or None; h_step: relative error of the hidden activations as an operand of the down projection.
+    Operands may be scaled fp16 numbers (largest magnitude in [2^14, 2^15), smallest step 2^-24): what is far below the
+    largest of its row is off by at most 2^-38 of that."""
     n, k = idx.shape
     y = torch.zeros(x.shape, dtype=torch.float64, device=x.device)
     d = torch.zeros_like(y)
@@ -114,14 +116,15 @@ def moe_few(x, idx, w, mats, biases, act, h_step):
         rows = x[who].double()
         w1, w2 = get("1", e), get("2", e)
         g, dg = rows @ w1.T + bias("1", e), dot_bound(rows, w1.T)
-        dg = dg + 2.0 ** -23 * g.abs()
+        far = 2.0 ** -38 * rows.abs().amax(1, keepdim=True)
+        dg = dg + 2.0 ** -23 * g.abs() + far * w1.abs().sum(1)
         u = du = None
         if act == 2:
             w3 = get("3", e)
             u, du = rows @ w3.T + bias("3", e), dot_bound(rows, w3.T)
-            du = du + 2.0 ** -23 * u.abs()
+            du = du + 2.0 ** -23 * u.abs() + far * w3.abs().sum(1)
         h = act64(g, u, act)
-        dh = act_bound(g, u, dg, du, act) + h_step * h.abs() + 2.0 ** -25
+        dh = act_bound(g, u, dg, du, act) + h_step * h.abs() + 2.0 ** -38 * h.abs().amax(1, keepdim=True)
         out = h @ w2.T + bias("2", e)
         do = dh @ w2.T.abs() + dot_bound(h, w2.T) + 2.0 ** -23 * out.abs()
         p = w[who, j].double()[:, None]

@@ -55,8 +55,9 @@ class Case:
         want_idx, want_w = self.layer.gate_topk(x, self.wg, self.k, gate_bias=self.gate_bias, **self.kw)
         assert torch.equal(idx, want_idx), "the routing is the gate's"
         assert torch.equal(w, want_w), "the combine weights are the gate's, bit for bit"
-        # value and remainder of a 16-bit type: two half steps
-        ref, bound = R.moe_few(x, idx, w, self.mats, self.b, self.act, R.half_step(self.dt) ** 2)
+        # bf16 weights: h as value and remainder, two half steps of bf16; else one rounding to fp16
+        h_step = 2.0 ** -18 if self.weights == "16" and self.dt == torch.bfloat16 else 2.0 ** -12
+        ref, bound = R.moe_few(x, idx, w, self.mats, self.b, self.act, h_step)
         R.assert_within(out, ref, bound + R.half_step(self.dt) * (ref.abs() + bound) * 1.01 + 2.0 ** -25)
 
 
