@@ -11,16 +11,18 @@
 //  * few_ffn_kernel: one CTA per SM, launched while the gate still runs. Every CTA does the (small) top-k and the
 //    expert lists for itself, so no further kernel or grid barrier is needed. The work is a list of items (chosen expert,
 //    8 * RG weight rows, part of K): all of the up projection, then all of the down projection, dealt out in turn to
-//    groups of W warps. The warps of a group cut K among themselves (64-byte pieces in turn, so together they read a
-//    row's bytes in order) and leave their sums in shared memory; a helper warp per group adds them in a fixed order and
-//    does the epilogue, the stores and the bookkeeping, so that the streaming warps never wait for any of it.
-//  * Weights travel by cp.async into a ring that every lane has for itself, D steps ahead of the arithmetic and across
-//    item boundaries, from the up into the down projection: the stream does not stop for reductions or for the wait below.
+//    groups of W warps. The warps of a group cut K among themselves (128-byte pieces of all rows in turn, so together they
+//    read a row's bytes in order) and leave their sums in shared memory; a helper warp per group adds them in a fixed
+//    order and does the epilogue, the stores and the bookkeeping, so that the streaming warps never wait for any of it.
+//  * Weights travel by TMA into a ring that every warp has for itself, up to D steps (4 KB each) ahead of the arithmetic
+//    and across item boundaries, from the up into the down projection: the stream does not stop for reductions or for the
+//    wait below. (Through cp.async or plain loads the tokens' loads queue behind the weights' in the L1 and every step
+//    takes as long as a DRAM access: 190 us for what takes 125 us this way.)
 //  * An item of the down projection waits until all of its expert's up items are done (a counter per expert; the wait is
 //    bounded). Up items never wait and come first in every group's list, so the wait ends.
 //  * The products run on the warp-level matrix instruction m16n8k16: 16 weight rows (gate and up rows of the same
 //    columns for SwiGLU) x 8 tokens x 16 of K. The order of K inside a step does not matter to the sum, so a lane uses
-//    the bytes as they lie and the tokens are read in the same order. The 5th-generation tensor cores would need 128
+//    whole 16-byte pieces of a row (4-bit: 4 bytes of each block) and reads the tokens in the same order. The 5th-generation tensor cores would need 128
 //    weight rows per instruction and both operands in shared memory, for a rate that this stream cannot use.
 //  * Expert outputs are summed per block of rows by the helper that finishes the block last, in the order of j.
 //
@@ -37,13 +39,14 @@
 #include "fp4_format.cuh"
 #include "gate_contract.cuh"
 #include "ptx_sm100.cuh"
+#include "tensor_map.cuh"
 
 namespace aristos {
 
 namespace {
 
 constexpr int FEW_MAX_TOKENS = ARISTOS_FEW_TOKENS_MAX;
-constexpr int FEW_MAX_EXPERTS = 1024;
+constexpr int FEW_MAX_EXPERTS = 512;
 constexpr int FEW_MAX_SLOTS = FEW_MAX_TOKENS * MAX_TOPK;
 static_assert(FEW_MAX_TOKENS <= 64, "the expert lists keep the tokens of an expert in 64 bits");
 
@@ -53,13 +56,14 @@ constexpr int FEW_STREAM_WARPS = FEW_W * FEW_GROUPS;
 constexpr int FEW_WARPS = FEW_STREAM_WARPS + FEW_GROUPS;  // and a helper per group
 constexpr int FEW_THREADS = 32 * FEW_WARPS;
 
+constexpr int FEW_MAX_DEPTH = 6;
+
 enum { FEW_BF16 = 0, FEW_F16 = 1, FEW_FP8 = 2, FEW_FP4 = 3 };      // weight formats
 
 struct FewParams {
     const float* logits;
     const uint16_t* x;             // (n, H) in the operand type
     const float* x_scale;          // (n) what the sums of a token are multiplied with, or NULL: 1
-    const uint8_t *w1, *w3, *w2;
     const uint8_t *s1, *s3, *s2;   // fp8: fp32 per 128 x 128; fp4: scale tiles
     const void *b1, *b3, *b2;      // activations' dtype, or NULL
     float* h;                      // (slots, I)
@@ -159,6 +163,7 @@ few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* 
 // ---- the experts ---------------------------------------------------------------------------------------------------------
 struct FewLists {
     uint64_t bars[FEW_GROUPS * 4];             // per group: sums written (2 buffers), buffer free (2)
+    uint64_t full[FEW_STREAM_WARPS * FEW_MAX_DEPTH];   // per streaming warp: step arrived
     float w[FEW_MAX_SLOTS];                    // combine weights (t, j)
     uint32_t mask[FEW_MAX_EXPERTS][2];         // tokens that chose an expert
     uint16_t idx[FEW_MAX_SLOTS];               // chosen experts (t, j)
@@ -170,26 +175,22 @@ struct FewLists {
     int abort;
 };
 
-// Top-k of one token by one warp: the selection and the weights of the gate kernels, bit for bit (gate.cu).
+// Top-k of one token by one warp: the selection and the weights of the gate kernels, bit for bit (gate.cu). PER logits
+// per lane; lane j ends up with the choice number j. Kept small: every CTA runs it once, out of a cold instruction cache.
+template <int PER>
 __device__ __forceinline__ void few_topk(const float* __restrict__ l, const FewParams& p, int t, int lane, FewLists& s) {
-    constexpr int PER_LANE = FEW_MAX_EXPERTS / 32;
-    float v[PER_LANE];
+    float v[PER];
 #pragma unroll
-    for (int i = 0; i < PER_LANE; ++i)
-        if (i * 32 < p.E) v[i] = i * 32 + lane < p.E ? __ldcg(l + i * 32 + lane) : 0.0f;
+    for (int i = 0; i < PER; ++i) v[i] = i * 32 + lane < p.E ? __ldcg(l + i * 32 + lane) : 0.0f;
     uint32_t taken = 0;
-    float chosen_l[MAX_TOPK], w_sel[MAX_TOPK];
-#pragma unroll
-    for (int j = 0; j < MAX_TOPK; ++j) {
-        if (j >= p.k) break;
+    float my_l = 0.0f;
+#pragma unroll 1
+    for (int j = 0; j < p.k; ++j) {
         float bv = 0.0f;
         int bi = -1;
 #pragma unroll
-        for (int i = 0; i < PER_LANE; ++i)
-            if (i * 32 < p.E) {
-                const int e = i * 32 + lane;
-                if (e < p.E && !(taken >> i & 1) && (bi < 0 || v[i] > bv)) { bv = v[i]; bi = e; }
-            }
+        for (int i = 0; i < PER; ++i)
+            if (i * 32 + lane < p.E && !(taken >> i & 1) && (bi < 0 || v[i] > bv)) { bv = v[i]; bi = i * 32 + lane; }
 #pragma unroll
         for (int m = 16; m >= 1; m >>= 1) {
             const float ov = __shfl_xor_sync(0xffffffffu, bv, m);
@@ -201,48 +202,43 @@ __device__ __forceinline__ void few_topk(const float* __restrict__ l, const FewP
         bi = __shfl_sync(0xffffffffu, bi, 0);
         bv = __shfl_sync(0xffffffffu, bv, 0);
         if ((bi & 31) == lane) taken |= 1u << (bi >> 5);
-        chosen_l[j] = bv;
-        if (lane == 0) s.idx[t * p.k + j] = (uint16_t)bi;
+        if (lane == j) {
+            my_l = bv;
+            s.idx[t * p.k + j] = (uint16_t)bi;
+        }
     }
+    float w;
     if (p.gate_fn == ARISTOS_GATE_SOFTMAX) {
-        const float mx = chosen_l[0];
+        const float mx = __shfl_sync(0xffffffffu, my_l, 0);
         float den = 0.0f;
 #pragma unroll
-        for (int i = 0; i < PER_LANE; ++i)
-            if (i * 32 < p.E && i * 32 + lane < p.E) den += expf(v[i] - mx);
+        for (int i = 0; i < PER; ++i)
+            if (i * 32 + lane < p.E) den += expf(v[i] - mx);
 #pragma unroll
         for (int m = 16; m >= 1; m >>= 1) den += __shfl_xor_sync(0xffffffffu, den, m);
-#pragma unroll
-        for (int j = 0; j < MAX_TOPK; ++j)
-            if (j < p.k) w_sel[j] = expf(chosen_l[j] - mx) / den;
+        w = expf(my_l - mx) / den;
     } else {
-#pragma unroll
-        for (int j = 0; j < MAX_TOPK; ++j)
-            if (j < p.k) w_sel[j] = 1.0f / (1.0f + expf(-chosen_l[j]));
+        w = 1.0f / (1.0f + expf(-my_l));
     }
     if (p.renorm) {
         float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < MAX_TOPK; ++j)
-            if (j < p.k) sum += w_sel[j];
-#pragma unroll
-        for (int j = 0; j < MAX_TOPK; ++j)
-            if (j < p.k) w_sel[j] = w_sel[j] / sum;
+#pragma unroll 1
+        for (int j = 0; j < p.k; ++j) sum += __shfl_sync(0xffffffffu, w, j);
+        w = w / sum;
     }
-#pragma unroll
-    for (int j = 0; j < MAX_TOPK; ++j)
-        if (j < p.k && lane == j) s.w[t * p.k + j] = w_sel[j];
+    if (lane < p.k) s.w[t * p.k + lane] = w;
 }
 
-
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void copy_async4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint2 ld_shared2(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
     uint32_t v;
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -254,6 +250,14 @@ __device__ __forceinline__ uint4 load_act(const void* ptr) {
     uint4 v;
     asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
     return v;
+}
+
+// Counts an item whose results this warp has written. Only a release: a full fence would also empty the L1 cache, from
+// which the streaming warps read the tokens again for every item.
+__device__ __forceinline__ int add_release(int32_t* counter) {
+    int old;
+    asm volatile("atom.add.release.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+    return old;
 }
 
 template <bool F16>
@@ -277,33 +281,63 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
 }
 __device__ __forceinline__ uint32_t half_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
-template <int WF> struct FewFormat;
-template <> struct FewFormat<FEW_BF16> { static constexpr int SUBS = 1; };
-template <> struct FewFormat<FEW_F16> { static constexpr int SUBS = 1; };
-template <> struct FewFormat<FEW_FP8> { static constexpr int SUBS = 2; };
-template <> struct FewFormat<FEW_FP4> { static constexpr int SUBS = 4; };
+// The eight e2m1 codes of a word as fp16 pairs, adjacent codes together. All eight magnitudes have an empty low byte in
+// fp16, so the high bytes of four codes come out of one byte permutation (the codes select from the table), their signs
+// out of another (which spreads the top bits of bytes), and two more put zero bytes between them: 13 instructions, where
+// four conversions took 24.
+__device__ __forceinline__ void unpack_e2m1(uint32_t w, uint32_t (&v)[4]) {
+    const uint32_t mag = w & 0x77777777u, up = w << 4;
+    // high bytes of 0, 0.5, 1, 1.5 | 2, 3, 4, 6
+    const uint32_t lo = __byte_perm(0x3E3C3800u, 0x46444240u, mag), hi = __byte_perm(0x3E3C3800u, 0x46444240u, mag >> 16);
+    uint32_t sl, sh;                                    // byte i: the sign of code i (of code 4 + i) in every bit
+    asm("prmt.b32 %0, %1, %2, 0x9D8C;" : "=r"(sl) : "r"(w), "r"(up));
+    asm("prmt.b32 %0, %1, %2, 0xBFAE;" : "=r"(sh) : "r"(w), "r"(up));
+    const uint32_t a = lo | (sl & 0x80808080u), b = hi | (sh & 0x80808080u);
+    v[0] = __byte_perm(a, 0, 0x1404);
+    v[1] = __byte_perm(a, 0, 0x3424);
+    v[2] = __byte_perm(b, 0, 0x1404);
+    v[3] = __byte_perm(b, 0, 0x3424);
+}
 
-// NT: token tiles of 8 (at least ceil(n / 8)); RG: groups of 8 weight rows per item; D: steps in flight; BUFS: buffers for
+// Four e4m3 codes as fp16 pairs (exact).
+__device__ __forceinline__ void unpack_e4m3(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    lo = half_bits(*reinterpret_cast<const __half2*>(&a));
+    hi = half_bits(*reinterpret_cast<const __half2*>(&b));
+}
+
+template <int WF> struct FewFormat;                    // elements per byte of weights, doubled
+template <> struct FewFormat<FEW_BF16> { static constexpr int PACK = 1; };
+template <> struct FewFormat<FEW_F16> { static constexpr int PACK = 1; };
+template <> struct FewFormat<FEW_FP8> { static constexpr int PACK = 2; };
+template <> struct FewFormat<FEW_FP4> { static constexpr int PACK = 4; };
+
+// NT: token tiles of 8 (at least ceil(n / 8)); RG: groups of 8 weight rows per item; D: steps in the ring; BUFS: buffers for
 // the sums of an item.
 template <int WF, int NT, int RG_, int D_, int BUFS_>
 struct FewShape {
     static constexpr int RG = RG_, D = D_, BUFS = BUFS_;
-    static constexpr int SUBS = FewFormat<WF>::SUBS;
-    static constexpr int STEP_K = 32 * SUBS;            // elements of K per step: 64 bytes of a row
+    static constexpr int STEP_K = 64 * FewFormat<WF>::PACK;     // elements of K per step: 128 bytes of a row
     static constexpr int TILES = RG / 2;                // m16 tiles: row groups (2 t, 2 t + 1)
-    static constexpr int SCALE_BYTES = WF == FEW_FP4 ? 32 * RG : (WF == FEW_FP8 ? 16 : 0);
-    static constexpr int SLOT = RG * 512 + SCALE_BYTES;
+    static constexpr int SLOT = RG * 1024;              // 8 rows x 128 bytes per row group
+    static constexpr int SCALES = WF == FEW_FP4 ? 2 * 32 * RG : (WF == FEW_FP8 ? 16 : 0);   // bytes of scales per step
     static constexpr int RED = TILES * NT * 128;        // floats per warp of one buffer
-    static constexpr size_t SMEM = (size_t)FEW_STREAM_WARPS * (D * SLOT + BUFS * RED * 4);
-    static_assert(RG == 2 || RG == 4, "a lane of a quad copies the scale word of one row group");
+    static constexpr size_t SMEM = 1024 + (size_t)FEW_STREAM_WARPS * (D * (SLOT + SCALES) + BUFS * RED * 4);
+    static_assert(RG == 2 || RG == 4, "a lane of a quad copies the scale words of one row group");
+    static_assert(D <= FEW_MAX_DEPTH && D >= 2, "ring depth");
 };
 
+template <int N> struct Tiles { static constexpr int value = N; };
+
 template <int WF, int NT, class S>
-__global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constant__ CUtensorMap tm3,
+                                                                 const __grid_constant__ CUtensorMap tm2, const __grid_constant__ FewParams p) {
     constexpr bool F16 = WF != FEW_BF16;                // operand type
-    constexpr int RG = S::RG, TILES = S::TILES, SUBS = S::SUBS, STEP_K = S::STEP_K, RED = S::RED;
+    constexpr int RG = S::RG, TILES = S::TILES, STEP_K = S::STEP_K, RED = S::RED;
     __shared__ FewLists s;
-    extern __shared__ __align__(16) uint8_t few_smem[];
+    extern __shared__ uint8_t few_smem_raw[];
+    uint8_t* few_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(few_smem_raw) + 1023) & ~uintptr_t(1023));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool gated = p.act == ARISTOS_ACT_SWIGLU;
@@ -311,13 +345,22 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     for (int i = threadIdx.x; i < 2 * p.E; i += FEW_THREADS) s.mask[i >> 1][i & 1] = 0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < FEW_GROUPS * 4; ++i) ptx::mbar_init(ptx::smem_u32(&s.bars[i]), (i & 2) ? 1 : FEW_W);
+        for (int i = 0; i < FEW_STREAM_WARPS * S::D; ++i) ptx::mbar_init(ptx::smem_u32(&s.full[i]), 1);
         s.abort = 0;
         ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&tm1);
+        if (gated) ptx::prefetch_tensormap(&tm3);
+        ptx::prefetch_tensormap(&tm2);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     // ---- routing and expert lists (every CTA for itself) ------------------------------------------------------------------
-    for (int t = warp; t < p.n; t += FEW_WARPS) few_topk(p.logits + (size_t)t * p.E, p, t, lane, s);
+    for (int t = warp; t < p.n; t += FEW_WARPS) {
+        const float* l = p.logits + (size_t)t * p.E;
+        if (p.E <= 32) few_topk<1>(l, p, t, lane, s);
+        else if (p.E <= 256) few_topk<8>(l, p, t, lane, s);
+        else few_topk<FEW_MAX_EXPERTS / 32>(l, p, t, lane, s);
+    }
     __syncthreads();
     const int slots = p.n * p.k;
     for (int i = threadIdx.x; i < slots; i += FEW_THREADS) {
@@ -365,47 +408,50 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     const int actives = s.actives;
     const int up_rows = gated ? 4 * RG : 8 * RG, down_rows = 8 * RG;
     const int up_blocks = p.I / up_rows, down_blocks = p.H / down_rows;
-    const int up_items = actives * up_blocks, items = up_items + actives * down_blocks * p.parts;
     const int up_steps = (p.H + STEP_K - 1) / STEP_K, down_steps = (p.I + STEP_K - 1) / STEP_K;
     const int part_steps = (down_steps + p.parts - 1) / p.parts;
     const int grp = warp < FEW_STREAM_WARPS ? warp / FEW_W : warp - FEW_STREAM_WARPS;
     const int stride = gridDim.x * FEW_GROUPS, first = blockIdx.x * FEW_GROUPS + grp;
 
+    // A position in the list. It advances by `stride` items without a division: the list is ordered by expert, then (down
+    // projection) by part of K, then by block of rows.
     struct Item {
         bool up;
-        int a, row, part;          // chosen expert, first weight row, part of K
-        int begin, end;            // steps
+        int a, part, block;        // chosen expert, part of K, block of rows
     };
-    auto item_at = [&](int it) {
-        Item i;
-        i.up = it < up_items;
+    auto forward = [&](Item& i, int by) {      // returns false past the end
+        i.block += by;
         if (i.up) {
-            i.a = it / up_blocks;
-            i.row = (it - i.a * up_blocks) * up_rows;
-            i.part = 0;
-            i.begin = 0;
-            i.end = up_steps;
-        } else {
-            const int local = it - up_items, per = down_blocks * p.parts;
-            i.a = local / per;
-            const int r = local - i.a * per;
-            const int rb = r / p.parts;
-            i.row = rb * down_rows;
-            i.part = r - rb * p.parts;
-            i.begin = i.part * part_steps;
-            i.end = min(i.begin + part_steps, down_steps);
+            while (i.block >= up_blocks) {
+                i.block -= up_blocks;
+                if (++i.a == actives) { i.up = false; i.a = 0; break; }
+            }
         }
-        return i;
+        if (!i.up) {
+            while (i.block >= down_blocks) {
+                i.block -= down_blocks;
+                if (++i.part == p.parts) {
+                    i.part = 0;
+                    if (++i.a == actives) return false;
+                }
+            }
+        }
+        return true;
     };
+    auto begin_of = [&](const Item& i) { return i.up ? 0 : i.part * part_steps; };
+    auto end_of = [&](const Item& i) { return i.up ? up_steps : min((i.part + 1) * part_steps, down_steps); };
+    // The warps of a group start at another step of every item: who has one step more than the others changes.
+    auto turn = [&](int wk, int nth) { return (wk + nth) % FEW_W; };
     auto tokens_of = [&](int e) { return __popc(s.mask[e][0]) + __popc(s.mask[e][1]); };
     const uint32_t bar_full = ptx::smem_u32(&s.bars[grp * 4]), bar_free = bar_full + 16;
-    float* red = reinterpret_cast<float*>(few_smem + FEW_STREAM_WARPS * S::D * S::SLOT) + grp * FEW_W * S::BUFS * RED;
+    float* red = reinterpret_cast<float*>(few_smem + FEW_STREAM_WARPS * S::D * (S::SLOT + S::SCALES)) + grp * FEW_W * S::BUFS * RED;
 
     if (warp >= FEW_STREAM_WARPS) {
         // ============================================================ helper: sums, epilogue, bookkeeping
         int nth = 0;
-        for (int it = first; it < items; it += stride, ++nth) {
-            const Item item = item_at(it);
+        Item item{true, 0, 0, 0};
+        for (bool more = forward(item, first); more; more = forward(item, stride), ++nth) {
+            const int row0 = item.block * (item.up ? up_rows : down_rows);
             const int e = s.active[item.a], base = s.base[e], m = tokens_of(e);
             const int b = nth % S::BUFS;
             const float* buf = red + b * FEW_W * RED;
@@ -434,7 +480,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                     if (tok < m) {
                         const int slot = base + tok;
                         const float f = p.x_scale ? __ldg(p.x_scale + s.token[slot]) : 1.0f;
-                        const size_t col = (size_t)e * p.I + item.row + j;
+                        const size_t col = (size_t)e * p.I + row0 + j;
                         float v;
                         if (gated) {
                             // row groups alternate between gate and up rows
@@ -446,7 +492,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                             v = total(j, tok) * f + bias_at(p.b1, col);
                             v = p.act == ARISTOS_ACT_RELU ? act_relu(v) : act_gelu(v);
                         }
-                        p.h[(size_t)slot * p.I + item.row + j] = v;
+                        p.h[(size_t)slot * p.I + row0 + j] = v;
                         mag = __float_as_uint(v) & 0x7FFFFFFFu;
                     }
                     if constexpr (F16) {
@@ -457,8 +503,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 __syncwarp();
                 if (lane == 0) {
                     ptx::mbar_arrive(bar_free + 8 * b);
-                    __threadfence();
-                    atomicAdd(p.done + item.a, 1);
+                    add_release(p.done + item.a);
                 }
             } else {
                 for (int i = lane; i < down_rows * m; i += 32) {
@@ -466,16 +511,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                     const int slot = base + tok;
                     float v = total(j, tok);
                     if constexpr (F16) v *= few_norm(__ldcg(p.h_max + slot), true);
-                    if (item.part == 0) v += bias_at(p.b2, (size_t)e * p.H + item.row + j);
-                    p.partial[((size_t)item.part * slots + slot) * p.H + item.row + j] = v;
+                    if (item.part == 0) v += bias_at(p.b2, (size_t)e * p.H + row0 + j);
+                    p.partial[((size_t)item.part * slots + slot) * p.H + row0 + j] = v;
                 }
                 __syncwarp();
                 int last = 0;
                 if (lane == 0) {
                     ptx::mbar_arrive(bar_free + 8 * b);
-                    __threadfence();
-                    last = atomicAdd(p.ticket + item.row / down_rows, 1) == actives * p.parts - 1;
-                    __threadfence();
+                    last = add_release(p.ticket + item.block) == actives * p.parts - 1;
+                    if (last) __threadfence();
                 }
                 if (__shfl_sync(0xffffffffu, last, 0)) {
                     // every chosen expert has delivered these rows: the weighted sum of each token, in the order of j
@@ -483,12 +527,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                         const int tok = i / down_rows, j = i - tok * down_rows;
                         float v = 0.0f;
                         for (int c = 0; c < p.k; ++c) {
-                            const float* src = p.partial + (size_t)s.slot[tok * p.k + c] * p.H + item.row + j;
+                            const float* src = p.partial + (size_t)s.slot[tok * p.k + c] * p.H + row0 + j;
                             float y = __ldcg(src);
                             for (int q = 1; q < p.parts; ++q) y += __ldcg(src + (size_t)q * slots * p.H);
                             v = fmaf(s.w[tok * p.k + c], y, v);
                         }
-                        const size_t at = (size_t)tok * p.H + item.row + j;
+                        const size_t at = (size_t)tok * p.H + row0 + j;
                         if (p.f16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
                         else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
                     }
@@ -502,72 +546,83 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     const int g = lane >> 2, q = lane & 3;
     const int wk = warp % FEW_W;
     const uint32_t ring = ptx::smem_u32(few_smem) + warp * (S::D * S::SLOT);
-    // where this lane's 16 bytes of a row group go: as they lie, but 4-bit rows block by block (32 elements = 16 bytes),
-    // so that the 8 codes a lane takes of every block can be read without bank conflicts
-    const uint32_t put = WF == FEW_FP4 ? (q * 8 + g) * 16 : lane * 16;
+    const uint32_t ring_scale = ptx::smem_u32(few_smem) + FEW_STREAM_WARPS * S::D * S::SLOT + warp * (S::D * S::SCALES);
+    const uint32_t bar_step = ptx::smem_u32(&s.full[warp * S::D]);
 
     // ---- position of the loads
-    int l_it = first - stride, l_s = 0, l_end = 0, l_K = 0, l_slot = 0;
-    const uint8_t* l_ptr[RG];
+    Item l_item{true, 0, 0, 0};
+    int l_nth = 0, l_s = 0, l_end = 0, l_slot = 0, l_e = 0;
+    int in_flight = 0;                                  // steps asked for and not yet used
     const uint8_t* l_scale = nullptr;                   // fp4: the words of this lane's row in row group q; fp8: group `lane`
-    auto next_load_item = [&]() {
-        Item i;
-        do {
-            l_it += stride;
-            if (l_it >= items) return;
-            i = item_at(l_it);
-            l_s = i.begin + wk;
-        } while (l_s >= i.end);
-        l_end = i.end;
-        const int e = s.active[i.a];
-        const int rows = i.up ? p.I : p.H, K = i.up ? p.H : p.I;
-        l_K = K;
-        const size_t row_bytes = (size_t)K * 2 / SUBS;
-        const bool alternate = i.up && gated;
-        // weight row 8 * group of the item: SwiGLU alternates between gate and up rows
-        auto row_of = [&](int group) { return i.row + 8 * (alternate ? group >> 1 : group); };
-#pragma unroll
-        for (int r = 0; r < RG; ++r) {
-            const uint8_t* w = i.up ? (alternate && (r & 1) ? p.w3 : p.w1) : p.w2;
-            l_ptr[r] = w + ((size_t)e * rows + row_of(r) + g) * row_bytes + q * 16;
+    bool l_more = forward(l_item, first);
+    // weight row of row group `group` of an item, SwiGLU: gate and up rows of the same number in turn
+    auto row_of = [&](const Item& i, int group) {
+        return i.up && gated ? i.block * up_rows + 8 * (group >> 1) : i.block * 8 * RG + 8 * group;
+    };
+    auto start_loads = [&]() {                          // l_item: the first item from here on that this warp has a step of
+        for (;; l_more = forward(l_item, stride), ++l_nth) {
+            if (!l_more) return;
+            l_s = begin_of(l_item) + turn(wk, l_nth);
+            l_end = end_of(l_item);
+            if (l_s < l_end) break;
         }
+        l_e = s.active[l_item.a];
+        const bool alternate = l_item.up && gated;
+        const int rows = l_item.up ? p.I : p.H, K = l_item.up ? p.H : p.I;
         if constexpr (WF == FEW_FP4) {
-            const int group = min(q, RG - 1), row = row_of(group) + g;
-            const uint8_t* sc = i.up ? (alternate && (group & 1) ? p.s3 : p.s1) : p.s2;
-            l_scale = sc + ((size_t)e * fp4_row_tiles(rows) + (row >> 7)) * fp4_col_tiles(K) * FP4_TILE_BYTES + fp4_tile_word(row);
+            const int group = min(q, RG - 1), row = row_of(l_item, group) + g;
+            const uint8_t* sc = l_item.up ? (alternate && (group & 1) ? p.s3 : p.s1) : p.s2;
+            l_scale = sc + ((size_t)l_e * fp4_row_tiles(rows) + (row >> 7)) * fp4_col_tiles(K) * FP4_TILE_BYTES + fp4_tile_word(row);
         } else if constexpr (WF == FEW_FP8) {
             const int group = min(lane, RG - 1);
-            const uint8_t* sc = i.up ? (alternate && (group & 1) ? p.s3 : p.s1) : p.s2;
-            l_scale = sc + ((size_t)e * ((rows + 127) / 128) + (row_of(group) >> 7)) * (K / 128) * 4;
+            const uint8_t* sc = l_item.up ? (alternate && (group & 1) ? p.s3 : p.s1) : p.s2;
+            l_scale = sc + ((size_t)l_e * ((rows + 127) / 128) + (row_of(l_item, group) >> 7)) * (K / 128) * 4;
         }
     };
     auto issue = [&]() {
-        if (l_it < items) {
-            const uint32_t to = ring + l_slot * S::SLOT;
-            // a lane whose part of the last step lies past K (4-bit weights, K an odd multiple of 64) gets zeros
-            const int bytes = WF != FEW_FP4 || l_s * STEP_K + q * 32 < l_K ? 16 : 0;
-#pragma unroll
-            for (int r = 0; r < RG; ++r) copy_async16(to + r * 512 + put, l_ptr[r] + (bytes ? (size_t)l_s * 64 : 0), bytes);
+        if (l_more) {
+            if (ptx::elect_one()) {
+                const uint32_t to = ring + l_slot * S::SLOT, bar = bar_step + 8 * l_slot;
+                ptx::mbar_arrive_expect_tx(bar, S::SLOT);
+                if (l_item.up && gated) {
+                    ptx::tma_load_3d(to, &tm1, l_s * 128, l_item.block * up_rows, l_e, bar);
+                    ptx::tma_load_3d(to + S::SLOT / 2, &tm3, l_s * 128, l_item.block * up_rows, l_e, bar);
+                } else {
+                    ptx::tma_load_3d(to, l_item.up ? &tm1 : &tm2, l_s * 128, l_item.block * 8 * RG, l_e, bar);
+                }
+            }
             if constexpr (WF == FEW_FP4) {
-                if (q < RG) copy_async4(to + RG * 512 + (g * RG + q) * 4, l_scale + (size_t)l_s * FP4_TILE_BYTES);
+                // two scale words per row and step (256 elements), if the row has as many
+                if (q < RG) {
+                    const uint32_t to = ring_scale + l_slot * S::SCALES + (g * RG + q) * 8;
+                    const uint8_t* from = l_scale + (size_t)l_s * (2 * FP4_TILE_BYTES);
+                    copy_async4(to, from);
+                    if (l_s * STEP_K + FP4_TILE_COLS < (l_item.up ? p.H : p.I)) copy_async4(to + 4, from + FP4_TILE_BYTES);
+                }
             } else if constexpr (WF == FEW_FP8) {
-                if (lane < RG) copy_async4(to + RG * 512 + lane * 4, l_scale + (l_s >> 1) * 4);
+                if (lane < RG) copy_async4(ring_scale + l_slot * S::SCALES + lane * 4, l_scale + l_s * 4);
             }
             if (++l_slot == S::D) l_slot = 0;
+            ++in_flight;
             l_s += FEW_W;
-            if (l_s >= l_end) next_load_item();
+            if (l_s >= l_end) {
+                l_more = forward(l_item, stride);
+                ++l_nth;
+                start_loads();
+            }
         }
-        copy_commit();                                  // one group per step, empty ones at the end
+        if constexpr (S::SCALES > 0) copy_commit();     // one group per step, empty ones at the end
     };
 
-    if (first >= items) return;
-    next_load_item();
+    if (!l_more) return;
+    start_loads();
 #pragma unroll 1
     for (int d = 0; d < S::D - 1; ++d) issue();
 
     int c_slot = 0, nth = 0, ready = -1;
-    for (int it = first; it < items; it += stride, ++nth) {
-        const Item item = item_at(it);
+    uint32_t c_phase = 0;
+    Item item{true, 0, 0, 0};
+    for (bool more = forward(item, first); more; more = forward(item, stride), ++nth) {
         const int e = s.active[item.a], base = s.base[e], m = tokens_of(e);
         const int K = item.up ? p.H : p.I;
         if (!item.up && ready < item.a) {
@@ -577,7 +632,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 uint64_t t0 = 0;
                 for (uint32_t i = 0;; ++i) {
                     int32_t v;
-                    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.done + item.a) : "memory");
+                    asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.done + item.a) : "memory");
                     if (v >= up_blocks) break;
                     if (i == 0) t0 = ptx::globaltimer_ns();
                     if ((i & 63u) == 63u) {
@@ -592,173 +647,222 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 }
             }
             if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+            asm volatile("fence.acq_rel.gpu;" ::: "memory");
             ready = item.a;
         }
-        // this lane's token row in every tile; rows past the expert's last one repeat it, their sums are not used
-        uint32_t row_at[NT];
-        float norm[NT];
+        // with as many token tiles as this expert has tokens for: most experts have a few, whatever the batch is
+        auto run = [&](auto tiles) -> bool {
+            constexpr int N = decltype(tiles)::value;
+            // this lane's token row in every tile; rows past the expert's last one repeat it, their sums are not used
+            uint32_t row_at[N];
+            float norm[N];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int slot = base + min(nt * 8 + g, m - 1);
-            row_at[nt] = item.up ? s.token[slot] : slot;
-            norm[nt] = F16 && !item.up ? few_norm(__ldcg(p.h_max + slot), false) : 1.0f;
-        }
-        float acc[TILES][NT][4];
+            for (int nt = 0; nt < N; ++nt) {
+                const int slot = base + min(nt * 8 + g, m - 1);
+                row_at[nt] = item.up ? s.token[slot] : slot;
+                norm[nt] = F16 && !item.up ? few_norm(__ldcg(p.h_max + slot), false) : 1.0f;
+            }
+            float acc[TILES][N][4];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
+            for (int t = 0; t < TILES; ++t)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < N; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[t][nt][i] = 0.0f;
+                    for (int i = 0; i < 4; ++i) acc[t][nt][i] = 0.0f;
 
-        for (int st = item.begin + wk; st < item.end; st += FEW_W) {
-            const int k0 = st * STEP_K;
-            // elements k0 + sub_at(sub) .. + 7 of the token row are this lane's share of sub-step `sub`
-            auto sub_at = [&](int sub) { return WF == FEW_FP4 ? sub * 32 + q * 8 : q * 8 * SUBS + sub * 8; };
-            const int subs = WF == FEW_FP4 ? min(SUBS, (K - k0) >> 5) : SUBS;
-            // operand of token tile nt, sub-step sub: value, and (bf16 hidden activations) remainder
-            auto load_tokens = [&](int nt, int sub, uint4& hi, uint4& lo) {
-                if (item.up) {
-                    hi = load_act(p.x + (size_t)row_at[nt] * p.H + k0 + sub_at(sub));
-                } else {
-                    const float* src = p.h + (size_t)row_at[nt] * p.I + k0 + sub_at(sub);
-                    hi = load_act(src);
-                    lo = load_act(src + 4);
-                }
-            };
-            auto convert_tokens = [&](int nt, uint4& hi, uint4& lo) {
-                if (item.up) return;
-                const float v[8] = {__uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w),
-                                    __uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w)};
-                uint32_t a[4], b[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (F16) {
-                        a[i] = half_pair(v[2 * i] * norm[nt], v[2 * i + 1] * norm[nt]);
-                        b[i] = 0;
+            // where row group r of a step lies: SwiGLU steps hold all gate rows, then all up rows
+            const uint32_t odd = item.up && gated ? RG / 2 * 1024 : 1024, pair = item.up && gated ? 1024 : 2048;
+            auto group_at = [&](int r) { return (r >> 1) * pair + (r & 1) * odd; };
+            const int end = end_of(item);
+            for (int st = begin_of(item) + turn(wk, nth); st < end; st += FEW_W) {
+                const int k0 = st * STEP_K;
+                // operand of token tile nt at element k: value, and (bf16 hidden activations) remainder
+                auto load_tokens = [&](int nt, int k, uint4& hi, uint4& lo) {
+                    if (item.up) {
+                        hi = load_act(p.x + (size_t)row_at[nt] * p.H + k);
                     } else {
-                        a[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
-                        const float r0 = v[2 * i] - __uint_as_float(a[i] << 16), r1 = v[2 * i + 1] - __uint_as_float(a[i] & 0xFFFF0000u);
-                        // a value that rounds to infinity has no remainder
-                        b[i] = bf16_pair((a[i] & 0x7F80u) == 0x7F80u ? 0.0f : r0, (a[i] & 0x7F800000u) == 0x7F800000u ? 0.0f : r1);
+                        const float* src = p.h + (size_t)row_at[nt] * p.I + k;
+                        hi = load_act(src);
+                        lo = load_act(src + 4);
                     }
-                }
-                hi = make_uint4(a[0], a[1], a[2], a[3]);
-                lo = make_uint4(b[0], b[1], b[2], b[3]);
-            };
-            // the first tile's tokens are asked for before the wait for the weights
-            uint4 hi0[SUBS], lo0[SUBS];
+                };
+                auto convert_tokens = [&](int nt, uint4& hi, uint4& lo) {
+                    if (item.up) return;
+                    const float v[8] = {__uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w),
+                                        __uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w)};
+                    uint32_t a[4], b[4];
 #pragma unroll
-            for (int sub = 0; sub < SUBS; ++sub)
-                if (sub < subs) load_tokens(0, sub, hi0[sub], lo0[sub]);
-
-            copy_wait<S::D - 2>();
-            __syncwarp();
-            const uint32_t from = ring + c_slot * S::SLOT;
-            if (++c_slot == S::D) c_slot = 0;
-
-            uint4 raw[RG];
-            if constexpr (WF != FEW_FP4) {
-#pragma unroll
-                for (int r = 0; r < RG; ++r) raw[r] = ptx::ld_shared_v4(from + r * 512 + lane * 16);
-            }
-            uint32_t scale[RG];
-            if constexpr (WF == FEW_FP4) {
-#pragma unroll
-                for (int r = 0; r < RG; ++r) scale[r] = ld_shared(from + RG * 512 + (g * RG + r) * 4);
-            } else if constexpr (WF == FEW_FP8) {
-#pragma unroll
-                for (int r = 0; r < RG; ++r) scale[r] = ld_shared(from + RG * 512 + r * 4);
-            }
-            float part[TILES][NT][4];                   // quantised weights: sums that still need their scale
-            if constexpr (WF == FEW_FP8) {
-#pragma unroll
-                for (int t = 0; t < TILES; ++t)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) part[t][nt][i] = 0.0f;
-            }
-#pragma unroll
-            for (int sub = 0; sub < SUBS; ++sub) {
-                if (sub >= subs) break;
-                uint32_t a[RG][4];
-#pragma unroll
-                for (int r = 0; r < RG; ++r) {
-                    if constexpr (WF == FEW_FP4) {
-                        const uint32_t w = ld_shared(from + r * 512 + (sub * 8 + g) * 16 + q * 4);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) a[r][i] = half_bits(fp4_unpack2((w >> (8 * i)) & 255u));
-                    } else if constexpr (WF == FEW_FP8) {
-                        const uint32_t w[2] = {sub == 0 ? raw[r].x : raw[r].z, sub == 0 ? raw[r].y : raw[r].w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu), __NV_E4M3);
-                            a[r][i] = half_bits(*reinterpret_cast<const __half2*>(&hr));
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (F16) {
+                            a[i] = half_pair(v[2 * i] * norm[nt], v[2 * i + 1] * norm[nt]);
+                            b[i] = 0;
+                        } else {
+                            a[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
+                            const float r0 = v[2 * i] - __uint_as_float(a[i] << 16), r1 = v[2 * i + 1] - __uint_as_float(a[i] & 0xFFFF0000u);
+                            // a value that rounds to infinity has no remainder
+                            b[i] = bf16_pair((a[i] & 0x7F80u) == 0x7F80u ? 0.0f : r0, (a[i] & 0x7F800000u) == 0x7F800000u ? 0.0f : r1);
                         }
-                    } else {
-                        a[r][0] = raw[r].x; a[r][1] = raw[r].y; a[r][2] = raw[r].z; a[r][3] = raw[r].w;
                     }
-                }
+                    hi = make_uint4(a[0], a[1], a[2], a[3]);
+                    lo = make_uint4(b[0], b[1], b[2], b[3]);
+                };
+                // 16 x 8 x 16 twice: the eight elements of a lane's share, a[r] = row group r's
+                auto multiply = [&](const uint32_t (&a)[RG][4], int t, const uint4& hi, const uint4& lo, float (&c)[4]) {
+                    mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], hi.x, hi.y);
+                    mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], hi.z, hi.w);
+                    if (!F16 && !item.up) {
+                        mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], lo.x, lo.y);
+                        mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], lo.z, lo.w);
+                    }
+                };
+                // With one token tile the tokens of up to four chunks of a lane are asked for at once, the first ones before
+                // the wait for the weights.
+                constexpr int CHUNKS = WF == FEW_FP4 ? 8 : 2 * FewFormat<WF>::PACK;     // of 8 elements per lane and step
+                constexpr int AHEAD = N == 1 ? (CHUNKS < 4 ? CHUNKS : 4) : 1;
+                auto element = [&](int c) { return WF == FEW_FP4 ? c * 32 + q * 8 : (q * CHUNKS + c) * 8; };
+                const int chunks = WF == FEW_FP4 ? min(CHUNKS, (K - k0) >> 5) : CHUNKS;
+                uint4 hi_ahead[AHEAD], lo_ahead[AHEAD];
+                auto look_ahead = [&](int c0) {
+                    if constexpr (N == 1) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (nt * 8 >= m) break;
-                    uint4 hi, lo;
-                    if (nt == 0) { hi = hi0[sub]; lo = lo0[sub]; }
-                    else load_tokens(nt, sub, hi, lo);
+                        for (int c = 0; c < AHEAD; ++c)
+                            if (c0 + c < chunks) load_tokens(0, k0 + element(c0 + c), hi_ahead[c], lo_ahead[c]);
+                    }
+                };
+                auto tokens = [&](int nt, int c, uint4& hi, uint4& lo) {
+                    if constexpr (N == 1) { hi = hi_ahead[c % AHEAD]; lo = lo_ahead[c % AHEAD]; }
+                    else load_tokens(nt, k0 + element(c), hi, lo);
                     convert_tokens(nt, hi, lo);
+                };
+                look_ahead(0);
+                if constexpr (S::SCALES > 0) copy_wait<S::D - 2>();
+                if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_step + 8 * c_slot, c_phase, &s.abort, p.dev_status)))
+                    return false;
+                const uint32_t from = ring + c_slot * S::SLOT + g * 128;
+                [[maybe_unused]] const uint32_t scales = ring_scale + c_slot * S::SCALES;
+                if (++c_slot == S::D) { c_slot = 0; c_phase ^= 1u; }
+                --in_flight;
+
+                if constexpr (WF == FEW_FP4) {
+                    // a block of 32 at a time: its scale multiplies the sums of its products. Scale byte as the exponent
+                    // of an fp32 number: 0 (2^-127) counts as zero, 255 (NaN) as infinity
+                    uint2 sw[RG];
 #pragma unroll
-                    for (int t = 0; t < TILES; ++t) {
-                        float fresh[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        float (&c)[4] = WF == FEW_FP4 ? fresh : (WF == FEW_FP8 ? part[t][nt] : acc[t][nt]);
-                        mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], hi.x, hi.y);
-                        mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], hi.z, hi.w);
-                        if (!F16 && !item.up) {
-                            mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], lo.x, lo.y);
-                            mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], lo.z, lo.w);
+                    for (int r = 0; r < RG; ++r) sw[r] = ld_shared2(scales + (g * RG + r) * 8);
+#pragma unroll
+                    for (int b = 0; b < 8; ++b) {
+                        if (b >= chunks) break;
+                        if (b == 4) look_ahead(4);
+                        uint32_t a[RG][4];
+#pragma unroll
+                        for (int r = 0; r < RG; ++r) unpack_e2m1(ld_shared(from + group_at(r) + ((b ^ g) << 4) + q * 4), a[r]);
+                        float f[RG];
+#pragma unroll
+                        for (int r = 0; r < RG; ++r) {
+                            const uint32_t w = b < 4 ? sw[r].x : sw[r].y;
+                            f[r] = __uint_as_float(((b & 3) < 3 ? w << (23 - 8 * (b & 3)) : w >> 1) & 0x7F800000u);
                         }
-                        if constexpr (WF == FEW_FP4) {
-                            // scale byte `sub` as the exponent of an fp32 number: 0 (2^-127) counts as zero, 255 (NaN) as
-                            // infinity
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t sw = scale[2 * t + (i >> 1)];
-                                const uint32_t f = (sub < 3 ? sw << (23 - 8 * sub) : sw >> 1) & 0x7F800000u;
-                                acc[t][nt][i] = fmaf(fresh[i], __uint_as_float(f), acc[t][nt][i]);
+                        for (int nt = 0; nt < N; ++nt) {
+                            if (nt * 8 >= m) break;
+                            uint4 hi, lo;
+                            tokens(nt, b, hi, lo);
+#pragma unroll
+                            for (int t = 0; t < TILES; ++t) {
+                                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                multiply(a, t, hi, lo, c);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) acc[t][nt][i] = fmaf(c[i], f[2 * t + (i >> 1)], acc[t][nt][i]);
                             }
                         }
                     }
+                } else if constexpr (WF == FEW_FP8) {
+                    float part[TILES][N][4];            // sums of this step (one scale block of K), to be scaled
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                        for (int nt = 0; nt < N; ++nt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) part[t][nt][i] = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {       // eight codes each
+                        uint32_t a[RG][4];
+#pragma unroll
+                        for (int r = 0; r < RG; ++r) {
+                            const uint2 w = ld_shared2(from + group_at(r) + (((2 * q + (c >> 1)) ^ g) << 4) + (c & 1) * 8);
+                            unpack_e4m3(w.x, a[r][0], a[r][1]);
+                            unpack_e4m3(w.y, a[r][2], a[r][3]);
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < N; ++nt) {
+                            if (nt * 8 >= m) break;
+                            uint4 hi, lo;
+                            tokens(nt, c, hi, lo);
+#pragma unroll
+                            for (int t = 0; t < TILES; ++t) multiply(a, t, hi, lo, part[t][nt]);
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float f = __uint_as_float(ld_shared(scales + (2 * t + (i >> 1)) * 4));
+#pragma unroll
+                            for (int nt = 0; nt < N; ++nt) acc[t][nt][i] = fmaf(part[t][nt][i], f, acc[t][nt][i]);
+                        }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t a[RG][4];
+#pragma unroll
+                        for (int r = 0; r < RG; ++r) {
+                            const uint4 w = ptx::ld_shared_v4(from + group_at(r) + (((2 * q + c) ^ g) << 4));
+                            a[r][0] = w.x; a[r][1] = w.y; a[r][2] = w.z; a[r][3] = w.w;
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < N; ++nt) {
+                            if (nt * 8 >= m) break;
+                            uint4 hi, lo;
+                            tokens(nt, c, hi, lo);
+#pragma unroll
+                            for (int t = 0; t < TILES; ++t) multiply(a, t, hi, lo, acc[t][nt]);
+                        }
+                    }
                 }
+                __syncwarp();                           // every lane has read the slot that the next issue may refill
+                issue();
             }
-            if constexpr (WF == FEW_FP8) {
+            // ---- leave the sums to the helper
+            const int b = nth % S::BUFS;
+            if (nth >= S::BUFS &&
+                !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_free + 8 * b, (nth / S::BUFS - 1) & 1, &s.abort, p.dev_status)))
+                return false;
+            float* buf = red + (b * FEW_W + wk) * RED;
 #pragma unroll
-                for (int t = 0; t < TILES; ++t)
+            for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < N; ++nt)
+                    if (nt * 8 < m)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            acc[t][nt][i] = fmaf(part[t][nt][i], __uint_as_float(scale[2 * t + (i >> 1)]), acc[t][nt][i]);
-            }
-            __syncwarp();                               // every lane has read the slot that the next issue may refill
-            issue();
-        }
-        // ---- leave the sums to the helper
-        const int b = nth % S::BUFS;
-        if (nth >= S::BUFS &&
-            !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_free + 8 * b, (nth / S::BUFS - 1) & 1, &s.abort, p.dev_status)))
-            break;
-        float* buf = red + (b * FEW_W + wk) * RED;
-#pragma unroll
-        for (int t = 0; t < TILES; ++t)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                if (nt * 8 < m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) buf[((t * NT + nt) * 4 + i) * 32 + lane] = acc[t][nt][i];
+                        for (int i = 0; i < 4; ++i) buf[((t * NT + nt) * 4 + i) * 32 + lane] = acc[t][nt][i];
+            return true;
+        };
+        bool ok;
+        if constexpr (NT == 1) ok = run(Tiles<1>{});
+        else if constexpr (NT == 2) ok = m <= 8 ? run(Tiles<1>{}) : run(Tiles<2>{});
+        else if constexpr (NT == 4) ok = m <= 8 ? run(Tiles<1>{}) : (m <= 16 ? run(Tiles<2>{}) : run(Tiles<4>{}));
+        else ok = m <= 8 ? run(Tiles<1>{}) : (m <= 16 ? run(Tiles<2>{}) : (m <= 32 ? run(Tiles<4>{}) : run(Tiles<8>{})));
+        if (!ok) break;
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar_full + 8 * b);
+        if (lane == 0) ptx::mbar_arrive(bar_full + 8 * (nth % S::BUFS));
     }
-    copy_wait<0>();
+    if constexpr (S::SCALES > 0) copy_wait<0>();
+    // after a wait that gave up: the copies in flight still write to this CTA's shared memory
+    for (; in_flight > 0; --in_flight) {
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (!ptx::mbar_try_wait(bar_step + 8 * c_slot, c_phase) && ptx::globaltimer_ns() - t0 < ptx::WAIT_LIMIT_NS) {}
+        if (++c_slot == S::D) { c_slot = 0; c_phase ^= 1u; }
+    }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -789,8 +893,17 @@ FewPlan few_plan(int n, int H, int I, int E, int k) {
     return f;
 }
 
+struct FewWeights { const void *w1, *w3, *w2; };
+
 template <int WF, int NT, class S>
-aristos_status_t launch_few(const FewParams& p, cudaStream_t st) {
+aristos_status_t launch_few(const FewParams& p, const FewWeights& w, cudaStream_t st) {
+    CUtensorMap tm1, tm3, tm2;
+    // weights as bytes: (experts, rows, bytes of a row), boxes of 128 bytes x the rows of an item
+    const int h_bytes = p.H * 2 / FewFormat<WF>::PACK, i_bytes = p.I * 2 / FewFormat<WF>::PACK;
+    const bool gated = p.act == ARISTOS_ACT_SWIGLU;
+    ARISTOS_TRY(encode_map_3d(&tm1, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w.w1, h_bytes, p.I, p.E, gated ? 4 * S::RG : 8 * S::RG));
+    ARISTOS_TRY(encode_map_3d(&tm3, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, gated ? w.w3 : w.w1, h_bytes, p.I, p.E, 4 * S::RG));
+    ARISTOS_TRY(encode_map_3d(&tm2, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w.w2, i_bytes, p.H, p.E, 8 * S::RG));
     auto kernel = few_ffn_kernel<WF, NT, S>;
     static_assert(S::SMEM + sizeof(FewLists) <= 227 * 1024, "few tokens: shared memory");
     ARISTOS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
@@ -811,17 +924,17 @@ aristos_status_t launch_few(const FewParams& p, cudaStream_t st) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    ARISTOS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
+    ARISTOS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tm1, tm3, tm2, p));
     ARISTOS_COUNT_LAUNCH();
     return ARISTOS_OK;
 }
 
 template <int WF>
-aristos_status_t launch_few_tokens(const FewParams& p, cudaStream_t st) {
-    if (p.n <= 8) return launch_few<WF, 1, FewShape<WF, 1, 4, 5, 2>>(p, st);
-    if (p.n <= 16) return launch_few<WF, 2, FewShape<WF, 2, 4, 4, 2>>(p, st);
-    if (p.n <= 32) return launch_few<WF, 4, FewShape<WF, 4, 4, 4, 1>>(p, st);
-    return launch_few<WF, 8, FewShape<WF, 8, 2, 6, 1>>(p, st);
+aristos_status_t launch_few_tokens(const FewParams& p, const FewWeights& w, cudaStream_t st) {
+    if (p.n <= 8) return launch_few<WF, 1, FewShape<WF, 1, 4, 3, 2>>(p, w, st);
+    if (p.n <= 16) return launch_few<WF, 2, FewShape<WF, 2, 4, 3, 1>>(p, w, st);
+    if (p.n <= 32) return launch_few<WF, 4, FewShape<WF, 4, 2, 4, 2>>(p, w, st);
+    return launch_few<WF, 8, FewShape<WF, 8, 2, 4, 1>>(p, w, st);
 }
 
 aristos_status_t few_check(int tokens, int H, int I, int E, int k, int weights_dtype) {
@@ -894,9 +1007,7 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
     p.logits = reinterpret_cast<float*>(ws + f.logits);
     p.x = static_cast<const uint16_t*>(norm ? static_cast<const void*>(ws + f.x_norm) : x);
     p.x_scale = norm ? reinterpret_cast<const float*>(ws + f.x_scale) : nullptr;
-    p.w1 = static_cast<const uint8_t*>(w1);
-    p.w3 = static_cast<const uint8_t*>(gated ? w3 : nullptr);
-    p.w2 = static_cast<const uint8_t*>(w2);
+    const FewWeights w{w1, w3, w2};
     p.s1 = static_cast<const uint8_t*>(s1);
     p.s3 = static_cast<const uint8_t*>(s3);
     p.s2 = static_cast<const uint8_t*>(s2);
@@ -929,7 +1040,7 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
             const_cast<float*>(p.logits), p.done, f.ncounters, x_norm, x_scale);
     ARISTOS_COUNT_LAUNCH();
     ARISTOS_CUDA_TRY(cudaGetLastError());
-    if (fp4) return launch_few_tokens<FEW_FP4>(p, st);
-    if (fp8) return launch_few_tokens<FEW_FP8>(p, st);
-    return f16 ? launch_few_tokens<FEW_F16>(p, st) : launch_few_tokens<FEW_BF16>(p, st);
+    if (fp4) return launch_few_tokens<FEW_FP4>(p, w, st);
+    if (fp8) return launch_few_tokens<FEW_FP8>(p, w, st);
+    return f16 ? launch_few_tokens<FEW_F16>(p, w, st) : launch_few_tokens<FEW_BF16>(p, w, st);
 }
