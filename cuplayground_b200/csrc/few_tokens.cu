@@ -171,7 +171,8 @@ struct FewLists {
     uint16_t base[FEW_MAX_EXPERTS];            // first row of an expert
     uint16_t active[FEW_MAX_EXPERTS];          // chosen experts, increasing
     uint8_t token[FEW_MAX_SLOTS];              // token of a row
-    int actives;
+    uint8_t chunks[FEW_MAX_EXPERTS];           // per chosen expert: its tokens are taken in so many passes
+    int actives, all_chunks;
     int abort;
 };
 
@@ -313,7 +314,7 @@ template <> struct FewFormat<FEW_F16> { static constexpr int PACK = 1; };
 template <> struct FewFormat<FEW_FP8> { static constexpr int PACK = 2; };
 template <> struct FewFormat<FEW_FP4> { static constexpr int PACK = 4; };
 
-// NT: token tiles of 8 (at least ceil(n / 8)); RG: groups of 8 weight rows per item; D: steps in the ring; BUFS: buffers for
+// NT: token tiles of 8 per pass; RG: groups of 8 weight rows per item; D: steps in the ring; BUFS: buffers for
 // the sums of an item.
 template <int WF, int NT, int RG_, int D_, int BUFS_>
 struct FewShape {
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     }
     __syncthreads();
     if (warp == 0) {
-        int rows = 0, n_active = 0;
+        int rows = 0, n_active = 0, all = 0;
         for (int e0 = 0; e0 < p.E; e0 += 32) {
             const int e = e0 + lane;
             const int m = e < p.E ? __popc(s.mask[e][0]) + __popc(s.mask[e][1]) : 0;
@@ -386,12 +387,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             const uint32_t on = __ballot_sync(0xffffffffu, m > 0);
             if (m > 0) {
                 s.base[e] = (uint16_t)(rows + incl - m);
-                s.active[n_active + __popc(on & ((1u << lane) - 1))] = (uint16_t)e;
+                const int a = n_active + __popc(on & ((1u << lane) - 1));
+                s.active[a] = (uint16_t)e;
+                s.chunks[a] = (uint8_t)((m + 8 * NT - 1) / (8 * NT));
             }
             rows += __shfl_sync(0xffffffffu, incl, 31);
             n_active += __popc(on);
+            all += __reduce_add_sync(0xffffffffu, (m + 8 * NT - 1) / (8 * NT));
         }
-        if (lane == 0) s.actives = n_active;
+        if (lane == 0) { s.actives = n_active; s.all_chunks = all; }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < slots; i += FEW_THREADS) {
@@ -414,22 +418,22 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     const int stride = gridDim.x * FEW_GROUPS, first = blockIdx.x * FEW_GROUPS + grp;
 
     // A position in the list. It advances by `stride` items without a division: the list is ordered by expert, then (down
-    // projection) by part of K, then by block of rows.
+    // projection) by part of K, then by block of rows, then by pass over the expert's tokens.
     struct Item {
         bool up;
-        int a, part, block;        // chosen expert, part of K, block of rows
+        int a, part, at;           // chosen expert, part of K, block of rows * passes + pass
     };
     auto forward = [&](Item& i, int by) {      // returns false past the end
-        i.block += by;
+        i.at += by;
         if (i.up) {
-            while (i.block >= up_blocks) {
-                i.block -= up_blocks;
+            for (int len; i.at >= (len = up_blocks * s.chunks[i.a]);) {
+                i.at -= len;
                 if (++i.a == actives) { i.up = false; i.a = 0; break; }
             }
         }
         if (!i.up) {
-            while (i.block >= down_blocks) {
-                i.block -= down_blocks;
+            for (int len; i.at >= (len = down_blocks * s.chunks[i.a]);) {
+                i.at -= len;
                 if (++i.part == p.parts) {
                     i.part = 0;
                     if (++i.a == actives) return false;
@@ -438,6 +442,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
         }
         return true;
     };
+    auto block_of = [&](const Item& i) { const int c = s.chunks[i.a]; return c == 1 ? i.at : i.at / c; };
+    auto pass_of = [&](const Item& i) { const int c = s.chunks[i.a]; return c == 1 ? 0 : i.at % c; };
     auto begin_of = [&](const Item& i) { return i.up ? 0 : i.part * part_steps; };
     auto end_of = [&](const Item& i) { return i.up ? up_steps : min((i.part + 1) * part_steps, down_steps); };
     // The warps of a group start at another step of every item: who has one step more than the others changes.
@@ -448,16 +454,51 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
 
     if (warp >= FEW_STREAM_WARPS) {
         // ============================================================ helper: sums, epilogue, bookkeeping
+        // Finished items are counted together: a release takes as long as the stores before it, so counters are put off
+        // until a few have come together or there is nothing else to do. Lane j holds the j-th one, as an offset from
+        // p.done.
+        constexpr int TOGETHER = 4;
+        const int ticket0 = (int)(p.ticket - p.done);
+        int pending = 0, counter = 0;
+        auto count_items = [&]() {
+            if (pending == 0) return;
+            __syncwarp();
+            bool last = false;
+            if (lane < pending) {
+                const int old = add_release(p.done + counter);
+                last = counter >= ticket0 && old == s.all_chunks * p.parts - 1;
+            }
+            uint32_t todo = __ballot_sync(0xffffffffu, last);
+            pending = 0;
+            if (todo == 0) return;
+            __threadfence();
+            for (; todo; todo &= todo - 1) {
+                // every chosen expert has delivered this block of rows: the weighted sum of each token, in the order of j
+                const int row0 = (__shfl_sync(0xffffffffu, counter, __ffs(todo) - 1) - ticket0) * down_rows;
+                for (int i = lane; i < down_rows * p.n; i += 32) {
+                    const int tok = i / down_rows, row = row0 + i - tok * down_rows;
+                    float v = 0.0f;
+                    for (int c = 0; c < p.k; ++c) {
+                        const float* src = p.partial + (size_t)s.slot[tok * p.k + c] * p.H + row;
+                        float y = __ldcg(src);
+                        for (int part = 1; part < p.parts; ++part) y += __ldcg(src + (size_t)part * slots * p.H);
+                        v = fmaf(s.w[tok * p.k + c], y, v);
+                    }
+                    const size_t at = (size_t)tok * p.H + row;
+                    if (p.f16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+                    else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+                }
+            }
+        };
         int nth = 0;
         Item item{true, 0, 0, 0};
         for (bool more = forward(item, first); more; more = forward(item, stride), ++nth) {
-            const int row0 = item.block * (item.up ? up_rows : down_rows);
-            const int e = s.active[item.a], base = s.base[e], m = tokens_of(e);
+            const int block = block_of(item), row0 = block * (item.up ? up_rows : down_rows);
+            const int e = s.active[item.a], pass = pass_of(item);
+            const int base = s.base[e] + pass * 8 * NT, m = min(tokens_of(e) - pass * 8 * NT, 8 * NT);
             const int b = nth % S::BUFS;
             const float* buf = red + b * FEW_W * RED;
-            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_full + 8 * b, (nth / S::BUFS) & 1, &s.abort, p.dev_status)))
-                return;
-            // the sum of row `j` of the item (in the order of its row groups) for token `tok` of the expert
+            // the sum of row `j` of the item (in the order of its row groups) for token `tok` of the pass
             auto total = [&](int j, int tok) {
                 const int at = (((j >> 4) * NT + (tok >> 3)) * 4 + ((j >> 3) & 1) * 2 + (tok & 1)) * 32 + (j & 7) * 4 + ((tok & 7) >> 1);
                 float v = 0.0f;
@@ -470,75 +511,55 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 return p.f16 ? __half2float(static_cast<const __half*>(bias)[i])
                              : __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[i]);
             };
+            const int rows = item.up ? up_rows : down_rows;    // 8, 16 or 32: a warp holds whole columns of the item
+            const int j = lane & (rows - 1), tok0 = lane / rows, step = 32 / rows;
+            // what does not depend on the sums is asked for before the wait
+            float bias1 = 0.0f, bias3 = 0.0f;
             if (item.up) {
-                const int rows = up_rows;                  // 8, 16 or 32: a power of two that a warp holds evenly
-                const int span = min(rows, 32);
-                for (int i0 = 0; i0 < rows * m; i0 += 32) {
-                    const int i = i0 + lane;
-                    const int tok = i / rows, j = i - tok * rows;
-                    uint32_t mag = 0;
-                    if (tok < m) {
-                        const int slot = base + tok;
+                bias1 = bias_at(p.b1, (size_t)e * p.I + row0 + j);
+                bias3 = bias_at(p.b3, (size_t)e * p.I + row0 + j);
+            } else if (item.part == 0) {
+                bias1 = bias_at(p.b2, (size_t)e * p.H + row0 + j);
+            }
+            const uint32_t full = bar_full + 8 * b, parity = (nth / S::BUFS) & 1;
+            if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(full, parity))) {
+                count_items();
+                if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(full, parity, &s.abort, p.dev_status))) return;
+            }
+            for (int tok = tok0; tok - tok0 < m; tok += step) {
+                const bool in = tok < m;
+                const int slot = base + (in ? tok : 0);
+                if (item.up) {
+                    float v = 0.0f;
+                    if (in) {
                         const float f = p.x_scale ? __ldg(p.x_scale + s.token[slot]) : 1.0f;
-                        const size_t col = (size_t)e * p.I + row0 + j;
-                        float v;
                         if (gated) {
                             // row groups alternate between gate and up rows
                             const int jg = (j >> 3) * 16 + (j & 7);
-                            const float gate = total(jg, tok) * f + bias_at(p.b1, col);
-                            const float lin = total(jg + 8, tok) * f + bias_at(p.b3, col);
-                            v = act_silu(gate) * lin;
+                            v = act_silu(total(jg, tok) * f + bias1) * (total(jg + 8, tok) * f + bias3);
                         } else {
-                            v = total(j, tok) * f + bias_at(p.b1, col);
+                            v = total(j, tok) * f + bias1;
                             v = p.act == ARISTOS_ACT_RELU ? act_relu(v) : act_gelu(v);
                         }
                         p.h[(size_t)slot * p.I + row0 + j] = v;
-                        mag = __float_as_uint(v) & 0x7FFFFFFFu;
                     }
                     if constexpr (F16) {
-                        for (int d = span >> 1; d >= 1; d >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, d));
-                        if (tok < m && (lane & (span - 1)) == 0) atomicMax(p.h_max + base + tok, mag);
+                        uint32_t mag = __float_as_uint(v) & 0x7FFFFFFFu;
+                        for (int d = rows >> 1; d >= 1; d >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, d));
+                        if (in && j == 0) atomicMax(p.h_max + slot, mag);
                     }
-                }
-                __syncwarp();
-                if (lane == 0) {
-                    ptx::mbar_arrive(bar_free + 8 * b);
-                    add_release(p.done + item.a);
-                }
-            } else {
-                for (int i = lane; i < down_rows * m; i += 32) {
-                    const int tok = i / down_rows, j = i - tok * down_rows;
-                    const int slot = base + tok;
+                } else if (in) {
                     float v = total(j, tok);
                     if constexpr (F16) v *= few_norm(__ldcg(p.h_max + slot), true);
-                    if (item.part == 0) v += bias_at(p.b2, (size_t)e * p.H + row0 + j);
-                    p.partial[((size_t)item.part * slots + slot) * p.H + row0 + j] = v;
-                }
-                __syncwarp();
-                int last = 0;
-                if (lane == 0) {
-                    ptx::mbar_arrive(bar_free + 8 * b);
-                    last = add_release(p.ticket + item.block) == actives * p.parts - 1;
-                    if (last) __threadfence();
-                }
-                if (__shfl_sync(0xffffffffu, last, 0)) {
-                    // every chosen expert has delivered these rows: the weighted sum of each token, in the order of j
-                    for (int i = lane; i < down_rows * p.n; i += 32) {
-                        const int tok = i / down_rows, j = i - tok * down_rows;
-                        float v = 0.0f;
-                        for (int c = 0; c < p.k; ++c) {
-                            const float* src = p.partial + (size_t)s.slot[tok * p.k + c] * p.H + row0 + j;
-                            float y = __ldcg(src);
-                            for (int q = 1; q < p.parts; ++q) y += __ldcg(src + (size_t)q * slots * p.H);
-                            v = fmaf(s.w[tok * p.k + c], y, v);
-                        }
-                        const size_t at = (size_t)tok * p.H + row0 + j;
-                        if (p.f16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
-                        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-                    }
+                    p.partial[((size_t)item.part * slots + slot) * p.H + row0 + j] = v + bias1;
                 }
             }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar_free + 8 * b);
+            if (lane == pending) counter = item.up ? item.a : ticket0 + block;
+            if (++pending == TOGETHER) count_items();
         }
+        count_items();
         return;
     }
 
@@ -551,13 +572,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
 
     // ---- position of the loads
     Item l_item{true, 0, 0, 0};
-    int l_nth = 0, l_s = 0, l_end = 0, l_slot = 0, l_e = 0;
+    int l_nth = 0, l_s = 0, l_end = 0, l_slot = 0, l_e = 0, l_block = 0;
     int in_flight = 0;                                  // steps asked for and not yet used
     const uint8_t* l_scale = nullptr;                   // fp4: the words of this lane's row in row group q; fp8: group `lane`
     bool l_more = forward(l_item, first);
     // weight row of row group `group` of an item, SwiGLU: gate and up rows of the same number in turn
     auto row_of = [&](const Item& i, int group) {
-        return i.up && gated ? i.block * up_rows + 8 * (group >> 1) : i.block * 8 * RG + 8 * group;
+        return i.up && gated ? l_block * up_rows + 8 * (group >> 1) : l_block * 8 * RG + 8 * group;
     };
     auto start_loads = [&]() {                          // l_item: the first item from here on that this warp has a step of
         for (;; l_more = forward(l_item, stride), ++l_nth) {
@@ -567,6 +588,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             if (l_s < l_end) break;
         }
         l_e = s.active[l_item.a];
+        l_block = block_of(l_item);
         const bool alternate = l_item.up && gated;
         const int rows = l_item.up ? p.I : p.H, K = l_item.up ? p.H : p.I;
         if constexpr (WF == FEW_FP4) {
@@ -585,10 +607,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 const uint32_t to = ring + l_slot * S::SLOT, bar = bar_step + 8 * l_slot;
                 ptx::mbar_arrive_expect_tx(bar, S::SLOT);
                 if (l_item.up && gated) {
-                    ptx::tma_load_3d(to, &tm1, l_s * 128, l_item.block * up_rows, l_e, bar);
-                    ptx::tma_load_3d(to + S::SLOT / 2, &tm3, l_s * 128, l_item.block * up_rows, l_e, bar);
+                    ptx::tma_load_3d(to, &tm1, l_s * 128, l_block * up_rows, l_e, bar);
+                    ptx::tma_load_3d(to + S::SLOT / 2, &tm3, l_s * 128, l_block * up_rows, l_e, bar);
                 } else {
-                    ptx::tma_load_3d(to, l_item.up ? &tm1 : &tm2, l_s * 128, l_item.block * 8 * RG, l_e, bar);
+                    ptx::tma_load_3d(to, l_item.up ? &tm1 : &tm2, l_s * 128, l_block * 8 * RG, l_e, bar);
                 }
             }
             if constexpr (WF == FEW_FP4) {
@@ -619,38 +641,43 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
 #pragma unroll 1
     for (int d = 0; d < S::D - 1; ++d) issue();
 
-    int c_slot = 0, nth = 0, ready = -1;
+    int c_slot = 0, nth = 0, ready = 0;               // experts below `ready` have all their hidden activations
     uint32_t c_phase = 0;
     Item item{true, 0, 0, 0};
     for (bool more = forward(item, first); more; more = forward(item, stride), ++nth) {
-        const int e = s.active[item.a], base = s.base[e], m = tokens_of(e);
+        const int e = s.active[item.a], pass = pass_of(item);
+        const int base = s.base[e] + pass * 8 * NT, m = min(tokens_of(e) - pass * 8 * NT, 8 * NT);
         const int K = item.up ? p.H : p.I;
-        if (!item.up && ready < item.a) {
-            // all of this expert's hidden activations must be there (the list is in expert order)
+        if (!item.up && ready <= item.a) {
+            // All of this expert's hidden activations must be there. The next experts' counters are read along with it:
+            // by now most of them are complete, and a fence is paid once for all.
             bool ok = true;
-            if (lane == 0) {
-                uint64_t t0 = 0;
-                for (uint32_t i = 0;; ++i) {
+            uint64_t t0 = 0;
+            for (uint32_t i = 0;; ++i) {
+                bool there = true;
+                if (item.a + lane < actives) {
                     int32_t v;
-                    asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.done + item.a) : "memory");
-                    if (v >= up_blocks) break;
-                    if (i == 0) t0 = ptx::globaltimer_ns();
-                    if ((i & 63u) == 63u) {
-                        ok = !*static_cast<volatile int*>(&s.abort);
-                        if (ok && ptx::globaltimer_ns() - t0 > ptx::WAIT_LIMIT_NS) {
-                            s.abort = 1;
-                            if (p.dev_status) atomicOr(p.dev_status, DEV_FAULT_TIMEOUT);
-                            ok = false;
-                        }
-                        if (!ok) break;
+                    asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.done + item.a + lane) : "memory");
+                    there = v >= up_blocks * s.chunks[item.a + lane];
+                }
+                const uint32_t missing = ~__ballot_sync(0xffffffffu, there);
+                ready = item.a + (missing ? __ffs(missing) - 1 : 32);
+                if (ready > item.a) break;
+                if (i == 0) t0 = ptx::globaltimer_ns();
+                if ((i & 63u) == 63u) {
+                    ok = !*static_cast<volatile int*>(&s.abort);
+                    if (ok && ptx::globaltimer_ns() - t0 > ptx::WAIT_LIMIT_NS) {
+                        s.abort = 1;
+                        if (p.dev_status && lane == 0) atomicOr(p.dev_status, DEV_FAULT_TIMEOUT);
+                        ok = false;
                     }
+                    if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
                 }
             }
-            if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+            if (!ok) break;
             asm volatile("fence.acq_rel.gpu;" ::: "memory");
-            ready = item.a;
         }
-        // with as many token tiles as this expert has tokens for: most experts have a few, whatever the batch is
+        // with as many token tiles as this pass has tokens for: most experts have a few, whatever the batch is
         auto run = [&](auto tiles) -> bool {
             constexpr int N = decltype(tiles)::value;
             // this lane's token row in every tile; rows past the expert's last one repeat it, their sums are not used
@@ -849,9 +876,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
         };
         bool ok;
         if constexpr (NT == 1) ok = run(Tiles<1>{});
-        else if constexpr (NT == 2) ok = m <= 8 ? run(Tiles<1>{}) : run(Tiles<2>{});
-        else if constexpr (NT == 4) ok = m <= 8 ? run(Tiles<1>{}) : (m <= 16 ? run(Tiles<2>{}) : run(Tiles<4>{}));
-        else ok = m <= 8 ? run(Tiles<1>{}) : (m <= 16 ? run(Tiles<2>{}) : (m <= 32 ? run(Tiles<4>{}) : run(Tiles<8>{})));
+        else ok = m <= 8 ? run(Tiles<1>{}) : run(Tiles<2>{});
         if (!ok) break;
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar_full + 8 * (nth % S::BUFS));
@@ -931,10 +956,10 @@ aristos_status_t launch_few(const FewParams& p, const FewWeights& w, cudaStream_
 
 template <int WF>
 aristos_status_t launch_few_tokens(const FewParams& p, const FewWeights& w, cudaStream_t st) {
+    // Up to 16 tokens of an expert in one pass over its weights; more (few experts, many tokens) take further passes,
+    // whose weights come from L2. Wider passes would cost every small one registers and shared memory.
     if (p.n <= 8) return launch_few<WF, 1, FewShape<WF, 1, 4, 3, 2>>(p, w, st);
-    if (p.n <= 16) return launch_few<WF, 2, FewShape<WF, 2, 4, 3, 1>>(p, w, st);
-    if (p.n <= 32) return launch_few<WF, 4, FewShape<WF, 4, 2, 4, 2>>(p, w, st);
-    return launch_few<WF, 8, FewShape<WF, 8, 2, 4, 1>>(p, w, st);
+    return launch_few<WF, 2, FewShape<WF, 2, 4, 3, 1>>(p, w, st);
 }
 
 aristos_status_t few_check(int tokens, int H, int I, int E, int k, int weights_dtype) {
@@ -953,7 +978,7 @@ aristos_status_t few_check(int tokens, int H, int I, int E, int k, int weights_d
         return ARISTOS_ERR_CONFIG;
     }
     // items are numbered in 31 bits
-    if ((int64_t)E * ((int64_t)H * few_parts(H, I) + I) / 8 >= (int64_t)1 << 30) { set_last_error("moe_few_tokens: too many weight rows"); return ARISTOS_ERR_CONFIG; }
+    if ((int64_t)E * ((int64_t)H * few_parts(H, I) + I) >= (int64_t)1 << 30) { set_last_error("moe_few_tokens: too many weight rows"); return ARISTOS_ERR_CONFIG; }
     return ARISTOS_OK;
 }
 
