@@ -7,24 +7,27 @@
 //
 // With few tokens every weight is used a handful of times, so the layer is bound by reading the chosen experts' weights
 // once: 2, 1 or 0.53 bytes each. Everything else is arranged around that stream:
-//  * few_gate_kernel: a warp per expert and four tokens computes the logits; it also clears the counters.
+//  * few_gate_kernel: a warp per expert and one or four tokens computes the logits; it also clears the counters.
 //  * few_ffn_kernel: one CTA per SM, launched while the gate still runs. Every CTA does the (small) top-k and the
 //    expert lists for itself, so no further kernel or grid barrier is needed. The work is a list of items (chosen expert,
-//    8 * RG weight rows, part of K): all of the up projection, then all of the down projection, dealt out in turn to
-//    groups of W warps. The warps of a group cut K among themselves (128-byte pieces of all rows in turn, so together they
-//    read a row's bytes in order) and leave their sums in shared memory; a helper warp per group adds them in a fixed
-//    order and does the epilogue, the stores and the bookkeeping, so that the streaming warps never wait for any of it.
+//    8 * RG weight rows, part of K): all of the up projection, then all of the down projection; of both a group of W warps
+//    takes a contiguous share. The warps of a group cut K among themselves (128-byte pieces of all rows in turn, so
+//    together they read a row's bytes in order) and leave their sums in shared memory; a helper warp per group adds them
+//    in a fixed order and does the epilogue, the stores and the bookkeeping, so that the streaming warps never wait for
+//    any of it.
 //  * Weights travel by TMA into a ring that every warp has for itself, up to D steps (4 KB each) ahead of the arithmetic
 //    and across item boundaries, from the up into the down projection: the stream does not stop for reductions or for the
 //    wait below. (Through cp.async or plain loads the tokens' loads queue behind the weights' in the L1 and every step
 //    takes as long as a DRAM access: 190 us for what takes 125 us this way.)
-//  * An item of the down projection waits until all of its expert's up items are done (a counter per expert; the wait is
-//    bounded). Up items never wait and come first in every group's list, so the wait ends.
+//  * An item of the down projection waits until all of its expert's up items are done (a counter per expert, to which a
+//    group adds its items of that expert at once: a release takes microseconds in a busy memory system; the wait is
+//    bounded). Up items never wait and come first in every group's share, so the wait ends.
 //  * The products run on the warp-level matrix instruction m16n8k16: 16 weight rows (gate and up rows of the same
 //    columns for SwiGLU) x 8 tokens x 16 of K. The order of K inside a step does not matter to the sum, so a lane uses
 //    whole 16-byte pieces of a row (4-bit: 4 bytes of each block) and reads the tokens in the same order. The 5th-generation tensor cores would need 128
 //    weight rows per instruction and both operands in shared memory, for a rate that this stream cannot use.
-//  * Expert outputs are summed per block of rows by the helper that finishes the block last, in the order of j.
+//  * When all down items are done (counted once per group), all streaming warps add up the expert outputs of the tokens,
+//    in the order of j.
 //
 // Operand types. The instruction multiplies 16-bit numbers. bf16 weights meet tokens in bf16 (as they are) and hidden
 // activations as two bf16 numbers, value and remainder: a single rounding of h to bf16 would by itself be as large as
@@ -34,6 +37,8 @@
 // activations are rounded once to 11 bits. h itself is kept in fp32. Scales of quantised weights multiply fp32 sums:
 // e4m3's per step (half of its 128 columns), e2m1's per block of 32.
 #include <cuda_fp8.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "fp4_format.cuh"
@@ -70,7 +75,7 @@ struct FewParams {
     uint32_t* h_max;               // (slots) bits of the largest |h| of a row
     float* partial;                // (parts, slots, H)
     int32_t* done;                 // up items finished, per chosen expert
-    int32_t* ticket;               // down items finished, per block of rows
+    int32_t* finished;             // groups that have written all their expert outputs
     void* out;
     int32_t* topk_idx;
     float* topk_w;
@@ -90,68 +95,84 @@ __device__ __forceinline__ float few_norm(uint32_t max_bits, bool undo) {
 }
 
 // ---- gate --------------------------------------------------------------------------------------------------------------
-constexpr int FEW_GATE_WARPS = 8, FEW_GATE_TOK = 4;
+constexpr int FEW_GATE_WARPS = 8;
 
-template <typename T>
+// TOK: tokens per warp (the gate weights are read once for them). With x_norm the first n blocks bring a token each into
+// fp16, scaled by a power of two.
+template <typename T, int TOK>
 __global__ void __launch_bounds__(FEW_GATE_WARPS * 32)
 few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* __restrict__ bias, int n, int H, int E,
                 float* __restrict__ logits, int32_t* __restrict__ counters, int ncounters, __half* __restrict__ x_norm,
                 float* __restrict__ x_scale) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int gt = blockIdx.x * blockDim.x + threadIdx.x, threads = gridDim.x * blockDim.x;
-    for (int i = gt; i < ncounters; i += threads) counters[i] = 0;
-    const int lane = gt & 31;
-    int warp = gt >> 5;
+    const int lane = threadIdx.x & 31;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < ncounters; i += gridDim.x * blockDim.x) counters[i] = 0;
     const int nchunk = H >> 3;
+    int block = blockIdx.x;
     if (x_norm) {
-        // the first n warps: a token in fp16, scaled by a power of two
-        if (warp < n) {
-            const T* row = x + (size_t)warp * H;
+        if (block < n) {
+            __shared__ uint32_t s_max;
+            if (threadIdx.x == 0) s_max = 0;
+            __syncthreads();
+            const T* row = x + (size_t)block * H;
             uint32_t m = 0;
-            for (int q = lane; q < nchunk; q += 32) {
+#pragma unroll 4
+            for (int q = threadIdx.x; q < nchunk; q += FEW_GATE_WARPS * 32) {
                 float v[8];
                 load8(row + q * 8, v);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
             }
             m = __reduce_max_sync(0xffffffffu, m);
-            const float f = few_norm(m, false);
-            for (int q = lane; q < nchunk; q += 32) {
+            if (lane == 0) atomicMax(&s_max, m);
+            __syncthreads();
+            const float f = few_norm(s_max, false);
+#pragma unroll 4
+            for (int q = threadIdx.x; q < nchunk; q += FEW_GATE_WARPS * 32) {
                 float v[8];
                 load8(row + q * 8, v);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] *= f;
-                store8(x_norm + (size_t)warp * H + q * 8, v);
+                store8(x_norm + (size_t)block * H + q * 8, v);
             }
-            if (lane == 0) x_scale[warp] = few_norm(m, true);
+            if (threadIdx.x == 0) x_scale[block] = few_norm(s_max, true);
+            return;
         }
-        warp -= n;
-        if (warp < 0) return;
+        block -= n;
     }
-    const int tgroups = (n + FEW_GATE_TOK - 1) / FEW_GATE_TOK;
+    const int warp = block * FEW_GATE_WARPS + (threadIdx.x >> 5);
+    const int tgroups = (n + TOK - 1) / TOK;
     if (warp >= E * tgroups) return;
-    const int e = warp / tgroups, t0 = (warp - e * tgroups) * FEW_GATE_TOK;
+    const int e = warp / tgroups, t0 = (warp - e * tgroups) * TOK;
     const T* w = wg + (size_t)e * H;
-    const T* xr[FEW_GATE_TOK];
+    const T* xr[TOK];
 #pragma unroll
-    for (int i = 0; i < FEW_GATE_TOK; ++i) xr[i] = x + (size_t)min(t0 + i, n - 1) * H;
-    float2 acc[FEW_GATE_TOK];
+    for (int i = 0; i < TOK; ++i) xr[i] = x + (size_t)min(t0 + i, n - 1) * H;
+    float2 acc[TOK];
 #pragma unroll
-    for (int i = 0; i < FEW_GATE_TOK; ++i) acc[i] = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-    for (int q = lane; q < nchunk; q += 32) {
-        GateChunk<T> wc;
-        load_chunk(w + q * 8, wc);
+    for (int i = 0; i < TOK; ++i) acc[i] = make_float2(0.0f, 0.0f);
+    // the loads of a round are all in flight together: the kernel is a handful of memory latencies long
+    constexpr int ROUND = TOK == 1 ? 8 : 4;
+    for (int q0 = lane; q0 < nchunk; q0 += 32 * ROUND) {
+        GateChunk<T> wc[ROUND], xc[ROUND][TOK];
 #pragma unroll
-        for (int i = 0; i < FEW_GATE_TOK; ++i) {
-            GateChunk<T> xc;
-            load_chunk(xr[i] + q * 8, xc);
+        for (int r = 0; r < ROUND; ++r)
+            if (q0 + 32 * r < nchunk) {
+                load_chunk(w + (q0 + 32 * r) * 8, wc[r]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) fma_pair(acc[i], xc, wc, j);
-        }
+                for (int i = 0; i < TOK; ++i) load_chunk(xr[i] + (q0 + 32 * r) * 8, xc[r][i]);
+            }
+#pragma unroll
+        for (int r = 0; r < ROUND; ++r)
+            if (q0 + 32 * r < nchunk) {
+#pragma unroll
+                for (int i = 0; i < TOK; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) fma_pair(acc[i], xc[r][i], wc[r], j);
+            }
     }
 #pragma unroll
-    for (int i = 0; i < FEW_GATE_TOK; ++i) {
+    for (int i = 0; i < TOK; ++i) {
         float s = acc[i].x + acc[i].y;
 #pragma unroll
         for (int m = 16; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
@@ -172,7 +193,7 @@ struct FewLists {
     uint16_t active[FEW_MAX_EXPERTS];          // chosen experts, increasing
     uint8_t token[FEW_MAX_SLOTS];              // token of a row
     uint8_t chunks[FEW_MAX_EXPERTS];           // per chosen expert: its tokens are taken in so many passes
-    int actives, all_chunks;
+    int actives, passes;                       // chosen experts; the passes of all of them
     int abort;
 };
 
@@ -253,12 +274,10 @@ __device__ __forceinline__ uint4 load_act(const void* ptr) {
     return v;
 }
 
-// Counts an item whose results this warp has written. Only a release: a full fence would also empty the L1 cache, from
+// Counts items whose results this warp has written. Only a release: a full fence would also empty the L1 cache, from
 // which the streaming warps read the tokens again for every item.
-__device__ __forceinline__ int add_release(int32_t* counter) {
-    int old;
-    asm volatile("atom.add.release.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
-    return old;
+__device__ __forceinline__ void add_release(int32_t* counter, int by) {
+    asm volatile("red.add.release.gpu.global.s32 [%0], %1;" ::"l"(counter), "r"(by) : "memory");
 }
 
 template <bool F16>
@@ -395,7 +414,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             n_active += __popc(on);
             all += __reduce_add_sync(0xffffffffu, (m + 8 * NT - 1) / (8 * NT));
         }
-        if (lane == 0) { s.actives = n_active; s.all_chunks = all; }
+        if (lane == 0) { s.actives = n_active; s.passes = all; }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < slots; i += FEW_THREADS) {
@@ -408,39 +427,48 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     }
     __syncthreads();
 
-    // ---- the list of items ------------------------------------------------------------------------------------------------
+    // ---- the items of this group ------------------------------------------------------------------------------------------
     const int actives = s.actives;
     const int up_rows = gated ? 4 * RG : 8 * RG, down_rows = 8 * RG;
     const int up_blocks = p.I / up_rows, down_blocks = p.H / down_rows;
     const int up_steps = (p.H + STEP_K - 1) / STEP_K, down_steps = (p.I + STEP_K - 1) / STEP_K;
     const int part_steps = (down_steps + p.parts - 1) / p.parts;
     const int grp = warp < FEW_STREAM_WARPS ? warp / FEW_W : warp - FEW_STREAM_WARPS;
-    const int stride = gridDim.x * FEW_GROUPS, first = blockIdx.x * FEW_GROUPS + grp;
-
-    // A position in the list. It advances by `stride` items without a division: the list is ordered by expert, then (down
-    // projection) by part of K, then by block of rows, then by pass over the expert's tokens.
+    // The up items are ordered by expert, block of rows and pass over the expert's tokens, the down items by expert, part
+    // of K, block of rows and pass. A group has [first, last) of either list.
+    const int groups = gridDim.x * FEW_GROUPS, group = blockIdx.x * FEW_GROUPS + grp;
+    const int up_items = s.passes * up_blocks, down_items = s.passes * down_blocks * p.parts;
+    auto share = [&](int items, int i) { return (int)((int64_t)items * i / groups); };
+    const int up_first = share(up_items, group), up_count = share(up_items, group + 1) - up_first;
+    const int down_first = share(down_items, group), my_items = up_count + share(down_items, group + 1) - down_first;
     struct Item {
         bool up;
         int a, part, at;           // chosen expert, part of K, block of rows * passes + pass
     };
-    auto forward = [&](Item& i, int by) {      // returns false past the end
-        i.at += by;
-        if (i.up) {
-            for (int len; i.at >= (len = up_blocks * s.chunks[i.a]);) {
-                i.at -= len;
-                if (++i.a == actives) { i.up = false; i.a = 0; break; }
-            }
+    // the item at place `index` of a list
+    auto locate = [&](bool up, int index) {
+        Item i{up, 0, 0, 0};
+        const int per_pass = up ? up_blocks : down_blocks * p.parts;
+        if (s.passes == actives) {                         // one pass each
+            i.a = index / per_pass;
+            index -= i.a * per_pass;
+        } else {
+            for (int len; index >= (len = per_pass * s.chunks[i.a]); ++i.a) index -= len;
         }
-        if (!i.up) {
-            for (int len; i.at >= (len = down_blocks * s.chunks[i.a]);) {
-                i.at -= len;
-                if (++i.part == p.parts) {
-                    i.part = 0;
-                    if (++i.a == actives) return false;
-                }
-            }
-        }
-        return true;
+        const int blocks = (up ? up_blocks : down_blocks) * s.chunks[i.a];
+        i.part = index / blocks;
+        i.at = index - i.part * blocks;
+        return i;
+    };
+    // item number `nth` of this group, given the one before it
+    auto next_item = [&](Item& i, int nth) {
+        if (nth == 0 && up_count > 0) { i = locate(true, up_first); return; }
+        if (nth == up_count) { i = locate(false, down_first); return; }
+        if (++i.at < (i.up ? up_blocks : down_blocks) * s.chunks[i.a]) return;
+        i.at = 0;
+        if (!i.up && ++i.part < p.parts) return;
+        i.part = 0;
+        ++i.a;
     };
     auto block_of = [&](const Item& i) { const int c = s.chunks[i.a]; return c == 1 ? i.at : i.at / c; };
     auto pass_of = [&](const Item& i) { const int c = s.chunks[i.a]; return c == 1 ? 0 : i.at % c; };
@@ -454,45 +482,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
 
     if (warp >= FEW_STREAM_WARPS) {
         // ============================================================ helper: sums, epilogue, bookkeeping
-        // Finished items are counted together: a release takes as long as the stores before it, so counters are put off
-        // until a few have come together or there is nothing else to do. Lane j holds the j-th one, as an offset from
-        // p.done.
-        constexpr int TOGETHER = 4;
-        const int ticket0 = (int)(p.ticket - p.done);
-        int pending = 0, counter = 0;
-        auto count_items = [&]() {
-            if (pending == 0) return;
-            __syncwarp();
-            bool last = false;
-            if (lane < pending) {
-                const int old = add_release(p.done + counter);
-                last = counter >= ticket0 && old == s.all_chunks * p.parts - 1;
-            }
-            uint32_t todo = __ballot_sync(0xffffffffu, last);
-            pending = 0;
-            if (todo == 0) return;
-            __threadfence();
-            for (; todo; todo &= todo - 1) {
-                // every chosen expert has delivered this block of rows: the weighted sum of each token, in the order of j
-                const int row0 = (__shfl_sync(0xffffffffu, counter, __ffs(todo) - 1) - ticket0) * down_rows;
-                for (int i = lane; i < down_rows * p.n; i += 32) {
-                    const int tok = i / down_rows, row = row0 + i - tok * down_rows;
-                    float v = 0.0f;
-                    for (int c = 0; c < p.k; ++c) {
-                        const float* src = p.partial + (size_t)s.slot[tok * p.k + c] * p.H + row;
-                        float y = __ldcg(src);
-                        for (int part = 1; part < p.parts; ++part) y += __ldcg(src + (size_t)part * slots * p.H);
-                        v = fmaf(s.w[tok * p.k + c], y, v);
-                    }
-                    const size_t at = (size_t)tok * p.H + row;
-                    if (p.f16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
-                    else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-                }
-            }
-        };
-        int nth = 0;
+        // Finished up items are counted when the group goes on to another expert or to the down projection.
+        int uncounted = 0;
         Item item{true, 0, 0, 0};
-        for (bool more = forward(item, first); more; more = forward(item, stride), ++nth) {
+        for (int nth = 0; nth < my_items; ++nth) {
+            next_item(item, nth);
             const int block = block_of(item), row0 = block * (item.up ? up_rows : down_rows);
             const int e = s.active[item.a], pass = pass_of(item);
             const int base = s.base[e] + pass * 8 * NT, m = min(tokens_of(e) - pass * 8 * NT, 8 * NT);
@@ -521,11 +515,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             } else if (item.part == 0) {
                 bias1 = bias_at(p.b2, (size_t)e * p.H + row0 + j);
             }
-            const uint32_t full = bar_full + 8 * b, parity = (nth / S::BUFS) & 1;
-            if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(full, parity))) {
-                count_items();
-                if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(full, parity, &s.abort, p.dev_status))) return;
-            }
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_full + 8 * b, (nth / S::BUFS) & 1, &s.abort, p.dev_status)))
+                return;
             for (int tok = tok0; tok - tok0 < m; tok += step) {
                 const bool in = tok < m;
                 const int slot = base + (in ? tok : 0);
@@ -556,10 +547,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             }
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(bar_free + 8 * b);
-            if (lane == pending) counter = item.up ? item.a : ticket0 + block;
-            if (++pending == TOGETHER) count_items();
+            if (item.up) {
+                ++uncounted;
+                const bool leaves = nth + 1 == up_count || item.at + 1 == up_blocks * s.chunks[item.a];
+                if (leaves && lane == 0) add_release(p.done + item.a, uncounted);
+                if (leaves) uncounted = 0;
+            }
         }
-        count_items();
+        __syncwarp();
+        if (lane == 0) add_release(p.finished, 1);
         return;
     }
 
@@ -575,14 +571,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     int l_nth = 0, l_s = 0, l_end = 0, l_slot = 0, l_e = 0, l_block = 0;
     int in_flight = 0;                                  // steps asked for and not yet used
     const uint8_t* l_scale = nullptr;                   // fp4: the words of this lane's row in row group q; fp8: group `lane`
-    bool l_more = forward(l_item, first);
+    bool l_more = my_items > 0;
     // weight row of row group `group` of an item, SwiGLU: gate and up rows of the same number in turn
     auto row_of = [&](const Item& i, int group) {
         return i.up && gated ? l_block * up_rows + 8 * (group >> 1) : l_block * 8 * RG + 8 * group;
     };
     auto start_loads = [&]() {                          // l_item: the first item from here on that this warp has a step of
-        for (;; l_more = forward(l_item, stride), ++l_nth) {
+        for (;; ++l_nth) {
+            l_more = l_nth < my_items;
             if (!l_more) return;
+            next_item(l_item, l_nth);
             l_s = begin_of(l_item) + turn(wk, l_nth);
             l_end = end_of(l_item);
             if (l_s < l_end) break;
@@ -628,7 +626,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             ++in_flight;
             l_s += FEW_W;
             if (l_s >= l_end) {
-                l_more = forward(l_item, stride);
                 ++l_nth;
                 start_loads();
             }
@@ -636,22 +633,22 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
         if constexpr (S::SCALES > 0) copy_commit();     // one group per step, empty ones at the end
     };
 
-    if (!l_more) return;
     start_loads();
 #pragma unroll 1
     for (int d = 0; d < S::D - 1; ++d) issue();
 
-    int c_slot = 0, nth = 0, ready = 0;               // experts below `ready` have all their hidden activations
+    int c_slot = 0, ready = 0;               // experts below `ready` have all their hidden activations
     uint32_t c_phase = 0;
     Item item{true, 0, 0, 0};
-    for (bool more = forward(item, first); more; more = forward(item, stride), ++nth) {
+    bool ok = true;
+    for (int nth = 0; nth < my_items; ++nth) {
+        next_item(item, nth);
         const int e = s.active[item.a], pass = pass_of(item);
         const int base = s.base[e] + pass * 8 * NT, m = min(tokens_of(e) - pass * 8 * NT, 8 * NT);
         const int K = item.up ? p.H : p.I;
         if (!item.up && ready <= item.a) {
             // All of this expert's hidden activations must be there. The next experts' counters are read along with it:
             // by now most of them are complete, and a fence is paid once for all.
-            bool ok = true;
             uint64_t t0 = 0;
             for (uint32_t i = 0;; ++i) {
                 bool there = true;
@@ -874,7 +871,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                         for (int i = 0; i < 4; ++i) buf[((t * NT + nt) * 4 + i) * 32 + lane] = acc[t][nt][i];
             return true;
         };
-        bool ok;
         if constexpr (NT == 1) ok = run(Tiles<1>{});
         else ok = m <= 8 ? run(Tiles<1>{}) : run(Tiles<2>{});
         if (!ok) break;
@@ -887,6 +883,46 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
         const uint64_t t0 = ptx::globaltimer_ns();
         while (!ptx::mbar_try_wait(bar_step + 8 * c_slot, c_phase) && ptx::globaltimer_ns() - t0 < ptx::WAIT_LIMIT_NS) {}
         if (++c_slot == S::D) { c_slot = 0; c_phase ^= 1u; }
+    }
+    if (!ok) return;
+
+    // ---- the tokens' sums over their experts, once every group has written its expert outputs: a warp takes 64 columns of a
+    // token at a time
+    const int columns = p.H / 64;
+    const int me = blockIdx.x * FEW_STREAM_WARPS + warp, warps = gridDim.x * FEW_STREAM_WARPS;
+    if (me >= columns * p.n) return;
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+        int32_t v;
+        asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.finished) : "memory");
+        if (v >= groups) break;
+        if (i == 0) t0 = ptx::globaltimer_ns();
+        if ((i & 63u) == 63u && (*static_cast<volatile int*>(&s.abort) || ptx::globaltimer_ns() - t0 > ptx::WAIT_LIMIT_NS)) {
+            if (p.dev_status && lane == 0) atomicOr(p.dev_status, DEV_FAULT_TIMEOUT);
+            return;
+        }
+    }
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    for (int c = me; c < columns * p.n; c += warps) {
+        const int tok = c / columns;
+        const size_t col = (size_t)(c - tok * columns) * 64 + 2 * lane;
+        float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+        for (int j = 0; j < p.k; ++j) {
+            const float* src = p.partial + (size_t)s.slot[tok * p.k + j] * p.H + col;
+            float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+            for (int part = 1; part < p.parts; ++part) {
+                const float2 z = __ldcg(reinterpret_cast<const float2*>(src + (size_t)part * slots * p.H));
+                y.x += z.x;
+                y.y += z.y;
+            }
+            const float w = s.w[tok * p.k + j];
+            v.x = fmaf(w, y.x, v.x);
+            v.y = fmaf(w, y.y, v.y);
+        }
+        const size_t at = (size_t)tok * p.H + col;
+        if (p.f16) *reinterpret_cast<uint32_t*>(static_cast<__half*>(p.out) + at) = half_pair(v.x, v.y);
+        else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(p.out) + at) = bf16_pair(v.x, v.y);
     }
 }
 
@@ -908,7 +944,7 @@ FewPlan few_plan(int n, int H, int I, int E, int k) {
     auto take = [&](size_t bytes) { const size_t here = at; at = align_up(at + bytes, 256); return here; };
     const size_t slots = (size_t)n * k;
     f.logits = take((size_t)n * E * 4);
-    f.ncounters = FEW_MAX_EXPERTS + FEW_MAX_SLOTS + H / 16;
+    f.ncounters = FEW_MAX_EXPERTS + FEW_MAX_SLOTS + 1;
     f.counters = take((size_t)f.ncounters * 4);
     f.x_norm = take((size_t)n * H * 2);
     f.x_scale = take((size_t)n * 4);
@@ -1041,7 +1077,7 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
     p.partial = reinterpret_cast<float*>(ws + f.partial);
     p.done = reinterpret_cast<int32_t*>(ws + f.counters);
     p.h_max = reinterpret_cast<uint32_t*>(p.done + FEW_MAX_EXPERTS);
-    p.ticket = p.done + FEW_MAX_EXPERTS + FEW_MAX_SLOTS;
+    p.finished = p.done + FEW_MAX_EXPERTS + FEW_MAX_SLOTS;
     p.out = out;
     p.topk_idx = topk_idx;
     p.topk_w = topk_w;
@@ -1051,18 +1087,20 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
     p.parts = few_parts(H, I);
     p.f16 = f16 ? 1 : 0;
 
-    const int gate_warps = E * ceil_div(tokens, FEW_GATE_TOK) + (norm ? tokens : 0);
-    const int gate_grid = ceil_div(gate_warps, FEW_GATE_WARPS);
+    // A warp per (expert, token) while that does not ask for more warps than run at once, else four tokens per warp.
+    const int tok = (int64_t)E * tokens <= 2048 ? 1 : 4;
+    const int gate_grid = ceil_div(E * ceil_div(tokens, tok), FEW_GATE_WARPS) + (norm ? tokens : 0);
     __half* x_norm = norm ? reinterpret_cast<__half*>(ws + f.x_norm) : nullptr;
     float* x_scale = norm ? reinterpret_cast<float*>(ws + f.x_scale) : nullptr;
-    if (f16)
-        few_gate_kernel<__half><<<gate_grid, FEW_GATE_WARPS * 32, 0, st>>>(
-            static_cast<const __half*>(x), static_cast<const __half*>(w_gate), gate_bias, tokens, H, E,
-            const_cast<float*>(p.logits), p.done, f.ncounters, x_norm, x_scale);
-    else
-        few_gate_kernel<__nv_bfloat16><<<gate_grid, FEW_GATE_WARPS * 32, 0, st>>>(
-            static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(w_gate), gate_bias, tokens, H, E,
-            const_cast<float*>(p.logits), p.done, f.ncounters, x_norm, x_scale);
+    auto gate = [&](auto kernel, auto* type) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        kernel<<<gate_grid, FEW_GATE_WARPS * 32, 0, st>>>(static_cast<const T*>(x), static_cast<const T*>(w_gate), gate_bias,
+                                                          tokens, H, E, const_cast<float*>(p.logits), p.done, f.ncounters,
+                                                          x_norm, x_scale);
+    };
+    if (f16) tok == 1 ? gate(few_gate_kernel<__half, 1>, (__half*)nullptr) : gate(few_gate_kernel<__half, 4>, (__half*)nullptr);
+    else tok == 1 ? gate(few_gate_kernel<__nv_bfloat16, 1>, (__nv_bfloat16*)nullptr)
+                  : gate(few_gate_kernel<__nv_bfloat16, 4>, (__nv_bfloat16*)nullptr);
     ARISTOS_COUNT_LAUNCH();
     ARISTOS_CUDA_TRY(cudaGetLastError());
     if (fp4) return launch_few_tokens<FEW_FP4>(p, w, st);
