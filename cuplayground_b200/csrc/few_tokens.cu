@@ -10,18 +10,17 @@
 //  * few_gate_kernel: a warp per expert and one or four tokens computes the logits; it also clears the counters.
 //  * few_ffn_kernel: one CTA per SM, launched while the gate still runs. Every CTA does the (small) top-k and the
 //    expert lists for itself, so no further kernel or grid barrier is needed. The work is a list of items (chosen expert,
-//    8 * RG weight rows, part of K): all of the up projection, then all of the down projection; of both a group of W warps
-//    takes a contiguous share. The warps of a group cut K among themselves (128-byte pieces of all rows in turn, so
-//    together they read a row's bytes in order) and leave their sums in shared memory; a helper warp per group adds them
-//    in a fixed order and does the epilogue, the stores and the bookkeeping, so that the streaming warps never wait for
-//    any of it.
+//    8 * RG weight rows, part of K): all of the up projection, then all of the down projection, dealt out in turn to
+//    groups of W warps. The warps of a group cut K among themselves (128-byte pieces of all rows in turn, so together they
+//    read a row's bytes in order) and leave their sums in shared memory; a helper warp adds them in a fixed order and does
+//    the epilogue and the stores, another one the counting, so that the streaming warps never wait for any of it (a
+//    release takes some 10000 cycles in a memory system that is kept this busy).
 //  * Weights travel by TMA into a ring that every warp has for itself, up to D steps (4 KB each) ahead of the arithmetic
 //    and across item boundaries, from the up into the down projection: the stream does not stop for reductions or for the
 //    wait below. (Through cp.async or plain loads the tokens' loads queue behind the weights' in the L1 and every step
 //    takes as long as a DRAM access: 190 us for what takes 125 us this way.)
-//  * An item of the down projection waits until all of its expert's up items are done (a counter per expert, to which a
-//    group adds its items of that expert at once: a release takes microseconds in a busy memory system; the wait is
-//    bounded). Up items never wait and come first in every group's share, so the wait ends.
+//  * An item of the down projection waits until all of its expert's up items are done (a counter per expert; the wait is
+//    bounded). Up items never wait and come first in every group's list, so the wait ends.
 //  * The products run on the warp-level matrix instruction m16n8k16: 16 weight rows (gate and up rows of the same
 //    columns for SwiGLU) x 8 tokens x 16 of K. The order of K inside a step does not matter to the sum, so a lane uses
 //    whole 16-byte pieces of a row (4-bit: 4 bytes of each block) and reads the tokens in the same order. The 5th-generation tensor cores would need 128
@@ -55,10 +54,10 @@ constexpr int FEW_MAX_EXPERTS = 512;
 constexpr int FEW_MAX_SLOTS = FEW_MAX_TOKENS * MAX_TOPK;
 static_assert(FEW_MAX_TOKENS <= 64, "the expert lists keep the tokens of an expert in 64 bits");
 
-constexpr int FEW_W = 7;                                  // warps that share an item (7 + a helper, twice: 128 registers each)
+constexpr int FEW_W = 7;                                  // warps that share an item (two groups and two helpers: 16 warps of 128 registers)
 constexpr int FEW_GROUPS = 2;                             // groups per CTA
 constexpr int FEW_STREAM_WARPS = FEW_W * FEW_GROUPS;
-constexpr int FEW_WARPS = FEW_STREAM_WARPS + FEW_GROUPS;  // and a helper per group
+constexpr int FEW_WARPS = FEW_STREAM_WARPS + 2;           // and one that adds and stores, and one that counts
 constexpr int FEW_THREADS = 32 * FEW_WARPS;
 
 constexpr int FEW_MAX_DEPTH = 6;
@@ -75,7 +74,7 @@ struct FewParams {
     uint32_t* h_max;               // (slots) bits of the largest |h| of a row
     float* partial;                // (parts, slots, H)
     int32_t* done;                 // up items finished, per chosen expert
-    int32_t* finished;             // groups that have written all their expert outputs
+    int32_t* finished;             // CTAs that have written all their expert outputs
     void* out;
     int32_t* topk_idx;
     float* topk_w;
@@ -182,6 +181,8 @@ few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* 
 }
 
 // ---- the experts ---------------------------------------------------------------------------------------------------------
+constexpr int FEW_POST = 64;               // finished items that may wait to be counted
+
 struct FewLists {
     uint64_t bars[FEW_GROUPS * 4];             // per group: sums written (2 buffers), buffer free (2)
     uint64_t full[FEW_STREAM_WARPS * FEW_MAX_DEPTH];   // per streaming warp: step arrived
@@ -193,7 +194,9 @@ struct FewLists {
     uint16_t active[FEW_MAX_EXPERTS];          // chosen experts, increasing
     uint8_t token[FEW_MAX_SLOTS];              // token of a row
     uint8_t chunks[FEW_MAX_EXPERTS];           // per chosen expert: its tokens are taken in so many passes
-    int actives, passes;                       // chosen experts; the passes of all of them
+    int actives;                               // chosen experts
+    int post[FEW_POST];                        // from the adding to the counting helper: whose up item is done; -1: the end
+    int posted, counted;
     int abort;
 };
 
@@ -256,6 +259,14 @@ __device__ __forceinline__ void copy_async4(uint32_t dst, const void* src) {
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ int ld_acquire_shared(uint32_t addr) {
+    int v;
+    asm volatile("ld.acquire.cta.shared::cta.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_release_shared(uint32_t addr, int v) {
+    asm volatile("st.release.cta.shared::cta.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 __device__ __forceinline__ uint2 ld_shared2(uint32_t addr) {
     uint2 v;
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
@@ -366,7 +377,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     if (threadIdx.x == 0) {
         for (int i = 0; i < FEW_GROUPS * 4; ++i) ptx::mbar_init(ptx::smem_u32(&s.bars[i]), (i & 2) ? 1 : FEW_W);
         for (int i = 0; i < FEW_STREAM_WARPS * S::D; ++i) ptx::mbar_init(ptx::smem_u32(&s.full[i]), 1);
-        s.abort = 0;
+        s.abort = s.posted = s.counted = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tm1);
         if (gated) ptx::prefetch_tensormap(&tm3);
@@ -393,7 +404,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     }
     __syncthreads();
     if (warp == 0) {
-        int rows = 0, n_active = 0, all = 0;
+        int rows = 0, n_active = 0;
         for (int e0 = 0; e0 < p.E; e0 += 32) {
             const int e = e0 + lane;
             const int m = e < p.E ? __popc(s.mask[e][0]) + __popc(s.mask[e][1]) : 0;
@@ -412,9 +423,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             }
             rows += __shfl_sync(0xffffffffu, incl, 31);
             n_active += __popc(on);
-            all += __reduce_add_sync(0xffffffffu, (m + 8 * NT - 1) / (8 * NT));
         }
-        if (lane == 0) { s.actives = n_active; s.passes = all; }
+        if (lane == 0) s.actives = n_active;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < slots; i += FEW_THREADS) {
@@ -427,48 +437,37 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     }
     __syncthreads();
 
-    // ---- the items of this group ------------------------------------------------------------------------------------------
+    // ---- the list of items ------------------------------------------------------------------------------------------
     const int actives = s.actives;
     const int up_rows = gated ? 4 * RG : 8 * RG, down_rows = 8 * RG;
     const int up_blocks = p.I / up_rows, down_blocks = p.H / down_rows;
     const int up_steps = (p.H + STEP_K - 1) / STEP_K, down_steps = (p.I + STEP_K - 1) / STEP_K;
     const int part_steps = (down_steps + p.parts - 1) / p.parts;
-    const int grp = warp < FEW_STREAM_WARPS ? warp / FEW_W : warp - FEW_STREAM_WARPS;
-    // The up items are ordered by expert, block of rows and pass over the expert's tokens, the down items by expert, part
-    // of K, block of rows and pass. A group has [first, last) of either list.
-    const int groups = gridDim.x * FEW_GROUPS, group = blockIdx.x * FEW_GROUPS + grp;
-    const int up_items = s.passes * up_blocks, down_items = s.passes * down_blocks * p.parts;
-    auto share = [&](int items, int i) { return (int)((int64_t)items * i / groups); };
-    const int up_first = share(up_items, group), up_count = share(up_items, group + 1) - up_first;
-    const int down_first = share(down_items, group), my_items = up_count + share(down_items, group + 1) - down_first;
+    const int stride = gridDim.x * FEW_GROUPS;
+    // A position in the list of items. It advances without a division: the list is ordered by expert, then (down
+    // projection) by part of K, then by block of rows, then by pass over the expert's tokens.
     struct Item {
         bool up;
         int a, part, at;           // chosen expert, part of K, block of rows * passes + pass
     };
-    // the item at place `index` of a list
-    auto locate = [&](bool up, int index) {
-        Item i{up, 0, 0, 0};
-        const int per_pass = up ? up_blocks : down_blocks * p.parts;
-        if (s.passes == actives) {                         // one pass each
-            i.a = index / per_pass;
-            index -= i.a * per_pass;
-        } else {
-            for (int len; index >= (len = per_pass * s.chunks[i.a]); ++i.a) index -= len;
+    auto forward = [&](Item& i, int by) {      // returns false past the end
+        i.at += by;
+        if (i.up) {
+            for (int len; i.at >= (len = up_blocks * s.chunks[i.a]);) {
+                i.at -= len;
+                if (++i.a == actives) { i.up = false; i.a = 0; break; }
+            }
         }
-        const int blocks = (up ? up_blocks : down_blocks) * s.chunks[i.a];
-        i.part = index / blocks;
-        i.at = index - i.part * blocks;
-        return i;
-    };
-    // item number `nth` of this group, given the one before it
-    auto next_item = [&](Item& i, int nth) {
-        if (nth == 0 && up_count > 0) { i = locate(true, up_first); return; }
-        if (nth == up_count) { i = locate(false, down_first); return; }
-        if (++i.at < (i.up ? up_blocks : down_blocks) * s.chunks[i.a]) return;
-        i.at = 0;
-        if (!i.up && ++i.part < p.parts) return;
-        i.part = 0;
-        ++i.a;
+        if (!i.up) {
+            for (int len; i.at >= (len = down_blocks * s.chunks[i.a]);) {
+                i.at -= len;
+                if (++i.part == p.parts) {
+                    i.part = 0;
+                    if (++i.a == actives) return false;
+                }
+            }
+        }
+        return true;
     };
     auto block_of = [&](const Item& i) { const int c = s.chunks[i.a]; return c == 1 ? i.at : i.at / c; };
     auto pass_of = [&](const Item& i) { const int c = s.chunks[i.a]; return c == 1 ? 0 : i.at % c; };
@@ -477,16 +476,64 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     // The warps of a group start at another step of every item: who has one step more than the others changes.
     auto turn = [&](int wk, int nth) { return (wk + nth) % FEW_W; };
     auto tokens_of = [&](int e) { return __popc(s.mask[e][0]) + __popc(s.mask[e][1]); };
-    const uint32_t bar_full = ptx::smem_u32(&s.bars[grp * 4]), bar_free = bar_full + 16;
-    float* red = reinterpret_cast<float*>(few_smem + FEW_STREAM_WARPS * S::D * (S::SLOT + S::SCALES)) + grp * FEW_W * S::BUFS * RED;
+    float* const red_all = reinterpret_cast<float*>(few_smem + FEW_STREAM_WARPS * S::D * (S::SLOT + S::SCALES));
 
-    if (warp >= FEW_STREAM_WARPS) {
+    if (warp == FEW_STREAM_WARPS + 1) {
+        // ============================================================ counting helper: publishes finished up items, several
+        // at once when they have come together meanwhile (a lane each)
+        int got = 0;
+        for (bool end = false; !end;) {
+            int have = 0;
+            uint64_t t0 = 0;
+            for (uint32_t i = 0;; ++i) {
+                have = ld_acquire_shared(ptx::smem_u32(&s.posted)) - got;
+                if (have > 0) break;
+                if (i == 0) t0 = ptx::globaltimer_ns();
+                if ((i & 15u) == 15u && (*static_cast<volatile int*>(&s.abort) || ptx::globaltimer_ns() - t0 > 2 * ptx::WAIT_LIMIT_NS))
+                    break;
+                __nanosleep(100);
+            }
+            have = min(__shfl_sync(0xffffffffu, have, 0), 32);
+            __syncwarp();
+            if (have <= 0) return;
+            const int a = lane < have ? s.post[(got + lane) % FEW_POST] : 0;
+            if (lane < have && a >= 0) add_release(p.done + a, 1);
+            end = __any_sync(0xffffffffu, a < 0);
+            got += have;
+            __syncwarp();
+            if (lane == 0) st_release_shared(ptx::smem_u32(&s.counted), got);
+        }
+        if (lane == 0) add_release(p.finished, 1);
+        return;
+    }
+
+    if (warp == FEW_STREAM_WARPS) {
         // ============================================================ helper: sums, epilogue, bookkeeping
-        // Finished up items are counted when the group goes on to another expert or to the down projection.
-        int uncounted = 0;
-        Item item{true, 0, 0, 0};
-        for (int nth = 0; nth < my_items; ++nth) {
-            next_item(item, nth);
+        // Takes the items of the CTA's groups in turn.
+        Item items[FEW_GROUPS];
+        bool more[FEW_GROUPS];
+#pragma unroll
+        for (int grp = 0; grp < FEW_GROUPS; ++grp) {
+            items[grp] = Item{true, 0, 0, 0};
+            more[grp] = forward(items[grp], blockIdx.x * FEW_GROUPS + grp);
+        }
+        int posts = 0;
+        auto post = [&](int a) {
+            // room in the post (it holds more than the groups can have done while one release takes place)
+            const uint64_t t0 = ptx::globaltimer_ns();
+            while (posts - ld_acquire_shared(ptx::smem_u32(&s.counted)) >= FEW_POST &&
+                   ptx::globaltimer_ns() - t0 < ptx::WAIT_LIMIT_NS) {}
+            __syncwarp();
+            if (lane == 0) {
+                s.post[posts % FEW_POST] = a;
+                st_release_shared(ptx::smem_u32(&s.posted), posts + 1);
+            }
+            ++posts;
+        };
+        // one item; returns false after a wait that gave up
+        auto add_up = [&](const Item& item, int grp, int nth) -> bool {
+            const uint32_t bar_full = ptx::smem_u32(&s.bars[grp * 4]), bar_free = bar_full + 16;
+            const float* red = red_all + grp * FEW_W * S::BUFS * RED;
             const int block = block_of(item), row0 = block * (item.up ? up_rows : down_rows);
             const int e = s.active[item.a], pass = pass_of(item);
             const int base = s.base[e] + pass * 8 * NT, m = min(tokens_of(e) - pass * 8 * NT, 8 * NT);
@@ -516,7 +563,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 bias1 = bias_at(p.b2, (size_t)e * p.H + row0 + j);
             }
             if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_full + 8 * b, (nth / S::BUFS) & 1, &s.abort, p.dev_status)))
-                return;
+                return false;
             for (int tok = tok0; tok - tok0 < m; tok += step) {
                 const bool in = tok < m;
                 const int slot = base + (in ? tok : 0);
@@ -547,21 +594,29 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             }
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(bar_free + 8 * b);
-            if (item.up) {
-                ++uncounted;
-                const bool leaves = nth + 1 == up_count || item.at + 1 == up_blocks * s.chunks[item.a];
-                if (leaves && lane == 0) add_release(p.done + item.a, uncounted);
-                if (leaves) uncounted = 0;
+            if (item.up) post(item.a);
+            return true;
+        };
+        for (int nth = 0;; ++nth) {
+            bool any = false;
+#pragma unroll
+            for (int grp = 0; grp < FEW_GROUPS; ++grp) {
+                if (!more[grp]) continue;
+                any = true;
+                if (!add_up(items[grp], grp, nth)) return;
+                more[grp] = forward(items[grp], stride);
             }
+            if (!any) break;
         }
-        __syncwarp();
-        if (lane == 0) add_release(p.finished, 1);
+        post(-1);
         return;
     }
 
     // ================================================================ streaming warps
     const int g = lane >> 2, q = lane & 3;
-    const int wk = warp % FEW_W;
+    const int wk = warp % FEW_W, grp = warp / FEW_W, first = blockIdx.x * FEW_GROUPS + grp;
+    const uint32_t bar_full = ptx::smem_u32(&s.bars[grp * 4]), bar_free = bar_full + 16;
+    float* red = red_all + grp * FEW_W * S::BUFS * RED;
     const uint32_t ring = ptx::smem_u32(few_smem) + warp * (S::D * S::SLOT);
     const uint32_t ring_scale = ptx::smem_u32(few_smem) + FEW_STREAM_WARPS * S::D * S::SLOT + warp * (S::D * S::SCALES);
     const uint32_t bar_step = ptx::smem_u32(&s.full[warp * S::D]);
@@ -571,16 +626,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     int l_nth = 0, l_s = 0, l_end = 0, l_slot = 0, l_e = 0, l_block = 0;
     int in_flight = 0;                                  // steps asked for and not yet used
     const uint8_t* l_scale = nullptr;                   // fp4: the words of this lane's row in row group q; fp8: group `lane`
-    bool l_more = my_items > 0;
+    bool l_more = forward(l_item, first);
     // weight row of row group `group` of an item, SwiGLU: gate and up rows of the same number in turn
     auto row_of = [&](const Item& i, int group) {
         return i.up && gated ? l_block * up_rows + 8 * (group >> 1) : l_block * 8 * RG + 8 * group;
     };
     auto start_loads = [&]() {                          // l_item: the first item from here on that this warp has a step of
-        for (;; ++l_nth) {
-            l_more = l_nth < my_items;
+        for (;; l_more = forward(l_item, stride), ++l_nth) {
             if (!l_more) return;
-            next_item(l_item, l_nth);
             l_s = begin_of(l_item) + turn(wk, l_nth);
             l_end = end_of(l_item);
             if (l_s < l_end) break;
@@ -626,6 +679,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             ++in_flight;
             l_s += FEW_W;
             if (l_s >= l_end) {
+                l_more = forward(l_item, stride);
                 ++l_nth;
                 start_loads();
             }
@@ -641,8 +695,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     uint32_t c_phase = 0;
     Item item{true, 0, 0, 0};
     bool ok = true;
-    for (int nth = 0; nth < my_items; ++nth) {
-        next_item(item, nth);
+    int nth = 0;
+    for (bool more = forward(item, first); more; more = forward(item, stride), ++nth) {
         const int e = s.active[item.a], pass = pass_of(item);
         const int base = s.base[e] + pass * 8 * NT, m = min(tokens_of(e) - pass * 8 * NT, 8 * NT);
         const int K = item.up ? p.H : p.I;
@@ -886,7 +940,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     }
     if (!ok) return;
 
-    // ---- the tokens' sums over their experts, once every group has written its expert outputs: a warp takes 64 columns of a
+    // ---- the tokens' sums over their experts, once every CTA has written its expert outputs: a warp takes 64 columns of a
     // token at a time
     const int columns = p.H / 64;
     const int me = blockIdx.x * FEW_STREAM_WARPS + warp, warps = gridDim.x * FEW_STREAM_WARPS;
@@ -895,7 +949,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     for (uint32_t i = 0;; ++i) {
         int32_t v;
         asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.finished) : "memory");
-        if (v >= groups) break;
+        if (v >= (int)gridDim.x) break;
         if (i == 0) t0 = ptx::globaltimer_ns();
         if ((i & 63u) == 63u && (*static_cast<volatile int*>(&s.abort) || ptx::globaltimer_ns() - t0 > ptx::WAIT_LIMIT_NS)) {
             if (p.dev_status && lane == 0) atomicOr(p.dev_status, DEV_FAULT_TIMEOUT);
