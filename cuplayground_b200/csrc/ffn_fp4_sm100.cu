@@ -8,17 +8,19 @@
 // path, whose fp32 scales per 128 elements have to be applied outside. What is left to the other warps is loading and
 // the epilogue.
 //
-// Tile 128 x 256 (SwiGLU: 128 gate and 128 up columns in one instruction), K in stages of 256 elements = one 128-byte
-// swizzled row, four stages of 51 KB. Per stage the producer loads the codes by TMA and the scales by untiled bulk copies
-// (they lie in global memory in the very tiles that tcgen05.cp takes to TMEM); the issuing thread copies the scales to
-// one of two TMEM buffers and issues up to four MMAs. Only whole 64-element steps that exist are issued, so nothing of a
-// row's padding is ever read.
+// Tile 256 x 256 per pair of CTAs (cta_group::2; SwiGLU: 128 gate and 128 up columns in one instruction), K in stages of
+// 256 elements = one 128-byte swizzled row. Each CTA loads its own 128 rows of A and one half of B, and the scales of its
+// rows and of all of B's: 35 KB, six stages. (A single CTA with all of B needs 51 KB and has room for four: the tensor
+// core then waits for TMA, 900 cycles per stage instead of the 512 that the instructions take.) Codes and scales come by
+// TMA; the scales lie in global memory in the very tiles that tcgen05.cp takes to TMEM. The issuing thread of the first
+// CTA copies a stage's scales to one of two TMEM buffers (in both CTAs) and issues up to four MMAs. Only whole 64-element
+// steps that exist are issued, so nothing of a row's padding is ever used.
 //
 // TMEM holds 512 columns; two accumulators of 256 would leave none for the scales. They overlap instead: columns
 // [0, 256) and [192, 448), scales from 448. The epilogue reads the 64 shared columns of a finished tile first and then
 // lets the issuer start the next one, which fills the other buffer while the rest is drained.
 //
-// Roles (320 threads): warp 0 TMA, warp 1 TMEM + MMA, warps 2-9 epilogue, two warps per lane quarter that take the
+// Roles (320 threads per CTA): warp 0 TMA, warp 1 TMEM + MMA, warps 2-9 epilogue, two warps per lane quarter that take the
 // 32-column chunks in turn. Every wait is bounded.
 //
 // The up projection of the FFN writes its output as MXFP4 again: a thread holds 32 adjacent columns of its row, i.e. a
@@ -34,12 +36,13 @@ namespace aristos {
 
 namespace {
 
-constexpr int F4_BM = 128;
+constexpr int F4_BM = 128;                               // rows per CTA
+constexpr int F4_PM = 256;                               // rows per pair
 constexpr int F4_BN = 256;
 constexpr int F4_KB = 256;                               // elements of K per stage: 128 bytes
-constexpr int F4_STAGES = 4;
+constexpr int F4_STAGES = 6;
 constexpr int F4_A_BYTES = F4_BM * F4_KB / 2;            // 16 KB
-constexpr int F4_B_BYTES = F4_BN * F4_KB / 2;            // 32 KB: two boxes of 128 weight rows
+constexpr int F4_B_BYTES = F4_BN / 2 * F4_KB / 2;        // 16 KB: this CTA's half of the weight rows
 constexpr int F4_SF_BYTES = 2 * FP4_TILE_BYTES;          // scales of 128 rows and one stage of K
 constexpr int F4_STAGE_BYTES = F4_A_BYTES + F4_B_BYTES + 3 * F4_SF_BYTES;
 static_assert(F4_STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
@@ -58,7 +61,7 @@ struct Fp4GemmParams {
     int groups, experts, rows_per_group;
     int N, K;
     int gated, act;
-    const uint8_t* sa;       // scale tiles of A: [groups][row tiles][K tiles][512]
+    const uint8_t* sa;       // scale tiles of A: [groups][row tiles][K tiles][512] (host side: they come by TMA)
     const uint8_t* sb0;      // of B: [experts][N tiles][K tiles][512]
     const uint8_t* sb1;      // SwiGLU: of the up projection's weights
     void* out;               // [groups * rows_per_group][N], bf16 / fp16 / fp32; or (quantised) codes, two per byte
@@ -66,14 +69,14 @@ struct Fp4GemmParams {
     int32_t* dev_status;
 };
 
-// D[tmem] (+)= A[smem] * B[smem]^T with block scales from TMEM; K = 64 elements, issued by ONE thread.
-__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+// D[tmem of both CTAs] (+)= A[smem] * B[smem]^T with block scales from TMEM; K = 64 elements, issued by ONE thread.
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
                                           uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
     asm volatile(
         "{\n\t"
         ".reg .pred p;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
         "}"
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
         : "memory");
@@ -85,18 +88,14 @@ __host__ __device__ constexpr uint32_t umma_idesc_mxf4(int M, int N, uint32_t sf
            (static_cast<uint32_t>(M >> 7) << 27) | (sf << 29);
 }
 
-// 32 rows x 16 bytes of shared memory (512 contiguous bytes) to 4 TMEM columns of every lane quarter.
+// 32 rows x 16 bytes of shared memory (512 contiguous bytes) to 4 TMEM columns of every lane quarter, in both CTAs from
+// their own shared memory.
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
     uint64_t d = 0;
     d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
     d |= static_cast<uint64_t>(128 >> 4) << 32;          // 8-row groups are 128 bytes apart, no swizzle
     d |= static_cast<uint64_t>(1) << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
-
-__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
 __device__ __forceinline__ float activate(float v, int act) {
@@ -119,9 +118,11 @@ template <typename T> __device__ __forceinline__ void store_row32(T* dst, const 
 enum { OUT_F32 = ARISTOS_DTYPE_F32, OUT_BF16 = ARISTOS_DTYPE_BF16, OUT_F16 = ARISTOS_DTYPE_F16, OUT_FP4 = 5 };
 
 template <int OUT>
-__global__ void __launch_bounds__(F4_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F4_THREADS, 1)
 ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
-                            const __grid_constant__ CUtensorMap tmB1, const Fp4GemmParams p) {
+                            const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmSA,
+                            const __grid_constant__ CUtensorMap tmSB0, const __grid_constant__ CUtensorMap tmSB1,
+                            const Fp4GemmParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* aux = smem + F4_STAGES * F4_STAGE_BYTES;
@@ -131,16 +132,17 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     int* prefix = reinterpret_cast<int*>(aux + 256);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t bar_full = ptx::smem_u32(bars);
-    const uint32_t bar_empty = bar_full + 8 * F4_STAGES;
-    const uint32_t bar_tfull = bar_empty + 8 * F4_STAGES;
-    const uint32_t bar_tempty = bar_tfull + 16;
+    const uint32_t cta = ptx::cluster_ctarank();           // 0 = the CTA that issues the MMAs
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const uint32_t bar_full = ptx::smem_u32(bars);         // used in CTA 0 only
+    const uint32_t bar_empty = bar_full + 8 * F4_STAGES;   // one per CTA
+    const uint32_t bar_tfull = bar_empty + 8 * F4_STAGES;  // one per CTA
+    const uint32_t bar_tempty = bar_tfull + 16;            // used in CTA 0 only
     const uint32_t smem_base = ptx::smem_u32(smem);
 
     const int out_w = p.gated ? 128 : 256;
     const int n_tiles = (p.N + out_w - 1) / out_w;
     const int kblocks = (p.K + F4_KB - 1) / F4_KB;
-    const int ktiles = fp4_col_tiles(p.K);                 // scale tiles along K (128 elements each)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < F4_STAGES; ++s) {
@@ -148,7 +150,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             ptx::mbar_init(bar_empty + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) ptx::mbar_init(bar_tfull + 8 * b, 1);
-        ptx::mbar_init(bar_tempty, F4_EPI_WARPS);
+        ptx::mbar_init(bar_tempty, 2 * F4_EPI_WARPS);
         *abort_flag = 0;
         ptx::fence_mbar_init();
     }
@@ -161,7 +163,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             int v = 0;
             if (g < p.groups) {
                 const int rows = max(0, min(p.count[ordered_group(g, p.groups, p.experts)], p.rows_per_group));
-                v = ((rows + F4_BM - 1) / F4_BM) * n_tiles;
+                v = ((rows + F4_PM - 1) / F4_PM) * n_tiles;
             }
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -172,64 +174,67 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             running += __shfl_sync(0xffffffffu, v, 31);
         }
     } else if (warp == 1) {
-        ptx::tmem_alloc(ptx::smem_u32(tmem_slot), F4_TMEM_COLS);
+        ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), F4_TMEM_COLS);
     }
     ptx::tcgen05_fence_before();
     __syncthreads();
+    ptx::cluster_sync();               // both CTAs' barriers are initialised before anything signals them
     ptx::tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = prefix[p.groups];
 
     if (warp == 0) {
-        // ------------------------------------------------------------------ producer
+        // ------------------------------------------------------------------ TMA producer (both CTAs)
         if (ptx::elect_one()) {
             ptx::prefetch_tensormap(&tmA);
             ptx::prefetch_tensormap(&tmB0);
             ptx::prefetch_tensormap(&tmB1);
-            const int a_row_tiles = fp4_row_tiles(p.rows_per_group), b_row_tiles = fp4_row_tiles(p.N);
+            ptx::prefetch_tensormap(&tmSA);
+            ptx::prefetch_tensormap(&tmSB0);
+            ptx::prefetch_tensormap(&tmSB1);
+            const CUtensorMap* tmB = cta == 0 ? &tmB0 : &tmB1;
+            const uint32_t full0 = ptx::mapa_shared(bar_full, 0);
             int stage = 0;
             uint32_t phase = 0;
             int vg = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+            for (int tile = pair; ok && tile < total_tiles; tile += num_pairs) {
                 while (tile >= prefix[vg + 1]) ++vg;
                 const int g = ordered_group(vg, p.groups, p.experts);
                 const int local = tile - prefix[vg];
                 const int mt = (prefix[vg + 1] - prefix[vg]) / n_tiles;
-                const int m0 = (local % mt) * F4_BM;
+                const int m0 = (local % mt) * F4_PM + (int)cta * F4_BM;
                 const int n0 = (local / mt) * out_w;
                 const int e = g % p.experts;
-                const int n1 = p.gated ? n0 : n0 + 128;     // second 128-row box of B
-                const bool second = n1 < p.N;               // its scale tiles exist (its codes read as zeros otherwise)
-                const uint8_t* sfa = p.sa + ((size_t)g * a_row_tiles + m0 / 128) * ktiles * FP4_TILE_BYTES;
-                const uint8_t* sfb0 = p.sb0 + ((size_t)e * b_row_tiles + n0 / 128) * ktiles * FP4_TILE_BYTES;
-                const uint8_t* sfb1 = p.sb1 + ((size_t)e * b_row_tiles + n1 / 128) * ktiles * FP4_TILE_BYTES;
+                const int n1 = p.gated ? n0 : n0 + 128;     // first weight row of the second half of B
+                const int nb = cta == 0 ? n0 : n1;
                 for (int kb = 0; kb < kblocks; ++kb) {
                     ok = ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.dev_status);
                     if (!ok) break;
-                    const uint32_t full = bar_full + 8 * stage;
+                    const uint32_t full = full0 + 8 * stage;
                     const uint32_t sa = smem_base + stage * F4_STAGE_BYTES;
                     const uint32_t sf = sa + F4_A_BYTES + F4_B_BYTES;
-                    const uint32_t sf_bytes = min(2, ktiles - 2 * kb) * FP4_TILE_BYTES;
-                    const size_t sf_off = (size_t)kb * F4_SF_BYTES;
-                    ptx::mbar_arrive_expect_tx(full, F4_A_BYTES + F4_B_BYTES + (second ? 3 : 2) * sf_bytes);
-                    ptx::tma_load_3d(sa, &tmA, kb * (F4_KB / 2), m0, g, full);
-                    ptx::tma_load_3d(sa + F4_A_BYTES, &tmB0, kb * (F4_KB / 2), n0, e, full);
-                    ptx::tma_load_3d(sa + F4_A_BYTES + F4_B_BYTES / 2, &tmB1, kb * (F4_KB / 2), n1, e, full);
-                    bulk_load(sf, sfa + sf_off, sf_bytes, full);
-                    bulk_load(sf + F4_SF_BYTES, sfb0 + sf_off, sf_bytes, full);
-                    if (second) bulk_load(sf + 2 * F4_SF_BYTES, sfb1 + sf_off, sf_bytes, full);
+                    if (cta == 0) ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, 2 * F4_STAGE_BYTES);
+                    ptx::tma_load_3d_pair(sa, &tmA, kb * (F4_KB / 2), m0, g, full);
+                    ptx::tma_load_3d_pair(sa + F4_A_BYTES, tmB, kb * (F4_KB / 2), nb, e, full);
+                    // scale tiles as rows of 32-bit words: two tiles (256 elements of K) of a row of tiles. What lies
+                    // outside reads as zeros, or belongs to columns that are not stored.
+                    ptx::tma_load_3d_pair(sf, &tmSA, kb * (F4_SF_BYTES / 4), m0 / FP4_TILE_ROWS, g, full);
+                    ptx::tma_load_3d_pair(sf + F4_SF_BYTES, &tmSB0, kb * (F4_SF_BYTES / 4), n0 / FP4_TILE_ROWS, e, full);
+                    ptx::tma_load_3d_pair(sf + 2 * F4_SF_BYTES, &tmSB1, kb * (F4_SF_BYTES / 4), n1 / FP4_TILE_ROWS, e, full);
                     if (++stage == F4_STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ------------------------------------------------------------------ MMA issuer
-        if (ptx::elect_one()) {
+        // ------------------------------------------------------------------ MMA issuer (CTA 0 only)
+        if (cta == 0 && ptx::elect_one()) {
+            const uint32_t empty_peer = ptx::mapa_shared(bar_empty, 1);
+            const uint32_t tfull_peer = ptx::mapa_shared(bar_tfull, 1);
             int it = 0, t = 0;                             // stages and tiles issued so far
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x, ++t) {
+            for (int tile = pair; ok && tile < total_tiles; tile += num_pairs, ++t) {
                 const uint32_t tmem_d = tmem_base + (t & 1) * F4_ACC1;
                 if (t > 0) {
                     // the columns that this accumulator shares with the previous tile's have been read (and all of
@@ -266,27 +271,31 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
 #pragma unroll
                     for (int k = 0; k < 4; ++k)            // K = 64 elements = 32 bytes per instruction
                         if (k < steps)
-                            umma_mxf4(tmem_d, da + 2 * k, db + 2 * k, umma_idesc_mxf4(F4_BM, F4_BN, (k & 1) * 2),
+                            umma_mxf4_pair(tmem_d, da + 2 * k, db + 2 * k, umma_idesc_mxf4(F4_PM, F4_BN, (k & 1) * 2),
                                       tsf + 4 * (k >> 1), tsf + 8 + 8 * (k >> 1), (kb | k) != 0 ? 1u : 0u);
-                    ptx::umma_commit(bar_empty + 8 * stage);
+                    // release the stage in both CTAs
+                    ptx::umma_commit_pair(bar_empty + 8 * stage);
+                    ptx::umma_commit_pair(empty_peer + 8 * stage);
                 }
                 if (!ok) break;
-                ptx::umma_commit(bar_tfull + 8 * (t & 1));
+                ptx::umma_commit_pair(bar_tfull + 8 * (t & 1));
+                ptx::umma_commit_pair(tfull_peer + 8 * (t & 1));
             }
         }
         __syncwarp();
     } else {
-        // ------------------------------------------------------------------ epilogue
+        // ------------------------------------------------------------------ epilogue (both CTAs, their own rows)
+        const uint32_t tempty0 = ptx::mapa_shared(bar_tempty, 0);
         const int quarter = warp & 3;                       // TMEM lanes this warp may read
         const int sub = (warp - 2) >> 2;                    // 0 / 1: even or odd 32-column chunks
         const int row_in_tile = quarter * 32 + lane;
         int vg = 0, t = 0;
-        for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++t) {
+        for (int tile = pair; tile < total_tiles; tile += num_pairs, ++t) {
             while (tile >= prefix[vg + 1]) ++vg;
             const int g = ordered_group(vg, p.groups, p.experts);
             const int local = tile - prefix[vg];
             const int mt = (prefix[vg + 1] - prefix[vg]) / n_tiles;
-            const int m0 = (local % mt) * F4_BM;
+            const int m0 = (local % mt) * F4_PM + (int)cta * F4_BM;
             const int n0 = (local / mt) * out_w;
             const int row = m0 + row_in_tile;
             const bool row_ok = row < min(p.count[g], p.rows_per_group);
@@ -309,7 +318,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                 if (c == 0) {
                     ptx::tcgen05_fence_before();
                     __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(bar_tempty);
+                    if (lane == 0) ptx::mbar_arrive_cluster(tempty0);
                 }
                 if (!row_ok || n0 + col >= p.N) continue;
                 float v[32];
@@ -354,26 +363,66 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
 
     ptx::tcgen05_fence_before();
     __syncthreads();
+    ptx::cluster_sync();               // nobody leaves (or frees TMEM) while the other CTA may still signal it
     if (warp == 1) {
         ptx::tcgen05_fence_after();
-        ptx::tmem_dealloc(tmem_base, F4_TMEM_COLS);
+        ptx::tmem_dealloc_pair(tmem_base, F4_TMEM_COLS);
     }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
+// Scale tiles as (outer, row tiles, 32-bit words of a row of tiles), read two tiles at a time.
+aristos_status_t encode_scale_map(CUtensorMap* tm, const void* base, int K, int rows, int outer) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) { set_last_error("cuTensorMapEncodeTiled is not available from the driver"); return ARISTOS_ERR_CUDA; }
+    const cuuint64_t words = (cuuint64_t)fp4_col_tiles(K) * (FP4_TILE_BYTES / 4), tiles = (cuuint64_t)fp4_row_tiles(rows);
+    const cuuint64_t dims[3] = {words, tiles, (cuuint64_t)outer};
+    const cuuint64_t strides[2] = {words * 4, words * 4 * tiles};
+    const cuuint32_t box[3] = {F4_SF_BYTES / 4, 1, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_last_error("cuTensorMapEncodeTiled failed with %d (scales of K=%d rows=%d outer=%d)", (int)r, K, rows, outer);
+        return ARISTOS_ERR_CUDA;
+    }
+    return ARISTOS_OK;
+}
+
 aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, const Fp4GemmParams& p, int out,
                                  cudaStream_t st) {
     CUtensorMap tmA, tmB0, tmB1;
     ARISTOS_TRY(encode_map_3d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A, p.K / 2, p.rows_per_group, p.groups, 128));
     ARISTOS_TRY(encode_map_3d(&tmB0, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B0, p.K / 2, p.N, p.experts, 128));
     ARISTOS_TRY(encode_map_3d(&tmB1, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B1, p.K / 2, p.N, p.experts, 128));
+    CUtensorMap tmSA, tmSB0, tmSB1;
+    ARISTOS_TRY(encode_scale_map(&tmSA, p.sa, p.K, p.rows_per_group, p.groups));
+    ARISTOS_TRY(encode_scale_map(&tmSB0, p.sb0, p.K, p.N, p.experts));
+    ARISTOS_TRY(encode_scale_map(&tmSB1, p.sb1, p.K, p.N, p.experts));
     const int sms = device_sm_count();
     if (sms <= 0) { set_last_error("no CUDA device"); return ARISTOS_ERR_CUDA; }
-    const int64_t bound = (int64_t)p.groups * ceil_div(p.rows_per_group, F4_BM) * ceil_div(p.N, p.gated ? 128 : 256);
-    const int grid = (int)(bound < sms ? bound : sms);
+    const int64_t bound = (int64_t)p.groups * ceil_div(p.rows_per_group, F4_PM) * ceil_div(p.N, p.gated ? 128 : 256);
     auto run = [&](auto kernel) -> aristos_status_t {
         ARISTOS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F4_SMEM_BYTES));
-        kernel<<<grid, F4_THREADS, F4_SMEM_BYTES, st>>>(tmA, tmB0, tmB1, p);
+        // one pair per two SMs, as many as the device holds at once (not every SM has a partner in its cluster's reach)
+        static int most = 0;
+        if (most == 0) {
+            cudaLaunchConfig_t lc = {};
+            lc.gridDim = dim3(2 * (sms / 2));
+            lc.blockDim = dim3(F4_THREADS);
+            lc.dynamicSmemBytes = F4_SMEM_BYTES;
+            cudaLaunchAttribute at;
+            at.id = cudaLaunchAttributeClusterDimension;
+            at.val.clusterDim.x = 2; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+            lc.attrs = &at;
+            lc.numAttrs = 1;
+            int n = 0;
+            ARISTOS_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &lc));
+            most = n > 0 ? n : 1;
+        }
+        const int pairs = (int)(bound < most ? bound : most);
+        kernel<<<2 * pairs, F4_THREADS, F4_SMEM_BYTES, st>>>(tmA, tmB0, tmB1, tmSA, tmSB0, tmSB1, p);
         ARISTOS_COUNT_LAUNCH();
         ARISTOS_CUDA_TRY(cudaGetLastError());
         return ARISTOS_OK;
