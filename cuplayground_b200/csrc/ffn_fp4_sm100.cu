@@ -10,21 +10,22 @@
 //
 // Tile 256 x 256 per pair of CTAs (cta_group::2; SwiGLU: 128 gate and 128 up columns in one instruction), K in stages of
 // 256 elements = one 128-byte swizzled row. Each CTA loads its own 128 rows of A and one half of B, and the scales of its
-// rows and of all of B's: 35 KB, six stages. (A single CTA with all of B needs 51 KB and has room for four: the tensor
-// core then waits for TMA, 900 cycles per stage instead of the 512 that the instructions take.) Codes and scales come by
-// TMA; the scales lie in global memory in the very tiles that tcgen05.cp takes to TMEM. The issuing thread of the first
-// CTA copies a stage's scales to one of two TMEM buffers (in both CTAs) and issues up to four MMAs. Only whole 64-element
-// steps that exist are issued, so nothing of a row's padding is ever used.
+// rows and of all of B's: 35 KB, five stages. (A single CTA with all of B needs 51 KB and has room for four: the tensor
+// core then waits for TMA.) Codes and scales come by
+// TMA; the scales lie in global memory in the very tiles that tcgen05.cp takes to TMEM. Two threads of the first CTA issue:
+// one copies a stage's scales to one of four TMEM buffers (in both CTAs), the other the up to four MMAs (one thread needs
+// 670 cycles for both, longer than the tensor core computes). Only whole 64-element steps that exist are issued, so
+// nothing of a row's padding is ever used.
 //
 // TMEM holds 512 columns; two accumulators of 256 would leave none for the scales. They overlap instead: columns
-// [0, 256) and [192, 448), scales from 448. The epilogue reads the 64 shared columns of a finished tile first and then
-// lets the issuer start the next one, which fills the other buffer while the rest is drained.
+// [0, 256) and [128, 384), scales from 384. The epilogue reads the shared half of a finished tile first and then lets the
+// issuer start the next one, which fills the other buffer while the rest is worked on.
 //
-// Roles (320 threads per CTA): warp 0 TMA, warp 1 TMEM + MMA, warps 2-9 epilogue, two warps per lane quarter that take the
-// 32-column chunks in turn. Every wait is bounded.
+// Roles (352 threads per CTA): warp 0 TMA, warp 1 TMEM + MMA, warps 2-9 epilogue, two warps per lane quarter with half of
+// the columns each, warp 10 scales. Every wait is bounded.
 //
-// The up projection of the FFN writes its output as MXFP4 again: a thread holds 32 adjacent columns of its row, i.e. a
-// whole block, so scale and codes come out of its registers, rounded once from fp32. Only valid rows are written.
+// The up projection of the FFN writes its output as MXFP4 again: a thread holds 64 adjacent columns of its row, i.e. two
+// whole blocks, so scale and codes come out of its registers, rounded once from fp32. Only valid rows are written.
 #include <cuda.h>
 
 #include "common.cuh"
@@ -40,21 +41,25 @@ constexpr int F4_BM = 128;                               // rows per CTA
 constexpr int F4_PM = 256;                               // rows per pair
 constexpr int F4_BN = 256;
 constexpr int F4_KB = 256;                               // elements of K per stage: 128 bytes
-constexpr int F4_STAGES = 6;
+constexpr int F4_STAGES = 5;
 constexpr int F4_A_BYTES = F4_BM * F4_KB / 2;            // 16 KB
 constexpr int F4_B_BYTES = F4_BN / 2 * F4_KB / 2;        // 16 KB: this CTA's half of the weight rows
 constexpr int F4_SF_BYTES = 2 * FP4_TILE_BYTES;          // scales of 128 rows and one stage of K
 constexpr int F4_STAGE_BYTES = F4_A_BYTES + F4_B_BYTES + 3 * F4_SF_BYTES;
 static_assert(F4_STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
 constexpr int F4_EPI_WARPS = 8;
-constexpr int F4_THREADS = 32 * (2 + F4_EPI_WARPS);
+constexpr int F4_SCALE_WARP = 2 + F4_EPI_WARPS;
+constexpr int F4_THREADS = 32 * (3 + F4_EPI_WARPS);
 constexpr int F4_MAX_GROUPS = 1024;
 constexpr int F4_AUX_BYTES = (256 + (F4_MAX_GROUPS + 1) * 4 + 127) & ~127;
-constexpr int F4_SMEM_BYTES = 1024 + F4_STAGES * F4_STAGE_BYTES + F4_AUX_BYTES;
+constexpr int F4_OUT_BYTES = 32 * 128;                   // output staging of an epilogue warp: 32 rows x 128 bytes
+constexpr int F4_SMEM_BYTES = 1024 + F4_STAGES * F4_STAGE_BYTES + F4_EPI_WARPS * F4_OUT_BYTES + F4_AUX_BYTES;
 static_assert(F4_SMEM_BYTES <= 227 * 1024, "fp4 GEMM: shared memory");
 constexpr int F4_TMEM_COLS = 512;
-constexpr int F4_ACC1 = 192;                             // first column of the second accumulator
-constexpr int F4_SF_COL = 448, F4_SF_COLS = 32;          // two scale buffers: A 2 x 4 columns, B 2 x 8 columns
+constexpr int F4_ACC1 = 128;                             // first column of the second accumulator
+constexpr int F4_SF_BUFS = 4;                            // scale buffers: A 2 x 4 columns, B 2 x 8 columns, of 32 each
+constexpr int F4_SF_COL = 384, F4_SF_COLS = 32;
+static_assert(F4_ACC1 + F4_BN <= F4_SF_COL && F4_SF_COL + F4_SF_BUFS * F4_SF_COLS <= F4_TMEM_COLS, "TMEM columns");
 
 struct Fp4GemmParams {
     const int32_t* count;
@@ -98,24 +103,98 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_a
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
+// Arrive on the barrier at this offset in both CTAs of the pair when the MMAs issued so far have completed.
+__device__ __forceinline__ void umma_commit_both(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == ARISTOS_ACT_RELU) return act_relu(v);
     if (act == ARISTOS_ACT_GELU) return act_gelu(v);
     return v;
 }
 
-// 32 fp32 values of one row to memory.
-template <typename T> __device__ __forceinline__ void store_row32(T* dst, const float (&v)[32]) {
+enum { OUT_F32 = ARISTOS_DTYPE_F32, OUT_BF16 = ARISTOS_DTYPE_BF16, OUT_F16 = ARISTOS_DTYPE_F16, OUT_FP4 = 5 };
+
+// 32 adjacent columns of one row as one block of MXFP4: codes, and the scale byte.
+__device__ __forceinline__ uint32_t quantize_block(const float (&v)[32], uint32_t (&w)[4]) {
+    float m = 0.0f;                                     // the bits of |NaN| are above infinity's: NaN is kept
+#pragma unroll
+    for (int i = 0; i < 32; ++i) m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(v[i]) & 0x7FFFFFFFu));
+    const uint32_t s = fp4_scale_of(m);
+    const float inv = fp4_inverse_scale(s);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float w[8];
+        w[i] = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = v[8 * i + j];
-        store8(dst + 8 * i, w);
+        for (int q = 0; q < 4; ++q) w[i] |= fp4_pack2(v[8 * i + 2 * q] * inv, v[8 * i + 2 * q + 1] * inv) << (8 * q);
+        if (s == 255u) w[i] = 0;
     }
+    return s;
 }
 
-enum { OUT_F32 = ARISTOS_DTYPE_F32, OUT_BF16 = ARISTOS_DTYPE_BF16, OUT_F16 = ARISTOS_DTYPE_F16, OUT_FP4 = 5 };
+// A warp's 32 rows of UNITS 16-byte units each (w: this lane's row) to memory, through its staging area, so that a store
+// instruction writes whole lines instead of 32 separate pieces (those took longer than the tensor core's work on a tile).
+// Rows from `valid` on are left out. dst: row 0, `pitch` bytes between rows.
+template <int UNITS>
+__device__ __forceinline__ void store_rows(uint32_t stage, int lane, const uint32_t (&w)[4 * UNITS], uint8_t* dst, size_t pitch,
+                                           int valid) {
+    // unit u of row r lies at unit u ^ (r % 8) of 8 (UNITS 8), u ^ (r / 4 % 2) of 2 (UNITS 2): no bank conflicts either way
+    auto place = [&](int r, int u) { return stage + r * (16 * UNITS) + ((u ^ (UNITS == 8 ? r & 7 : (r >> 2) & 1)) << 4); };
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) ptx::st_shared_v4(place(lane, u), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+    __syncwarp();
+    const int u = lane % UNITS;
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+        const int r = i * (32 / UNITS) + lane / UNITS;
+        const uint4 v = ptx::ld_shared_v4(place(r, u));
+        if (r < valid) *reinterpret_cast<uint4*>(dst + r * pitch + u * 16) = v;
+    }
+    __syncwarp();
+}
+
+// 64 adjacent columns of a warp's 32 rows to the output; v: this lane's row.
+template <int OUT>
+__device__ __forceinline__ void store_columns(const Fp4GemmParams& p, uint32_t stage, int lane, int g, int row0, int valid, int col,
+                                              const float (&v)[2][32]) {
+    if (col >= p.N) return;
+    const size_t grow = (size_t)g * p.rows_per_group + row0;
+    if constexpr (OUT == OUT_FP4) {
+        uint32_t w[8], lo[4], hi[4];
+        const uint32_t s = quantize_block(v[0], lo) | quantize_block(v[1], hi) << 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { w[i] = lo[i]; w[4 + i] = hi[i]; }
+        store_rows<2>(stage, lane, w, static_cast<uint8_t*>(p.out) + grow * (p.N / 2) + col / 2, p.N / 2, valid);
+        const size_t tile_at = ((size_t)g * fp4_row_tiles(p.rows_per_group) + row0 / 128) * fp4_col_tiles(p.N) + col / 128;
+        if (lane < valid)
+            *reinterpret_cast<uint16_t*>(p.out_scales + tile_at * FP4_TILE_BYTES + fp4_tile_word(row0 + lane) + (col / 32) % 4) = (uint16_t)s;
+    } else if constexpr (OUT == OUT_F32) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[c][i]);
+            store_rows<8>(stage, lane, w, static_cast<uint8_t*>(p.out) + (grow * p.N + col + 32 * c) * 4, (size_t)p.N * 4, valid);
+        }
+    } else {
+        uint32_t w[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if constexpr (OUT == OUT_BF16) {
+                    const __nv_bfloat162 t = __floats2bfloat162_rn(v[c][2 * i], v[c][2 * i + 1]);
+                    w[16 * c + i] = *reinterpret_cast<const uint32_t*>(&t);
+                } else {
+                    const __half2 t = __floats2half2_rn(v[c][2 * i], v[c][2 * i + 1]);
+                    w[16 * c + i] = *reinterpret_cast<const uint32_t*>(&t);
+                }
+            }
+        store_rows<8>(stage, lane, w, static_cast<uint8_t*>(p.out) + (grow * p.N + col) * 2, (size_t)p.N * 2, valid);
+    }
+}
 
 template <int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F4_THREADS, 1)
@@ -125,8 +204,8 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                             const Fp4GemmParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* aux = smem + F4_STAGES * F4_STAGE_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(aux);     // full[S], empty[S], tfull[2], tempty
+    uint8_t* aux = smem + F4_STAGES * F4_STAGE_BYTES + F4_EPI_WARPS * F4_OUT_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(aux);     // full[S], empty[S], tfull[2], tempty, scales[4]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 192);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(aux + 196);
     int* prefix = reinterpret_cast<int*>(aux + 256);
@@ -138,6 +217,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     const uint32_t bar_empty = bar_full + 8 * F4_STAGES;   // one per CTA
     const uint32_t bar_tfull = bar_empty + 8 * F4_STAGES;  // one per CTA
     const uint32_t bar_tempty = bar_tfull + 16;            // used in CTA 0 only
+    const uint32_t bar_scales = bar_tempty + 8;            // used in CTA 0 only
     const uint32_t smem_base = ptx::smem_u32(smem);
 
     const int out_w = p.gated ? 128 : 256;
@@ -151,6 +231,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
         }
         for (int b = 0; b < 2; ++b) ptx::mbar_init(bar_tfull + 8 * b, 1);
         ptx::mbar_init(bar_tempty, 2 * F4_EPI_WARPS);
+        for (int b = 0; b < F4_SF_BUFS; ++b) ptx::mbar_init(bar_scales + 8 * b, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
     }
@@ -230,8 +311,6 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer (CTA 0 only)
         if (cta == 0 && ptx::elect_one()) {
-            const uint32_t empty_peer = ptx::mapa_shared(bar_empty, 1);
-            const uint32_t tfull_peer = ptx::mapa_shared(bar_tfull, 1);
             int it = 0, t = 0;                             // stages and tiles issued so far
             bool ok = true;
             for (int tile = pair; ok && tile < total_tiles; tile += num_pairs, ++t) {
@@ -244,19 +323,48 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                     ptx::tcgen05_fence_after();
                 }
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    const int stage = it % F4_STAGES;
+                    const int stage = it % F4_STAGES, buf = it % F4_SF_BUFS;
+                    ok = ptx::mbar_wait_bounded(bar_scales + 8 * buf, (it / F4_SF_BUFS) & 1, abort_flag, p.dev_status) &&
+                         ptx::mbar_wait_bounded(bar_full + 8 * stage, (it / F4_STAGES) & 1, abort_flag, p.dev_status);
+                    if (!ok) break;
+                    ptx::tcgen05_fence_after();
+                    const uint32_t sa = smem_base + stage * F4_STAGE_BYTES;
+                    const uint32_t tsf = tmem_base + F4_SF_COL + buf * F4_SF_COLS;
+                    const int steps = min(4, (p.K - kb * F4_KB) / 64);
+                    const uint64_t da = ptx::umma_desc_k_sw128(sa);
+                    const uint64_t db = ptx::umma_desc_k_sw128(sa + F4_A_BYTES);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)            // K = 64 elements = 32 bytes per instruction
+                        if (k < steps)
+                            umma_mxf4_pair(tmem_d, da + 2 * k, db + 2 * k, umma_idesc_mxf4(F4_PM, F4_BN, (k & 1) * 2),
+                                           tsf + 4 * (k >> 1), tsf + 8 + 8 * (k >> 1), (kb | k) != 0 ? 1u : 0u);
+                    umma_commit_both(bar_empty + 8 * stage);   // release the stage in both CTAs
+                }
+                if (!ok) break;
+                umma_commit_both(bar_tfull + 8 * (t & 1));
+            }
+        }
+        __syncwarp();
+    } else if (warp == F4_SCALE_WARP) {
+        // ------------------------------------------------------------------ scales to TMEM (CTA 0 only)
+        if (cta == 0 && ptx::elect_one()) {
+            int it = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < total_tiles; tile += num_pairs) {
+                for (int kb = 0; kb < kblocks; ++kb, ++it) {
+                    const int stage = it % F4_STAGES, buf = it % F4_SF_BUFS;
                     ok = ptx::mbar_wait_bounded(bar_full + 8 * stage, (it / F4_STAGES) & 1, abort_flag, p.dev_status);
                     if (!ok) break;
-                    // the scale buffer of this stage was read by the MMAs of two stages ago
-                    if (it >= 2) {
-                        ok = ptx::mbar_wait_bounded(bar_empty + 8 * ((it - 2) % F4_STAGES), ((it - 2) / F4_STAGES) & 1,
-                                                    abort_flag, p.dev_status);
+                    // the buffer was read by the MMAs of four stages ago
+                    if (it >= F4_SF_BUFS) {
+                        const int old = it - F4_SF_BUFS;
+                        ok = ptx::mbar_wait_bounded(bar_empty + 8 * (old % F4_STAGES), (old / F4_STAGES) & 1, abort_flag,
+                                                    p.dev_status);
                         if (!ok) break;
                     }
                     ptx::tcgen05_fence_after();
-                    const uint32_t sa = smem_base + stage * F4_STAGE_BYTES;
-                    const uint32_t sf = sa + F4_A_BYTES + F4_B_BYTES;
-                    const uint32_t tsf = tmem_base + F4_SF_COL + (it & 1) * F4_SF_COLS;
+                    const uint32_t sf = smem_base + stage * F4_STAGE_BYTES + F4_A_BYTES + F4_B_BYTES;
+                    const uint32_t tsf = tmem_base + F4_SF_COL + buf * F4_SF_COLS;
                     const int steps = min(4, (p.K - kb * F4_KB) / 64);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -266,20 +374,8 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                             tmem_copy_scales(tsf + 8 + 8 * h + 4, sf + 2 * F4_SF_BYTES + h * FP4_TILE_BYTES);
                         }
                     }
-                    const uint64_t da = ptx::umma_desc_k_sw128(sa);
-                    const uint64_t db = ptx::umma_desc_k_sw128(sa + F4_A_BYTES);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)            // K = 64 elements = 32 bytes per instruction
-                        if (k < steps)
-                            umma_mxf4_pair(tmem_d, da + 2 * k, db + 2 * k, umma_idesc_mxf4(F4_PM, F4_BN, (k & 1) * 2),
-                                      tsf + 4 * (k >> 1), tsf + 8 + 8 * (k >> 1), (kb | k) != 0 ? 1u : 0u);
-                    // release the stage in both CTAs
-                    ptx::umma_commit_pair(bar_empty + 8 * stage);
-                    ptx::umma_commit_pair(empty_peer + 8 * stage);
+                    ptx::umma_commit_pair(bar_scales + 8 * buf);
                 }
-                if (!ok) break;
-                ptx::umma_commit_pair(bar_tfull + 8 * (t & 1));
-                ptx::umma_commit_pair(tfull_peer + 8 * (t & 1));
             }
         }
         __syncwarp();
@@ -287,8 +383,8 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
         // ------------------------------------------------------------------ epilogue (both CTAs, their own rows)
         const uint32_t tempty0 = ptx::mapa_shared(bar_tempty, 0);
         const int quarter = warp & 3;                       // TMEM lanes this warp may read
-        const int sub = (warp - 2) >> 2;                    // 0 / 1: even or odd 32-column chunks
-        const int row_in_tile = quarter * 32 + lane;
+        const int sub = (warp - 2) >> 2;                    // 0 / 1: lower or upper 64 columns of either half of the tile
+        const uint32_t stage = smem_base + F4_STAGES * F4_STAGE_BYTES + (warp - 2) * F4_OUT_BYTES;
         int vg = 0, t = 0;
         for (int tile = pair; tile < total_tiles; tile += num_pairs, ++t) {
             while (tile >= prefix[vg + 1]) ++vg;
@@ -297,66 +393,51 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             const int mt = (prefix[vg + 1] - prefix[vg]) / n_tiles;
             const int m0 = (local % mt) * F4_PM + (int)cta * F4_BM;
             const int n0 = (local / mt) * out_w;
-            const int row = m0 + row_in_tile;
-            const bool row_ok = row < min(p.count[g], p.rows_per_group);
-            const size_t grow = (size_t)g * p.rows_per_group + row;
+            const int row0 = m0 + quarter * 32;
+            const int valid = min(p.count[g], p.rows_per_group) - row0;   // of this warp's 32 rows
             bool ok = ptx::mbar_wait_bounded(bar_tfull + 8 * (t & 1), (t >> 1) & 1, abort_flag, p.dev_status);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             ptx::tcgen05_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (t & 1) * F4_ACC1;
-            const int chunks = p.gated ? 2 : 4;             // of this warp: sub, sub + 2, ...
-            for (int c = 0; c < chunks; ++c) {
-                // first the chunk whose columns the next tile needs: the last one in the first accumulator (columns
-                // 192-255; SwiGLU: with its gate columns), the first one in the second
-                const int j = (t & 1) ? c : (c == 0 ? chunks - 1 : c - 1);
-                const int col = (sub + 2 * j) * 32;
-                uint32_t a[32], b[32];
-                ptx::tmem_ld_32x32b_x32(taddr + col, a);
-                if (p.gated) ptx::tmem_ld_32x32b_x32(taddr + 128 + col, b);
+            // First the half of the columns that the next tile's accumulator shares: the upper one of the first accumulator,
+            // the lower one of the second. A warp has 64 columns of either half; SwiGLU: gate columns in the lower half,
+            // up columns in the upper.
+            const int half0 = (t & 1) ? 0 : 1;
+            uint32_t a[2][32], b[2][32];
+            float v[2][32];
+            ptx::tmem_ld_32x32b_x32(taddr + half0 * 128 + sub * 64, a[0]);
+            ptx::tmem_ld_32x32b_x32(taddr + half0 * 128 + sub * 64 + 32, a[1]);
+            ptx::tmem_ld_wait();
+            ptx::tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster(tempty0);
+            if (p.gated) {
+                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64, b[0]);
+                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64 + 32, b[1]);
                 ptx::tmem_ld_wait();
-                if (c == 0) {
-                    ptx::tcgen05_fence_before();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive_cluster(tempty0);
-                }
-                if (!row_ok || n0 + col >= p.N) continue;
-                float v[32];
-                if (p.gated) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = act_silu(__uint_as_float(a[i])) * __uint_as_float(b[i]);
-                } else {
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = activate(__uint_as_float(a[i]), p.act);
-                }
-                if constexpr (OUT == OUT_FP4) {
-                    float m = 0.0f;                         // the bits of |NaN| are above infinity's: NaN is kept
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(v[i]) & 0x7FFFFFFFu));
-                    const uint32_t s = fp4_scale_of(m);
-                    const float inv = fp4_inverse_scale(s);
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        w[i] = 0;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            w[i] |= fp4_pack2(v[8 * i + 2 * q] * inv, v[8 * i + 2 * q + 1] * inv) << (8 * q);
-                        if (s == 255u) w[i] = 0;
+                    for (int i = 0; i < 32; ++i) {
+                        const float gate = __uint_as_float(half0 == 0 ? a[c][i] : b[c][i]);
+                        v[c][i] = act_silu(gate) * __uint_as_float(half0 == 0 ? b[c][i] : a[c][i]);
                     }
-                    uint8_t* codes = static_cast<uint8_t*>(p.out) + grow * (p.N / 2) + (n0 + col) / 2;
-                    *reinterpret_cast<uint4*>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
-                    const size_t tile_at = ((size_t)g * fp4_row_tiles(p.rows_per_group) + row / 128) * fp4_col_tiles(p.N) +
-                                           (n0 + col) / 128;
-                    p.out_scales[tile_at * FP4_TILE_BYTES + fp4_tile_word(row) + (col / 32) % 4] = (uint8_t)s;
-                } else if constexpr (OUT == OUT_F32) {
-                    store_row32(static_cast<float*>(p.out) + grow * p.N + n0 + col, v);
-                } else if constexpr (OUT == OUT_BF16) {
-                    store_row32(static_cast<__nv_bfloat16*>(p.out) + grow * p.N + n0 + col, v);
-                } else {
-                    store_row32(static_cast<__half*>(p.out) + grow * p.N + n0 + col, v);
-                }
+                store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + sub * 64, v);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[c][i] = activate(__uint_as_float(a[c][i]), p.act);
+                store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + half0 * 128 + sub * 64, v);
+                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64, b[0]);
+                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64 + 32, b[1]);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[c][i] = activate(__uint_as_float(b[c][i]), p.act);
+                store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + (half0 ^ 1) * 128 + sub * 64, v);
             }
         }
     }
