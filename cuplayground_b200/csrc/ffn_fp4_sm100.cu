@@ -9,20 +9,20 @@
 // the epilogue.
 //
 // Tile 256 x 256 per pair of CTAs (cta_group::2; SwiGLU: 128 gate and 128 up columns in one instruction), K in stages of
-// 256 elements = one 128-byte swizzled row. Each CTA loads its own 128 rows of A and one half of B, and the scales of its
-// rows and of all of B's: 35 KB, five stages. (A single CTA with all of B needs 51 KB and has room for four: the tensor
-// core then waits for TMA.) Codes and scales come by
-// TMA; the scales lie in global memory in the very tiles that tcgen05.cp takes to TMEM. Two threads of the first CTA issue:
-// one copies a stage's scales to one of four TMEM buffers (in both CTAs), the other the up to four MMAs (one thread needs
-// 670 cycles for both, longer than the tensor core computes). Only whole 64-element steps that exist are issued, so
-// nothing of a row's padding is ever used.
+// 256 elements = one 128-byte swizzled row. Each CTA loads its own 128 rows of A and one half of B, 32 KB, in five stages.
+// (A single CTA with all of B needs 48 KB and has room for four: the tensor core then waits for TMA.) The scales of its rows
+// and of all of B's, 3 KB a stage, take a ring of their own and run ahead: they lie in global memory in the very tiles that
+// tcgen05.cp takes to TMEM, and one thread of the first CTA copies them there, to one of four buffers in both CTAs, while
+// another one issues the up to four MMAs of a stage. (With the scales in the stage, copying them lies between the arrival
+// of a stage and its MMAs, and five stages do not cover that.) Only whole 64-element steps that exist are issued, so nothing
+// of a row's padding is ever used.
 //
 // TMEM holds 512 columns; two accumulators of 256 would leave none for the scales. They overlap instead: columns
 // [0, 256) and [128, 384), scales from 384. The epilogue reads the shared half of a finished tile first and then lets the
 // issuer start the next one, which fills the other buffer while the rest is worked on.
 //
-// Roles (352 threads per CTA): warp 0 TMA, warp 1 TMEM + MMA, warps 2-9 epilogue, two warps per lane quarter with half of
-// the columns each, warp 10 scales. Every wait is bounded.
+// Roles (384 threads per CTA): warp 0 TMA, warp 1 TMEM + MMA, warps 2-9 epilogue, two warps per lane quarter with half of
+// the columns each, warp 10 TMA of the scales, warp 11 scales to TMEM. Every wait is bounded.
 //
 // The up projection of the FFN writes its output as MXFP4 again: a thread holds 64 adjacent columns of its row, i.e. two
 // whole blocks, so scale and codes come out of its registers, rounded once from fp32. Only valid rows are written.
@@ -45,15 +45,18 @@ constexpr int F4_STAGES = 5;
 constexpr int F4_A_BYTES = F4_BM * F4_KB / 2;            // 16 KB
 constexpr int F4_B_BYTES = F4_BN / 2 * F4_KB / 2;        // 16 KB: this CTA's half of the weight rows
 constexpr int F4_SF_BYTES = 2 * FP4_TILE_BYTES;          // scales of 128 rows and one stage of K
-constexpr int F4_STAGE_BYTES = F4_A_BYTES + F4_B_BYTES + 3 * F4_SF_BYTES;
+constexpr int F4_STAGE_BYTES = F4_A_BYTES + F4_B_BYTES;
+constexpr int F4_SF_STAGES = 8;
+constexpr int F4_SF_STAGE_BYTES = 3 * F4_SF_BYTES;       // of A's rows, of B's first and second 128 rows
 static_assert(F4_STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
 constexpr int F4_EPI_WARPS = 8;
-constexpr int F4_SCALE_WARP = 2 + F4_EPI_WARPS;
-constexpr int F4_THREADS = 32 * (3 + F4_EPI_WARPS);
+constexpr int F4_SF_LOAD_WARP = 2 + F4_EPI_WARPS, F4_SF_COPY_WARP = 3 + F4_EPI_WARPS;
+constexpr int F4_THREADS = 32 * (4 + F4_EPI_WARPS);
 constexpr int F4_MAX_GROUPS = 1024;
-constexpr int F4_AUX_BYTES = (256 + (F4_MAX_GROUPS + 1) * 4 + 127) & ~127;
+constexpr int F4_AUX_BYTES = (512 + (F4_MAX_GROUPS + 1) * 4 + 127) & ~127;
 constexpr int F4_OUT_BYTES = 32 * 128;                   // output staging of an epilogue warp: 32 rows x 128 bytes
-constexpr int F4_SMEM_BYTES = 1024 + F4_STAGES * F4_STAGE_BYTES + F4_EPI_WARPS * F4_OUT_BYTES + F4_AUX_BYTES;
+constexpr int F4_SMEM_BYTES = 1024 + F4_STAGES * F4_STAGE_BYTES + F4_SF_STAGES * F4_SF_STAGE_BYTES +
+                              F4_EPI_WARPS * F4_OUT_BYTES + F4_AUX_BYTES;
 static_assert(F4_SMEM_BYTES <= 227 * 1024, "fp4 GEMM: shared memory");
 constexpr int F4_TMEM_COLS = 512;
 constexpr int F4_ACC1 = 128;                             // first column of the second accumulator
@@ -109,9 +112,29 @@ __device__ __forceinline__ void umma_commit_both(uint32_t bar) {
                  ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 
+// v * Phi(v) = v / 2 * erfc(-v / sqrt 2), with erfc by the Chebyshev fit of Numerical Recipes (routine erfcc, section 6.2;
+// fractional error below 1.2e-7): erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), z >= 0, and 2 - erfc(-z) for z < 0.
+// Half the instructions of the library's erff, which would take longer than the tensor cores' work on a tile of K = 2048.
+__device__ __forceinline__ float gelu_erfc(float v) {
+    const float z = fabsf(v) * 0.70710678f;
+    const float t = __fdividef(1.0f, fmaf(0.5f, z, 1.0f));
+    float q = 0.17087277f;
+    q = fmaf(q, t, -0.82215223f);
+    q = fmaf(q, t, 1.48851587f);
+    q = fmaf(q, t, -1.13520398f);
+    q = fmaf(q, t, 0.27886807f);
+    q = fmaf(q, t, -0.18628806f);
+    q = fmaf(q, t, 0.09678418f);
+    q = fmaf(q, t, 0.37409196f);
+    q = fmaf(q, t, 1.00002368f);
+    q = fmaf(q, t, -1.26551223f);
+    const float e = t * __expf(fmaf(-0.5f * v, v, q));
+    return 0.5f * v * (v < 0.0f ? e : 2.0f - e);
+}
+
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == ARISTOS_ACT_RELU) return act_relu(v);
-    if (act == ARISTOS_ACT_GELU) return act_gelu(v);
+    if (act == ARISTOS_ACT_GELU) return gelu_erfc(v);
     return v;
 }
 
@@ -204,11 +227,11 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                             const Fp4GemmParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* aux = smem + F4_STAGES * F4_STAGE_BYTES + F4_EPI_WARPS * F4_OUT_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(aux);     // full[S], empty[S], tfull[2], tempty, scales[4]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 192);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(aux + 196);
-    int* prefix = reinterpret_cast<int*>(aux + 256);
+    uint8_t* aux = smem + F4_STAGES * F4_STAGE_BYTES + F4_SF_STAGES * F4_SF_STAGE_BYTES + F4_EPI_WARPS * F4_OUT_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(aux);     // full[S], empty[S], tfull[2], tempty, scales[4], sfull[8], sempty[8]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 384);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(aux + 388);
+    int* prefix = reinterpret_cast<int*>(aux + 512);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cta = ptx::cluster_ctarank();           // 0 = the CTA that issues the MMAs
@@ -217,8 +240,12 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     const uint32_t bar_empty = bar_full + 8 * F4_STAGES;   // one per CTA
     const uint32_t bar_tfull = bar_empty + 8 * F4_STAGES;  // one per CTA
     const uint32_t bar_tempty = bar_tfull + 16;            // used in CTA 0 only
-    const uint32_t bar_scales = bar_tempty + 8;            // used in CTA 0 only
+    const uint32_t bar_scales = bar_tempty + 8;            // used in CTA 0 only: a stage's scales are in TMEM
+    const uint32_t bar_sfull = bar_scales + 8 * F4_SF_BUFS;        // used in CTA 0 only
+    const uint32_t bar_sempty = bar_sfull + 8 * F4_SF_STAGES;      // one per CTA
+    static_assert(8 * (2 * F4_STAGES + 3 + F4_SF_BUFS + 2 * F4_SF_STAGES) <= 384, "barriers");
     const uint32_t smem_base = ptx::smem_u32(smem);
+    const uint32_t smem_sf = smem_base + F4_STAGES * F4_STAGE_BYTES;
 
     const int out_w = p.gated ? 128 : 256;
     const int n_tiles = (p.N + out_w - 1) / out_w;
@@ -232,6 +259,10 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
         for (int b = 0; b < 2; ++b) ptx::mbar_init(bar_tfull + 8 * b, 1);
         ptx::mbar_init(bar_tempty, 2 * F4_EPI_WARPS);
         for (int b = 0; b < F4_SF_BUFS; ++b) ptx::mbar_init(bar_scales + 8 * b, 1);
+        for (int s = 0; s < F4_SF_STAGES; ++s) {
+            ptx::mbar_init(bar_sfull + 8 * s, 1);
+            ptx::mbar_init(bar_sempty + 8 * s, 1);
+        }
         *abort_flag = 0;
         ptx::fence_mbar_init();
     }
@@ -270,9 +301,6 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             ptx::prefetch_tensormap(&tmA);
             ptx::prefetch_tensormap(&tmB0);
             ptx::prefetch_tensormap(&tmB1);
-            ptx::prefetch_tensormap(&tmSA);
-            ptx::prefetch_tensormap(&tmSB0);
-            ptx::prefetch_tensormap(&tmSB1);
             const CUtensorMap* tmB = cta == 0 ? &tmB0 : &tmB1;
             const uint32_t full0 = ptx::mapa_shared(bar_full, 0);
             int stage = 0;
@@ -287,22 +315,15 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                 const int m0 = (local % mt) * F4_PM + (int)cta * F4_BM;
                 const int n0 = (local / mt) * out_w;
                 const int e = g % p.experts;
-                const int n1 = p.gated ? n0 : n0 + 128;     // first weight row of the second half of B
-                const int nb = cta == 0 ? n0 : n1;
+                const int nb = cta == 0 || p.gated ? n0 : n0 + 128;     // this CTA's half of B
                 for (int kb = 0; kb < kblocks; ++kb) {
                     ok = ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.dev_status);
                     if (!ok) break;
                     const uint32_t full = full0 + 8 * stage;
                     const uint32_t sa = smem_base + stage * F4_STAGE_BYTES;
-                    const uint32_t sf = sa + F4_A_BYTES + F4_B_BYTES;
                     if (cta == 0) ptx::mbar_arrive_expect_tx(bar_full + 8 * stage, 2 * F4_STAGE_BYTES);
                     ptx::tma_load_3d_pair(sa, &tmA, kb * (F4_KB / 2), m0, g, full);
                     ptx::tma_load_3d_pair(sa + F4_A_BYTES, tmB, kb * (F4_KB / 2), nb, e, full);
-                    // scale tiles as rows of 32-bit words: two tiles (256 elements of K) of a row of tiles. What lies
-                    // outside reads as zeros, or belongs to columns that are not stored.
-                    ptx::tma_load_3d_pair(sf, &tmSA, kb * (F4_SF_BYTES / 4), m0 / FP4_TILE_ROWS, g, full);
-                    ptx::tma_load_3d_pair(sf + F4_SF_BYTES, &tmSB0, kb * (F4_SF_BYTES / 4), n0 / FP4_TILE_ROWS, e, full);
-                    ptx::tma_load_3d_pair(sf + 2 * F4_SF_BYTES, &tmSB1, kb * (F4_SF_BYTES / 4), n1 / FP4_TILE_ROWS, e, full);
                     if (++stage == F4_STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -345,15 +366,51 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             }
         }
         __syncwarp();
-    } else if (warp == F4_SCALE_WARP) {
+    } else if (warp == F4_SF_LOAD_WARP) {
+        // ------------------------------------------------------------------ TMA of the scales (both CTAs)
+        if (ptx::elect_one()) {
+            ptx::prefetch_tensormap(&tmSA);
+            ptx::prefetch_tensormap(&tmSB0);
+            ptx::prefetch_tensormap(&tmSB1);
+            const uint32_t sfull0 = ptx::mapa_shared(bar_sfull, 0);
+            int stage = 0;
+            uint32_t phase = 0;
+            int vg = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < total_tiles; tile += num_pairs) {
+                while (tile >= prefix[vg + 1]) ++vg;
+                const int g = ordered_group(vg, p.groups, p.experts);
+                const int local = tile - prefix[vg];
+                const int mt = (prefix[vg + 1] - prefix[vg]) / n_tiles;
+                const int m0 = (local % mt) * F4_PM + (int)cta * F4_BM;
+                const int n0 = (local / mt) * out_w;
+                const int e = g % p.experts;
+                const int n1 = p.gated ? n0 : n0 + 128;     // first weight row of the second half of B
+                for (int kb = 0; kb < kblocks; ++kb) {
+                    ok = ptx::mbar_wait_bounded(bar_sempty + 8 * stage, phase ^ 1u, abort_flag, p.dev_status);
+                    if (!ok) break;
+                    const uint32_t full = sfull0 + 8 * stage;
+                    const uint32_t sf = smem_sf + stage * F4_SF_STAGE_BYTES;
+                    // scale tiles as rows of 32-bit words: two tiles (256 elements of K) of a row of tiles. What lies
+                    // outside reads as zeros, or belongs to columns that are not stored.
+                    if (cta == 0) ptx::mbar_arrive_expect_tx(bar_sfull + 8 * stage, 2 * F4_SF_STAGE_BYTES);
+                    ptx::tma_load_3d_pair(sf, &tmSA, kb * (F4_SF_BYTES / 4), m0 / FP4_TILE_ROWS, g, full);
+                    ptx::tma_load_3d_pair(sf + F4_SF_BYTES, &tmSB0, kb * (F4_SF_BYTES / 4), n0 / FP4_TILE_ROWS, e, full);
+                    ptx::tma_load_3d_pair(sf + 2 * F4_SF_BYTES, &tmSB1, kb * (F4_SF_BYTES / 4), n1 / FP4_TILE_ROWS, e, full);
+                    if (++stage == F4_SF_STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == F4_SF_COPY_WARP) {
         // ------------------------------------------------------------------ scales to TMEM (CTA 0 only)
         if (cta == 0 && ptx::elect_one()) {
             int it = 0;
             bool ok = true;
             for (int tile = pair; ok && tile < total_tiles; tile += num_pairs) {
                 for (int kb = 0; kb < kblocks; ++kb, ++it) {
-                    const int stage = it % F4_STAGES, buf = it % F4_SF_BUFS;
-                    ok = ptx::mbar_wait_bounded(bar_full + 8 * stage, (it / F4_STAGES) & 1, abort_flag, p.dev_status);
+                    const int stage = it % F4_SF_STAGES, buf = it % F4_SF_BUFS;
+                    ok = ptx::mbar_wait_bounded(bar_sfull + 8 * stage, (it / F4_SF_STAGES) & 1, abort_flag, p.dev_status);
                     if (!ok) break;
                     // the buffer was read by the MMAs of four stages ago
                     if (it >= F4_SF_BUFS) {
@@ -363,7 +420,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                         if (!ok) break;
                     }
                     ptx::tcgen05_fence_after();
-                    const uint32_t sf = smem_base + stage * F4_STAGE_BYTES + F4_A_BYTES + F4_B_BYTES;
+                    const uint32_t sf = smem_sf + stage * F4_SF_STAGE_BYTES;
                     const uint32_t tsf = tmem_base + F4_SF_COL + buf * F4_SF_COLS;
                     const int steps = min(4, (p.K - kb * F4_KB) / 64);
 #pragma unroll
@@ -375,6 +432,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                         }
                     }
                     ptx::umma_commit_pair(bar_scales + 8 * buf);
+                    umma_commit_both(bar_sempty + 8 * stage);
                 }
             }
         }
@@ -384,7 +442,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
         const uint32_t tempty0 = ptx::mapa_shared(bar_tempty, 0);
         const int quarter = warp & 3;                       // TMEM lanes this warp may read
         const int sub = (warp - 2) >> 2;                    // 0 / 1: lower or upper 64 columns of either half of the tile
-        const uint32_t stage = smem_base + F4_STAGES * F4_STAGE_BYTES + (warp - 2) * F4_OUT_BYTES;
+        const uint32_t stage = smem_sf + F4_SF_STAGES * F4_SF_STAGE_BYTES + (warp - 2) * F4_OUT_BYTES;
         int vg = 0, t = 0;
         for (int tile = pair; tile < total_tiles; tile += num_pairs, ++t) {
             while (tile >= prefix[vg + 1]) ++vg;
