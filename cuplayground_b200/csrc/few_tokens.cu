@@ -312,24 +312,6 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
 }
 __device__ __forceinline__ uint32_t half_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
-// The eight e2m1 codes of a word as fp16 pairs, adjacent codes together. All eight magnitudes have an empty low byte in
-// fp16, so the high bytes of four codes come out of one byte permutation (the codes select from the table), their signs
-// out of another (which spreads the top bits of bytes), and two more put zero bytes between them: 13 instructions, where
-// four conversions took 24.
-__device__ __forceinline__ void unpack_e2m1(uint32_t w, uint32_t (&v)[4]) {
-    const uint32_t mag = w & 0x77777777u, up = w << 4;
-    // high bytes of 0, 0.5, 1, 1.5 | 2, 3, 4, 6
-    const uint32_t lo = __byte_perm(0x3E3C3800u, 0x46444240u, mag), hi = __byte_perm(0x3E3C3800u, 0x46444240u, mag >> 16);
-    uint32_t sl, sh;                                    // byte i: the sign of code i (of code 4 + i) in every bit
-    asm("prmt.b32 %0, %1, %2, 0x9D8C;" : "=r"(sl) : "r"(w), "r"(up));
-    asm("prmt.b32 %0, %1, %2, 0xBFAE;" : "=r"(sh) : "r"(w), "r"(up));
-    const uint32_t a = lo | (sl & 0x80808080u), b = hi | (sh & 0x80808080u);
-    v[0] = __byte_perm(a, 0, 0x1404);
-    v[1] = __byte_perm(a, 0, 0x3424);
-    v[2] = __byte_perm(b, 0, 0x1404);
-    v[3] = __byte_perm(b, 0, 0x3424);
-}
-
 // Four e4m3 codes as fp16 pairs (exact).
 __device__ __forceinline__ void unpack_e4m3(uint32_t w, uint32_t& lo, uint32_t& hi) {
     const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
@@ -833,7 +815,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                         if (b == 4) look_ahead(4);
                         uint32_t a[RG][4];
 #pragma unroll
-                        for (int r = 0; r < RG; ++r) unpack_e2m1(ld_shared(from + group_at(r) + ((b ^ g) << 4) + q * 4), a[r]);
+                        for (int r = 0; r < RG; ++r) fp4_unpack8(ld_shared(from + group_at(r) + ((b ^ g) << 4) + q * 4), a[r]);
                         float f[RG];
 #pragma unroll
                         for (int r = 0; r < RG; ++r) {

@@ -112,47 +112,58 @@ __device__ __forceinline__ void umma_commit_both(uint32_t bar) {
                  ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 
-// v * Phi(v) = v / 2 * erfc(-v / sqrt 2), with erfc by the Chebyshev fit of Numerical Recipes (routine erfcc, section 6.2;
-// fractional error below 1.2e-7): erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), z >= 0, and 2 - erfc(-z) for z < 0.
-// Half the instructions of the library's erff, which would take longer than the tensor cores' work on a tile of K = 2048.
-__device__ __forceinline__ float gelu_erfc(float v) {
-    const float z = fabsf(v) * 0.70710678f;
-    const float t = __fdividef(1.0f, fmaf(0.5f, z, 1.0f));
-    float q = 0.17087277f;
-    q = fmaf(q, t, -0.82215223f);
-    q = fmaf(q, t, 1.48851587f);
-    q = fmaf(q, t, -1.13520398f);
-    q = fmaf(q, t, 0.27886807f);
-    q = fmaf(q, t, -0.18628806f);
-    q = fmaf(q, t, 0.09678418f);
-    q = fmaf(q, t, 0.37409196f);
-    q = fmaf(q, t, 1.00002368f);
-    q = fmaf(q, t, -1.26551223f);
-    const float e = t * __expf(fmaf(-0.5f * v, v, q));
-    return 0.5f * v * (v < 0.0f ? e : 2.0f - e);
+// Two values through v * Phi(v) = v / 2 * erfc(-v / sqrt 2), with erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2),
+// t = 1 / (1 + p z), z >= 0 (Abramowitz and Stegun 7.1.26: off by at most 1.5e-7), and 2 - erfc(-z) for z < 0. A third of the
+// instructions of the library's erff, with which the epilogue takes several times as long as the tensor cores' work on a
+// tile of K = 2048.
+__device__ __forceinline__ float2 gelu2(float2 v) {
+    const float2 z = make_float2(fabsf(v.x), fabsf(v.y));
+    const float2 one = make_float2(1.0f, 1.0f);
+    const float p = 0.3275911f * 0.70710678f;
+    const float2 d = __ffma2_rn(z, make_float2(p, p), one);
+    const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+    float2 q = __ffma2_rn(t, make_float2(1.061405429f, 1.061405429f), make_float2(-1.453152027f, -1.453152027f));
+    q = __ffma2_rn(q, t, make_float2(1.421413741f, 1.421413741f));
+    q = __ffma2_rn(q, t, make_float2(-0.284496736f, -0.284496736f));
+    q = __ffma2_rn(q, t, make_float2(0.254829592f, 0.254829592f));
+    const float2 half = make_float2(0.5f * v.x, 0.5f * v.y);
+    // half of erfc's factor t, the exponential, and v
+    const float2 e = make_float2(q.x * t.x * __expf(-half.x * v.x), q.y * t.y * __expf(-half.y * v.y));
+    return make_float2(half.x * (v.x < 0.0f ? e.x : 2.0f - e.x), half.y * (v.y < 0.0f ? e.y : 2.0f - e.y));
 }
 
-__device__ __forceinline__ float activate(float v, int act) {
-    if (act == ARISTOS_ACT_RELU) return act_relu(v);
-    if (act == ARISTOS_ACT_GELU) return gelu_erfc(v);
-    return v;
+template <int ACT>
+__device__ __forceinline__ void activate(float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        if constexpr (ACT == ARISTOS_ACT_RELU) {
+            v[i] = act_relu(v[i]);
+            v[i + 1] = act_relu(v[i + 1]);
+        } else if constexpr (ACT == ARISTOS_ACT_GELU) {
+            const float2 r = gelu2(make_float2(v[i], v[i + 1]));
+            v[i] = r.x;
+            v[i + 1] = r.y;
+        }
+    }
 }
 
 enum { OUT_F32 = ARISTOS_DTYPE_F32, OUT_BF16 = ARISTOS_DTYPE_BF16, OUT_F16 = ARISTOS_DTYPE_F16, OUT_FP4 = 5 };
 
 // 32 adjacent columns of one row as one block of MXFP4: codes, and the scale byte.
 __device__ __forceinline__ uint32_t quantize_block(const float (&v)[32], uint32_t (&w)[4]) {
-    float m = 0.0f;                                     // the bits of |NaN| are above infinity's: NaN is kept
+    float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};              // the maximum that keeps a NaN
 #pragma unroll
-    for (int i = 0; i < 32; ++i) m = __uint_as_float(max(__float_as_uint(m), __float_as_uint(v[i]) & 0x7FFFFFFFu));
-    const uint32_t s = fp4_scale_of(m);
+    for (int i = 0; i < 32; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m[i & 3]) : "f"(fabsf(v[i])));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m[0]) : "f"(m[1]));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m[2]) : "f"(m[3]));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m[0]) : "f"(m[2]));
+    const uint32_t s = fp4_scale_of(m[0]);
     const float inv = fp4_inverse_scale(s);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        w[i] = 0;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) w[i] |= fp4_pack2(v[8 * i + 2 * q] * inv, v[8 * i + 2 * q + 1] * inv) << (8 * q);
-        if (s == 255u) w[i] = 0;
+        const uint32_t codes = fp4_pack8(v[8 * i] * inv, v[8 * i + 1] * inv, v[8 * i + 2] * inv, v[8 * i + 3] * inv,
+                                         v[8 * i + 4] * inv, v[8 * i + 5] * inv, v[8 * i + 6] * inv, v[8 * i + 7] * inv);
+        w[i] = s == 255u ? 0u : codes;
     }
     return s;
 }
@@ -219,12 +230,14 @@ __device__ __forceinline__ void store_columns(const Fp4GemmParams& p, uint32_t s
     }
 }
 
-template <int OUT>
+// One kernel per output type and activation (which is part of the up projection, whose output is MXFP4).
+template <int OUT, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F4_THREADS, 1)
 ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
                             const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmSA,
                             const __grid_constant__ CUtensorMap tmSB0, const __grid_constant__ CUtensorMap tmSB1,
                             const Fp4GemmParams p) {
+    constexpr bool GATED = ACT == ARISTOS_ACT_SWIGLU;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* aux = smem + F4_STAGES * F4_STAGE_BYTES + F4_SF_STAGES * F4_SF_STAGE_BYTES + F4_EPI_WARPS * F4_OUT_BYTES;
@@ -247,7 +260,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     const uint32_t smem_base = ptx::smem_u32(smem);
     const uint32_t smem_sf = smem_base + F4_STAGES * F4_STAGE_BYTES;
 
-    const int out_w = p.gated ? 128 : 256;
+    const int out_w = GATED ? 128 : 256;
     const int n_tiles = (p.N + out_w - 1) / out_w;
     const int kblocks = (p.K + F4_KB - 1) / F4_KB;
 
@@ -315,7 +328,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                 const int m0 = (local % mt) * F4_PM + (int)cta * F4_BM;
                 const int n0 = (local / mt) * out_w;
                 const int e = g % p.experts;
-                const int nb = cta == 0 || p.gated ? n0 : n0 + 128;     // this CTA's half of B
+                const int nb = cta == 0 || GATED ? n0 : n0 + 128;     // this CTA's half of B
                 for (int kb = 0; kb < kblocks; ++kb) {
                     ok = ptx::mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.dev_status);
                     if (!ok) break;
@@ -385,7 +398,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                 const int m0 = (local % mt) * F4_PM + (int)cta * F4_BM;
                 const int n0 = (local / mt) * out_w;
                 const int e = g % p.experts;
-                const int n1 = p.gated ? n0 : n0 + 128;     // first weight row of the second half of B
+                const int n1 = GATED ? n0 : n0 + 128;     // first weight row of the second half of B
                 for (int kb = 0; kb < kblocks; ++kb) {
                     ok = ptx::mbar_wait_bounded(bar_sempty + 8 * stage, phase ^ 1u, abort_flag, p.dev_status);
                     if (!ok) break;
@@ -470,7 +483,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             ptx::tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive_cluster(tempty0);
-            if (p.gated) {
+            if constexpr (GATED) {
                 ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64, b[0]);
                 ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64 + 32, b[1]);
                 ptx::tmem_ld_wait();
@@ -486,7 +499,9 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[c][i] = activate(__uint_as_float(a[c][i]), p.act);
+                    for (int i = 0; i < 32; ++i) v[c][i] = __uint_as_float(a[c][i]);
+                activate<ACT>(v[0]);
+                activate<ACT>(v[1]);
                 store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + half0 * 128 + sub * 64, v);
                 ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64, b[0]);
                 ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64 + 32, b[1]);
@@ -494,7 +509,9 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[c][i] = activate(__uint_as_float(b[c][i]), p.act);
+                    for (int i = 0; i < 32; ++i) v[c][i] = __uint_as_float(b[c][i]);
+                activate<ACT>(v[0]);
+                activate<ACT>(v[1]);
                 store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + (half0 ^ 1) * 128 + sub * 64, v);
             }
         }
@@ -567,10 +584,15 @@ aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, 
         return ARISTOS_OK;
     };
     switch (out) {
-        case OUT_F32: return run(ffn_fp4_grouped_gemm_kernel<OUT_F32>);
-        case OUT_BF16: return run(ffn_fp4_grouped_gemm_kernel<OUT_BF16>);
-        case OUT_F16: return run(ffn_fp4_grouped_gemm_kernel<OUT_F16>);
-        default: return run(ffn_fp4_grouped_gemm_kernel<OUT_FP4>);
+        case OUT_F32: return run(ffn_fp4_grouped_gemm_kernel<OUT_F32, ARISTOS_ACT_IDENTITY>);
+        case OUT_BF16: return run(ffn_fp4_grouped_gemm_kernel<OUT_BF16, ARISTOS_ACT_IDENTITY>);
+        case OUT_F16: return run(ffn_fp4_grouped_gemm_kernel<OUT_F16, ARISTOS_ACT_IDENTITY>);
+        default: break;
+    }
+    switch (p.act) {
+        case ARISTOS_ACT_RELU: return run(ffn_fp4_grouped_gemm_kernel<OUT_FP4, ARISTOS_ACT_RELU>);
+        case ARISTOS_ACT_GELU: return run(ffn_fp4_grouped_gemm_kernel<OUT_FP4, ARISTOS_ACT_GELU>);
+        default: return run(ffn_fp4_grouped_gemm_kernel<OUT_FP4, ARISTOS_ACT_SWIGLU>);
     }
 }
 

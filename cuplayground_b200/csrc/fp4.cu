@@ -88,11 +88,9 @@ quantize_fp4_kernel(const T* __restrict__ src, int64_t mats, int rows, int cols,
                 m = magnitude_max(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 const uint32_t sb = fp4_scale_of(m);
                 const float inv = fp4_inverse_scale(sb);
-                uint32_t packed = 0;
-                if (sb != 255u) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) packed |= fp4_pack2(v[2 * j] * inv, v[2 * j + 1] * inv) << (8 * j);
-                }
+                const uint32_t codes8 = fp4_pack8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, v[4] * inv, v[5] * inv,
+                                                  v[6] * inv, v[7] * inv);
+                const uint32_t packed = sb != 255u ? codes8 : 0u;
                 uint32_t word = sb << (8 * (l >> 2));
                 word |= __shfl_xor_sync(0xffffffffu, word, 4);
                 word |= __shfl_xor_sync(0xffffffffu, word, 8);
@@ -141,9 +139,11 @@ dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
                 if (!in[i]) continue;
                 const float f = fp4_scale_value((sword[i] >> (8 * (l >> 2))) & 255u);
                 float v[8];
+                uint32_t h[4];
+                fp4_unpack8(word[i], h);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 p = __half22float2(fp4_unpack2((word[i] >> (8 * j)) & 255u));
+                    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
                     v[2 * j] = p.x * f;
                     v[2 * j + 1] = p.y * f;
                 }

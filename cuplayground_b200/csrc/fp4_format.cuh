@@ -6,7 +6,6 @@
 //   byte (row, block) of a matrix = tile (row / 128, block / 4), [row % 32][row / 32 % 4][block % 4],
 // tiles of a matrix row-tile-major. Rows and blocks that only fill up a tile have scale 0 (2^-127).
 #pragma once
-#include <cuda_fp4.h>
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -45,14 +44,37 @@ __device__ __forceinline__ uint32_t fp4_scale_of(float amax) {
 // the factor is a normal number and the products are exact (or so small that they round to zero either way).
 __device__ __forceinline__ float fp4_inverse_scale(uint32_t s) { return __uint_as_float((254u - min(s, 253u)) << 23); }
 
-// Two values, already divided by their scale, to one byte (a in the low half); round to nearest even, saturate at 6.
-__device__ __forceinline__ uint32_t fp4_pack2(float a, float b) {
-    return (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(a, b), __NV_E2M1, cudaRoundNearest);
+// Eight values, already divided by their scale, to a word of codes (v[0] in the lowest four bits); round to nearest even,
+// saturate at 6.
+__device__ __forceinline__ uint32_t fp4_pack8(float v0, float v1, float v2, float v3, float v4, float v5, float v6, float v7) {
+    uint32_t w;
+    asm("{\n\t"
+        ".reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t"
+        "}"
+        : "=r"(w)
+        : "f"(v0), "f"(v1), "f"(v2), "f"(v3), "f"(v4), "f"(v5), "f"(v6), "f"(v7));
+    return w;
 }
-// The two elements of a byte as fp16 (exact).
-__device__ __forceinline__ __half2 fp4_unpack2(uint32_t byte) {
-    const __half2_raw r = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)byte, __NV_E2M1);
-    return *reinterpret_cast<const __half2*>(&r);
+// The eight elements of a word as fp16 pairs (exact), adjacent ones together. All magnitudes have an empty low byte in
+// fp16, so the high bytes of four codes come out of one byte permutation (the codes select from the table), their signs out
+// of another (which spreads the top bits of bytes), and two more put zero bytes between them.
+__device__ __forceinline__ void fp4_unpack8(uint32_t w, uint32_t (&v)[4]) {
+    const uint32_t mag = w & 0x77777777u, up = w << 4;
+    // high bytes of 0, 0.5, 1, 1.5 | 2, 3, 4, 6
+    const uint32_t lo = __byte_perm(0x3E3C3800u, 0x46444240u, mag), hi = __byte_perm(0x3E3C3800u, 0x46444240u, mag >> 16);
+    uint32_t sl, sh;                                    // byte i: the sign of code i (of code 4 + i) in every bit
+    asm("prmt.b32 %0, %1, %2, 0x9D8C;" : "=r"(sl) : "r"(w), "r"(up));
+    asm("prmt.b32 %0, %1, %2, 0xBFAE;" : "=r"(sh) : "r"(w), "r"(up));
+    const uint32_t a = lo | (sl & 0x80808080u), b = hi | (sh & 0x80808080u);
+    v[0] = __byte_perm(a, 0, 0x1404);
+    v[1] = __byte_perm(a, 0, 0x3424);
+    v[2] = __byte_perm(b, 0, 0x1404);
+    v[3] = __byte_perm(b, 0, 0x3424);
 }
 #endif
 
