@@ -21,11 +21,12 @@
 // [0, 256) and [128, 384), scales from 384. The epilogue reads the shared half of a finished tile first and then lets the
 // issuer start the next one, which fills the other buffer while the rest is worked on.
 //
-// Roles (384 threads per CTA): warp 0 TMA, warp 1 TMEM + MMA, warps 2-9 epilogue, two warps per lane quarter with half of
-// the columns each, warp 10 TMA of the scales, warp 11 scales to TMEM. Every wait is bounded.
+// Roles (640 threads per CTA): warp 0 TMA, warp 1 TMEM + MMA, warps 2-17 epilogue, four warps per lane quarter with a
+// quarter of the columns each (eight warps of twice the columns left an activation's latencies uncovered: GELU took them
+// 15000 cycles a tile), warp 18 TMA of the scales, warp 19 scales to TMEM. Every wait is bounded.
 //
-// The up projection of the FFN writes its output as MXFP4 again: a thread holds 64 adjacent columns of its row, i.e. two
-// whole blocks, so scale and codes come out of its registers, rounded once from fp32. Only valid rows are written.
+// The up projection of the FFN writes its output as MXFP4 again: a thread holds 32 adjacent columns of its row, i.e. a
+// whole block, so scale and codes come out of its registers, rounded once from fp32. Only valid rows are written.
 #include <cuda.h>
 
 #include "common.cuh"
@@ -49,12 +50,12 @@ constexpr int F4_STAGE_BYTES = F4_A_BYTES + F4_B_BYTES;
 constexpr int F4_SF_STAGES = 8;
 constexpr int F4_SF_STAGE_BYTES = 3 * F4_SF_BYTES;       // of A's rows, of B's first and second 128 rows
 static_assert(F4_STAGE_BYTES % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
-constexpr int F4_EPI_WARPS = 8;
+constexpr int F4_EPI_WARPS = 16;
 constexpr int F4_SF_LOAD_WARP = 2 + F4_EPI_WARPS, F4_SF_COPY_WARP = 3 + F4_EPI_WARPS;
 constexpr int F4_THREADS = 32 * (4 + F4_EPI_WARPS);
 constexpr int F4_MAX_GROUPS = 1024;
 constexpr int F4_AUX_BYTES = (512 + (F4_MAX_GROUPS + 1) * 4 + 127) & ~127;
-constexpr int F4_OUT_BYTES = 32 * 128;                   // output staging of an epilogue warp: 32 rows x 128 bytes
+constexpr int F4_OUT_BYTES = 32 * 64;                    // output staging of an epilogue warp: 32 rows x 64 bytes
 constexpr int F4_SMEM_BYTES = 1024 + F4_STAGES * F4_STAGE_BYTES + F4_SF_STAGES * F4_SF_STAGE_BYTES +
                               F4_EPI_WARPS * F4_OUT_BYTES + F4_AUX_BYTES;
 static_assert(F4_SMEM_BYTES <= 227 * 1024, "fp4 GEMM: shared memory");
@@ -112,6 +113,22 @@ __device__ __forceinline__ void umma_commit_both(uint32_t bar) {
                  ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 
+// Reciprocal and power of two in one instruction each (subnormal arguments and results count as zero: the arguments here are
+// at least 1, and a factor below 2^-126 is none).
+__device__ __forceinline__ float fast_rcp(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float fast_exp2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+constexpr float LOG2_E = 1.44269504f;
+
+__device__ __forceinline__ float silu(float v) { return v * fast_rcp(1.0f + fast_exp2(-LOG2_E * v)); }
+
 // Two values through v * Phi(v) = v / 2 * erfc(-v / sqrt 2), with erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2),
 // t = 1 / (1 + p z), z >= 0 (Abramowitz and Stegun 7.1.26: off by at most 1.5e-7), and 2 - erfc(-z) for z < 0. A third of the
 // instructions of the library's erff, with which the epilogue takes several times as long as the tensor cores' work on a
@@ -121,14 +138,13 @@ __device__ __forceinline__ float2 gelu2(float2 v) {
     const float2 one = make_float2(1.0f, 1.0f);
     const float p = 0.3275911f * 0.70710678f;
     const float2 d = __ffma2_rn(z, make_float2(p, p), one);
-    const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+    const float2 t = make_float2(fast_rcp(d.x), fast_rcp(d.y));
     float2 q = __ffma2_rn(t, make_float2(1.061405429f, 1.061405429f), make_float2(-1.453152027f, -1.453152027f));
     q = __ffma2_rn(q, t, make_float2(1.421413741f, 1.421413741f));
     q = __ffma2_rn(q, t, make_float2(-0.284496736f, -0.284496736f));
     q = __ffma2_rn(q, t, make_float2(0.254829592f, 0.254829592f));
     const float2 half = make_float2(0.5f * v.x, 0.5f * v.y);
-    // half of erfc's factor t, the exponential, and v
-    const float2 e = make_float2(q.x * t.x * __expf(-half.x * v.x), q.y * t.y * __expf(-half.y * v.y));
+    const float2 e = make_float2(q.x * t.x * fast_exp2(-LOG2_E * half.x * v.x), q.y * t.y * fast_exp2(-LOG2_E * half.y * v.y));
     return make_float2(half.x * (v.x < 0.0f ? e.x : 2.0f - e.x), half.y * (v.y < 0.0f ? e.y : 2.0f - e.y));
 }
 
@@ -168,65 +184,59 @@ __device__ __forceinline__ uint32_t quantize_block(const float (&v)[32], uint32_
     return s;
 }
 
-// A warp's 32 rows of UNITS 16-byte units each (w: this lane's row) to memory, through its staging area, so that a store
-// instruction writes whole lines instead of 32 separate pieces (those took longer than the tensor core's work on a tile).
-// Rows from `valid` on are left out. dst: row 0, `pitch` bytes between rows.
-template <int UNITS>
-__device__ __forceinline__ void store_rows(uint32_t stage, int lane, const uint32_t (&w)[4 * UNITS], uint8_t* dst, size_t pitch,
-                                           int valid) {
-    // unit u of row r lies at unit u ^ (r % 8) of 8 (UNITS 8), u ^ (r / 4 % 2) of 2 (UNITS 2): no bank conflicts either way
-    auto place = [&](int r, int u) { return stage + r * (16 * UNITS) + ((u ^ (UNITS == 8 ? r & 7 : (r >> 2) & 1)) << 4); };
+// A warp's 32 rows of 64 bytes each (w: this lane's row) to memory, through its staging area, so that a store instruction
+// writes 64 bytes in a row instead of 32 separate pieces (those took longer than the tensor core's work on a tile). Rows from
+// `valid` on are left out. dst: row 0, `pitch` bytes between rows.
+__device__ __forceinline__ void store_rows(uint32_t stage, int lane, const uint32_t (&w)[16], uint8_t* dst, size_t pitch, int valid) {
+    // unit u of row r lies at unit u ^ (r / 2 % 4): no bank conflicts either way
+    auto place = [&](int r, int u) { return stage + r * 64 + ((u ^ ((r >> 1) & 3)) << 4); };
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) ptx::st_shared_v4(place(lane, u), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+    for (int u = 0; u < 4; ++u) ptx::st_shared_v4(place(lane, u), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
     __syncwarp();
-    const int u = lane % UNITS;
+    const int u = lane & 3;
 #pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-        const int r = i * (32 / UNITS) + lane / UNITS;
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
         const uint4 v = ptx::ld_shared_v4(place(r, u));
         if (r < valid) *reinterpret_cast<uint4*>(dst + r * pitch + u * 16) = v;
     }
     __syncwarp();
 }
 
-// 64 adjacent columns of a warp's 32 rows to the output; v: this lane's row.
+// 32 adjacent columns of a warp's 32 rows to the output; v: this lane's row.
 template <int OUT>
 __device__ __forceinline__ void store_columns(const Fp4GemmParams& p, uint32_t stage, int lane, int g, int row0, int valid, int col,
-                                              const float (&v)[2][32]) {
+                                              const float (&v)[32]) {
     if (col >= p.N) return;
     const size_t grow = (size_t)g * p.rows_per_group + row0;
     if constexpr (OUT == OUT_FP4) {
-        uint32_t w[8], lo[4], hi[4];
-        const uint32_t s = quantize_block(v[0], lo) | quantize_block(v[1], hi) << 8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { w[i] = lo[i]; w[4 + i] = hi[i]; }
-        store_rows<2>(stage, lane, w, static_cast<uint8_t*>(p.out) + grow * (p.N / 2) + col / 2, p.N / 2, valid);
+        uint32_t w[4];
+        const uint32_t s = quantize_block(v, w);
+        if (lane >= valid) return;
+        *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + (grow + lane) * (p.N / 2) + col / 2) = make_uint4(w[0], w[1], w[2], w[3]);
         const size_t tile_at = ((size_t)g * fp4_row_tiles(p.rows_per_group) + row0 / 128) * fp4_col_tiles(p.N) + col / 128;
-        if (lane < valid)
-            *reinterpret_cast<uint16_t*>(p.out_scales + tile_at * FP4_TILE_BYTES + fp4_tile_word(row0 + lane) + (col / 32) % 4) = (uint16_t)s;
+        p.out_scales[tile_at * FP4_TILE_BYTES + fp4_tile_word(row0 + lane) + (col / 32) % 4] = (uint8_t)s;
     } else if constexpr (OUT == OUT_F32) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            uint32_t w[32];
+            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[c][i]);
-            store_rows<8>(stage, lane, w, static_cast<uint8_t*>(p.out) + (grow * p.N + col + 32 * c) * 4, (size_t)p.N * 4, valid);
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[16 * c + i]);
+            store_rows(stage, lane, w, static_cast<uint8_t*>(p.out) + (grow * p.N + col + 16 * c) * 4, (size_t)p.N * 4, valid);
         }
     } else {
-        uint32_t w[32];
+        uint32_t w[16];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if constexpr (OUT == OUT_BF16) {
-                    const __nv_bfloat162 t = __floats2bfloat162_rn(v[c][2 * i], v[c][2 * i + 1]);
-                    w[16 * c + i] = *reinterpret_cast<const uint32_t*>(&t);
-                } else {
-                    const __half2 t = __floats2half2_rn(v[c][2 * i], v[c][2 * i + 1]);
-                    w[16 * c + i] = *reinterpret_cast<const uint32_t*>(&t);
-                }
+        for (int i = 0; i < 16; ++i) {
+            if constexpr (OUT == OUT_BF16) {
+                const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&t);
+            } else {
+                const __half2 t = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&t);
             }
-        store_rows<8>(stage, lane, w, static_cast<uint8_t*>(p.out) + (grow * p.N + col) * 2, (size_t)p.N * 2, valid);
+        }
+        store_rows(stage, lane, w, static_cast<uint8_t*>(p.out) + (grow * p.N + col) * 2, (size_t)p.N * 2, valid);
     }
 }
 
@@ -454,7 +464,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
         // ------------------------------------------------------------------ epilogue (both CTAs, their own rows)
         const uint32_t tempty0 = ptx::mapa_shared(bar_tempty, 0);
         const int quarter = warp & 3;                       // TMEM lanes this warp may read
-        const int sub = (warp - 2) >> 2;                    // 0 / 1: lower or upper 64 columns of either half of the tile
+        const int sub = (warp - 2) >> 2;                    // 0 .. 3: which 32 columns of either half of the tile
         const uint32_t stage = smem_sf + F4_SF_STAGES * F4_SF_STAGE_BYTES + (warp - 2) * F4_OUT_BYTES;
         int vg = 0, t = 0;
         for (int tile = pair; tile < total_tiles; tile += num_pairs, ++t) {
@@ -472,47 +482,37 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             ptx::tcgen05_fence_after();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (t & 1) * F4_ACC1;
             // First the half of the columns that the next tile's accumulator shares: the upper one of the first accumulator,
-            // the lower one of the second. A warp has 64 columns of either half; SwiGLU: gate columns in the lower half,
+            // the lower one of the second. A warp has 32 columns of either half; SwiGLU: gate columns in the lower half,
             // up columns in the upper.
             const int half0 = (t & 1) ? 0 : 1;
-            uint32_t a[2][32], b[2][32];
-            float v[2][32];
-            ptx::tmem_ld_32x32b_x32(taddr + half0 * 128 + sub * 64, a[0]);
-            ptx::tmem_ld_32x32b_x32(taddr + half0 * 128 + sub * 64 + 32, a[1]);
+            uint32_t a[32];
+            float v[32];
+            ptx::tmem_ld_32x32b_x32(taddr + half0 * 128 + sub * 32, a);
             ptx::tmem_ld_wait();
             ptx::tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive_cluster(tempty0);
             if constexpr (GATED) {
-                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64, b[0]);
-                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64 + 32, b[1]);
+                uint32_t b[32];
+                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 32, b);
                 ptx::tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float gate = __uint_as_float(half0 == 0 ? a[c][i] : b[c][i]);
-                        v[c][i] = act_silu(gate) * __uint_as_float(half0 == 0 ? b[c][i] : a[c][i]);
-                    }
-                store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + sub * 64, v);
+                for (int i = 0; i < 32; ++i) {
+                    const float gate = __uint_as_float(half0 == 0 ? a[i] : b[i]);
+                    v[i] = silu(gate) * __uint_as_float(half0 == 0 ? b[i] : a[i]);
+                }
+                store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + sub * 32, v);
             } else {
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[c][i] = __uint_as_float(a[c][i]);
-                activate<ACT>(v[0]);
-                activate<ACT>(v[1]);
-                store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + half0 * 128 + sub * 64, v);
-                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64, b[0]);
-                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 64 + 32, b[1]);
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(a[i]);
+                activate<ACT>(v);
+                store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + half0 * 128 + sub * 32, v);
+                ptx::tmem_ld_32x32b_x32(taddr + (half0 ^ 1) * 128 + sub * 32, a);
                 ptx::tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[c][i] = __uint_as_float(b[c][i]);
-                activate<ACT>(v[0]);
-                activate<ACT>(v[1]);
-                store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + (half0 ^ 1) * 128 + sub * 64, v);
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(a[i]);
+                activate<ACT>(v);
+                store_columns<OUT>(p, stage, lane, g, row0, valid, n0 + (half0 ^ 1) * 128 + sub * 32, v);
             }
         }
     }
