@@ -232,12 +232,42 @@ def expert_ffn_fp8(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, hidden_act: int, de
 
 
 # ---- microscaled 4-bit operands -------------------------------------------------------------------------------------
-def _one_device(*tensors) -> torch.device:
-    """The CUDA device that all the given tensors (None: not given) are on."""
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1 or next(iter(devices)).type != "cuda":
-        raise ValueError(f"tensors must all be on one CUDA device, got {sorted(map(str, devices))}")
-    return next(iter(devices))
+class _Device:
+    """Makes the device that all the given tensors (None: not given) are on the current one for a call of the library, and
+    gives the call its current stream. Only another device than the current one costs a switch."""
+    __slots__ = ("index", "previous", "stream")
+
+    def __init__(self, *tensors):
+        device = None
+        for t in tensors:
+            if t is None:
+                continue
+            if device is None:
+                device = t.device
+            if t.device != device or device.type != "cuda":
+                raise ValueError("tensors must all be on one CUDA device, got "
+                                 f"{sorted({str(t.device) for t in tensors if t is not None})}")
+        self.index = device.index
+
+    def __enter__(self):
+        self.previous = torch.cuda.current_device()
+        if self.previous != self.index:
+            torch.cuda.set_device(self.index)
+        self.stream = torch.cuda.current_stream(self.index).cuda_stream
+        return self
+
+    def __exit__(self, *_):
+        if self.previous != self.index:
+            torch.cuda.set_device(self.previous)
+
+
+def _addr(t: Optional[torch.Tensor]):
+    """The address that the C ABI takes for a tensor (ctypes makes a pointer of it)."""
+    if t is None:
+        return None
+    if not t.is_contiguous():
+        raise ValueError("tensors passed to the C ABI must be contiguous")
+    return t.data_ptr()
 
 
 def _fp4_scale_shape(lead, rows: int, cols: int):
@@ -245,7 +275,7 @@ def _fp4_scale_shape(lead, rows: int, cols: int):
 
 
 def _expect(name: str, t: torch.Tensor, shape, dtype: torch.dtype) -> None:
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -256,11 +286,11 @@ def quantize_fp4(src: torch.Tensor):
     [..., r / 128, b / 4, r % 32, r / 32 % 4, b % 4]. See aristos_quantize_fp4."""
     rows, cols = src.shape[-2], src.shape[-1]
     lead = src.shape[:-2]
-    with torch.cuda.device(_one_device(src)):
+    with _Device(src) as on:
         q = torch.empty((*lead, rows, cols // 2), dtype=torch.uint8, device=src.device)
         scales = torch.empty(_fp4_scale_shape(lead, rows, cols), dtype=torch.uint8, device=src.device)
-        _lib.check(_lib.load().aristos_quantize_fp4(_ptr(src), lead.numel(), rows, cols, _dt(src), _ptr(q), _ptr(scales),
-                                                    _stream_ptr()))
+        _lib.check(_lib.load().aristos_quantize_fp4(_addr(src), lead.numel(), rows, cols, _dt(src), _addr(q), _addr(scales),
+                                                    on.stream))
     return q, scales
 
 
@@ -270,10 +300,10 @@ def dequantize_fp4(q: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     lead = q.shape[:-2]
     _expect("q", q, q.shape, torch.uint8)
     _expect("scales", scales, _fp4_scale_shape(lead, rows, cols), torch.uint8)
-    with torch.cuda.device(_one_device(q, scales)):
+    with _Device(q, scales) as on:
         out = torch.empty((*lead, rows, cols), dtype=dtype, device=q.device)
-        _lib.check(_lib.load().aristos_dequantize_fp4(_ptr(q), _ptr(scales), lead.numel(), rows, cols, _dt(out),
-                                                      _ptr(out), _stream_ptr()))
+        _lib.check(_lib.load().aristos_dequantize_fp4(_addr(q), _addr(scales), lead.numel(), rows, cols, _dt(out),
+                                                      _addr(out), on.stream))
     return out
 
 
@@ -294,11 +324,11 @@ def expert_product_fp4(aq, sa, count, bq, sb, y=None, dtype: Optional[torch.dtyp
                            ("bq", bq, (experts, N, half)), ("sb", sb, _fp4_scale_shape((experts,), N, 2 * half))):
         _expect(name, t, shape, torch.uint8)
     _expect("count", count, (groups,), torch.int32)
-    with torch.cuda.device(_one_device(aq, sa, count, bq, sb, y, dev_status)):
+    with _Device(aq, sa, count, bq, sb, y, dev_status) as on:
         y = _fp4_output(y, (groups, rows, N), dtype, aq.device)
-        _lib.check(_lib.load().aristos_expert_product_fp4(_ptr(aq), _ptr(sa), _ptr(count), groups, rows, experts, _ptr(bq),
-                                                          _ptr(sb), N, 2 * half, _dt(y), _ptr(y), _ptr(dev_status),
-                                                          _stream_ptr()))
+        _lib.check(_lib.load().aristos_expert_product_fp4(_addr(aq), _addr(sa), _addr(count), groups, rows, experts, _addr(bq),
+                                                          _addr(sb), N, 2 * half, _dt(y), _addr(y), _addr(dev_status),
+                                                          on.stream))
     return y
 
 
@@ -322,14 +352,14 @@ def expert_ffn_fp4(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, hidden_act: int, y=
     for name, t, shape in checks:
         _expect(name, t, shape, torch.uint8)
     _expect("count", count, (groups,), torch.int32)
-    with torch.cuda.device(_one_device(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, y, dev_status)):
+    with _Device(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, y, dev_status) as on:
         y = _fp4_output(y, (groups, rows, H), dtype, xq.device)
         hq = torch.empty((groups, rows, I // 2), dtype=torch.uint8, device=xq.device)
         sh = torch.empty(_fp4_scale_shape((groups,), rows, I), dtype=torch.uint8, device=xq.device)
-        _lib.check(_lib.load().aristos_expert_ffn_fp4(_ptr(xq), _ptr(sx), _ptr(count), groups, rows, experts, _ptr(w1q),
-                                                      _ptr(s1), _ptr(w3q), _ptr(s3), _ptr(w2q), _ptr(s2), _ptr(hq),
-                                                      _ptr(sh), _ptr(y), H, I, hidden_act, _dt(y), _ptr(dev_status),
-                                                      _stream_ptr()))
+        _lib.check(_lib.load().aristos_expert_ffn_fp4(_addr(xq), _addr(sx), _addr(count), groups, rows, experts, _addr(w1q),
+                                                      _addr(s1), _addr(w3q), _addr(s3), _addr(w2q), _addr(s2), _addr(hq),
+                                                      _addr(sh), _addr(y), H, I, hidden_act, _dt(y), _addr(dev_status),
+                                                      on.stream))
     return y
 
 
@@ -374,17 +404,17 @@ def moe_few_tokens(x, w_gate, w1, w3, w2, k: int, hidden_act: int, *, gate_fn: i
         if t is not None:
             _expect(name, t, shape, d)
     lib = _lib.load()
-    with torch.cuda.device(_one_device(x, w_gate, w1, w3, w2, s1, s3, s2, gate_bias, b1, b3, b2, out, dev_status)):
+    with _Device(x, w_gate, w1, w3, w2, s1, s3, s2, gate_bias, b1, b3, b2, out, dev_status) as on:
         if out is None:
             out = torch.empty_like(x)
         idx = torch.empty((n, k), dtype=torch.int32, device=x.device)
         w = torch.empty((n, k), dtype=torch.float32, device=x.device)
         nbytes = lib.aristos_moe_few_tokens_workspace_bytes(n, H, I, E, k)
         ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
-        _lib.check(lib.aristos_moe_few_tokens(_ptr(x), _ptr(w_gate), _ptr(gate_bias), _ptr(w1), _ptr(w3), _ptr(w2),
-                                              _ptr(s1), _ptr(s3), _ptr(s2), _ptr(b1), _ptr(b3), _ptr(b2), n, H, I, E, k,
-                                              gate_fn, renorm, hidden_act, dt, wdt, _ptr(out), _ptr(idx), _ptr(w),
-                                              _ptr(ws), nbytes, _ptr(dev_status), _stream_ptr()))
+        _lib.check(lib.aristos_moe_few_tokens(_addr(x), _addr(w_gate), _addr(gate_bias), _addr(w1), _addr(w3), _addr(w2),
+                                              _addr(s1), _addr(s3), _addr(s2), _addr(b1), _addr(b3), _addr(b2), n, H, I, E, k,
+                                              gate_fn, renorm, hidden_act, dt, wdt, _addr(out), _addr(idx), _addr(w),
+                                              _addr(ws), nbytes, _addr(dev_status), on.stream))
     return out, idx, w
 
 
