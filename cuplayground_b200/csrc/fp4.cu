@@ -4,9 +4,10 @@
 // rounded to nearest even and saturated at 6. Multiplying by a power of two is exact, so the only rounding is the one to
 // e2m1 and the codes do not depend on how the work is cut up.
 //
-// Both directions are bound by HBM. A unit of work is one row's 128 columns = one 4-byte scale word: a half warp takes it,
-// 8 columns (16 bytes of a 16-bit tensor) per lane, so loads and stores of a warp are contiguous; four lanes share a
-// block and find its maximum with two shuffles. UNITS units are in flight per half warp.
+// Both directions are bound by HBM, and close to being bound by instructions: a 16-bit element is two bytes of traffic.
+// Quantising, a thread takes a whole block (64 bytes of a 16-bit tensor): no exchange between threads, 4 instructions an
+// element (four threads per block, with shuffles for the maximum and the scale word, needed 9 and took 1.4 times as long).
+// The other way a thread takes 8 codes, so that a warp's stores are contiguous.
 #include "common.cuh"
 #include "fp4_format.cuh"
 
@@ -31,75 +32,97 @@ __device__ __forceinline__ uint32_t divide(uint32_t u, const Divider& v) {
     return (uint32_t)(((uint64_t)u * v.magic) >> v.shift);
 }
 
-template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
+// A block of 32 elements as it lies in memory.
+template <typename T> struct RawBlock { uint4 v[2 * sizeof(T)]; };
 template <typename T>
-__device__ __forceinline__ void load_raw(const T* p, Raw8<T>& r) {
+__device__ __forceinline__ void load_block(const T* p, RawBlock<T>& r) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-}
-template <typename T>
-__device__ __forceinline__ void raw_to_float(const Raw8<T>& r, float (&v)[8]) {
-    load8(reinterpret_cast<const T*>(&r.v[0]), v);
+    for (int i = 0; i < 2 * (int)sizeof(T); ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
 }
 
-// The largest magnitude as an fp32 number, except that a NaN stays one (the bits of NaN are above those of infinity).
-__device__ __forceinline__ float magnitude_max(float a, float b) {
-    return __uint_as_float(max(__float_as_uint(a) & 0x7FFFFFFFu, __float_as_uint(b) & 0x7FFFFFFFu));
+// The largest magnitude of a block as fp32, NaN if there is one: 16-bit elements are compared in pairs as they are.
+__device__ __forceinline__ uint32_t max_pair(const __nv_bfloat16*, uint32_t a, uint32_t b) {
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b & 0x7FFF7FFFu));
+    return a;
 }
+__device__ __forceinline__ uint32_t max_pair(const __half*, uint32_t a, uint32_t b) {
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(a) : "r"(b & 0x7FFF7FFFu));
+    return a;
+}
+__device__ __forceinline__ float2 to_float2(const __nv_bfloat16*, uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ float2 to_float2(const __half*, uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(fabsf(b)));
+    return a;
+}
+__device__ __forceinline__ uint32_t raw_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+template <typename T>
+__device__ __forceinline__ float largest(const RawBlock<T>& r) {
+    const T* tag = nullptr;
+    uint32_t m[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m[i & 1] = max_pair(tag, m[i & 1], raw_word(r.v[i >> 2], i & 3));
+    const float2 f = to_float2(tag, max_pair(tag, m[0], m[1]));
+    return max_nan(f.x, f.y);
+}
+template <>
+__device__ __forceinline__ float largest<float>(const RawBlock<float>& r) {
+    float m[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) m[i & 1] = max_nan(m[i & 1], __uint_as_float(raw_word(r.v[i >> 2], i & 3)));
+    return max_nan(m[0], m[1]);
+}
+// Eight elements from number 8 * i on.
+template <typename T>
+__device__ __forceinline__ void eight(const RawBlock<T>& r, int i, float (&v)[8]) {
+    load8(reinterpret_cast<const T*>(&r.v[i * (int)sizeof(T) / 2]), v);
+}
+
+constexpr int Q4_BLOCKS = 2;                 // blocks in flight per thread
 
 template <typename T>
 __global__ void __launch_bounds__(Q4_THREADS)
-quantize_fp4_kernel(const T* __restrict__ src, int64_t mats, int rows, int cols, uint32_t units, Divider tiles,
+quantize_fp4_kernel(const T* __restrict__ src, int64_t mats, int rows, int cols, uint32_t blocks, Divider per_row,
                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    const int l = threadIdx.x & 15;
-    const uint32_t half = blockIdx.x * Q4_HALVES + (threadIdx.x >> 4);
-    const uint32_t stride = gridDim.x * Q4_HALVES;
+    // a matrix's blocks are numbered with its rows and columns filled up to whole scale tiles
+    const uint32_t first = blockIdx.x * Q4_THREADS + threadIdx.x, stride = gridDim.x * Q4_THREADS;
     const size_t mat_scales = fp4_matrix_scale_bytes(rows, cols);
     for (int64_t mat = blockIdx.y; mat < mats; mat += gridDim.y) {
         const T* s = src + (size_t)mat * rows * cols;
         uint8_t* c = codes + (size_t)mat * rows * (cols / 2);
         uint8_t* sc = scales + (size_t)mat * mat_scales;
-        // the loop bound is the same for both halves of a warp, so that the shuffles below are reached together
-        for (uint32_t u0 = 0; u0 < units; u0 += stride * Q4_UNITS) {
-            Raw8<T> raw[Q4_UNITS];
-            uint32_t row[Q4_UNITS], tile[Q4_UNITS];
-            bool in[Q4_UNITS];
+        for (uint32_t u0 = first; u0 < blocks; u0 += stride * Q4_BLOCKS) {
+            RawBlock<T> raw[Q4_BLOCKS];
+            uint32_t row[Q4_BLOCKS], block[Q4_BLOCKS];
+            bool in[Q4_BLOCKS];
 #pragma unroll
-            for (int i = 0; i < Q4_UNITS; ++i) {
-                const uint32_t u = u0 + i * stride + half;
-                row[i] = divide(u, tiles);
-                tile[i] = u - row[i] * tiles.d;
-                in[i] = u < units && row[i] < (uint32_t)rows && tile[i] * 128 + l * 8 < (uint32_t)cols;
-                if (in[i]) {
-                    load_raw(s + (size_t)row[i] * cols + tile[i] * 128 + l * 8, raw[i]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) raw[i].v[j] = make_uint4(0, 0, 0, 0);
-                }
+            for (int i = 0; i < Q4_BLOCKS; ++i) {
+                const uint32_t u = u0 + i * stride;
+                row[i] = divide(u, per_row);
+                block[i] = u - row[i] * per_row.d;
+                in[i] = u < blocks && row[i] < (uint32_t)rows && block[i] * FP4_BLOCK < (uint32_t)cols;
+                if (in[i]) load_block(s + (size_t)row[i] * cols + block[i] * FP4_BLOCK, raw[i]);
             }
 #pragma unroll
-            for (int i = 0; i < Q4_UNITS; ++i) {
-                float v[8];
-                raw_to_float(raw[i], v);
-                float m = 0.0f;
+            for (int i = 0; i < Q4_BLOCKS; ++i) {
+                if (u0 + i * stride >= blocks) continue;
+                uint32_t sb = 0;                        // what only fills up a scale tile gets scale 0
+                if (in[i]) {
+                    sb = fp4_scale_of(largest(raw[i]));
+                    const float inv = fp4_inverse_scale(sb);
+                    uint32_t w[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) m = magnitude_max(m, v[j]);
-                m = magnitude_max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = magnitude_max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                const uint32_t sb = fp4_scale_of(m);
-                const float inv = fp4_inverse_scale(sb);
-                const uint32_t codes8 = fp4_pack8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, v[4] * inv, v[5] * inv,
-                                                  v[6] * inv, v[7] * inv);
-                const uint32_t packed = sb != 255u ? codes8 : 0u;
-                uint32_t word = sb << (8 * (l >> 2));
-                word |= __shfl_xor_sync(0xffffffffu, word, 4);
-                word |= __shfl_xor_sync(0xffffffffu, word, 8);
-                if (in[i])
-                    *reinterpret_cast<uint32_t*>(c + (size_t)row[i] * (cols / 2) + tile[i] * 64 + l * 4) = packed;
-                // rows that only fill up a tile of 128 get scale 0, as the missing blocks of a row do
-                if (l == 0 && u0 + i * stride + half < units)
-                    *reinterpret_cast<uint32_t*>(sc + ((size_t)(row[i] >> 7) * tiles.d + tile[i]) * FP4_TILE_BYTES +
-                                                 fp4_tile_word(row[i])) = word;
+                    for (int j = 0; j < 4; ++j) {
+                        float v[8];
+                        eight(raw[i], j, v);
+                        w[j] = fp4_pack8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+                        if (sb == 255u) w[j] = 0;
+                    }
+                    *reinterpret_cast<uint4*>(c + (size_t)row[i] * (cols / 2) + block[i] * (FP4_BLOCK / 2)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                sc[((size_t)(row[i] >> 7) * (per_row.d >> 2) + (block[i] >> 2)) * FP4_TILE_BYTES + fp4_tile_word(row[i]) + (block[i] & 3)] = (uint8_t)sb;
             }
         }
     }
@@ -158,17 +181,17 @@ aristos_status_t check_fp4_shape(const char* what, int64_t mats, int64_t rows, i
         set_last_error("%s: sizes must not be negative and cols must be a multiple of 64", what);
         return ARISTOS_ERR_INVALID_ARG;
     }
-    // a matrix's units (row, 128 columns) are numbered in 31 bits
-    if (rows > (1 << 30) || (rows + 127) / 128 * 128 * (int64_t)fp4_col_tiles(cols) > (int64_t)1 << 30) {
-        set_last_error("%s: a matrix of more than 2^37 elements", what);
+    // a matrix's blocks are numbered in 31 bits
+    if (rows > (1 << 30) || (rows + 127) / 128 * 128 * 4 * (int64_t)fp4_col_tiles(cols) > (int64_t)1 << 30) {
+        set_last_error("%s: a matrix of more than 2^35 elements", what);
         return ARISTOS_ERR_CONFIG;
     }
     return ARISTOS_OK;
 }
 
-dim3 unit_grid(uint32_t units, int64_t mats) {
+dim3 unit_grid(uint32_t units, uint32_t per_cta, int64_t mats) {
     // enough CTAs to fill the device, no more than the units of a matrix ask for
-    const uint32_t need = (units + Q4_HALVES - 1) / Q4_HALVES;
+    const uint32_t need = (units + per_cta - 1) / per_cta;
     const int64_t fill = (int64_t)device_sm_count() * 8;
     const uint32_t y = (uint32_t)(mats < 65535 ? mats : 65535);
     int64_t x = (fill + y - 1) / y;
@@ -195,23 +218,23 @@ extern "C" aristos_status_t aristos_quantize_fp4(const void* src, int64_t mats, 
         set_last_error("quantize_fp4: pointers must be 16-byte aligned");
         return ARISTOS_ERR_INVALID_ARG;
     }
-    const Divider tiles = make_divider((uint32_t)fp4_col_tiles(cols));
-    const uint32_t units = (uint32_t)fp4_row_tiles((int)rows) * FP4_TILE_ROWS * tiles.d;
-    const dim3 grid = unit_grid(units, mats);
+    const Divider per_row = make_divider(4 * (uint32_t)fp4_col_tiles(cols));
+    const uint32_t blocks = (uint32_t)fp4_row_tiles((int)rows) * FP4_TILE_ROWS * per_row.d;
+    const dim3 grid = unit_grid(blocks, Q4_THREADS, mats);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     uint8_t *c = static_cast<uint8_t*>(codes), *s = static_cast<uint8_t*>(scales);
     switch (src_dtype) {
         case ARISTOS_DTYPE_F32:
             quantize_fp4_kernel<float><<<grid, Q4_THREADS, 0, st>>>(static_cast<const float*>(src), mats, (int)rows, cols,
-                                                                    units, tiles, c, s);
+                                                                    blocks, per_row, c, s);
             break;
         case ARISTOS_DTYPE_BF16:
             quantize_fp4_kernel<__nv_bfloat16><<<grid, Q4_THREADS, 0, st>>>(static_cast<const __nv_bfloat16*>(src), mats,
-                                                                            (int)rows, cols, units, tiles, c, s);
+                                                                            (int)rows, cols, blocks, per_row, c, s);
             break;
         case ARISTOS_DTYPE_F16:
             quantize_fp4_kernel<__half><<<grid, Q4_THREADS, 0, st>>>(static_cast<const __half*>(src), mats, (int)rows,
-                                                                     cols, units, tiles, c, s);
+                                                                     cols, blocks, per_row, c, s);
             break;
         default:
             set_last_error("quantize_fp4: source dtype must be f32, bf16 or f16");
@@ -233,7 +256,7 @@ extern "C" aristos_status_t aristos_dequantize_fp4(const void* codes, const void
     }
     const Divider tiles = make_divider((uint32_t)fp4_col_tiles(cols));
     const uint32_t units = (uint32_t)rows * tiles.d;
-    const dim3 grid = unit_grid(units, mats);
+    const dim3 grid = unit_grid(units, Q4_HALVES, mats);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint8_t *c = static_cast<const uint8_t*>(codes), *s = static_cast<const uint8_t*>(scales);
     switch (dst_dtype) {
