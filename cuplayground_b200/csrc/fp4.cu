@@ -17,7 +17,7 @@ namespace {
 
 constexpr int Q4_THREADS = 256;
 constexpr int Q4_HALVES = Q4_THREADS / 16;
-constexpr int Q4_UNITS = 4;
+constexpr int Q4_TILES = 4;                  // scale tiles (128 columns) of a row that a half warp turns back at a time
 
 // Division by a constant found at launch: u / d for u < 2^31.
 struct Divider {
@@ -128,50 +128,74 @@ quantize_fp4_kernel(const T* __restrict__ src, int64_t mats, int rows, int cols,
     }
 }
 
+// Eight codes with their scale byte to eight elements at dst.
+template <typename T>
+__device__ __forceinline__ void expand8(uint32_t w, uint32_t sb, T* dst) {
+    const float f = fp4_scale_value(sb);
+    float v[8];
+    uint32_t h[4];
+    fp4_unpack8(w, h);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+        v[2 * j] = p.x * f;
+        v[2 * j + 1] = p.y * f;
+    }
+    store8(dst, v);
+}
+// bf16 holds every element and every scale: the two bytes of an element come out of two byte tables, and one product of
+// pairs applies the scale exactly (half the instructions of the way through fp32).
+__device__ __forceinline__ void expand8(uint32_t w, uint32_t sb, __nv_bfloat16* dst) {
+    const uint32_t scale = sb == 255u ? 0x7FFFu : (sb == 0u ? 0x0040u : sb << 7);
+    const uint32_t scale2 = scale | scale << 16, mag = w & 0x77777777u, up = w << 4;
+    uint32_t v[4];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const uint32_t sel = half == 0 ? mag : mag >> 16;
+        // 0, 0.5, 1, 1.5 | 2, 3, 4, 6 = 0000 3F00 3F80 3FC0 | 4000 4040 4080 40C0
+        uint32_t hi = __byte_perm(0x3F3F3F00u, 0x40404040u, sel), sign;
+        const uint32_t lo = __byte_perm(0xC0800000u, 0xC0804000u, sel);
+        if (half == 0) asm("prmt.b32 %0, %1, %2, 0x9D8C;" : "=r"(sign) : "r"(w), "r"(up));
+        else asm("prmt.b32 %0, %1, %2, 0xBFAE;" : "=r"(sign) : "r"(w), "r"(up));
+        hi |= sign & 0x80808080u;
+        v[2 * half] = __byte_perm(lo, hi, 0x5140);
+        v[2 * half + 1] = __byte_perm(lo, hi, 0x7362);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(v[j]) : "r"(scale2));
+    *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(Q4_THREADS)
 dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t mats, int rows,
-                      int cols, uint32_t units, Divider tiles, T* __restrict__ dst) {
+                      int cols, uint32_t units, Divider per_row, T* __restrict__ dst) {
     const int l = threadIdx.x & 15;
     const uint32_t half = blockIdx.x * Q4_HALVES + (threadIdx.x >> 4);
     const uint32_t stride = gridDim.x * Q4_HALVES;
+    const uint32_t tiles = (uint32_t)fp4_col_tiles(cols);
     const size_t mat_scales = fp4_matrix_scale_bytes(rows, cols);
     for (int64_t mat = blockIdx.y; mat < mats; mat += gridDim.y) {
         T* d = dst + (size_t)mat * rows * cols;
         const uint8_t* c = codes + (size_t)mat * rows * (cols / 2);
         const uint8_t* sc = scales + (size_t)mat * mat_scales;
-        for (uint32_t u0 = half; u0 < units; u0 += stride * Q4_UNITS) {
-            uint32_t word[Q4_UNITS], sword[Q4_UNITS];
-            size_t at[Q4_UNITS];
-            bool in[Q4_UNITS];
+        for (uint32_t u = half; u < units; u += stride) {
+            const uint32_t row = divide(u, per_row), tile = (u - row * per_row.d) * Q4_TILES;
+            const uint32_t col = tile * FP4_TILE_COLS + l * 8;
+            const size_t at = (size_t)row * cols + col;
+            const uint8_t* from = c + at / 2;
+            const uint8_t* sf = sc + ((size_t)(row >> 7) * tiles + tile) * FP4_TILE_BYTES + fp4_tile_word(row) + (l >> 2);
+            T* to = d + at;
+            uint32_t word[Q4_TILES], sb[Q4_TILES];
 #pragma unroll
-            for (int i = 0; i < Q4_UNITS; ++i) {
-                const uint32_t u = u0 + i * stride;
-                const uint32_t row = divide(u, tiles), tile = u - row * tiles.d;
-                in[i] = u < units && tile * 128 + l * 8 < (uint32_t)cols;
-                at[i] = (size_t)row * cols + tile * 128 + l * 8;
-                word[i] = sword[i] = 0;
-                if (in[i]) {
-                    word[i] = __ldcs(reinterpret_cast<const uint32_t*>(c + at[i] / 2));
-                    sword[i] = __ldg(reinterpret_cast<const uint32_t*>(
-                        sc + ((size_t)(row >> 7) * tiles.d + tile) * FP4_TILE_BYTES + fp4_tile_word(row)));
+            for (int i = 0; i < Q4_TILES; ++i)
+                if (col + i * FP4_TILE_COLS < (uint32_t)cols) {
+                    word[i] = __ldcs(reinterpret_cast<const uint32_t*>(from + i * (FP4_TILE_COLS / 2)));
+                    sb[i] = __ldg(sf + i * FP4_TILE_BYTES);
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < Q4_UNITS; ++i) {
-                if (!in[i]) continue;
-                const float f = fp4_scale_value((sword[i] >> (8 * (l >> 2))) & 255u);
-                float v[8];
-                uint32_t h[4];
-                fp4_unpack8(word[i], h);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-                    v[2 * j] = p.x * f;
-                    v[2 * j + 1] = p.y * f;
-                }
-                store8(d + at[i], v);
-            }
+            for (int i = 0; i < Q4_TILES; ++i)
+                if (col + i * FP4_TILE_COLS < (uint32_t)cols) expand8(word[i], sb[i], to + i * FP4_TILE_COLS);
         }
     }
 }
@@ -254,22 +278,22 @@ extern "C" aristos_status_t aristos_dequantize_fp4(const void* codes, const void
         set_last_error("dequantize_fp4: pointers must be 16-byte aligned");
         return ARISTOS_ERR_INVALID_ARG;
     }
-    const Divider tiles = make_divider((uint32_t)fp4_col_tiles(cols));
-    const uint32_t units = (uint32_t)rows * tiles.d;
+    const Divider per_row = make_divider((uint32_t)ceil_div(fp4_col_tiles(cols), Q4_TILES));
+    const uint32_t units = (uint32_t)rows * per_row.d;
     const dim3 grid = unit_grid(units, Q4_HALVES, mats);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint8_t *c = static_cast<const uint8_t*>(codes), *s = static_cast<const uint8_t*>(scales);
     switch (dst_dtype) {
         case ARISTOS_DTYPE_F32:
-            dequantize_fp4_kernel<float><<<grid, Q4_THREADS, 0, st>>>(c, s, mats, (int)rows, cols, units, tiles,
+            dequantize_fp4_kernel<float><<<grid, Q4_THREADS, 0, st>>>(c, s, mats, (int)rows, cols, units, per_row,
                                                                       static_cast<float*>(dst));
             break;
         case ARISTOS_DTYPE_BF16:
-            dequantize_fp4_kernel<__nv_bfloat16><<<grid, Q4_THREADS, 0, st>>>(c, s, mats, (int)rows, cols, units, tiles,
+            dequantize_fp4_kernel<__nv_bfloat16><<<grid, Q4_THREADS, 0, st>>>(c, s, mats, (int)rows, cols, units, per_row,
                                                                               static_cast<__nv_bfloat16*>(dst));
             break;
         case ARISTOS_DTYPE_F16:
-            dequantize_fp4_kernel<__half><<<grid, Q4_THREADS, 0, st>>>(c, s, mats, (int)rows, cols, units, tiles,
+            dequantize_fp4_kernel<__half><<<grid, Q4_THREADS, 0, st>>>(c, s, mats, (int)rows, cols, units, per_row,
                                                                        static_cast<__half*>(dst));
             break;
         default:
