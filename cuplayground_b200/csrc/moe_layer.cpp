@@ -78,6 +78,8 @@ struct aristos_moe {
     int32_t *send_base = nullptr, *dense_count = nullptr, *src_off = nullptr;
     int32_t* ffn_done = nullptr;             // counters of the one-launch expert FFN (groups x row tiles)
     size_t ffn_done_ints = 0;
+    void* few_ws = nullptr;                  // decode (few tokens): workspace for ARISTOS_FEW_TOKENS_MAX tokens
+    size_t few_ws_bytes = 0;                 // 0: this layer has no decode
     int64_t launches = 0;
     const void *b1 = nullptr, *b3 = nullptr, *b2 = nullptr;   // optional expert biases (caller-owned, device)
     // failure handling of the exchange: every wait for a forward's completion has a wall-clock limit; on expiry the
@@ -174,6 +176,7 @@ size_t plan_workspace(aristos_moe* L, char* base) {
         L->xr = L->xg;
         L->yg = L->yr;
     }
+    if (L->few_ws_bytes) CARVE(few_ws, void*, L->few_ws_bytes)
     for (int i = 0; i < aristos_moe::HOST_SLOTS; ++i) {
         CARVE(slots[i].x_dev, void*, S * H * elt)
         CARVE(slots[i].out_dev, void*, S * H * elt)
@@ -364,6 +367,8 @@ aristos_status_t aristos_moe_create(const aristos_config_t* cfg, int rank, int w
             }
         }
     }
+    if (world == 1 && (L->fp8 || cfg->torch_dtype == ARISTOS_DTYPE_BF16 || cfg->torch_dtype == ARISTOS_DTYPE_F16))
+        L->few_ws_bytes = aristos_moe_few_tokens_workspace_bytes(ARISTOS_FEW_TOKENS_MAX, L->H, L->I, L->E, L->k);
     L->ws_bytes = plan_workspace(L, nullptr);
     *out = L;
     return ARISTOS_OK;
@@ -426,15 +431,10 @@ aristos_status_t aristos_moe_forward(aristos_moe_t* L, const void* x, const void
     return s;
 }
 
-static aristos_status_t forward_impl(aristos_moe_t* L, const void* x, const void* w_gate, const float* gate_bias,
-                                     const void* w1, const void* w3, const void* w2, const void* scales, void* out,
-                                     void* stream, bool* exchange_started) {
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int64_t launches0 = launch_counter();
-    const int dt = L->fp8 ? ARISTOS_DTYPE_BF16 : L->cfg.torch_dtype;     // dtype of x, out and the expert outputs
-
-    const float* bias = gate_bias;
-    if (!bias && L->cfg.gate_bias_zipf_s > 0.0) {
+// The prior that the gate adds: the caller's, the layer's own Zipf prior (uploaded at its first use), or none.
+static aristos_status_t gate_prior(aristos_moe_t* L, const float* gate_bias, cudaStream_t st, const float** bias) {
+    *bias = gate_bias;
+    if (!gate_bias && L->cfg.gate_bias_zipf_s > 0.0) {
         if (!L->bias_ready) {
             std::vector<float> b(L->E);
             aristos_zipf_bias_host(b.data(), L->E, L->cfg.gate_bias_zipf_s);
@@ -442,8 +442,51 @@ static aristos_status_t forward_impl(aristos_moe_t* L, const void* x, const void
             ARISTOS_CUDA_TRY(cudaStreamSynchronize(st));   // b goes out of scope
             L->bias_ready = true;
         }
-        bias = L->gate_bias;
+        *bias = L->gate_bias;
     }
+    return ARISTOS_OK;
+}
+
+aristos_status_t aristos_moe_decode(aristos_moe_t* L, const void* x, int tokens, const void* w_gate,
+                                    const float* gate_bias, const void* w1, const void* w3, const void* w2,
+                                    const void* scales, void* out, int32_t* topk_idx, float* topk_w, void* stream) {
+    if (!L) { set_last_error("decode: NULL layer"); return ARISTOS_ERR_INVALID_ARG; }
+    if (L->few_ws_bytes == 0) {
+        set_last_error("decode: needs a layer on one rank with bf16, fp16 or fp8 (torch_dtype 2, 3, 4), H and I multiples "
+                       "of 64 and at most 512 experts");
+        return ARISTOS_ERR_UNSUPPORTED;
+    }
+    if (tokens < 0 || tokens > ARISTOS_FEW_TOKENS_MAX) {
+        set_last_error("decode: %d tokens, 0 to %d are possible", tokens, (int)ARISTOS_FEW_TOKENS_MAX);
+        return ARISTOS_ERR_INVALID_ARG;
+    }
+    if (tokens == 0) return ARISTOS_OK;
+    if (L->fp8 && !scales) { set_last_error("decode: fp8 needs the weight scales"); return ARISTOS_ERR_INVALID_ARG; }
+    ARISTOS_TRY(ensure_workspace(L));
+    const float* bias = nullptr;
+    ARISTOS_TRY(gate_prior(L, gate_bias, static_cast<cudaStream_t>(stream), &bias));
+    const bool swiglu = L->cfg.hidden_act == ARISTOS_ACT_SWIGLU;
+    const float* s1 = L->fp8 ? static_cast<const float*>(scales) : nullptr;
+    const size_t nb = (size_t)L->E * (L->I / 128) * (L->H / 128);
+    const int64_t launches0 = launch_counter();
+    const aristos_status_t s = aristos_moe_few_tokens(
+        x, w_gate, bias, w1, w3, w2, s1, L->fp8 && swiglu ? s1 + nb : nullptr, L->fp8 ? s1 + nb * (swiglu ? 2 : 1) : nullptr,
+        L->b1, L->b3, L->b2, tokens, L->H, L->I, L->E, L->k, L->cfg.gate_fn, L->cfg.renorm_topk, L->cfg.hidden_act,
+        L->fp8 ? ARISTOS_DTYPE_BF16 : L->cfg.torch_dtype, L->cfg.torch_dtype, out, topk_idx, topk_w, L->few_ws,
+        L->few_ws_bytes, L->dev_status, stream);
+    L->launches += launch_counter() - launches0;
+    return s;
+}
+
+static aristos_status_t forward_impl(aristos_moe_t* L, const void* x, const void* w_gate, const float* gate_bias,
+                                     const void* w1, const void* w3, const void* w2, const void* scales, void* out,
+                                     void* stream, bool* exchange_started) {
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int64_t launches0 = launch_counter();
+    const int dt = L->fp8 ? ARISTOS_DTYPE_BF16 : L->cfg.torch_dtype;     // dtype of x, out and the expert outputs
+
+    const float* bias = nullptr;
+    ARISTOS_TRY(gate_prior(L, gate_bias, st, &bias));
 
     const int prof_set = (int)(L->prof_n % aristos_moe::PROF_SETS) * aristos_moe::PROF_EVENTS;
     L->prof_sent = false;

@@ -497,6 +497,22 @@ class MoELayer:
     def wait_host(self) -> None:
         _lib.check(self._lib.aristos_moe_wait_host(self._h))
 
+    def decode(self, x, w_gate, w1, w3, w2, gate_bias=None, out=None, stream=None, scales=None):
+        """The forward for up to 64 tokens, x (tokens, H): two kernels, nothing dropped, activations not quantised. Returns
+        (out, topk_idx (tokens, k), topk_w (tokens, k)). See aristos_moe_decode."""
+        if x.dim() != 2 or x.shape[1] != self.H or x.dtype != self.dtype:
+            raise ValueError(f"x must be {self.dtype} (tokens, {self.H}), got {x.dtype} {tuple(x.shape)}")
+        with torch.cuda.stream(stream):              # outputs belong to the stream that writes them
+            out = torch.empty_like(x) if out is None else out
+            idx = torch.empty((x.shape[0], self.k), dtype=torch.int32, device=x.device)
+            w = torch.empty((x.shape[0], self.k), dtype=torch.float32, device=x.device)
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("out must have x's shape and dtype")
+        _lib.check(self._lib.aristos_moe_decode(self._h, _ptr(x), x.shape[0], _ptr(w_gate), _ptr(gate_bias), _ptr(w1),
+                                                _ptr(w3), _ptr(w2), _ptr(scales), _ptr(out), _ptr(idx), _ptr(w),
+                                                _stream_ptr(stream)))
+        return out, idx, w
+
     def routing(self) -> dict:
         """Host copies (CPU torch tensors) of the routing tensors of the last forward."""
         S, k, E, cap = self.S, self.k, self.E, self.cap

@@ -52,6 +52,22 @@ def _(x, w_gate, w1, w3, w2, scales, handle):
     return torch.empty_like(x)
 
 
+@torch.library.custom_op("aristos::moe_decode", mutates_args=(), device_types="cuda")
+def moe_decode(x: torch.Tensor, w_gate: torch.Tensor, w1: torch.Tensor, w3: Optional[torch.Tensor],
+               w2: torch.Tensor, scales: Optional[torch.Tensor], handle: int) -> torch.Tensor:
+    """out (tokens, H) of up to 64 tokens x (tokens, H) through aristos_moe_decode; the other arguments as moe_forward's."""
+    try:
+        layer = _LAYERS[handle]
+    except KeyError:
+        raise RuntimeError(f"aristos::moe_decode: unknown layer handle {handle}") from None
+    return layer.decode(x.contiguous(), w_gate, w1, w3, w2, scales=scales)[0]
+
+
+@moe_decode.register_fake
+def _(x, w_gate, w1, w3, w2, scales, handle):
+    return torch.empty_like(x)
+
+
 class AristosMoE(torch.nn.Module):
     """The layer as a module: owns the gate and (this rank's) expert weights as parameters in the reference layouts
     (weights (out, in) row-major) and a library handle. Forward only (the parameters do not receive gradients)."""
@@ -79,6 +95,13 @@ class AristosMoE(torch.nn.Module):
         shape = x.shape
         out = torch.ops.aristos.moe_forward(x.reshape(-1, shape[-1]), self.w_gate, self.w1, self.w3, self.w2, None,
                                             self._handle)
+        return out.reshape(shape)
+
+    def decode(self, x: torch.Tensor) -> torch.Tensor:
+        """The layer on up to 64 tokens, x (..., H): a serving step. No token is dropped."""
+        shape = x.shape
+        out = torch.ops.aristos.moe_decode(x.reshape(-1, shape[-1]), self.w_gate, self.w1, self.w3, self.w2, None,
+                                           self._handle)
         return out.reshape(shape)
 
     def close(self) -> None:

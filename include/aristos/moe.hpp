@@ -76,6 +76,11 @@ public:
                  void* stream = nullptr, const float* gate_bias = nullptr) {
         check(aristos_moe_forward(h_, x, w_gate, gate_bias, w1, w3, w2, nullptr, out, stream));
     }
+    // A few tokens (a serving step): x, out (tokens, H), tokens <= ARISTOS_FEW_TOKENS_MAX; scales: fp8 layers only.
+    void decode(const void* x, int tokens, const void* w_gate, const void* w1, const void* w3, const void* w2, void* out,
+                void* stream = nullptr, const float* gate_bias = nullptr, const void* scales = nullptr) {
+        check(aristos_moe_decode(h_, x, tokens, w_gate, gate_bias, w1, w3, w2, scales, out, nullptr, nullptr, stream));
+    }
     // Host activations in, host result out (weights stay on the device); returns when out_host is complete.
     void forward_host(const void* x_host, const void* w_gate, const void* w1, const void* w3, const void* w2,
                       void* out_host, void* stream = nullptr, const float* gate_bias = nullptr) {

@@ -115,6 +115,8 @@ ARISTOS_API int aristos_config_capacity(const aristos_config_t* cfg); /* rows pe
 /* Host helper: the Zipf prior of the skewed-routing case, bias_host[e] = -s*ln(e+1) as fp32. */
 ARISTOS_API aristos_status_t aristos_zipf_bias_host(float* bias_host, int num_experts, double s);
 
+enum { ARISTOS_FEW_TOKENS_MAX = 64 };   /* tokens of aristos_moe_few_tokens and aristos_moe_decode */
+
 /* ---- layer: replaces the allocate/launch/sync/free harnesses (mma.cuh:371-443, overlap.cuh:159-242) -------- */
 /* nccl_unique_id: 128 bytes from aristos_nccl_unique_id on rank 0, shared by the caller; NULL when world == 1.
  * The CUDA device current at this call becomes the layer's device. */
@@ -174,6 +176,19 @@ ARISTOS_API aristos_status_t aristos_moe_submit_host(aristos_moe_t* layer, const
                                                      const void* w2, const void* scales, void* out_host,
                                                      void* stream);
 ARISTOS_API aristos_status_t aristos_moe_wait_host(aristos_moe_t* layer);
+/*
+ * The layer's forward for a few tokens (a serving step; 0 <= tokens <= ARISTOS_FEW_TOKENS_MAX, whatever the layer's own
+ * token count is): two kernels that read the chosen experts' weights once (aristos_moe_few_tokens), with the layer's gate,
+ * activation and biases and the arguments of aristos_moe_forward. x, out (tokens, H). No token is dropped, fp8 layers do
+ * not quantise the activations, and nothing that aristos_moe_routing or aristos_moe_training_state returns changes;
+ * topk_idx / topk_w (tokens, k) receive this call's routing, or NULL. One rank, torch_dtype 2, 3 or 4, E <= 512, else
+ * ARISTOS_ERR_UNSUPPORTED. Uses the layer's workspace (which the first forward or decode allocates: outside a capture):
+ * calls of one handle are ordered by the caller, as forwards are.
+ */
+ARISTOS_API aristos_status_t aristos_moe_decode(aristos_moe_t* layer, const void* x, int tokens, const void* w_gate,
+                                                const float* gate_bias, const void* w1, const void* w3, const void* w2,
+                                                const void* scales, void* out, int32_t* topk_idx, float* topk_w,
+                                                void* stream);
 ARISTOS_API aristos_status_t aristos_moe_routing(const aristos_moe_t* layer, aristos_routing_t* out);
 /* Copies the routing tensors of the last forward into host buffers sized as in aristos_routing_t (any pointer may
  * be NULL); synchronises the device first. */
@@ -382,12 +397,12 @@ ARISTOS_API aristos_status_t aristos_expert_ffn_fp4(const void* xq, const void* 
  * ARISTOS_FEW_TOKENS_MAX; w_gate (E, H) and the optional biases b1 / b3 (E, I), b2 (E, H) in the same dtype; gate_bias
  * (E) fp32 or NULL. weights_dtype: `dtype` itself, ARISTOS_DTYPE_FP8_E4M3 (bf16 activations only; s1 / s3 / s2 fp32 as
  * aristos_quantize_fp8(block_rows = 128) writes them; H and I multiples of 128) or ARISTOS_DTYPE_FP4_E2M1 (codes and
- * scale tiles of aristos_quantize_fp4). Activations are not quantised. The routing is aristos_gate_topk's, bit for bit;
+ * scale tiles of aristos_quantize_fp4; a scale byte 0 counts as zero, 255 makes the row's results infinite or NaN). E <= 512.
+ * Activations are not quantised. The routing is aristos_gate_topk's, bit for bit;
  * no token is dropped. topk_idx / topk_w (tokens, k) receive it, or NULL. workspace:
  * aristos_moe_few_tokens_workspace_bytes (0: sizes out of range) on the device, owned by the caller; it needs no
  * initialisation, and calls that may overlap on the GPU need one each.
  */
-enum { ARISTOS_FEW_TOKENS_MAX = 64 };
 ARISTOS_API size_t aristos_moe_few_tokens_workspace_bytes(int tokens, int H, int I, int E, int k);
 ARISTOS_API aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_gate, const float* gate_bias,
                                                     const void* w1, const void* w3, const void* w2, const void* s1,

@@ -231,3 +231,74 @@ def test_refusals():
     with pytest.raises(cp.AristosError) as e:                          # 8-bit weights go with bf16 tokens
         f.run()
     assert e.value.status == 6
+
+
+# ---- through the layer handle -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("torch_dtype,H,I,act", [(2, 256, 320, 2), (3, 192, 256, 1), (4, 512, 256, 2), (2, 128, 128, 0)])
+def test_decode_of_a_layer(torch_dtype, H, I, act):
+    """decode on a handle made for many tokens: the same bits as the stage, between forwards that it leaves alone."""
+    torch, cp, layer = _mods()
+    E, k, n = 8, 2, 5
+    cfg = cp.AristosConfig(capacity_factor=1.25, drop_tokens=1, expert_top_k=k, hidden_act=act, hidden_size=H,
+                           intermediate_size=I, num_experts=E, torch_dtype=torch_dtype, tokens=256, renorm_topk=1,
+                           gate_bias_zipf_s=0.3)
+    c = Case(n, E, k, H, I, act, "8" if torch_dtype == 4 else "16", "float16" if torch_dtype == 3 else "bfloat16", renorm=1)
+    L = layer.MoELayer(cfg)
+    scales = None
+    if torch_dtype == 4:
+        scales = torch.cat([c.s[m].reshape(-1) for m in ("1", "3", "2") if m in c.s]).contiguous()
+    weights = (c.wg, c.w["1"], c.w.get("3"), c.w["2"])
+    big = torch.randn(256, H, device="cuda").to(c.dt)
+    full = L.forward(big, *weights, scales=scales)
+    routing = L.routing()
+    c.gate_bias = layer.zipf_prior(E, 0.3).cuda()
+    want = c.run()
+    launches = L.launch_count
+    got = L.decode(c.x, *weights, scales=scales)
+    assert L.launch_count - launches == 2
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    other = L.decode(c.x, *weights, scales=scales, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b, o in zip(got, want, other):
+        assert torch.equal(a, b) and torch.equal(o, b)
+    L.status()
+    again = L.routing()
+    assert all(torch.equal(routing[m], again[m]) for m in ("topk_idx", "topk_w", "slot_of", "count"))
+    assert torch.equal(L.forward(big, *weights, scales=scales), full)
+    if torch_dtype != 4:
+        b1, b2 = (torch.randn(E, s, device="cuda").to(c.dt) for s in (I, H))
+        L.set_bias(b1=b1, b2=b2)
+        c.b["1"], c.b["2"] = b1, b2
+        assert torch.equal(L.decode(c.x, *weights)[0], c.run()[0])
+    assert L.decode(c.x[:0], *weights, scales=scales)[0].shape == (0, H)
+    with pytest.raises(cp.AristosError) as e:
+        L.decode(big, *weights, scales=scales)
+    assert e.value.status == 1 and "64" in str(e.value)
+    with pytest.raises(ValueError):
+        L.decode(c.x.float(), *weights, scales=scales)
+    L.close()
+
+
+def test_decode_is_refused_where_the_layer_has_none():
+    torch, cp, layer = _mods()
+    L = layer.MoELayer(cp.AristosConfig(hidden_size=128, intermediate_size=128, num_experts=4, torch_dtype=0, tokens=128))
+    x, wg = torch.zeros(2, 128, device="cuda"), torch.zeros(4, 128, device="cuda")
+    w = torch.zeros(4, 128, 128, device="cuda")
+    with pytest.raises(cp.AristosError) as e:
+        L.decode(x, wg, w, None, w)
+    assert e.value.status == 6
+    L.close()
+
+
+def test_module_decode():
+    torch, cp, layer = _mods()
+    from cuplayground_b200.torch_op import AristosMoE
+    cfg = cp.AristosConfig(expert_top_k=2, hidden_act=2, hidden_size=256, intermediate_size=512, num_experts=8,
+                           torch_dtype=2, tokens=512, renorm_topk=1)
+    m = AristosMoE(cfg)
+    x = torch.randn(2, 3, 256, device="cuda", dtype=torch.bfloat16)
+    out = m.decode(x)
+    want = layer.moe_few_tokens(x.reshape(6, 256), m.w_gate, m.w1, m.w3, m.w2, 2, 2, renorm=1)[0]
+    assert torch.equal(out, want.reshape(2, 3, 256))
+    m.close()
