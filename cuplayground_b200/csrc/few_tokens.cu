@@ -1,5 +1,6 @@
 // The whole mixture-of-experts layer for a few tokens (aristos_moe_few_tokens): what a serving step with 1 to 64 tokens
-// runs instead of gate -> dispatch -> gather -> expert GEMMs -> combine, in two kernels.
+// runs instead of gate -> dispatch -> gather -> expert GEMMs -> combine, in two kernels. This file has the gate and, for
+// 16-bit and 8-bit weights, the experts; few_fp4_sm100.cu has them for 4-bit weights.
 //
 //   l[t, e] = x[t] . Wg[e] + bias[e] (the bit-exact contract of gate_contract.cuh), top-k, softmax or sigmoid weights w;
 //   h[t, j] = act(x[t] W1^T + b1) or silu(x[t] W1^T + b1) * (x[t] W3^T + b3) with the weights of expert idx[t, j];
@@ -23,24 +24,24 @@
 //    bounded). Up items never wait and come first in every group's list, so the wait ends.
 //  * The products run on the warp-level matrix instruction m16n8k16: 16 weight rows (gate and up rows of the same
 //    columns for SwiGLU) x 8 tokens x 16 of K. The order of K inside a step does not matter to the sum, so a lane uses
-//    whole 16-byte pieces of a row (4-bit: 4 bytes of each block) and reads the tokens in the same order. The 5th-generation tensor cores would need 128
+//    whole 16-byte pieces of a row and reads the tokens in the same order. The 5th-generation tensor cores would need 128
 //    weight rows per instruction and both operands in shared memory, for a rate that this stream cannot use.
 //  * When all down items are done (counted once per group), all streaming warps add up the expert outputs of the tokens,
 //    in the order of j.
 //
 // Operand types. The instruction multiplies 16-bit numbers. bf16 weights meet tokens in bf16 (as they are) and hidden
 // activations as two bf16 numbers, value and remainder: a single rounding of h to bf16 would by itself be as large as
-// that of the output. fp16, e4m3 and e2m1 weights meet fp16 numbers, in which all three are exact; bf16 tokens and the
-// hidden activations are brought into fp16's range by a power of two per token (the largest magnitude to [2^14, 2^15)),
+// that of the output. fp16 and e4m3 weights meet fp16 numbers, in which both are exact; bf16 tokens and the hidden
+// activations are brought into fp16's range by a power of two per token (the largest magnitude to [2^14, 2^15)),
 // which is undone on the fp32 sums: bf16 tokens lose nothing that is not 2^-40 of the token's largest element, hidden
-// activations are rounded once to 11 bits. h itself is kept in fp32. Scales of quantised weights multiply fp32 sums:
-// e4m3's per step (half of its 128 columns), e2m1's per block of 32.
+// activations are rounded once to 11 bits. h itself is kept in fp32. e4m3's scales multiply the fp32 sums of a step, which
+// is one of their blocks of 128 columns.
 #include <cuda_fp8.h>
 
 #include <type_traits>
 
 #include "common.cuh"
-#include "fp4_format.cuh"
+#include "few_common.cuh"
 #include "gate_contract.cuh"
 #include "ptx_sm100.cuh"
 #include "tensor_map.cuh"
@@ -48,11 +49,6 @@
 namespace aristos {
 
 namespace {
-
-constexpr int FEW_MAX_TOKENS = ARISTOS_FEW_TOKENS_MAX;
-constexpr int FEW_MAX_EXPERTS = 512;
-constexpr int FEW_MAX_SLOTS = FEW_MAX_TOKENS * MAX_TOPK;
-static_assert(FEW_MAX_TOKENS <= 64, "the expert lists keep the tokens of an expert in 64 bits");
 
 constexpr int FEW_W = 7;                                  // warps that share an item (two groups and two helpers: 16 warps of 128 registers)
 constexpr int FEW_GROUPS = 2;                             // groups per CTA
@@ -62,28 +58,7 @@ constexpr int FEW_THREADS = 32 * FEW_WARPS;
 
 constexpr int FEW_MAX_DEPTH = 6;
 
-enum { FEW_BF16 = 0, FEW_F16 = 1, FEW_FP8 = 2, FEW_FP4 = 3 };      // weight formats
-
-struct FewParams {
-    const float* logits;
-    const uint16_t* x;             // (n, H) in the operand type
-    const float* x_scale;          // (n) what the sums of a token are multiplied with, or NULL: 1
-    const uint8_t *s1, *s3, *s2;   // fp8: fp32 per 128 x 128; fp4: scale tiles
-    const void *b1, *b3, *b2;      // activations' dtype, or NULL
-    float* h;                      // (slots, I)
-    uint32_t* h_max;               // (slots) bits of the largest |h| of a row
-    float* partial;                // (parts, slots, H)
-    int32_t* done;                 // up items finished, per chosen expert
-    int32_t* finished;             // CTAs that have written all their expert outputs
-    void* out;
-    int32_t* topk_idx;
-    float* topk_w;
-    int32_t* dev_status;
-    int n, H, I, E, k;
-    int gate_fn, renorm, act;
-    int parts;                     // K of the down projection is cut into so many items
-    int f16;                       // dtype of out and of the biases: fp16, else bf16
-};
+enum { FEW_BF16 = 0, FEW_F16 = 1, FEW_FP8 = 2 };      // weight formats
 
 // The power of two that brings a largest magnitude (its bits) to [2^14, 2^15) and the one that undoes it. Zero, and what
 // is not finite, stays as it is; the exponent is bounded so that both are normal numbers.
@@ -96,19 +71,39 @@ __device__ __forceinline__ float few_norm(uint32_t max_bits, bool undo) {
 // ---- gate --------------------------------------------------------------------------------------------------------------
 constexpr int FEW_GATE_WARPS = 8;
 
-// TOK: tokens per warp (the gate weights are read once for them). With x_norm the first n blocks bring a token each into
-// fp16, scaled by a power of two.
-template <typename T, int TOK>
+// What the experts' kernel needs of the tokens: as they are, in fp16 (scaled by a power of two), or split into 4-bit terms.
+enum { PREP_NONE = 0, PREP_F16 = 1, PREP_TERMS = 2 };
+
+// TOK: tokens per warp (the gate weights are read once for them). The first n blocks prepare a token each: x_prep receives
+// the fp16 numbers or the terms, x_scale the factors (fp32) or the scale bytes.
+template <typename T, int TOK, int PREP>
 __global__ void __launch_bounds__(FEW_GATE_WARPS * 32)
 few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* __restrict__ bias, int n, int H, int E,
-                float* __restrict__ logits, int32_t* __restrict__ counters, int ncounters, __half* __restrict__ x_norm,
-                float* __restrict__ x_scale) {
+                float* __restrict__ logits, int32_t* __restrict__ counters, int ncounters, uint8_t* __restrict__ x_prep,
+                uint8_t* __restrict__ x_scale) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < ncounters; i += gridDim.x * blockDim.x) counters[i] = 0;
     const int nchunk = H >> 3;
     int block = blockIdx.x;
-    if (x_norm) {
+    if constexpr (PREP == PREP_TERMS) {
+        if (block < n) {
+            const int q = threadIdx.x & 7;
+            for (int c0 = 0; c0 < H; c0 += FEW_GATE_WARPS * 128) {      // 128 columns per warp, four per lane
+                const int c = c0 + (threadIdx.x >> 3) * 32 + 4 * q;
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (c < H) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(x[(size_t)block * H + c + j]);
+                }
+                few_split(v, c < H, x_prep + (size_t)block * FEW_TERMS * (H / 2) + c / 2, H / 2,
+                          x_scale + (size_t)block * few_scale_pitch(H) + c / 32);
+            }
+            return;
+        }
+        block -= n;
+    }
+    if constexpr (PREP == PREP_F16) {
         if (block < n) {
             __shared__ uint32_t s_max;
             if (threadIdx.x == 0) s_max = 0;
@@ -132,9 +127,9 @@ few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* 
                 load8(row + q * 8, v);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] *= f;
-                store8(x_norm + (size_t)block * H + q * 8, v);
+                store8(reinterpret_cast<__half*>(x_prep) + (size_t)block * H + q * 8, v);
             }
-            if (threadIdx.x == 0) x_scale[block] = few_norm(s_max, true);
+            if (threadIdx.x == 0) reinterpret_cast<float*>(x_scale)[block] = few_norm(s_max, true);
             return;
         }
         block -= n;
@@ -183,76 +178,12 @@ few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* 
 // ---- the experts ---------------------------------------------------------------------------------------------------------
 constexpr int FEW_POST = 64;               // finished items that may wait to be counted
 
-struct FewLists {
+struct FewLists : FewRouting {
     uint64_t bars[FEW_GROUPS * 4];             // per group: sums written (2 buffers), buffer free (2)
     uint64_t full[FEW_STREAM_WARPS * FEW_MAX_DEPTH];   // per streaming warp: step arrived
-    float w[FEW_MAX_SLOTS];                    // combine weights (t, j)
-    uint32_t mask[FEW_MAX_EXPERTS][2];         // tokens that chose an expert
-    uint16_t idx[FEW_MAX_SLOTS];               // chosen experts (t, j)
-    uint16_t slot[FEW_MAX_SLOTS];              // row of h / partial of (t, j)
-    uint16_t base[FEW_MAX_EXPERTS];            // first row of an expert
-    uint16_t active[FEW_MAX_EXPERTS];          // chosen experts, increasing
-    uint8_t token[FEW_MAX_SLOTS];              // token of a row
-    uint8_t chunks[FEW_MAX_EXPERTS];           // per chosen expert: its tokens are taken in so many passes
-    int actives;                               // chosen experts
     int post[FEW_POST];                        // from the adding to the counting helper: whose up item is done; -1: the end
     int posted, counted;
-    int abort;
 };
-
-// Top-k of one token by one warp: the selection and the weights of the gate kernels, bit for bit (gate.cu). PER logits
-// per lane; lane j ends up with the choice number j. Kept small: every CTA runs it once, out of a cold instruction cache.
-template <int PER>
-__device__ __forceinline__ void few_topk(const float* __restrict__ l, const FewParams& p, int t, int lane, FewLists& s) {
-    float v[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = i * 32 + lane < p.E ? __ldcg(l + i * 32 + lane) : 0.0f;
-    uint32_t taken = 0;
-    float my_l = 0.0f;
-#pragma unroll 1
-    for (int j = 0; j < p.k; ++j) {
-        float bv = 0.0f;
-        int bi = -1;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (i * 32 + lane < p.E && !(taken >> i & 1) && (bi < 0 || v[i] > bv)) { bv = v[i]; bi = i * 32 + lane; }
-#pragma unroll
-        for (int m = 16; m >= 1; m >>= 1) {
-            const float ov = __shfl_xor_sync(0xffffffffu, bv, m);
-            const int oi = __shfl_xor_sync(0xffffffffu, bi, m);
-            const bool take = (oi >= 0) && (bi < 0 || ov > bv || (ov == bv && oi < bi));
-            if (take) { bv = ov; bi = oi; }
-        }
-        // lanes can disagree only where NaN logits break the order: lane 0 decides
-        bi = __shfl_sync(0xffffffffu, bi, 0);
-        bv = __shfl_sync(0xffffffffu, bv, 0);
-        if ((bi & 31) == lane) taken |= 1u << (bi >> 5);
-        if (lane == j) {
-            my_l = bv;
-            s.idx[t * p.k + j] = (uint16_t)bi;
-        }
-    }
-    float w;
-    if (p.gate_fn == ARISTOS_GATE_SOFTMAX) {
-        const float mx = __shfl_sync(0xffffffffu, my_l, 0);
-        float den = 0.0f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (i * 32 + lane < p.E) den += expf(v[i] - mx);
-#pragma unroll
-        for (int m = 16; m >= 1; m >>= 1) den += __shfl_xor_sync(0xffffffffu, den, m);
-        w = expf(my_l - mx) / den;
-    } else {
-        w = 1.0f / (1.0f + expf(-my_l));
-    }
-    if (p.renorm) {
-        float sum = 0.0f;
-#pragma unroll 1
-        for (int j = 0; j < p.k; ++j) sum += __shfl_sync(0xffffffffu, w, j);
-        w = w / sum;
-    }
-    if (lane < p.k) s.w[t * p.k + lane] = w;
-}
 
 __device__ __forceinline__ void copy_async4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -285,12 +216,6 @@ __device__ __forceinline__ uint4 load_act(const void* ptr) {
     return v;
 }
 
-// Counts items whose results this warp has written. Only a release: a full fence would also empty the L1 cache, from
-// which the streaming warps read the tokens again for every item.
-__device__ __forceinline__ void add_release(int32_t* counter, int by) {
-    asm volatile("red.add.release.gpu.global.s32 [%0], %1;" ::"l"(counter), "r"(by) : "memory");
-}
-
 template <bool F16>
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                             uint32_t b1) {
@@ -302,14 +227,6 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t half_pair(float a, float b) {
-    const __half2 t = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&t);
-}
-__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
-    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&t);
-}
 __device__ __forceinline__ uint32_t half_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
 // Four e4m3 codes as fp16 pairs (exact).
@@ -324,7 +241,6 @@ template <int WF> struct FewFormat;                    // elements per byte of w
 template <> struct FewFormat<FEW_BF16> { static constexpr int PACK = 1; };
 template <> struct FewFormat<FEW_F16> { static constexpr int PACK = 1; };
 template <> struct FewFormat<FEW_FP8> { static constexpr int PACK = 2; };
-template <> struct FewFormat<FEW_FP4> { static constexpr int PACK = 4; };
 
 // NT: token tiles of 8 per pass; RG: groups of 8 weight rows per item; D: steps in the ring; BUFS: buffers for
 // the sums of an item.
@@ -334,10 +250,10 @@ struct FewShape {
     static constexpr int STEP_K = 64 * FewFormat<WF>::PACK;     // elements of K per step: 128 bytes of a row
     static constexpr int TILES = RG / 2;                // m16 tiles: row groups (2 t, 2 t + 1)
     static constexpr int SLOT = RG * 1024;              // 8 rows x 128 bytes per row group
-    static constexpr int SCALES = WF == FEW_FP4 ? 2 * 32 * RG : (WF == FEW_FP8 ? 16 : 0);   // bytes of scales per step
+    static constexpr int SCALES = WF == FEW_FP8 ? 16 : 0;       // bytes of scales per step
     static constexpr int RED = TILES * NT * 128;        // floats per warp of one buffer
     static constexpr size_t SMEM = 1024 + (size_t)FEW_STREAM_WARPS * (D * (SLOT + SCALES) + BUFS * RED * 4);
-    static_assert(RG == 2 || RG == 4, "a lane of a quad copies the scale words of one row group");
+    static_assert(RG == 2 || RG == 4, "at most one 16-byte group of scales per step");
     static_assert(D <= FEW_MAX_DEPTH && D >= 2, "ring depth");
 };
 
@@ -367,57 +283,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- routing and expert lists (every CTA for itself) ------------------------------------------------------------------
-    for (int t = warp; t < p.n; t += FEW_WARPS) {
-        const float* l = p.logits + (size_t)t * p.E;
-        if (p.E <= 32) few_topk<1>(l, p, t, lane, s);
-        else if (p.E <= 256) few_topk<8>(l, p, t, lane, s);
-        else few_topk<FEW_MAX_EXPERTS / 32>(l, p, t, lane, s);
-    }
-    __syncthreads();
+    few_route<8 * NT>(p, s);
     const int slots = p.n * p.k;
-    for (int i = threadIdx.x; i < slots; i += FEW_THREADS) {
-        const int t = i / p.k;
-        atomicOr(&s.mask[s.idx[i]][t >> 5], 1u << (t & 31));
-        if (blockIdx.x == 0) {
-            if (p.topk_idx) p.topk_idx[i] = s.idx[i];
-            if (p.topk_w) p.topk_w[i] = s.w[i];
-        }
-    }
-    __syncthreads();
-    if (warp == 0) {
-        int rows = 0, n_active = 0;
-        for (int e0 = 0; e0 < p.E; e0 += 32) {
-            const int e = e0 + lane;
-            const int m = e < p.E ? __popc(s.mask[e][0]) + __popc(s.mask[e][1]) : 0;
-            int incl = m;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int o = __shfl_up_sync(0xffffffffu, incl, d);
-                if (lane >= d) incl += o;
-            }
-            const uint32_t on = __ballot_sync(0xffffffffu, m > 0);
-            if (m > 0) {
-                s.base[e] = (uint16_t)(rows + incl - m);
-                const int a = n_active + __popc(on & ((1u << lane) - 1));
-                s.active[a] = (uint16_t)e;
-                s.chunks[a] = (uint8_t)((m + 8 * NT - 1) / (8 * NT));
-            }
-            rows += __shfl_sync(0xffffffffu, incl, 31);
-            n_active += __popc(on);
-        }
-        if (lane == 0) s.actives = n_active;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < slots; i += FEW_THREADS) {
-        const int t = i / p.k, e = s.idx[i];
-        const uint32_t lo = s.mask[e][0], hi = s.mask[e][1];
-        const int rank = t < 32 ? __popc(lo & ((1u << t) - 1)) : __popc(lo) + __popc(hi & ((1u << (t - 32)) - 1));
-        const int slot = s.base[e] + rank;
-        s.slot[i] = (uint16_t)slot;
-        s.token[slot] = (uint8_t)t;
-    }
-    __syncthreads();
 
     // ---- the list of items ------------------------------------------------------------------------------------------
     const int actives = s.actives;
@@ -426,33 +293,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     const int up_steps = (p.H + STEP_K - 1) / STEP_K, down_steps = (p.I + STEP_K - 1) / STEP_K;
     const int part_steps = (down_steps + p.parts - 1) / p.parts;
     const int stride = gridDim.x * FEW_GROUPS;
-    // A position in the list of items. It advances without a division: the list is ordered by expert, then (down
-    // projection) by part of K, then by block of rows, then by pass over the expert's tokens.
-    struct Item {
-        bool up;
-        int a, part, at;           // chosen expert, part of K, block of rows * passes + pass
-    };
-    auto forward = [&](Item& i, int by) {      // returns false past the end
-        i.at += by;
-        if (i.up) {
-            for (int len; i.at >= (len = up_blocks * s.chunks[i.a]);) {
-                i.at -= len;
-                if (++i.a == actives) { i.up = false; i.a = 0; break; }
-            }
-        }
-        if (!i.up) {
-            for (int len; i.at >= (len = down_blocks * s.chunks[i.a]);) {
-                i.at -= len;
-                if (++i.part == p.parts) {
-                    i.part = 0;
-                    if (++i.a == actives) return false;
-                }
-            }
-        }
-        return true;
-    };
-    auto block_of = [&](const Item& i) { const int c = s.chunks[i.a]; return c == 1 ? i.at : i.at / c; };
-    auto pass_of = [&](const Item& i) { const int c = s.chunks[i.a]; return c == 1 ? 0 : i.at % c; };
+    using Item = FewItem;
+    auto forward = [&](Item& i, int by) { return i.forward(by, s, actives, up_blocks, down_blocks, p.parts); };
+    auto block_of = [&](const Item& i) { return i.block(s); };
+    auto pass_of = [&](const Item& i) { return i.pass(s); };
     auto begin_of = [&](const Item& i) { return i.up ? 0 : i.part * part_steps; };
     auto end_of = [&](const Item& i) { return i.up ? up_steps : min((i.part + 1) * part_steps, down_steps); };
     // The warps of a group start at another step of every item: who has one step more than the others changes.
@@ -496,7 +340,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
         bool more[FEW_GROUPS];
 #pragma unroll
         for (int grp = 0; grp < FEW_GROUPS; ++grp) {
-            items[grp] = Item{true, 0, 0, 0};
+            items[grp] = Item{};
             more[grp] = forward(items[grp], blockIdx.x * FEW_GROUPS + grp);
         }
         int posts = 0;
@@ -529,11 +373,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 for (int w = 0; w < FEW_W; ++w) v += buf[w * RED + at];
                 return v;
             };
-            auto bias_at = [&](const void* bias, size_t i) {
-                if (!bias) return 0.0f;
-                return p.f16 ? __half2float(static_cast<const __half*>(bias)[i])
-                             : __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[i]);
-            };
+            auto bias_at = [&](const void* bias, size_t i) { return few_bias(p, bias, i); };
             const int rows = item.up ? up_rows : down_rows;    // 8, 16 or 32: a warp holds whole columns of the item
             const int j = lane & (rows - 1), tok0 = lane / rows, step = 32 / rows;
             // what does not depend on the sums is asked for before the wait
@@ -604,10 +444,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     const uint32_t bar_step = ptx::smem_u32(&s.full[warp * S::D]);
 
     // ---- position of the loads
-    Item l_item{true, 0, 0, 0};
+    Item l_item;
     int l_nth = 0, l_s = 0, l_end = 0, l_slot = 0, l_e = 0, l_block = 0;
     int in_flight = 0;                                  // steps asked for and not yet used
-    const uint8_t* l_scale = nullptr;                   // fp4: the words of this lane's row in row group q; fp8: group `lane`
+    const uint8_t* l_scale = nullptr;                   // fp8: of row group `lane`
     bool l_more = forward(l_item, first);
     // weight row of row group `group` of an item, SwiGLU: gate and up rows of the same number in turn
     auto row_of = [&](const Item& i, int group) {
@@ -624,11 +464,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
         l_block = block_of(l_item);
         const bool alternate = l_item.up && gated;
         const int rows = l_item.up ? p.I : p.H, K = l_item.up ? p.H : p.I;
-        if constexpr (WF == FEW_FP4) {
-            const int group = min(q, RG - 1), row = row_of(l_item, group) + g;
-            const uint8_t* sc = l_item.up ? (alternate && (group & 1) ? p.s3 : p.s1) : p.s2;
-            l_scale = sc + ((size_t)l_e * fp4_row_tiles(rows) + (row >> 7)) * fp4_col_tiles(K) * FP4_TILE_BYTES + fp4_tile_word(row);
-        } else if constexpr (WF == FEW_FP8) {
+        if constexpr (WF == FEW_FP8) {
             const int group = min(lane, RG - 1);
             const uint8_t* sc = l_item.up ? (alternate && (group & 1) ? p.s3 : p.s1) : p.s2;
             l_scale = sc + ((size_t)l_e * ((rows + 127) / 128) + (row_of(l_item, group) >> 7)) * (K / 128) * 4;
@@ -646,15 +482,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                     ptx::tma_load_3d(to, l_item.up ? &tm1 : &tm2, l_s * 128, l_block * 8 * RG, l_e, bar);
                 }
             }
-            if constexpr (WF == FEW_FP4) {
-                // two scale words per row and step (256 elements), if the row has as many
-                if (q < RG) {
-                    const uint32_t to = ring_scale + l_slot * S::SCALES + (g * RG + q) * 8;
-                    const uint8_t* from = l_scale + (size_t)l_s * (2 * FP4_TILE_BYTES);
-                    copy_async4(to, from);
-                    if (l_s * STEP_K + FP4_TILE_COLS < (l_item.up ? p.H : p.I)) copy_async4(to + 4, from + FP4_TILE_BYTES);
-                }
-            } else if constexpr (WF == FEW_FP8) {
+            if constexpr (WF == FEW_FP8) {
                 if (lane < RG) copy_async4(ring_scale + l_slot * S::SCALES + lane * 4, l_scale + l_s * 4);
             }
             if (++l_slot == S::D) l_slot = 0;
@@ -675,15 +503,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
 
     int c_slot = 0, ready = 0;               // experts below `ready` have all their hidden activations
     uint32_t c_phase = 0;
-    Item item{true, 0, 0, 0};
+    Item item;
     bool ok = true;
     int nth = 0;
     for (bool more = forward(item, first); more; more = forward(item, stride), ++nth) {
         const int e = s.active[item.a], pass = pass_of(item);
         const int base = s.base[e] + pass * 8 * NT, m = min(tokens_of(e) - pass * 8 * NT, 8 * NT);
-        const int K = item.up ? p.H : p.I;
         if (!item.up && ready <= item.a) {
-            // All of this expert's hidden activations must be there. The next experts' counters are read along with it:
+            // All of this expert's hidden activations must be there. (Written out here: as a function of its own, inlined, it
+            // costs the fp8 kernel more spilled registers and 4 % of its time.) The next experts' counters are read along with it:
             // by now most of them are complete, and a fence is paid once for all.
             uint64_t t0 = 0;
             for (uint32_t i = 0;; ++i) {
@@ -777,16 +605,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 };
                 // With one token tile the tokens of up to four chunks of a lane are asked for at once, the first ones before
                 // the wait for the weights.
-                constexpr int CHUNKS = WF == FEW_FP4 ? 8 : 2 * FewFormat<WF>::PACK;     // of 8 elements per lane and step
+                constexpr int CHUNKS = 2 * FewFormat<WF>::PACK;     // of 8 elements per lane and step
                 constexpr int AHEAD = N == 1 ? (CHUNKS < 4 ? CHUNKS : 4) : 1;
-                auto element = [&](int c) { return WF == FEW_FP4 ? c * 32 + q * 8 : (q * CHUNKS + c) * 8; };
-                const int chunks = WF == FEW_FP4 ? min(CHUNKS, (K - k0) >> 5) : CHUNKS;
+                auto element = [&](int c) { return (q * CHUNKS + c) * 8; };
                 uint4 hi_ahead[AHEAD], lo_ahead[AHEAD];
                 auto look_ahead = [&](int c0) {
                     if constexpr (N == 1) {
 #pragma unroll
                         for (int c = 0; c < AHEAD; ++c)
-                            if (c0 + c < chunks) load_tokens(0, k0 + element(c0 + c), hi_ahead[c], lo_ahead[c]);
+                            load_tokens(0, k0 + element(c0 + c), hi_ahead[c], lo_ahead[c]);
                     }
                 };
                 auto tokens = [&](int nt, int c, uint4& hi, uint4& lo) {
@@ -803,40 +630,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 if (++c_slot == S::D) { c_slot = 0; c_phase ^= 1u; }
                 --in_flight;
 
-                if constexpr (WF == FEW_FP4) {
-                    // a block of 32 at a time: its scale multiplies the sums of its products. Scale byte as the exponent
-                    // of an fp32 number: 0 (2^-127) counts as zero, 255 (NaN) as infinity
-                    uint2 sw[RG];
-#pragma unroll
-                    for (int r = 0; r < RG; ++r) sw[r] = ld_shared2(scales + (g * RG + r) * 8);
-#pragma unroll
-                    for (int b = 0; b < 8; ++b) {
-                        if (b >= chunks) break;
-                        if (b == 4) look_ahead(4);
-                        uint32_t a[RG][4];
-#pragma unroll
-                        for (int r = 0; r < RG; ++r) fp4_unpack8(ld_shared(from + group_at(r) + ((b ^ g) << 4) + q * 4), a[r]);
-                        float f[RG];
-#pragma unroll
-                        for (int r = 0; r < RG; ++r) {
-                            const uint32_t w = b < 4 ? sw[r].x : sw[r].y;
-                            f[r] = __uint_as_float(((b & 3) < 3 ? w << (23 - 8 * (b & 3)) : w >> 1) & 0x7F800000u);
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < N; ++nt) {
-                            if (nt * 8 >= m) break;
-                            uint4 hi, lo;
-                            tokens(nt, b, hi, lo);
-#pragma unroll
-                            for (int t = 0; t < TILES; ++t) {
-                                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                multiply(a, t, hi, lo, c);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) acc[t][nt][i] = fmaf(c[i], f[2 * t + (i >> 1)], acc[t][nt][i]);
-                            }
-                        }
-                    }
-                } else if constexpr (WF == FEW_FP8) {
+                if constexpr (WF == FEW_FP8) {
                     float part[TILES][N][4];            // sums of this step (one scale block of K), to be scaled
 #pragma unroll
                     for (int t = 0; t < TILES; ++t)
@@ -922,44 +716,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
     }
     if (!ok) return;
 
-    // ---- the tokens' sums over their experts, once every CTA has written its expert outputs: a warp takes 64 columns of a
-    // token at a time
-    const int columns = p.H / 64;
-    const int me = blockIdx.x * FEW_STREAM_WARPS + warp, warps = gridDim.x * FEW_STREAM_WARPS;
-    if (me >= columns * p.n) return;
-    uint64_t t0 = 0;
-    for (uint32_t i = 0;; ++i) {
-        int32_t v;
-        asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p.finished) : "memory");
-        if (v >= (int)gridDim.x) break;
-        if (i == 0) t0 = ptx::globaltimer_ns();
-        if ((i & 63u) == 63u && (*static_cast<volatile int*>(&s.abort) || ptx::globaltimer_ns() - t0 > ptx::WAIT_LIMIT_NS)) {
-            if (p.dev_status && lane == 0) atomicOr(p.dev_status, DEV_FAULT_TIMEOUT);
-            return;
-        }
-    }
-    asm volatile("fence.acq_rel.gpu;" ::: "memory");
-    for (int c = me; c < columns * p.n; c += warps) {
-        const int tok = c / columns;
-        const size_t col = (size_t)(c - tok * columns) * 64 + 2 * lane;
-        float2 v = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-        for (int j = 0; j < p.k; ++j) {
-            const float* src = p.partial + (size_t)s.slot[tok * p.k + j] * p.H + col;
-            float2 y = __ldcg(reinterpret_cast<const float2*>(src));
-            for (int part = 1; part < p.parts; ++part) {
-                const float2 z = __ldcg(reinterpret_cast<const float2*>(src + (size_t)part * slots * p.H));
-                y.x += z.x;
-                y.y += z.y;
-            }
-            const float w = s.w[tok * p.k + j];
-            v.x = fmaf(w, y.x, v.x);
-            v.y = fmaf(w, y.y, v.y);
-        }
-        const size_t at = (size_t)tok * p.H + col;
-        if (p.f16) *reinterpret_cast<uint32_t*>(static_cast<__half*>(p.out) + at) = half_pair(v.x, v.y);
-        else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(p.out) + at) = bf16_pair(v.x, v.y);
-    }
+    few_sum(p, s, blockIdx.x * FEW_STREAM_WARPS + warp, gridDim.x * FEW_STREAM_WARPS);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -971,7 +728,7 @@ int few_parts(int H, int I) {
 }
 
 struct FewPlan {
-    size_t logits, counters, x_norm, x_scale, h, partial, total;
+    size_t logits, counters, x, x_scale, h, h_scale, partial, total;
     int ncounters;
 };
 FewPlan few_plan(int n, int H, int I, int E, int k) {
@@ -982,15 +739,15 @@ FewPlan few_plan(int n, int H, int I, int E, int k) {
     f.logits = take((size_t)n * E * 4);
     f.ncounters = FEW_MAX_EXPERTS + FEW_MAX_SLOTS + 1;
     f.counters = take((size_t)f.ncounters * 4);
-    f.x_norm = take((size_t)n * H * 2);
-    f.x_scale = take((size_t)n * 4);
+    // the tokens in fp16 (2 bytes, a factor each) or as terms (4 bytes, scale bytes); h in fp32 or as terms
+    f.x = take((size_t)n * H * 4);
+    f.x_scale = take((size_t)n * (4 + few_scale_pitch(H)));
     f.h = take(slots * I * 4);
+    f.h_scale = take(slots * few_scale_pitch(I));
     f.partial = take(slots * H * 4 * few_parts(H, I));
     f.total = at;
     return f;
 }
-
-struct FewWeights { const void *w1, *w3, *w2; };
 
 template <int WF, int NT, class S>
 aristos_status_t launch_few(const FewParams& p, const FewWeights& w, cudaStream_t st) {
@@ -1099,17 +856,20 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f16 = dtype == ARISTOS_DTYPE_F16;
-    const bool norm = !f16 && (fp8 || fp4);                 // bf16 tokens meet quantised weights as scaled fp16 numbers
     FewParams p{};
     p.logits = reinterpret_cast<float*>(ws + f.logits);
-    p.x = static_cast<const uint16_t*>(norm ? static_cast<const void*>(ws + f.x_norm) : x);
-    p.x_scale = norm ? reinterpret_cast<const float*>(ws + f.x_scale) : nullptr;
+    p.x = static_cast<const uint16_t*>(fp8 ? static_cast<const void*>(ws + f.x) : x);
+    p.x_scale = fp8 ? reinterpret_cast<const float*>(ws + f.x_scale) : nullptr;
     const FewWeights w{w1, w3, w2};
     p.s1 = static_cast<const uint8_t*>(s1);
     p.s3 = static_cast<const uint8_t*>(s3);
     p.s2 = static_cast<const uint8_t*>(s2);
     p.b1 = b1; p.b3 = gated ? b3 : nullptr; p.b2 = b2;
     p.h = reinterpret_cast<float*>(ws + f.h);
+    p.x_codes = ws + f.x;
+    p.x_scales = ws + f.x_scale;
+    p.h_codes = ws + f.h;
+    p.h_scales = ws + f.h_scale;
     p.partial = reinterpret_cast<float*>(ws + f.partial);
     p.done = reinterpret_cast<int32_t*>(ws + f.counters);
     p.h_max = reinterpret_cast<uint32_t*>(p.done + FEW_MAX_EXPERTS);
@@ -1125,21 +885,29 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
 
     // A warp per (expert, token) while that does not ask for more warps than run at once, else four tokens per warp.
     const int tok = (int64_t)E * tokens <= 2048 ? 1 : 4;
-    const int gate_grid = ceil_div(E * ceil_div(tokens, tok), FEW_GATE_WARPS) + (norm ? tokens : 0);
-    __half* x_norm = norm ? reinterpret_cast<__half*>(ws + f.x_norm) : nullptr;
-    float* x_scale = norm ? reinterpret_cast<float*>(ws + f.x_scale) : nullptr;
+    const int gate_grid = ceil_div(E * ceil_div(tokens, tok), FEW_GATE_WARPS) + (fp8 || fp4 ? tokens : 0);
     auto gate = [&](auto kernel, auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
         kernel<<<gate_grid, FEW_GATE_WARPS * 32, 0, st>>>(static_cast<const T*>(x), static_cast<const T*>(w_gate), gate_bias,
                                                           tokens, H, E, const_cast<float*>(p.logits), p.done, f.ncounters,
-                                                          x_norm, x_scale);
+                                                          ws + f.x, ws + f.x_scale);
     };
-    if (f16) tok == 1 ? gate(few_gate_kernel<__half, 1>, (__half*)nullptr) : gate(few_gate_kernel<__half, 4>, (__half*)nullptr);
-    else tok == 1 ? gate(few_gate_kernel<__nv_bfloat16, 1>, (__nv_bfloat16*)nullptr)
-                  : gate(few_gate_kernel<__nv_bfloat16, 4>, (__nv_bfloat16*)nullptr);
+    auto gate_as = [&](auto* type, auto prep) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        constexpr int PREP = decltype(prep)::value;
+        tok == 1 ? gate(few_gate_kernel<T, 1, PREP>, type) : gate(few_gate_kernel<T, 4, PREP>, type);
+    };
+    using None = std::integral_constant<int, PREP_NONE>;
+    using Half = std::integral_constant<int, PREP_F16>;
+    using Terms = std::integral_constant<int, PREP_TERMS>;
+    __half* const as_f16 = nullptr;
+    __nv_bfloat16* const as_bf16 = nullptr;
+    if (fp4) f16 ? gate_as(as_f16, Terms{}) : gate_as(as_bf16, Terms{});
+    else if (fp8) gate_as(as_bf16, Half{});
+    else f16 ? gate_as(as_f16, None{}) : gate_as(as_bf16, None{});
     ARISTOS_COUNT_LAUNCH();
     ARISTOS_CUDA_TRY(cudaGetLastError());
-    if (fp4) return launch_few_tokens<FEW_FP4>(p, w, st);
+    if (fp4) return launch_few_fp4(p, w, st);
     if (fp8) return launch_few_tokens<FEW_FP8>(p, w, st);
     return f16 ? launch_few_tokens<FEW_F16>(p, w, st) : launch_few_tokens<FEW_BF16>(p, w, st);
 }

@@ -397,8 +397,8 @@ ARISTOS_API aristos_status_t aristos_expert_ffn_fp4(const void* xq, const void* 
  * ARISTOS_FEW_TOKENS_MAX; w_gate (E, H) and the optional biases b1 / b3 (E, I), b2 (E, H) in the same dtype; gate_bias
  * (E) fp32 or NULL. weights_dtype: `dtype` itself, ARISTOS_DTYPE_FP8_E4M3 (bf16 activations only; s1 / s3 / s2 fp32 as
  * aristos_quantize_fp8(block_rows = 128) writes them; H and I multiples of 128) or ARISTOS_DTYPE_FP4_E2M1 (codes and
- * scale tiles of aristos_quantize_fp4; a scale byte 0 counts as zero, 255 makes the row's results infinite or NaN). E <= 512.
- * Activations are not quantised. The routing is aristos_gate_topk's, bit for bit;
+ * scale tiles of aristos_quantize_fp4; scale byte 255 makes the row's results NaN). E <= 512.
+ * Activations are not quantised (for 4-bit weights they are split into 4-bit terms that hold 24 bits). The routing is aristos_gate_topk's, bit for bit;
  * no token is dropped. topk_idx / topk_w (tokens, k) receive it, or NULL. workspace:
  * aristos_moe_few_tokens_workspace_bytes (0: sizes out of range) on the device, owned by the caller; it needs no
  * initialisation, and calls that may overlap on the GPU need one each.

@@ -302,3 +302,93 @@ def test_module_decode():
     want = layer.moe_few_tokens(x.reshape(6, 256), m.w_gate, m.w1, m.w3, m.w2, 2, 2, renorm=1)[0]
     assert torch.equal(out, want.reshape(2, 3, 256))
     m.close()
+
+
+# ---- 4-bit weights: the split into terms, the parts of K, the order of tiles ----------------------------------------------
+@pytest.mark.parametrize("n,E,k,H,I,act", [
+    (5, 3, 2, 64, 1024, 0),             # more parts of K asked for than there are whole stages
+    (3, 4, 2, 128, 1600, 2),            # parts of unequal length, the last stage cut
+    (24, 64, 8, 512, 1024, 2),          # several rounds of up tiles, the CTAs with one tile less are dealt more
+    (24, 64, 8, 2048, 512, 1),          # the same with long up and short down tiles
+    (64, 3, 3, 320, 448, 2),            # four passes over every expert's weights
+    (64, 512, 16, 128, 192, 0),         # the most experts and choices
+])
+def test_tiles_of_4_bit_weights(n, E, k, H, I, act):
+    c = Case(n, E, k, H, I, act, "4", gate_fn=n % 2, bias=n % 3 == 0, seed=n + H)
+    got = c.run()
+    c.check(got)
+    again = c.run()
+    assert all(c.torch.equal(a, b) for a, b in zip(got, again)), "the same call gives the same bits"
+
+
+def test_most_experts_and_choices():
+    c = Case(64, 512, 16, 128, 64, 1, "16", seed=3)
+    c.check(c.run())
+
+
+def test_4_bit_products_scale_with_the_tokens():
+    """Everything behind a split is a power of two away: without biases, with ReLU and the same routing, tokens times 2^a give
+    outputs times 2^a, bit for bit, as long as all terms have a scale (2^-127 or more). Of tokens near 2^-110 the terms
+    below 2^-127 are left out: some 16 bits stay, of which the tolerance asks for 8 (the output is bf16)."""
+    torch, cp, layer = _mods()
+    c = Case(7, 6, 2, 256, 320, 0, "4", seed=9)
+    c.wg = torch.zeros_like(c.wg)
+    want = c.run()[0].double()
+    for a in (-60, -13, 1, 40, 60):
+        got = c.run((c.x.double() * 2.0 ** a).to(c.dt))[0].double()
+        assert torch.equal(got, want * 2.0 ** a), a
+    got = c.run((c.x.double() * 2.0 ** -110).to(c.dt))[0].double() * 2.0 ** 110
+    scale = want.abs().amax()
+    assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -9 * scale).all()
+
+
+def test_4_bit_weights_meet_all_24_bits_of_the_hidden_activations():
+    """W1 picks columns, so h is known exactly: every block of 32 holds one large and 31 small numbers, and W2 cancels the
+    large one. What is left are the small numbers, 2^-15 of the largest: an h rounded to 11 or 16 bits of its block would
+    lose them. Terms are off by at most 2^-23 of a block's largest magnitude (half a unit of the eighth: 2^(s0 - 22), the
+    largest being 2^(s0 + 1) or more), i.e. 2^-8 of the small numbers; fp32 sums of K = 128 add 128 * 2^-24 * 2^15 of them
+    at most where the large ones cancel: one of each sign per two blocks, exactly equal, so nothing is rounded on the way
+    but what is smaller than 2^-24 of the large ones."""
+    torch, cp, layer = _mods()
+    H, n = 128, 4
+    c = Case(n, 1, 1, H, H, 0, "4", seed=4)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    x = 1.0 + torch.randint(0, 128, (n, H), device="cuda", generator=g).float() / 128       # 8 bits, in [1, 2)
+    x[:, 0::32] = 2.0 ** 15
+    c.x = x.to(c.dt)
+    assert torch.equal(c.x.float(), x)
+    eye = torch.eye(H, device="cuda")[None]
+    w2 = torch.zeros(1, H, H, device="cuda")
+    for r in range(H):
+        for b in range(H // 32):
+            w2[0, r, 32 * b] = 1.0 if b % 2 else -1.0                                       # the large ones cancel
+        w2[0, r, 32 * (r % 4) + 1 + r % 31] += 1.0
+    for m, w in (("1", eye), ("2", w2)):
+        q, s = layer.quantize_fp4(w)
+        assert torch.equal(layer.dequantize_fp4(q, s, torch.float32), w)
+        c.w[m], c.s[m], c.mats[m] = q, s, None
+    out = c.run()[0].double()
+    want = torch.stack([x[:, 32 * (r % 4) + 1 + r % 31] for r in range(H)], 1).double()
+    # 2^-23 * 2^15 per number of the split, twice (x and h); sums within 2^-24 * 2^16 per added pair of large numbers, at most 8
+    bound = 2 * 2.0 ** -8 + 8 * 2.0 ** -8 + 2.0 ** -9 * want
+    assert ((out - want).abs() <= bound).all(), (out - want).abs().max()
+
+
+def test_4_bit_calls_that_overlap_on_two_streams():
+    torch, cp, layer = _mods()
+    cases = [Case(6, 16, 2, 512, 512, 2, "4", seed=1), Case(33, 16, 3, 512, 1024, 1, "4", seed=2)]
+    want = [c.run() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    results = [[], []]
+    for _ in range(20):
+        for i, (c, st) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(st):
+                results[i].append(c.run(dev_status=status))
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    for r, w in zip(results, want):
+        for got in r:
+            assert all(torch.equal(p, q) for p, q in zip(got, w))
