@@ -29,6 +29,8 @@
 // whole block, so scale and codes come out of its registers, rounded once from fp32. Only valid rows are written.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "fp4_format.cuh"
 #include "ptx_sm100.cuh"
@@ -111,6 +113,12 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_a
 __device__ __forceinline__ void umma_commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+
+// After a wait that gave up: the copies and MMAs in flight still use shared memory and TMEM. Waits for them, with a limit.
+__device__ __forceinline__ void wait_drained(uint32_t bar, uint32_t parity) {
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (!ptx::mbar_try_wait(bar, parity) && ptx::globaltimer_ns() - t0 < ptx::WAIT_LIMIT_NS) {}
 }
 
 // Reciprocal and power of two in one instruction each (subnormal arguments and results count as zero: the arguments here are
@@ -251,7 +259,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* aux = smem + F4_STAGES * F4_STAGE_BYTES + F4_SF_STAGES * F4_SF_STAGE_BYTES + F4_EPI_WARPS * F4_OUT_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(aux);     // full[S], empty[S], tfull[2], tempty, scales[4], sfull[8], sempty[8]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(aux);     // full[S], empty[S], tfull[2], tempty, scales[4], sfull[8], sempty[8], drained[2]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(aux + 384);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(aux + 388);
     int* prefix = reinterpret_cast<int*>(aux + 512);
@@ -266,7 +274,8 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     const uint32_t bar_scales = bar_tempty + 8;            // used in CTA 0 only: a stage's scales are in TMEM
     const uint32_t bar_sfull = bar_scales + 8 * F4_SF_BUFS;        // used in CTA 0 only
     const uint32_t bar_sempty = bar_sfull + 8 * F4_SF_STAGES;      // one per CTA
-    static_assert(8 * (2 * F4_STAGES + 3 + F4_SF_BUFS + 2 * F4_SF_STAGES) <= 384, "barriers");
+    const uint32_t bar_drained = bar_sempty + 8 * F4_SF_STAGES;    // used in CTA 0 only: by the issuers of MMAs and of copies to TMEM
+    static_assert(8 * (2 * F4_STAGES + 5 + F4_SF_BUFS + 2 * F4_SF_STAGES) <= 384, "barriers");
     const uint32_t smem_base = ptx::smem_u32(smem);
     const uint32_t smem_sf = smem_base + F4_STAGES * F4_STAGE_BYTES;
 
@@ -286,6 +295,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             ptx::mbar_init(bar_sfull + 8 * s, 1);
             ptx::mbar_init(bar_sempty + 8 * s, 1);
         }
+        for (int b = 0; b < 2; ++b) ptx::mbar_init(bar_drained + 8 * b, 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
     }
@@ -326,7 +336,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             ptx::prefetch_tensormap(&tmB1);
             const CUtensorMap* tmB = cta == 0 ? &tmB0 : &tmB1;
             const uint32_t full0 = ptx::mapa_shared(bar_full, 0);
-            int stage = 0;
+            int stage = 0, issued = 0;
             uint32_t phase = 0;
             int vg = 0;
             bool ok = true;
@@ -348,8 +358,12 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                     ptx::tma_load_3d_pair(sa, &tmA, kb * (F4_KB / 2), m0, g, full);
                     ptx::tma_load_3d_pair(sa + F4_A_BYTES, tmB, kb * (F4_KB / 2), nb, e, full);
                     if (++stage == F4_STAGES) { stage = 0; phase ^= 1u; }
+                    ++issued;
                 }
             }
+            // both CTAs' copies are counted in CTA 0; CTA 1 waits for it below
+            for (int i = max(issued - F4_STAGES, 0); !ok && cta == 0 && i < issued; ++i)
+                wait_drained(bar_full + 8 * (i % F4_STAGES), (i / F4_STAGES) & 1);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -387,6 +401,10 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                 if (!ok) break;
                 umma_commit_both(bar_tfull + 8 * (t & 1));
             }
+            if (!ok) {
+                ptx::umma_commit_pair(bar_drained);
+                wait_drained(bar_drained, 0);
+            }
         }
         __syncwarp();
     } else if (warp == F4_SF_LOAD_WARP) {
@@ -396,7 +414,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             ptx::prefetch_tensormap(&tmSB0);
             ptx::prefetch_tensormap(&tmSB1);
             const uint32_t sfull0 = ptx::mapa_shared(bar_sfull, 0);
-            int stage = 0;
+            int stage = 0, issued = 0;
             uint32_t phase = 0;
             int vg = 0;
             bool ok = true;
@@ -421,8 +439,11 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                     ptx::tma_load_3d_pair(sf + F4_SF_BYTES, &tmSB0, kb * (F4_SF_BYTES / 4), n0 / FP4_TILE_ROWS, e, full);
                     ptx::tma_load_3d_pair(sf + 2 * F4_SF_BYTES, &tmSB1, kb * (F4_SF_BYTES / 4), n1 / FP4_TILE_ROWS, e, full);
                     if (++stage == F4_SF_STAGES) { stage = 0; phase ^= 1u; }
+                    ++issued;
                 }
             }
+            for (int i = max(issued - F4_SF_STAGES, 0); !ok && cta == 0 && i < issued; ++i)
+                wait_drained(bar_sfull + 8 * (i % F4_SF_STAGES), (i / F4_SF_STAGES) & 1);
         }
         __syncwarp();
     } else if (warp == F4_SF_COPY_WARP) {
@@ -457,6 +478,10 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                     ptx::umma_commit_pair(bar_scales + 8 * buf);
                     umma_commit_both(bar_sempty + 8 * stage);
                 }
+            }
+            if (!ok) {
+                ptx::umma_commit_pair(bar_drained + 8);
+                wait_drained(bar_drained + 8, 0);
             }
         }
         __syncwarp();
@@ -562,7 +587,8 @@ aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, 
     auto run = [&](auto kernel) -> aristos_status_t {
         ARISTOS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F4_SMEM_BYTES));
         // one pair per two SMs, as many as the device holds at once (not every SM has a partner in its cluster's reach)
-        static int most = 0;
+        static std::atomic<int> most_pairs{0};
+        int most = most_pairs.load(std::memory_order_relaxed);
         if (most == 0) {
             cudaLaunchConfig_t lc = {};
             lc.gridDim = dim3(2 * (sms / 2));
@@ -576,6 +602,7 @@ aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, 
             int n = 0;
             ARISTOS_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &lc));
             most = n > 0 ? n : 1;
+            most_pairs.store(most, std::memory_order_relaxed);
         }
         const int pairs = (int)(bound < most ? bound : most);
         kernel<<<2 * pairs, F4_THREADS, F4_SMEM_BYTES, st>>>(tmA, tmB0, tmB1, tmSA, tmSB0, tmSB1, p);
