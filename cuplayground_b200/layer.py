@@ -307,6 +307,11 @@ def dequantize_fp4(q: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     return out
 
 
+def _expect_status(t: Optional[torch.Tensor]) -> None:
+    if t is not None and (t.dtype != torch.int32 or t.numel() < 1):
+        raise ValueError(f"dev_status must hold an int32, got {t.dtype} {tuple(t.shape)}")
+
+
 def _fp4_output(y, shape, dtype, device):
     if y is None:
         return torch.zeros(shape, dtype=dtype or torch.bfloat16, device=device)
@@ -324,6 +329,7 @@ def expert_product_fp4(aq, sa, count, bq, sb, y=None, dtype: Optional[torch.dtyp
                            ("bq", bq, (experts, N, half)), ("sb", sb, _fp4_scale_shape((experts,), N, 2 * half))):
         _expect(name, t, shape, torch.uint8)
     _expect("count", count, (groups,), torch.int32)
+    _expect_status(dev_status)
     with _Device(aq, sa, count, bq, sb, y, dev_status) as on:
         y = _fp4_output(y, (groups, rows, N), dtype, aq.device)
         _lib.check(_lib.load().aristos_expert_product_fp4(_addr(aq), _addr(sa), _addr(count), groups, rows, experts, _addr(bq),
@@ -352,6 +358,7 @@ def expert_ffn_fp4(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, hidden_act: int, y=
     for name, t, shape in checks:
         _expect(name, t, shape, torch.uint8)
     _expect("count", count, (groups,), torch.int32)
+    _expect_status(dev_status)
     with _Device(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, y, dev_status) as on:
         y = _fp4_output(y, (groups, rows, H), dtype, xq.device)
         hq = torch.empty((groups, rows, I // 2), dtype=torch.uint8, device=xq.device)
@@ -403,6 +410,7 @@ def moe_few_tokens(x, w_gate, w1, w3, w2, k: int, hidden_act: int, *, gate_fn: i
                               ("b3", b3, (E, I), x.dtype), ("b2", b2, (E, H), x.dtype), ("out", out, (n, H), x.dtype)):
         if t is not None:
             _expect(name, t, shape, d)
+    _expect_status(dev_status)
     lib = _lib.load()
     with _Device(x, w_gate, w1, w3, w2, s1, s3, s2, gate_bias, b1, b3, b2, out, dev_status) as on:
         if out is None:

@@ -126,3 +126,22 @@ def test_reference_finds_a_planted_mistake():
         R.assert_within(short @ w2.T, y, bound + 1e-30)
     with pytest.raises(AssertionError):
         R.assert_within(x[:, :-1] @ w1[:, :-1].T, x @ w1.T, R.dot_bound(x, w1.T))
+
+
+def test_a_status_word_of_another_type_is_refused():
+    """The kernels OR 32 bits into it: one byte would be followed by somebody else's memory."""
+    torch = pytest.importorskip("torch")
+    import cuplayground_b200.layer as layer
+    u8 = lambda *shape: torch.zeros(shape, dtype=torch.uint8)
+    tiles = lambda *lead: u8(*lead, 1, 1, 32, 4, 4)
+    count = torch.zeros(1, dtype=torch.int32)
+    for status in (u8(1), torch.zeros(0, dtype=torch.int32), torch.zeros(1)):
+        with pytest.raises(ValueError, match="dev_status"):
+            layer.expert_product_fp4(u8(1, 4, 32), tiles(1), count, u8(1, 64, 32), tiles(1), dev_status=status)
+        with pytest.raises(ValueError, match="dev_status"):
+            layer.expert_ffn_fp4(u8(1, 4, 32), tiles(1), count, u8(1, 64, 32), tiles(1), None, None, u8(1, 64, 32), tiles(1), 0,
+                                 dev_status=status)
+        x = torch.zeros(2, 64, dtype=torch.bfloat16)
+        w = torch.zeros(3, 64, 64, dtype=torch.bfloat16)
+        with pytest.raises(ValueError, match="dev_status"):
+            layer.moe_few_tokens(x, x.new_zeros(3, 64), w, None, w, 1, 0, dev_status=status)
