@@ -232,28 +232,33 @@ def expert_ffn_fp8(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, hidden_act: int, de
 
 
 # ---- microscaled 4-bit operands -------------------------------------------------------------------------------------
+# The current stream of a device as an address, without a Stream object around it (1 us of a small call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class _Device:
     """Makes the device that all the given tensors (None: not given) are on the current one for a call of the library, and
     gives the call its current stream. Only another device than the current one costs a switch."""
     __slots__ = ("index", "previous", "stream")
 
     def __init__(self, *tensors):
-        device = None
+        index = None
         for t in tensors:
             if t is None:
                 continue
-            if device is None:
-                device = t.device
-            if t.device != device or device.type != "cuda":
+            at = t.get_device()                  # -1: not on a GPU
+            if index is None:
+                index = at
+            if at != index or at < 0:
                 raise ValueError("tensors must all be on one CUDA device, got "
                                  f"{sorted({str(t.device) for t in tensors if t is not None})}")
-        self.index = device.index
+        self.index = index
 
     def __enter__(self):
         self.previous = torch.cuda.current_device()
         if self.previous != self.index:
             torch.cuda.set_device(self.index)
-        self.stream = torch.cuda.current_stream(self.index).cuda_stream
+        self.stream = _raw_stream(self.index)
         return self
 
     def __exit__(self, *_):
