@@ -283,10 +283,6 @@ few_ffn_fp4_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constan
                 if (!ok) break;
                 ptx::umma_commit(bar_acc);
             }
-            if (!ok) {                                   // MMAs in flight still read shared memory and write TMEM
-                ptx::umma_commit(bar_drained);
-                wait_drained(bar_drained, 0);
-            }
         }
         __syncwarp();
     } else if (warp == 2) {
@@ -431,6 +427,10 @@ few_ffn_fp4_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constan
         }
     }
 
+    if (warp == 1 && __any_sync(0xffffffffu, *abort_flag) && ptx::elect_one()) {   // MMAs in flight still read shared memory and write TMEM
+        ptx::umma_commit(bar_drained);
+        wait_drained(bar_drained, 0);
+    }
     ptx::tcgen05_fence_before();
     __syncthreads();
     if (warp == 1) {

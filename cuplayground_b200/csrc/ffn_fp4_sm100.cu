@@ -401,10 +401,6 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                 if (!ok) break;
                 umma_commit_both(bar_tfull + 8 * (t & 1));
             }
-            if (!ok) {
-                ptx::umma_commit_pair(bar_drained);
-                wait_drained(bar_drained, 0);
-            }
         }
         __syncwarp();
     } else if (warp == F4_SF_LOAD_WARP) {
@@ -479,10 +475,6 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                     umma_commit_both(bar_sempty + 8 * stage);
                 }
             }
-            if (!ok) {
-                ptx::umma_commit_pair(bar_drained + 8);
-                wait_drained(bar_drained + 8, 0);
-            }
         }
         __syncwarp();
     } else {
@@ -542,6 +534,12 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
         }
     }
 
+    // Behind the loops, not in the issuers' branches: there it costs their loops 5 % of the kernel's time.
+    if (cta == 0 && (warp == 1 || warp == F4_SF_COPY_WARP) && __any_sync(0xffffffffu, *abort_flag) && ptx::elect_one()) {
+        const uint32_t bar = bar_drained + (warp == 1 ? 0 : 8);
+        ptx::umma_commit_pair(bar);
+        wait_drained(bar, 0);
+    }
     ptx::tcgen05_fence_before();
     __syncthreads();
     ptx::cluster_sync();               // nobody leaves (or frees TMEM) while the other CTA may still signal it
