@@ -10,8 +10,9 @@
 //
 // A tile has 128 rows, of which a token takes eight: 16 tokens to a pass over an expert's weights. The tensor core computes
 // all of it whether there are 16 tokens or one, which does not matter here: it is busy for a quarter of the time. That case
-// takes 450 us (5.5 TB/s). The smallest calls pay for the larger tiles (1 token, 256 x 512: 32 us instead of 26 us with
-// 16-bit instructions and items of 32 rows); from some 10 MB of chosen weights on this kernel is the faster one.
+// takes 440 us with the gate, 418 us of it this kernel (5.9 TB/s). The smallest calls pay for the larger tiles (1 token, 256 x
+// 512: 31 us instead of 26 us with 16-bit instructions and items of 32 rows); from some 10 MB of chosen weights on this kernel
+// is the faster one.
 //
 // Tile: 16 tokens x 256 weight rows (SwiGLU: 128 gate and 128 up rows), K in stages of 256 columns (one 128-byte row):
 // 32 KB of weights, their scales, the tokens' terms (1 KB each, only those that are there) and their scales, four
@@ -189,7 +190,8 @@ few_ffn_fp4_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constan
     const int up_steps = (p.H + T4_KB - 1) / T4_KB, down_steps = (p.I + T4_KB - 1) / T4_KB;
     const int part_steps = (down_steps + p.parts - 1) / p.parts;
     // Tiles are dealt out in turn. An up tile takes as long as several down tiles, so the CTAs that have one up tile less
-    // than the others (those from `rest` on) are dealt the first `extra` rounds of down tiles among themselves.
+    // than the others (those from `rest` on) are dealt the first `extra` rounds of down tiles among themselves: 1 to 4 % (4
+    // tokens, 8 of 256: 163 us instead of 169 us). With fewer than two rounds of up tiles the first down tiles would wait.
     const int ups = up_blocks * s.passes, rest = ups % gridDim.x, my_ups = ups / gridDim.x + ((int)blockIdx.x < rest ? 1 : 0);
     const int lighter = gridDim.x - rest, extra = rest == 0 || ups < 2 * (int)gridDim.x ? 0 : up_steps / part_steps;
     int nth = 0;                                         // of this CTA's tiles

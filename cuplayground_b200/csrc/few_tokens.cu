@@ -29,6 +29,10 @@
 //  * When all down items are done (counted once per group), all streaming warps add up the expert outputs of the tokens,
 //    in the order of j.
 //
+// Measured on a B200 whose copies run at 6.47 TB/s, L2 cold, both kernels: one token, 2 of 8 experts, 4096 x 14336 SwiGLU,
+// bf16 131 us (0.70 GB of weights, 125 us of it this kernel at 5.6 TB/s); 64 tokens, 2 of 64, 2048 x 2048 GELU, bf16 188 us
+// (0.93 GB); 5 tokens, 8 of 256, 7168 x 2048 SwiGLU, e4m3 340 us (1.66 GB; here the conversions to fp16 count, too).
+//
 // Operand types. The instruction multiplies 16-bit numbers. bf16 weights meet tokens in bf16 (as they are) and hidden
 // activations as two bf16 numbers, value and remainder: a single rounding of h to bf16 would by itself be as large as
 // that of the output. fp16 and e4m3 weights meet fp16 numbers, in which both are exact; bf16 tokens and the hidden
@@ -723,7 +727,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
 
 // ---- host side ------------------------------------------------------------------------------------------------------
 // Parts of K of the down projection: so many that its items are about as long as those of the up projection. A group's
-// share of a small call is only a few items, and the call ends with the longest of them.
+// share of a small call is only a few items, and the call ends with the longest of them. (1 token, 4096 x 14336, four parts:
+// 146 us, uncut 150 us, L2 cold; where items are many, at 1024 x 4096 with 8 tokens, it costs 67 us against 65 us.)
 int few_parts(int H, int I) {
     const int parts = (I + H / 2) / H;
     return parts < 1 ? 1 : (parts > 8 ? 8 : parts);
@@ -788,7 +793,10 @@ aristos_status_t launch_few(const FewParams& p, const FewWeights& w, cudaStream_
 template <int WF>
 aristos_status_t launch_few_tokens(const FewParams& p, const FewWeights& w, cudaStream_t st) {
     // Up to 16 tokens of an expert in one pass over its weights; more (few experts, many tokens) take further passes,
-    // whose weights come from L2. Wider passes would cost every small one registers and shared memory.
+    // whose weights come from L2. Wider passes would cost every small one registers and shared memory. Up to 8 tokens a
+    // pass needs one token tile: the registers that this saves are worth 3 % with fp8 weights (345 us against 357 us for 5
+    // tokens of 256 experts, 7168 x 2048), nothing with 16-bit ones. Items of 32 rows: with 16 rows (and rings twice as
+    // deep) the same cases take 1.1 to 1.4 times as long, the tokens are read once per item.
     if (p.n <= 8) return launch_few<WF, 1, FewShape<WF, 1, 4, 3, 2>>(p, w, st);
     return launch_few<WF, 2, FewShape<WF, 2, 4, 3, 1>>(p, w, st);
 }
