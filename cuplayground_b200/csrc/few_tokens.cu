@@ -60,7 +60,7 @@ constexpr int FEW_STREAM_WARPS = FEW_W * FEW_GROUPS;
 constexpr int FEW_WARPS = FEW_STREAM_WARPS + 2;           // and one that adds and stores, and one that counts
 constexpr int FEW_THREADS = 32 * FEW_WARPS;
 
-constexpr int FEW_MAX_DEPTH = 6;
+constexpr int FEW_MAX_DEPTH = 3;
 
 enum { FEW_BF16 = 0, FEW_F16 = 1, FEW_FP8 = 2 };      // weight formats
 

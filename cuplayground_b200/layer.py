@@ -5,6 +5,7 @@ libaristos_moe.so. Nothing here falls back to PyTorch ops."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
@@ -292,8 +293,8 @@ def quantize_fp4(src: torch.Tensor):
     rows, cols = src.shape[-2], src.shape[-1]
     lead = src.shape[:-2]
     with _Device(src) as on:
-        q = torch.empty((*lead, rows, cols // 2), dtype=torch.uint8, device=src.device)
-        scales = torch.empty(_fp4_scale_shape(lead, rows, cols), dtype=torch.uint8, device=src.device)
+        q = src.new_empty((*lead, rows, cols // 2), dtype=torch.uint8)
+        scales = src.new_empty(_fp4_scale_shape(lead, rows, cols), dtype=torch.uint8)
         _lib.check(_lib.load().aristos_quantize_fp4(_addr(src), lead.numel(), rows, cols, _dt(src), _addr(q), _addr(scales),
                                                     on.stream))
     return q, scales
@@ -306,7 +307,7 @@ def dequantize_fp4(q: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     _expect("q", q, q.shape, torch.uint8)
     _expect("scales", scales, _fp4_scale_shape(lead, rows, cols), torch.uint8)
     with _Device(q, scales) as on:
-        out = torch.empty((*lead, rows, cols), dtype=dtype, device=q.device)
+        out = q.new_empty((*lead, rows, cols), dtype=dtype)
         _lib.check(_lib.load().aristos_dequantize_fp4(_addr(q), _addr(scales), lead.numel(), rows, cols, _dt(out),
                                                       _addr(out), on.stream))
     return out
@@ -366,8 +367,8 @@ def expert_ffn_fp4(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, hidden_act: int, y=
     _expect_status(dev_status)
     with _Device(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, y, dev_status) as on:
         y = _fp4_output(y, (groups, rows, H), dtype, xq.device)
-        hq = torch.empty((groups, rows, I // 2), dtype=torch.uint8, device=xq.device)
-        sh = torch.empty(_fp4_scale_shape((groups,), rows, I), dtype=torch.uint8, device=xq.device)
+        hq = xq.new_empty((groups, rows, I // 2))
+        sh = xq.new_empty(_fp4_scale_shape((groups,), rows, I))
         _lib.check(_lib.load().aristos_expert_ffn_fp4(_addr(xq), _addr(sx), _addr(count), groups, rows, experts, _addr(w1q),
                                                       _addr(s1), _addr(w3q), _addr(s3), _addr(w2q), _addr(s2), _addr(hq),
                                                       _addr(sh), _addr(y), H, I, hidden_act, _dt(y), _addr(dev_status),
@@ -376,6 +377,11 @@ def expert_ffn_fp4(xq, sx, count, w1q, s1, w3q, s3, w2q, s2, hidden_act: int, y=
 
 
 # ---- the layer for a few tokens ---------------------------------------------------------------------------------------
+@functools.lru_cache(maxsize=1024)
+def _few_workspace_bytes(n: int, H: int, I: int, E: int, k: int) -> int:
+    return _lib.load().aristos_moe_few_tokens_workspace_bytes(n, H, I, E, k)
+
+
 def moe_few_tokens(x, w_gate, w1, w3, w2, k: int, hidden_act: int, *, gate_fn: int = 0, renorm: int = 0, gate_bias=None,
                    scales=None, b1=None, b3=None, b2=None, out=None, dev_status=None):
     """The whole layer for up to 64 tokens in two kernels: x (tokens, H) bf16 or f16; w_gate (E, H); w1 / w3 (E, I, H) and
@@ -420,10 +426,10 @@ def moe_few_tokens(x, w_gate, w1, w3, w2, k: int, hidden_act: int, *, gate_fn: i
     with _Device(x, w_gate, w1, w3, w2, s1, s3, s2, gate_bias, b1, b3, b2, out, dev_status) as on:
         if out is None:
             out = torch.empty_like(x)
-        idx = torch.empty((n, k), dtype=torch.int32, device=x.device)
-        w = torch.empty((n, k), dtype=torch.float32, device=x.device)
-        nbytes = lib.aristos_moe_few_tokens_workspace_bytes(n, H, I, E, k)
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=x.device)
+        idx = x.new_empty((n, k), dtype=torch.int32)
+        w = x.new_empty((n, k), dtype=torch.float32)
+        nbytes = _few_workspace_bytes(n, H, I, E, k)
+        ws = x.new_empty(max(nbytes, 16), dtype=torch.uint8)
         _lib.check(lib.aristos_moe_few_tokens(_addr(x), _addr(w_gate), _addr(gate_bias), _addr(w1), _addr(w3), _addr(w2),
                                               _addr(s1), _addr(s3), _addr(s2), _addr(b1), _addr(b3), _addr(b2), n, H, I, E, k,
                                               gate_fn, renorm, hidden_act, dt, wdt, _addr(out), _addr(idx), _addr(w),
