@@ -138,6 +138,12 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
 }
 
 __device__ __forceinline__ float act_relu(float v) { return v > 0.0f ? v : 0.0f; }
+// The same, but a NaN stays one: the 4-bit operators and the few-token layer hide no NaN of a weight's scale.
+__device__ __forceinline__ float act_relu_nan(float v) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ __forceinline__ float act_gelu(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f)); }
 __device__ __forceinline__ float act_silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 #endif

@@ -400,7 +400,7 @@ few_ffn_fp4_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constan
                         for (int i = 0; i < 4; ++i) {
                             const float g = y[c][i] + few_bias(p, p.b1, bias_at + mine + i);
                             if (pair) v[i] = act_silu(g) * (y[c | 1][i] + few_bias(p, p.b3, bias_at + mine + i));
-                            else v[i] = p.act == ARISTOS_ACT_RELU ? act_relu(g) : act_gelu(g);
+                            else v[i] = p.act == ARISTOS_ACT_RELU ? act_relu_nan(g) : act_gelu(g);
                         }
                         store(col, v);
                     }

@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                             v = act_silu(total(jg, tok) * f + bias1) * (total(jg + 8, tok) * f + bias3);
                         } else {
                             v = total(j, tok) * f + bias1;
-                            v = p.act == ARISTOS_ACT_RELU ? act_relu(v) : act_gelu(v);
+                            v = p.act == ARISTOS_ACT_RELU ? act_relu_nan(v) : act_gelu(v);
                         }
                         p.h[(size_t)slot * p.I + row0 + j] = v;
                     }

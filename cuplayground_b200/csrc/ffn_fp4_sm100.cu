@@ -167,8 +167,8 @@ __device__ __forceinline__ void activate(float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
         if constexpr (ACT == ARISTOS_ACT_RELU) {
-            v[i] = act_relu(v[i]);
-            v[i + 1] = act_relu(v[i + 1]);
+            v[i] = act_relu_nan(v[i]);
+            v[i + 1] = act_relu_nan(v[i + 1]);
         } else if constexpr (ACT == ARISTOS_ACT_GELU) {
             const float2 r = gelu2(make_float2(v[i], v[i + 1]));
             v[i] = r.x;

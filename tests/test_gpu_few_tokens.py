@@ -392,3 +392,70 @@ def test_4_bit_calls_that_overlap_on_two_streams():
     for r, w in zip(results, want):
         for got in r:
             assert all(torch.equal(p, q) for p, q in zip(got, w))
+
+
+def test_a_nan_scale_of_a_4_bit_weight_row_reaches_its_expert_only():
+    torch, cp, layer = _mods()
+    c = Case(6, 4, 1, 256, 256, 0, "4", seed=6)
+    clean, idx, _ = c.run()
+    for m, row in (("2", 77), ("1", 200)):
+        s = c.s[m].clone()
+        e = int(idx[0, 0])
+        s[e, row // 128, 1, row % 32, row // 32 % 4, 2] = 255
+        keep, c.s[m] = c.s[m], s
+        out, again, _ = c.run()
+        c.s[m] = keep
+        assert torch.equal(again, idx)
+        mine = (idx == e).any(1)
+        assert torch.equal(out[~mine], clean[~mine])
+        if m == "2":
+            assert torch.isnan(out[mine][:, row]).all()
+            rest = torch.arange(256, device="cuda") != row
+            assert torch.equal(out[mine][:, rest], clean[mine][:, rest])
+        else:
+            assert torch.isnan(out[mine]).all()                     # that column of h is NaN, and every output reads it
+
+
+def test_4_bit_layer_beside_4_bit_products():
+    """Both kernels want all of an SM's tensor memory: whoever comes second waits, nobody waits for the other's end."""
+    torch, cp, layer = _mods()
+    c = Case(20, 32, 4, 512, 512, 2, "4", seed=8)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    q = [layer.quantize_fp4(torch.randn(s, device="cuda", generator=g)) for s in ((8, 300, 512), (8, 768, 512))]
+    count = torch.tensor([300, 0, 1, 129, 256, 299, 64, 200], dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    product = lambda: layer.expert_product_fp4(*q[0], count, *q[1], dev_status=status)
+    want, want_y = c.run(), product()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got, got_y = [], []
+    for _ in range(30):
+        with torch.cuda.stream(streams[0]):
+            got.append(c.run(dev_status=status))
+        with torch.cuda.stream(streams[1]):
+            got_y.append(product())
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
+    assert all(torch.equal(y, want_y) for y in got_y)
+
+
+def test_decode_in_a_graph():
+    torch, cp, layer = _mods()
+    cfg = cp.AristosConfig(expert_top_k=2, hidden_act=2, hidden_size=256, intermediate_size=320, num_experts=8, torch_dtype=2,
+                           tokens=256, renorm_topk=1)
+    c = Case(9, 8, 2, 256, 320, 2, renorm=1, seed=11)
+    weights = (c.wg, c.w["1"], c.w["3"], c.w["2"])
+    L = layer.MoELayer(cfg)
+    L.decode(c.x, *weights)                                          # allocates the layer's workspace
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = L.decode(c.x, *weights)
+    for seed in range(3):
+        c.x.copy_(torch.randn(c.x.shape, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, c.run()))
+    L.status()
+    L.close()

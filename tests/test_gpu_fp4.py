@@ -297,3 +297,22 @@ def test_tensors_that_do_not_fit_are_refused():
     assert q.shape == (0, 32) and layer.dequantize_fp4(q, s).shape == (0, 64)
     none = layer.expert_product_fp4(xq[:, :0].contiguous(), sx[:, :0].contiguous(), count, wq, sw)
     assert none.shape == (2, 0, 64)
+
+
+@pytest.mark.parametrize("act", [0, 1, 2])
+def test_ffn_keeps_a_nan_of_the_up_projection(act):
+    """One weight row with a NaN scale: that column of h is NaN (ReLU does not turn it into 0), its block of h gets the NaN
+    scale, and every output of the expert that reads the block is NaN; the other experts' are as before."""
+    torch, cp, layer = _mods()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    mk = lambda *s: layer.quantize_fp4(torch.randn(s, device="cuda", generator=g) * 0.1)
+    x, w1, w3, w2 = mk(2, 20, 256), mk(2, 320, 256), mk(2, 320, 256), mk(2, 256, 320)
+    count = torch.tensor([20, 17], dtype=torch.int32, device="cuda")
+    run = lambda: layer.expert_ffn_fp4(*x, count, *w1, *(w3 if act == 2 else (None, None)), *w2, act)
+    clean = run()
+    assert torch.isfinite(clean).all()
+    w1[1][1, 2, 1, 300 % 32, 300 // 32 % 4, 0] = 255
+    out = run()
+    assert torch.equal(out[0], clean[0])
+    assert torch.isnan(out[1, :17]).all() and (out[1, 17:] == 0).all()
