@@ -34,7 +34,7 @@
 // Measured (B200, bf16 matrix products of the library reach 1.67 PFLOP/s in bursts): 20969 rows of 7 experts, 14336 x 4096,
 // bf16 output 480 us = 5.1 PFLOP/s for some milliseconds, 560 us on and on: then the 1000 W cap holds the SM clock at 1470 of
 // 1965 MHz. The FFN of 24896 rows of 31 experts, 7168 x 2048, SwiGLU 527 us = 4.2 PFLOP/s (4.8 counting what fills up tiles);
-// 15163 rows of 63 experts, 2048 x 2048, GELU 129 us (1.45 times as many rows in tiles, 8 stages each). Tiles of 128 x 256 in single CTAs, with the same
+// 15163 rows of 63 experts, 2048 x 2048, GELU 124 us (1.45 times as many rows in tiles, 8 stages each). Tiles of 128 x 256 in single CTAs, with the same
 // epilogue, took 680 us where pairs took 615 us on the first, and 6 to 11 % less than pairs on the two others.
 #include <cuda.h>
 
@@ -288,6 +288,10 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     const uint32_t smem_base = ptx::smem_u32(smem);
     const uint32_t smem_sf = smem_base + F4_STAGES * F4_STAGE_BYTES;
 
+    // The down projection's launch follows the up projection's without a gap: its CTAs start as the others leave, and wait for
+    // the rest only where they need it.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
     const int out_w = GATED ? 128 : 256;
     const int n_tiles = (p.N + out_w - 1) / out_w;
     const int kblocks = (p.K + F4_KB - 1) / F4_KB;
@@ -334,6 +338,8 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     __syncthreads();
     ptx::cluster_sync();               // both CTAs' barriers are initialised before anything signals them
     ptx::tcgen05_fence_after();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("fence.proxy.async;" ::: "memory");   // TMA reads what the launch before has stored
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = prefix[p.groups];
 
@@ -578,8 +584,9 @@ aristos_status_t encode_scale_map(CUtensorMap* tm, const void* base, int K, int 
     return ARISTOS_OK;
 }
 
+// follows: the launch before this one on the stream is this kernel, too, with the same p.count (which is read before the wait).
 aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, const Fp4GemmParams& p, int out,
-                                 cudaStream_t st) {
+                                 cudaStream_t st, bool follows = false) {
     CUtensorMap tmA, tmB0, tmB1;
     ARISTOS_TRY(encode_map_3d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A, p.K / 2, p.rows_per_group, p.groups, 128));
     ARISTOS_TRY(encode_map_3d(&tmB0, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B0, p.K / 2, p.N, p.experts, 128));
@@ -612,9 +619,18 @@ aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, 
             most_pairs.store(most, std::memory_order_relaxed);
         }
         const int pairs = (int)(bound < most ? bound : most);
-        kernel<<<2 * pairs, F4_THREADS, F4_SMEM_BYTES, st>>>(tmA, tmB0, tmB1, tmSA, tmSB0, tmSB1, p);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * pairs);
+        cfg.blockDim = dim3(F4_THREADS);
+        cfg.dynamicSmemBytes = F4_SMEM_BYTES;
+        cfg.stream = st;
+        cudaLaunchAttribute serial;
+        serial.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        serial.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &serial;
+        cfg.numAttrs = follows ? 1 : 0;
+        ARISTOS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB0, tmB1, tmSA, tmSB0, tmSB1, p));
         ARISTOS_COUNT_LAUNCH();
-        ARISTOS_CUDA_TRY(cudaGetLastError());
         return ARISTOS_OK;
     };
     switch (out) {
@@ -734,5 +750,5 @@ extern "C" aristos_status_t aristos_expert_ffn_fp4(const void* xq, const void* s
     p.sb0 = p.sb1 = static_cast<const uint8_t*>(s2);
     p.out = y;
     p.out_scales = nullptr;
-    return launch_fp4_gemm(hq_scratch, w2q, w2q, p, out_dtype, st);
+    return launch_fp4_gemm(hq_scratch, w2q, w2q, p, out_dtype, st, true);
 }
