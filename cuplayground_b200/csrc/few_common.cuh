@@ -21,8 +21,9 @@ struct FewParams {
     const void *b1, *b3, *b2;      // activations' dtype, or NULL
     const uint8_t *x_codes, *x_scales;   // fp4: the tokens as terms: (n, FEW_TERMS, H / 2) and (n, few_scale_pitch(H))
     uint8_t *h_codes, *h_scales;         // fp4: the same of h: (slots, FEW_TERMS, I / 2) and (slots, few_scale_pitch(I))
-    float* h;                      // (slots, I); not fp4
-    uint32_t* h_max;               // (slots) bits of the largest |h| of a row
+    uint16_t* h;                   // not fp4: (slots, I) as terms
+    int8_t* h_exp;                 // fp16 and fp8: (slots, I / 16) exponents of the terms' scales
+    uint32_t* h_max;               // fp16 and fp8: (slots) bits of the largest |h| of a row
     float* partial;                // (parts, slots, H)
     int32_t* done;                 // up items finished, per chosen expert
     int32_t* finished;             // CTAs that have written all their expert outputs

@@ -30,18 +30,27 @@
 //    in the order of j.
 //
 // Measured on a B200 whose copies run at 6.47 TB/s, L2 cold, both kernels: one token, 2 of 8 experts, 4096 x 14336 SwiGLU,
-// bf16 131 us (0.70 GB of weights, 125 us of it this kernel at 5.6 TB/s); 64 tokens, 2 of 64, 2048 x 2048 GELU, bf16 188 us
-// (0.93 GB); 5 tokens, 8 of 256, 7168 x 2048 SwiGLU, e4m3 340 us (1.66 GB; here the conversions to fp16 count, too).
+// bf16 127 us (0.70 GB of weights, 5.5 TB/s); 64 tokens, 2 of 64, 2048 x 2048 GELU, bf16 178 us (0.93 GB); 5 tokens, 8 of 256,
+// 7168 x 2048 SwiGLU, e4m3 328 us (1.66 GB; here the conversions of the codes to fp16 count, too).
 //
-// Operand types. The instruction multiplies 16-bit numbers. bf16 weights meet tokens in bf16 (as they are) and hidden
-// activations as two bf16 numbers, value and remainder: a single rounding of h to bf16 would by itself be as large as
-// that of the output. fp16 and e4m3 weights meet fp16 numbers, in which both are exact; bf16 tokens and the hidden
-// activations are brought into fp16's range by a power of two per token (the largest magnitude to [2^14, 2^15)),
-// which is undone on the fp32 sums: bf16 tokens lose nothing that is not 2^-40 of the token's largest element, hidden
-// activations are rounded once to 11 bits. h itself is kept in fp32. e4m3's scales multiply the fp32 sums of a step, which
-// is one of their blocks of 128 columns.
+// Operand types. The instruction multiplies 16-bit numbers. bf16 weights meet tokens in bf16 (as they are); fp16 and e4m3
+// weights meet fp16 numbers, in which both are exact, bf16 tokens being brought into fp16's range by a power of two per
+// token (the largest magnitude to [2^14, 2^15)), which is undone on the fp32 sums: they lose nothing that is not 2^-40 of the
+// token's largest element. e4m3's scales multiply the fp32 sums of a step, which is one of their blocks of 128 columns.
+// h, fp32 when it is computed, meets the weights as a sum of such numbers: three bf16 (8 bits each, all 24 that there are) or
+// two fp16 (off by 2^-24, or by 2^-38 of the largest of the row). One number would round it by as much as the output is
+// rounded. The helper that computes h splits it: the streaming warps, which read every h once per item and whose time goes by
+// the number of their instructions, load the terms as they are. In fp16 the terms are scaled so that the largest of the
+// item is in [2^14, 2^15); a row's largest magnitude is known only when all of its items are done, and the streaming warps
+// bring the terms from the one scale to the other (a power of two: exact, down to 2^-24).
+// Three bf16 terms are three instructions. The two fp16 terms of up to 4 tokens are columns of one, the first in columns 0-3
+// and the second in 4-7 (most experts have no more tokens, and the columns would be empty otherwise): 5 tokens, 8 of 64
+// experts, 2048 x 2048, e4m3, 117 us against 126 with two instructions. More tokens take two (folded into tiles of four they
+// take longer, 8 tokens per expert 122 us against 101: their loads are not ahead of the wait). Either way the terms have sums of
+// their own, which are added when the item is done: the bits of a token do not depend on who else chose its experts.
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -64,13 +73,13 @@ constexpr int FEW_MAX_DEPTH = 3;
 
 enum { FEW_BF16 = 0, FEW_F16 = 1, FEW_FP8 = 2 };      // weight formats
 
-// The power of two that brings a largest magnitude (its bits) to [2^14, 2^15) and the one that undoes it. Zero, and what
-// is not finite, stays as it is; the exponent is bounded so that both are normal numbers.
-__device__ __forceinline__ float few_norm(uint32_t max_bits, bool undo) {
+// The exponent of the power of two that brings a largest magnitude (its bits) to [2^14, 2^15). Zero, and what is not finite,
+// stays as it is; it is bounded so that the power and its inverse are normal numbers (and fits a byte).
+__device__ __forceinline__ int few_exponent(uint32_t max_bits) {
     const int field = (int)(max_bits >> 23);
-    const int e = (max_bits == 0 || field == 255) ? 0 : max(min(127 + 14 - field, 120), -120);
-    return __uint_as_float((uint32_t)(127 + (undo ? -e : e)) << 23);
+    return (max_bits == 0 || field == 255) ? 0 : max(min(127 + 14 - field, 120), -120);
 }
+__device__ __forceinline__ float few_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // ---- gate --------------------------------------------------------------------------------------------------------------
 constexpr int FEW_GATE_WARPS = 4;
@@ -124,7 +133,7 @@ few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* 
             m = __reduce_max_sync(0xffffffffu, m);
             if (lane == 0) atomicMax(&s_max, m);
             __syncthreads();
-            const float f = few_norm(s_max, false);
+            const float f = few_power(few_exponent(s_max));
 #pragma unroll 4
             for (int q = threadIdx.x; q < nchunk; q += FEW_GATE_WARPS * 32) {
                 float v[8];
@@ -133,7 +142,7 @@ few_gate_kernel(const T* __restrict__ x, const T* __restrict__ wg, const float* 
                 for (int j = 0; j < 8; ++j) v[j] *= f;
                 store8(reinterpret_cast<__half*>(x_prep) + (size_t)block * H + q * 8, v);
             }
-            if (threadIdx.x == 0) reinterpret_cast<float*>(x_scale)[block] = few_norm(s_max, true);
+            if (threadIdx.x == 0) reinterpret_cast<float*>(x_scale)[block] = few_power(-few_exponent(s_max));
             return;
         }
         block -= n;
@@ -214,11 +223,40 @@ __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ uint32_t half_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// h as numbers of the operand type, largest first; each is what the ones before left over, which is exact. A value that
+// became an infinity or a NaN leaves nothing. bf16: the upper halves, 8 bits at a time; fp16: the nearest numbers.
+template <bool F16> constexpr int FEW_H_TERMS = F16 ? 2 : 3;
+template <bool F16>
+__device__ __forceinline__ void split_hidden(float v, uint16_t (&t)[FEW_H_TERMS<F16>]) {
+#pragma unroll
+    for (int i = 0; i < FEW_H_TERMS<F16>; ++i) {
+        const uint32_t bits = __float_as_uint(v);
+        if constexpr (F16) t[i] = __half_as_ushort(__float2half_rn(v));
+        else t[i] = v == v ? (uint16_t)(bits >> 16) : (uint16_t)0x7FFF;
+        const bool finite = F16 ? (t[i] & 0x7C00) != 0x7C00 : (t[i] & 0x7F80) != 0x7F80;
+        v = finite ? v - (F16 ? __half2float(__ushort_as_half(t[i])) : __uint_as_float(bits & 0xFFFF0000u)) : 0.0f;
+    }
+}
+// Terms of row `slot`, columns col .. col + 7: eight of a term, then eight of the next.
+template <bool F16>
+__device__ __forceinline__ size_t hidden_at(int slot, int I, int col) {
+    return ((size_t)slot * I + (col & ~7)) * FEW_H_TERMS<F16> + (col & 7);
+}
+__device__ __forceinline__ uint32_t scale_pair(uint32_t w, __half2 f) {
+    return half_bits(__hmul2(*reinterpret_cast<const __half2*>(&w), f));
+}
 // Activations. Not the read-only path: h is written in this kernel, and read only after the acquire that follows its
 // expert's counter.
 __device__ __forceinline__ uint4 load_act(const void* ptr) {
     uint4 v;
     asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(ptr));
+    return v;
+}
+__device__ __forceinline__ uint32_t load_exponents(const int8_t* ptr, bool two) {
+    uint32_t v;
+    if (two) asm volatile("ld.global.u16 %0, [%1];" : "=r"(v) : "l"(ptr));
+    else asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(ptr));
     return v;
 }
 
@@ -232,8 +270,6 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-
-__device__ __forceinline__ uint32_t half_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
 // Four e4m3 codes as fp16 pairs (exact).
 __device__ __forceinline__ void unpack_e4m3(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -264,11 +300,15 @@ struct FewShape {
 };
 
 template <int N> struct Tiles { static constexpr int value = N; };
+// What a streaming warp's loop works on: an up item; a down item; a down item whose tokens' two terms fill one tile.
+enum { MODE_UP, MODE_DOWN, MODE_FOLD };
+template <int N> struct Mode { static constexpr int value = N; };
 
 template <int WF, int NT, class S>
 __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constant__ CUtensorMap tm3,
                                                                  const __grid_constant__ CUtensorMap tm2, const __grid_constant__ FewParams p) {
     constexpr bool F16 = WF != FEW_BF16;                // operand type
+    constexpr int TERMS = FEW_H_TERMS<F16>;
     constexpr int RG = S::RG, TILES = S::TILES, STEP_K = S::STEP_K, RED = S::RED;
     __shared__ FewLists s;
     extern __shared__ uint8_t few_smem_raw[];
@@ -407,16 +447,25 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                             v = total(j, tok) * f + bias1;
                             v = p.act == ARISTOS_ACT_RELU ? act_relu_nan(v) : act_gelu(v);
                         }
-                        p.h[(size_t)slot * p.I + row0 + j] = v;
                     }
                     if constexpr (F16) {
                         uint32_t mag = __float_as_uint(v) & 0x7FFFFFFFu;
                         for (int d = rows >> 1; d >= 1; d >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, d));
+                        const int e = few_exponent(mag);
+                        v *= few_power(e);
                         if (in && j == 0) atomicMax(p.h_max + slot, mag);
+                        if (in && (j & 15) == 0) p.h_exp[(size_t)slot * (p.I / 16) + (row0 + j) / 16] = (int8_t)e;
+                    }
+                    if (in) {
+                        uint16_t t[TERMS];
+                        split_hidden<F16>(v, t);
+                        uint16_t* dst = p.h + hidden_at<F16>(slot, p.I, row0 + j);
+#pragma unroll
+                        for (int i = 0; i < TERMS; ++i) dst[8 * i] = t[i];
                     }
                 } else if (in) {
                     float v = total(j, tok);
-                    if constexpr (F16) v *= few_norm(__ldcg(p.h_max + slot), true);
+                    if constexpr (F16) v *= few_power(-few_exponent(__ldcg(p.h_max + slot)));
                     p.partial[((size_t)item.part * slots + slot) * p.H + row0 + j] = v + bias1;
                 }
             }
@@ -545,89 +594,81 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             asm volatile("fence.acq_rel.gpu;" ::: "memory");
         }
         // with as many token tiles as this pass has tokens for: most experts have a few, whatever the batch is
-        auto run = [&](auto tiles) -> bool {
-            constexpr int N = decltype(tiles)::value;
+        auto run = [&](auto tiles, auto what) -> bool {
+            constexpr int N = decltype(tiles)::value, MODE = decltype(what)::value;
+            constexpr bool UP = MODE == MODE_UP, FOLD = MODE == MODE_FOLD;
+            constexpr int TILE = FOLD ? 4 : 8;                          // tokens
+            constexpr int OPERANDS = MODE == MODE_DOWN ? TERMS : 1;     // of a column
+            constexpr int SETS = F16 ? OPERANDS : 1;                    // sums: fp16 terms have their own
             // this lane's token row in every tile; rows past the expert's last one repeat it, their sums are not used
             uint32_t row_at[N];
-            float norm[N];
+            [[maybe_unused]] int row_exp[N];                            // fp16: the scale of the row
 #pragma unroll
             for (int nt = 0; nt < N; ++nt) {
-                const int slot = base + min(nt * 8 + g, m - 1);
-                row_at[nt] = item.up ? s.token[slot] : slot;
-                norm[nt] = F16 && !item.up ? few_norm(__ldcg(p.h_max + slot), false) : 1.0f;
+                const int slot = base + min(nt * TILE + (g & (TILE - 1)), m - 1);
+                row_at[nt] = UP ? s.token[slot] : slot;
+                if constexpr (F16 && !UP) row_exp[nt] = few_exponent(__ldcg(p.h_max + slot));
             }
-            float acc[TILES][N][4];
+            float acc[SETS][TILES][N][4];
 #pragma unroll
-            for (int t = 0; t < TILES; ++t)
+            for (int j = 0; j < SETS; ++j)
 #pragma unroll
-                for (int nt = 0; nt < N; ++nt)
+                for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[t][nt][i] = 0.0f;
+                    for (int nt = 0; nt < N; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[j][t][nt][i] = 0.0f;
 
             // where row group r of a step lies: SwiGLU steps hold all gate rows, then all up rows
-            const uint32_t odd = item.up && gated ? RG / 2 * 1024 : 1024, pair = item.up && gated ? 1024 : 2048;
+            const uint32_t odd = UP && gated ? RG / 2 * 1024 : 1024, pair = UP && gated ? 1024 : 2048;
             auto group_at = [&](int r) { return (r >> 1) * pair + (r & 1) * odd; };
             const int end = end_of(item);
             for (int st = begin_of(item) + turn(wk, nth); st < end; st += FEW_W) {
                 const int k0 = st * STEP_K;
-                // operand of token tile nt at element k: value, and (bf16 hidden activations) remainder
-                auto load_tokens = [&](int nt, int k, uint4& hi, uint4& lo) {
-                    if (item.up) {
-                        hi = load_act(p.x + (size_t)row_at[nt] * p.H + k);
+                // eight elements of token tile nt from k on: tokens are one operand, hidden activations the sum of several
+                auto load_tokens = [&](int nt, int k, uint4 (&op)[OPERANDS]) {
+                    if constexpr (UP) {
+                        op[0] = load_act(p.x + (size_t)row_at[nt] * p.H + k);
                     } else {
-                        const float* src = p.h + (size_t)row_at[nt] * p.I + k;
-                        hi = load_act(src);
-                        lo = load_act(src + 4);
-                    }
-                };
-                auto convert_tokens = [&](int nt, uint4& hi, uint4& lo) {
-                    if (item.up) return;
-                    const float v[8] = {__uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w),
-                                        __uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w)};
-                    uint32_t a[4], b[4];
+                        const uint16_t* src = p.h + hidden_at<F16>(row_at[nt], p.I, k) + (FOLD ? 8 * (g >> 2) : 0);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (F16) {
-                            a[i] = half_pair(v[2 * i] * norm[nt], v[2 * i + 1] * norm[nt]);
-                            b[i] = 0;
-                        } else {
-                            a[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
-                            const float r0 = v[2 * i] - __uint_as_float(a[i] << 16), r1 = v[2 * i + 1] - __uint_as_float(a[i] & 0xFFFF0000u);
-                            // a value that rounds to infinity has no remainder
-                            b[i] = bf16_pair((a[i] & 0x7F80u) == 0x7F80u ? 0.0f : r0, (a[i] & 0x7F800000u) == 0x7F800000u ? 0.0f : r1);
-                        }
-                    }
-                    hi = make_uint4(a[0], a[1], a[2], a[3]);
-                    lo = make_uint4(b[0], b[1], b[2], b[3]);
-                };
-                // 16 x 8 x 16 twice: the eight elements of a lane's share, a[r] = row group r's
-                auto multiply = [&](const uint32_t (&a)[RG][4], int t, const uint4& hi, const uint4& lo, float (&c)[4]) {
-                    mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], hi.x, hi.y);
-                    mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], hi.z, hi.w);
-                    if (!F16 && !item.up) {
-                        mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], lo.x, lo.y);
-                        mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], lo.z, lo.w);
+                        for (int j = 0; j < OPERANDS; ++j) op[j] = load_act(src + 8 * j);
                     }
                 };
-                // With one token tile the tokens of up to four chunks of a lane are asked for at once, the first ones before
-                // the wait for the weights.
+                // 16 x 8 x 16 twice per operand: the eight elements of a lane's share, a[r] = row group r's
+                auto multiply = [&](const uint32_t (&a)[RG][4], int t, const uint4& op, float (&c)[4]) {
+                    mma_16x8x16<F16>(c, a[2 * t][0], a[2 * t + 1][0], a[2 * t][1], a[2 * t + 1][1], op.x, op.y);
+                    mma_16x8x16<F16>(c, a[2 * t][2], a[2 * t + 1][2], a[2 * t][3], a[2 * t + 1][3], op.z, op.w);
+                };
+                // With one token tile the tokens of a lane's chunks are asked for before the wait for the weights, as many as have
+                // place in the registers.
                 constexpr int CHUNKS = 2 * FewFormat<WF>::PACK;     // of 8 elements per lane and step
-                constexpr int AHEAD = N == 1 ? (CHUNKS < 4 ? CHUNKS : 4) : 1;
+                constexpr int AHEAD = N > 1 ? 0 : (CHUNKS * OPERANDS > 6 ? 2 : CHUNKS);
                 auto element = [&](int c) { return (q * CHUNKS + c) * 8; };
-                uint4 hi_ahead[AHEAD], lo_ahead[AHEAD];
-                auto look_ahead = [&](int c0) {
-                    if constexpr (N == 1) {
+                [[maybe_unused]] uint4 ahead[AHEAD > 0 ? AHEAD : 1][OPERANDS];
 #pragma unroll
-                        for (int c = 0; c < AHEAD; ++c)
-                            load_tokens(0, k0 + element(c0 + c), hi_ahead[c], lo_ahead[c]);
+                for (int c = 0; c < AHEAD; ++c) load_tokens(0, k0 + element(c), ahead[c]);
+                [[maybe_unused]] uint32_t exponents[N];             // fp16: of a lane's one (e4m3: two) blocks of 16 columns
+                if constexpr (F16 && !UP) {
+#pragma unroll
+                    for (int nt = 0; nt < N; ++nt)
+                        exponents[nt] = load_exponents(p.h_exp + (size_t)row_at[nt] * (p.I / 16) + (k0 + element(0)) / 16, CHUNKS == 4);
+                }
+                auto tokens = [&](int nt, int c, uint4 (&op)[OPERANDS]) {
+                    if (c < AHEAD) {
+#pragma unroll
+                        for (int j = 0; j < OPERANDS; ++j) op[j] = ahead[c][j];
+                    } else {
+                        load_tokens(nt, k0 + element(c), op);
+                    }
+                    if constexpr (F16 && !UP) {
+                        const int e = (int8_t)(exponents[nt] >> (8 * (c >> 1)));
+                        const __half2 f = __float2half2_rn(few_power(max(min(row_exp[nt] - e, 0), -100)));
+#pragma unroll
+                        for (int j = 0; j < OPERANDS; ++j)
+                            op[j] = make_uint4(scale_pair(op[j].x, f), scale_pair(op[j].y, f), scale_pair(op[j].z, f), scale_pair(op[j].w, f));
                     }
                 };
-                auto tokens = [&](int nt, int c, uint4& hi, uint4& lo) {
-                    if constexpr (N == 1) { hi = hi_ahead[c % AHEAD]; lo = lo_ahead[c % AHEAD]; }
-                    else load_tokens(nt, k0 + element(c), hi, lo);
-                    convert_tokens(nt, hi, lo);
-                };
-                look_ahead(0);
                 if constexpr (S::SCALES > 0) copy_wait<S::D - 2>();
                 if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_step + 8 * c_slot, c_phase, &s.abort, p.dev_status)))
                     return false;
@@ -637,13 +678,15 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 --in_flight;
 
                 if constexpr (WF == FEW_FP8) {
-                    float part[TILES][N][4];            // sums of this step (one scale block of K), to be scaled
+                    float part[SETS][TILES][N][4];      // sums of this step (one scale block of K), to be scaled
 #pragma unroll
-                    for (int t = 0; t < TILES; ++t)
+                    for (int j = 0; j < SETS; ++j)
 #pragma unroll
-                        for (int nt = 0; nt < N; ++nt)
+                        for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) part[t][nt][i] = 0.0f;
+                            for (int nt = 0; nt < N; ++nt)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) part[j][t][nt][i] = 0.0f;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {       // eight codes each
                         uint32_t a[RG][4];
@@ -655,11 +698,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                         }
 #pragma unroll
                         for (int nt = 0; nt < N; ++nt) {
-                            if (nt * 8 >= m) break;
-                            uint4 hi, lo;
-                            tokens(nt, c, hi, lo);
+                            if (nt * TILE >= m) break;
+                            uint4 op[OPERANDS];
+                            tokens(nt, c, op);
 #pragma unroll
-                            for (int t = 0; t < TILES; ++t) multiply(a, t, hi, lo, part[t][nt]);
+                            for (int j = 0; j < OPERANDS; ++j)
+#pragma unroll
+                                for (int t = 0; t < TILES; ++t) multiply(a, t, op[j], part[j][t][nt]);
                         }
                     }
 #pragma unroll
@@ -668,7 +713,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                         for (int i = 0; i < 4; ++i) {
                             const float f = __uint_as_float(ld_shared(scales + (2 * t + (i >> 1)) * 4));
 #pragma unroll
-                            for (int nt = 0; nt < N; ++nt) acc[t][nt][i] = fmaf(part[t][nt][i], f, acc[t][nt][i]);
+                            for (int j = 0; j < SETS; ++j)
+#pragma unroll
+                                for (int nt = 0; nt < N; ++nt) acc[j][t][nt][i] = fmaf(part[j][t][nt][i], f, acc[j][t][nt][i]);
                         }
                 } else {
 #pragma unroll
@@ -681,11 +728,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                         }
 #pragma unroll
                         for (int nt = 0; nt < N; ++nt) {
-                            if (nt * 8 >= m) break;
-                            uint4 hi, lo;
-                            tokens(nt, c, hi, lo);
+                            if (nt * TILE >= m) break;
+                            uint4 op[OPERANDS];
+                            tokens(nt, c, op);
 #pragma unroll
-                            for (int t = 0; t < TILES; ++t) multiply(a, t, hi, lo, acc[t][nt]);
+                            for (int j = 0; j < OPERANDS; ++j)
+#pragma unroll
+                                for (int t = 0; t < TILES; ++t) multiply(a, t, op[j], acc[SETS > 1 ? j : 0][t][nt]);
                         }
                     }
                 }
@@ -702,13 +751,26 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             for (int t = 0; t < TILES; ++t)
 #pragma unroll
                 for (int nt = 0; nt < N; ++nt)
-                    if (nt * 8 < m)
+                    if (nt * TILE < m)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) buf[((t * NT + nt) * 4 + i) * 32 + lane] = acc[t][nt][i];
+                        for (int i = 0; i < 4; ++i) {
+                            float v = acc[0][t][nt][i];
+                            if constexpr (SETS > 1) v += acc[1][t][nt][i];
+                            // columns c and c + 4 are a token's: the lanes two further have the other one
+                            if constexpr (FOLD) v += __shfl_xor_sync(0xffffffffu, v, 2);
+                            buf[((t * NT + nt) * 4 + i) * 32 + lane] = v;
+                        }
             return true;
         };
-        if constexpr (NT == 1) ok = run(Tiles<1>{});
-        else ok = m <= 8 ? run(Tiles<1>{}) : run(Tiles<2>{});
+        if (item.up) {
+            if constexpr (NT == 1) ok = run(Tiles<1>{}, Mode<MODE_UP>{});
+            else ok = m <= 8 ? run(Tiles<1>{}, Mode<MODE_UP>{}) : run(Tiles<2>{}, Mode<MODE_UP>{});
+        } else if (F16 && m <= 4) {
+            if constexpr (F16) ok = run(Tiles<1>{}, Mode<MODE_FOLD>{});
+        } else {
+            if constexpr (NT == 1) ok = run(Tiles<1>{}, Mode<MODE_DOWN>{});
+            else ok = m <= 8 ? run(Tiles<1>{}, Mode<MODE_DOWN>{}) : run(Tiles<2>{}, Mode<MODE_DOWN>{});
+        }
         if (!ok) break;
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar_full + 8 * (nth % S::BUFS));
@@ -746,11 +808,12 @@ FewPlan few_plan(int n, int H, int I, int E, int k) {
     f.logits = take((size_t)n * E * 4);
     f.ncounters = FEW_MAX_EXPERTS + FEW_MAX_SLOTS + 1;
     f.counters = take((size_t)f.ncounters * 4);
-    // the tokens in fp16 (2 bytes, a factor each) or as terms (4 bytes, scale bytes); h in fp32 or as terms
+    // the tokens in fp16 (2 bytes, a factor each) or as terms (4 bytes, scale bytes); h as terms: at most three of 2 bytes, and an
+    // exponent per 16 columns or a scale byte per 32
     f.x = take((size_t)n * H * 4);
     f.x_scale = take((size_t)n * (4 + few_scale_pitch(H)));
-    f.h = take(slots * I * 4);
-    f.h_scale = take(slots * few_scale_pitch(I));
+    f.h = take(slots * I * 6);
+    f.h_scale = take(slots * std::max(I / 16, few_scale_pitch(I)));
     f.partial = take(slots * H * 4 * few_parts(H, I));
     f.total = at;
     return f;
@@ -797,8 +860,12 @@ aristos_status_t launch_few_tokens(const FewParams& p, const FewWeights& w, cuda
     // pass needs one token tile: the registers that this saves are worth 3 % with fp8 weights (345 us against 357 us for 5
     // tokens of 256 experts, 7168 x 2048), nothing with 16-bit ones. Items of 32 rows: with 16 rows (and rings twice as
     // deep) the same cases take 1.1 to 1.4 times as long, the tokens are read once per item.
+    // Two token tiles and three steps of ring leave room for the sums of one item only. 16-bit weights do well with that; with
+    // fp8 ones the streaming warps then wait for the helper, and two steps with two buffers are faster where an item is long
+    // (12 tokens, 4 of 16 experts, 2048 x 4096: 114 us against 126; 32 tokens, 4 of 32, 4096 x 128, the other way round: 103, 101).
     if (p.n <= 8) return launch_few<WF, 1, FewShape<WF, 1, 4, 3, 2>>(p, w, st);
-    return launch_few<WF, 2, FewShape<WF, 2, 4, 3, 1>>(p, w, st);
+    if constexpr (WF == FEW_FP8) return launch_few<WF, 2, FewShape<WF, 2, 4, 2, 2>>(p, w, st);
+    else return launch_few<WF, 2, FewShape<WF, 2, 4, 3, 1>>(p, w, st);
 }
 
 aristos_status_t few_check(int tokens, int H, int I, int E, int k, int weights_dtype) {
@@ -875,7 +942,8 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
     p.s3 = static_cast<const uint8_t*>(s3);
     p.s2 = static_cast<const uint8_t*>(s2);
     p.b1 = b1; p.b3 = gated ? b3 : nullptr; p.b2 = b2;
-    p.h = reinterpret_cast<float*>(ws + f.h);
+    p.h = reinterpret_cast<uint16_t*>(ws + f.h);
+    p.h_exp = reinterpret_cast<int8_t*>(ws + f.h_scale);
     p.x_codes = ws + f.x;
     p.x_scales = ws + f.x_scale;
     p.h_codes = ws + f.h;
