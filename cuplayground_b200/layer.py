@@ -463,6 +463,7 @@ class MoELayer:
         self.rank, self.world = rank, world
         self._lib = _lib.load()
         self._h = C.c_void_p()
+        self.device = torch.cuda.current_device()
         s = cfg.to_struct()
         uid = C.create_string_buffer(nccl_uid, 128) if nccl_uid is not None else None
         _lib.check(self._lib.aristos_moe_create(C.byref(s), rank, world, uid, C.byref(self._h)))
@@ -517,19 +518,43 @@ class MoELayer:
         _lib.check(self._lib.aristos_moe_wait_host(self._h))
 
     def decode(self, x, w_gate, w1, w3, w2, gate_bias=None, out=None, stream=None, scales=None):
-        """The forward for up to 64 tokens, x (tokens, H): two kernels, nothing dropped, activations not quantised. Returns
-        (out, topk_idx (tokens, k), topk_w (tokens, k)). See aristos_moe_decode."""
+        """The forward for up to 64 tokens, x (tokens, H): two kernels, nothing dropped, activations not quantised. w_gate
+        (E, H); w1 / w3 (E, I, H) and w2 (E, H, I) in the layer's dtype (fp8: e4m3 codes, scales as for forward); all on the
+        layer's device. Returns (out, topk_idx (tokens, k), topk_w (tokens, k)). See aristos_moe_decode."""
         if x.dim() != 2 or x.shape[1] != self.H or x.dtype != self.dtype:
             raise ValueError(f"x must be {self.dtype} (tokens, {self.H}), got {x.dtype} {tuple(x.shape)}")
-        with torch.cuda.stream(stream):              # outputs belong to the stream that writes them
-            out = torch.empty_like(x) if out is None else out
-            idx = torch.empty((x.shape[0], self.k), dtype=torch.int32, device=x.device)
-            w = torch.empty((x.shape[0], self.k), dtype=torch.float32, device=x.device)
-        if out.shape != x.shape or out.dtype != x.dtype:
-            raise ValueError("out must have x's shape and dtype")
-        _lib.check(self._lib.aristos_moe_decode(self._h, _ptr(x), x.shape[0], _ptr(w_gate), _ptr(gate_bias), _ptr(w1),
-                                                _ptr(w3), _ptr(w2), _ptr(scales), _ptr(out), _ptr(idx), _ptr(w),
-                                                _stream_ptr(stream)))
+        n, E, H, I = x.shape[0], self.E_local, self.H, self.I
+        gated = self.cfg.hidden_act == _lib.ACT_SWIGLU
+        fp8 = self.cfg.torch_dtype == _lib.DTYPE_FP8_E4M3
+        w3, scales = w3 if gated else None, scales if fp8 else None
+        if w_gate is not None:
+            _expect("w_gate", w_gate, (self.E, H), self.dtype)
+        for name, t, shape in (("w1", w1, (E, I, H)), ("w3", w3, (E, I, H)), ("w2", w2, (E, H, I))):
+            if t is not None:
+                code = torch.float8_e4m3fn if fp8 and t.dtype == torch.float8_e4m3fn else torch.uint8 if fp8 else self.dtype
+                _expect(name, t, shape, code)
+        if gate_bias is not None:
+            _expect("gate_bias", gate_bias, (self.E,), torch.float32)
+        if scales is not None:
+            blocks = E * (I // 128) * (H // 128) * (3 if gated else 2)
+            if scales.dtype != torch.float32 or scales.numel() != blocks:
+                raise ValueError(f"scales must be {blocks} torch.float32, got {scales.numel()} {scales.dtype}")
+        if out is not None:
+            _expect("out", out, (n, H), self.dtype)
+        bias = getattr(self, "_bias", (None, None, None))
+        for name, t, cols in zip(("b1", "b3", "b2"), bias, (I, I, H)):
+            if t is not None and (t.dtype != self.dtype or t.numel() != E * cols):
+                raise ValueError(f"{name} must be {E * cols} {self.dtype}, got {t.numel()} {t.dtype}")
+        with _Device(x, w_gate, w1, w3, w2, gate_bias, scales, out, *bias) as on:
+            if on.index != self.device or (stream is not None and stream.device.index != self.device):
+                raise ValueError(f"the layer, its tensors and the stream must be on one device, the layer is on cuda:{self.device}")
+            with torch.cuda.stream(stream):              # outputs belong to the stream that writes them
+                out = torch.empty_like(x) if out is None else out
+                idx = x.new_empty((n, self.k), dtype=torch.int32)
+                w = x.new_empty((n, self.k), dtype=torch.float32)
+            _lib.check(self._lib.aristos_moe_decode(self._h, _addr(x), n, _addr(w_gate), _addr(gate_bias), _addr(w1), _addr(w3),
+                                                    _addr(w2), _addr(scales), _addr(out), _addr(idx), _addr(w),
+                                                    on.stream if stream is None else stream.cuda_stream))
         return out, idx, w
 
     def routing(self) -> dict:
