@@ -124,7 +124,9 @@ __device__ __forceinline__ bool wait_hidden(const FewParams& p, FewRouting& s, i
             if (__any_sync(0xffffffffu, !ok)) return false;
         }
     }
+    // the lane that read the counter in question orders the others behind it: the vote alone does not
     asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    __syncwarp();
     return true;
 }
 

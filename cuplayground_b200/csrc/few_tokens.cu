@@ -591,7 +591,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                 }
             }
             if (!ok) break;
+            // the lane that read the counter in question orders the others behind it: the vote alone does not
             asm volatile("fence.acq_rel.gpu;" ::: "memory");
+            __syncwarp();
         }
         // with as many token tiles as this pass has tokens for: most experts have a few, whatever the batch is
         auto run = [&](auto tiles, auto what) -> bool {
@@ -669,7 +671,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                             op[j] = make_uint4(scale_pair(op[j].x, f), scale_pair(op[j].y, f), scale_pair(op[j].z, f), scale_pair(op[j].w, f));
                     }
                 };
-                if constexpr (S::SCALES > 0) copy_wait<S::D - 2>();
+                if constexpr (S::SCALES > 0) {
+                    copy_wait<S::D - 2>();
+                    __syncwarp();                           // all lanes read the scales that RG lanes have asked for
+                }
                 if (!__all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_step + 8 * c_slot, c_phase, &s.abort, p.dev_status)))
                     return false;
                 const uint32_t from = ring + c_slot * S::SLOT + g * 128;
