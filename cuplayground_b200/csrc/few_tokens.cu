@@ -390,17 +390,29 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             more[grp] = forward(items[grp], blockIdx.x * FEW_GROUPS + grp);
         }
         int posts = 0;
-        auto post = [&](int a) {
+        auto post = [&](int a) -> bool {                // false after a wait that gave up: nothing has been posted
             // room in the post (it holds more than the groups can have done while one release takes place)
-            const uint64_t t0 = ptx::globaltimer_ns();
-            while (posts - ld_acquire_shared(ptx::smem_u32(&s.counted)) >= FEW_POST &&
-                   ptx::globaltimer_ns() - t0 < ptx::WAIT_LIMIT_NS) {}
+            bool room = true;
+            uint64_t t0 = 0;
+            for (uint32_t i = 0; posts - ld_acquire_shared(ptx::smem_u32(&s.counted)) >= FEW_POST; ++i) {
+                if (i == 0) t0 = ptx::globaltimer_ns();
+                if ((i & 15u) != 15u) continue;
+                if (*static_cast<volatile int*>(&s.abort)) { room = false; break; }
+                if (ptx::globaltimer_ns() - t0 > ptx::WAIT_LIMIT_NS) {
+                    s.abort = 1;
+                    if (p.dev_status) atomicOr(p.dev_status, DEV_FAULT_TIMEOUT);
+                    room = false;
+                    break;
+                }
+            }
+            if (!__all_sync(0xffffffffu, room)) return false;
             __syncwarp();
             if (lane == 0) {
                 s.post[posts % FEW_POST] = a;
                 st_release_shared(ptx::smem_u32(&s.posted), posts + 1);
             }
             ++posts;
+            return true;
         };
         // one item; returns false after a wait that gave up
         auto add_up = [&](const Item& item, int grp, int nth) -> bool {
@@ -471,8 +483,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
             }
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(bar_free + 8 * b);
-            if (item.up) post(item.a);
-            return true;
+            return !item.up || post(item.a);
         };
         for (int nth = 0;; ++nth) {
             bool any = false;
