@@ -938,8 +938,18 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
     if (!x || !w_gate || !w1 || !w2 || !out || !workspace) { set_last_error("moe_few_tokens: NULL pointer"); return ARISTOS_ERR_INVALID_ARG; }
     if (gated && !w3) { set_last_error("moe_few_tokens: SwiGLU needs w3"); return ARISTOS_ERR_INVALID_ARG; }
     if ((fp8 || fp4) && (!s1 || !s2 || (gated && !s3))) { set_last_error("moe_few_tokens: quantised weights need their scales"); return ARISTOS_ERR_INVALID_ARG; }
-    for (const void* q : {x, w_gate, w1, w2, (const void*)out, (const void*)workspace, gated ? w3 : w1, s1, s2, gated ? s3 : s1}) {
+    for (const void* q : {x, w_gate, w1, w2, (const void*)out, (const void*)workspace, gated ? w3 : w1}) {
         if (!aligned16(q)) { set_last_error("moe_few_tokens: pointers must be 16-byte aligned"); return ARISTOS_ERR_INVALID_ARG; }
+    }
+    if (fp8 || fp4) {
+        // fp8 scales are read one by one, 4-bit ones in whole tiles
+        const uintptr_t unit = fp8 ? sizeof(float) : 16;
+        for (const void* q : {s1, s2, gated ? s3 : s1}) {
+            if (reinterpret_cast<uintptr_t>(q) % unit != 0) {
+                set_last_error("moe_few_tokens: scales must be %d-byte aligned", (int)unit);
+                return ARISTOS_ERR_INVALID_ARG;
+            }
+        }
     }
     const FewPlan f = few_plan(tokens, H, I, E, k);
     if (workspace_bytes < f.total) {

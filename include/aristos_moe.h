@@ -397,7 +397,8 @@ ARISTOS_API aristos_status_t aristos_expert_ffn_fp4(const void* xq, const void* 
  * ARISTOS_FEW_TOKENS_MAX; w_gate (E, H) and the optional biases b1 / b3 (E, I), b2 (E, H) in the same dtype; gate_bias
  * (E) fp32 or NULL. weights_dtype: `dtype` itself, ARISTOS_DTYPE_FP8_E4M3 (bf16 activations only; s1 / s3 / s2 fp32 as
  * aristos_quantize_fp8(block_rows = 128) writes them; H and I multiples of 128) or ARISTOS_DTYPE_FP4_E2M1 (codes and
- * scale tiles of aristos_quantize_fp4; scale byte 255 makes the row's results NaN). E <= 512.
+ * scale tiles of aristos_quantize_fp4; scale byte 255 makes the row's results NaN). E <= 512. x, w_gate, weights, out, 4-bit
+ * scales and workspace 16-byte aligned.
  * Activations are not quantised. The hidden ones are computed in fp32 and meet the weights as sums of 16-bit numbers (bf16
  * weights: three, all 24 bits; fp16 and fp8 weights: two, off by 2^-24 of the value or 2^-38 of the largest of the row) or of
  * eight 4-bit numbers (4-bit weights: 24 bits of the largest of 32). A token's results do not depend on the other tokens of the

@@ -63,3 +63,18 @@ def test_fp8_weights_are_codes():
     for codes in (torch.uint8, torch.float8_e4m3fn):               # as they are, or typed: as far as the device
         with pytest.raises(ValueError, match="CUDA device"):
             L.decode(**_args(L, codes), scales=scales)
+
+
+def test_e4m3_scales_need_no_more_than_their_own_alignment():
+    """Scales may be parts of one tensor [s1 | s3 | s2], as a layer's are: with an odd number of blocks per matrix the second and
+    third start on 4 bytes. The kernels read them one at a time. (A workspace of 0 bytes is refused last: nothing is launched.)"""
+    import ctypes as C
+    lib = cp._lib.load()
+    P = 1 << 20
+    call = lambda s1, s3, s2, wdt: lib.aristos_moe_few_tokens(P, P, None, P, P, P, s1, s3, s2, None, None, None, 4, 128, 128, 3, 2, 0,
+                                                              0, 2, 2, wdt, P, None, None, P, 0, None, None)
+    WORKSPACE, INVALID = 7, 1
+    assert call(P, P + 12, P + 24, 4) == WORKSPACE
+    assert call(P + 4, P + 4, P + 4, 4) == WORKSPACE
+    assert call(P + 2, P, P, 4) == INVALID and call(P, P, P + 1, 4) == INVALID and call(P, P + 2, P, 4) == INVALID
+    assert call(P, P + 12, P + 24, 5) == INVALID               # scale tiles of 4-bit weights travel in pieces of 16 bytes

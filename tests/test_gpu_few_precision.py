@@ -83,3 +83,13 @@ def test_hidden_activations_of_very_different_size(weights, dtype, n):
     out, idx, w = c.run()
     ref, bound = R.moe_few(c.x, idx, w, c.mats, c.b, 0, 2.0 ** -24)
     R.assert_within(out, ref, bound + R.half_step(c.dt) * (ref.abs() + bound) * 1.01 + 2.0 ** -25)
+
+
+def test_e4m3_scales_that_are_parts_of_one_tensor():
+    """3 experts of one 128 x 128 block: the scales of w3 start 12 bytes behind those of w1."""
+    import torch
+    c = Case(5, 3, 2, 128, 128, 2, "8", seed=12)
+    want = c.run()
+    packed = torch.cat([c.s[m].reshape(-1) for m in ("1", "3", "2")])
+    c.s = {m: packed[3 * i:3 * i + 3].view(3, 1, 1) for i, m in enumerate(("1", "3", "2"))}
+    assert all(torch.equal(a, b) for a, b in zip(c.run(), want))
