@@ -39,10 +39,11 @@
 // on the two others.
 #include <cuda.h>
 
-#include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "fp4_format.cuh"
+#include "per_device.h"
 #include "ptx_sm100.cuh"
 #include "tensor_map.cuh"
 
@@ -599,11 +600,15 @@ aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, 
     const int sms = device_sm_count();
     if (sms <= 0) { set_last_error("no CUDA device"); return ARISTOS_ERR_CUDA; }
     const int64_t bound = (int64_t)p.groups * ceil_div(p.rows_per_group, F4_PM) * ceil_div(p.N, p.gated ? 128 : 256);
-    auto run = [&](auto kernel) -> aristos_status_t {
+    auto run = [&](auto output, auto activation) -> aristos_status_t {
+        const auto kernel = ffn_fp4_grouped_gemm_kernel<decltype(output)::value, decltype(activation)::value>;
         ARISTOS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F4_SMEM_BYTES));
-        // one pair per two SMs, as many as the device holds at once (not every SM has a partner in its cluster's reach)
-        static std::atomic<int> most_pairs{0};
-        int most = most_pairs.load(std::memory_order_relaxed);
+        // One pair per two SMs, as many as the device holds at once (not every SM has a partner in its cluster's reach): one table
+        // per kernel, this being a function per output type and activation.
+        static PerDevice most_pairs;
+        int device = 0;
+        ARISTOS_CUDA_TRY(cudaGetDevice(&device));
+        int most = most_pairs.get(device);
         if (most == 0) {
             cudaLaunchConfig_t lc = {};
             lc.gridDim = dim3(2 * (sms / 2));
@@ -617,7 +622,7 @@ aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, 
             int n = 0;
             ARISTOS_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &lc));
             most = n > 0 ? n : 1;
-            most_pairs.store(most, std::memory_order_relaxed);
+            most_pairs.set(device, most);
         }
         const int pairs = (int)(bound < most ? bound : most);
         cudaLaunchConfig_t cfg = {};
@@ -634,16 +639,19 @@ aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, 
         ARISTOS_COUNT_LAUNCH();
         return ARISTOS_OK;
     };
+    using std::integral_constant;
+    using Identity = integral_constant<int, ARISTOS_ACT_IDENTITY>;
+    using Fp4 = integral_constant<int, OUT_FP4>;
     switch (out) {
-        case OUT_F32: return run(ffn_fp4_grouped_gemm_kernel<OUT_F32, ARISTOS_ACT_IDENTITY>);
-        case OUT_BF16: return run(ffn_fp4_grouped_gemm_kernel<OUT_BF16, ARISTOS_ACT_IDENTITY>);
-        case OUT_F16: return run(ffn_fp4_grouped_gemm_kernel<OUT_F16, ARISTOS_ACT_IDENTITY>);
+        case OUT_F32: return run(integral_constant<int, OUT_F32>{}, Identity{});
+        case OUT_BF16: return run(integral_constant<int, OUT_BF16>{}, Identity{});
+        case OUT_F16: return run(integral_constant<int, OUT_F16>{}, Identity{});
         default: break;
     }
     switch (p.act) {
-        case ARISTOS_ACT_RELU: return run(ffn_fp4_grouped_gemm_kernel<OUT_FP4, ARISTOS_ACT_RELU>);
-        case ARISTOS_ACT_GELU: return run(ffn_fp4_grouped_gemm_kernel<OUT_FP4, ARISTOS_ACT_GELU>);
-        default: return run(ffn_fp4_grouped_gemm_kernel<OUT_FP4, ARISTOS_ACT_SWIGLU>);
+        case ARISTOS_ACT_RELU: return run(Fp4{}, integral_constant<int, ARISTOS_ACT_RELU>{});
+        case ARISTOS_ACT_GELU: return run(Fp4{}, integral_constant<int, ARISTOS_ACT_GELU>{});
+        default: return run(Fp4{}, integral_constant<int, ARISTOS_ACT_SWIGLU>{});
     }
 }
 
