@@ -49,7 +49,7 @@ def moe_forward(x: torch.Tensor, w_gate: torch.Tensor, w1: torch.Tensor, w3: Opt
 
 @moe_forward.register_fake
 def _(x, w_gate, w1, w3, w2, scales, handle):
-    return torch.empty_like(x)
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 @torch.library.custom_op("aristos::moe_decode", mutates_args=(), device_types="cuda")
@@ -65,7 +65,7 @@ def moe_decode(x: torch.Tensor, w_gate: torch.Tensor, w1: torch.Tensor, w3: Opti
 
 @moe_decode.register_fake
 def _(x, w_gate, w1, w3, w2, scales, handle):
-    return torch.empty_like(x)
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 class AristosMoE(torch.nn.Module):

@@ -44,3 +44,33 @@ def test_module_matches_layer_and_oracle(oracle):
     with pytest.raises(RuntimeError):
         m(x[:2])                                                           # the handle was created for 512 tokens
     m.close()
+
+
+def test_results_are_contiguous_where_the_inputs_are_not():
+    """The ops return contiguous tensors whatever x's strides are, and their fake implementations say so: a compiled graph indexes
+    by what the fake one says."""
+    import cuplayground_b200.torch_op  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(16, 8, dtype=torch.bfloat16, device="cuda").t()            # (8, 16), strides (1, 8)
+        w = torch.empty(4, 16, dtype=torch.bfloat16, device="cuda")
+        for op in (torch.ops.aristos.moe_decode, torch.ops.aristos.moe_forward):
+            out = op(x, w, w, None, w, None, 1)
+            assert out.shape == (8, 16) and out.stride() == (16, 1)
+        assert torch.ops.aristos.moe_decode(torch.empty(3, 16, device="cuda"), w, w, None, w, None, 1).stride() == (16, 1)
+
+
+@pytest.mark.gpu
+def test_the_real_ops_return_what_the_fake_ones_say():
+    import cuplayground_b200 as cp
+    from cuplayground_b200.torch_op import AristosMoE
+    cfg = cp.AristosConfig(expert_top_k=2, hidden_act=0, hidden_size=256, intermediate_size=256, num_experts=4, torch_dtype=2,
+                           tokens=128)
+    m = AristosMoE(cfg)
+    x = torch.randn(256, 128, device="cuda", dtype=torch.bfloat16).t()             # (128, 256), not contiguous
+    args = (m.w_gate, m.w1, None, m.w2, None, m._handle)
+    for op, v in ((torch.ops.aristos.moe_forward, x), (torch.ops.aristos.moe_decode, x[:5])):
+        out = op(v, *args)
+        assert out.stride() == (256, 1) and torch.equal(out, op(v.contiguous(), *args))
+        torch.library.opcheck(op.default, (v, *args), test_utils=("test_schema", "test_faketensor"))
+    m.close()
