@@ -82,6 +82,9 @@ inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 // Number of SMs of the current device (cached per device).
 int device_sm_count();
 
+// Workspace of the few-token layer for as many tokens as it takes; 0 (and no error text): sizes that it refuses.
+size_t few_layer_workspace_bytes(int H, int I, int E, int k);
+
 // Per-thread launch counter, read by the layer to report how many kernels it launched.
 int64_t& launch_counter();
 #define ARISTOS_COUNT_LAUNCH() (++::aristos::launch_counter())

@@ -884,27 +884,32 @@ aristos_status_t launch_few_tokens(const FewParams& p, const FewWeights& w, cuda
     else return launch_few<WF, 2, FewShape<WF, 2, 4, 3, 1>>(p, w, st);
 }
 
-aristos_status_t few_check(int tokens, int H, int I, int E, int k, int weights_dtype) {
-    if (tokens < 0 || H <= 0 || I <= 0 || E <= 0 || k <= 0) { set_last_error("moe_few_tokens: bad size"); return ARISTOS_ERR_INVALID_ARG; }
-    if (tokens > FEW_MAX_TOKENS) {
-        set_last_error("moe_few_tokens: %d tokens, at most %d", tokens, FEW_MAX_TOKENS);
-        return ARISTOS_ERR_CONFIG;
-    }
+// say: whether a refusal becomes the thread's error text.
+aristos_status_t few_check(int tokens, int H, int I, int E, int k, int weights_dtype, bool say = true) {
+    auto refuse = [&](aristos_status_t status, const char* fmt, auto... values) {
+        if (say) set_last_error(fmt, values...);
+        return status;
+    };
+    if (tokens < 0 || H <= 0 || I <= 0 || E <= 0 || k <= 0) return refuse(ARISTOS_ERR_INVALID_ARG, "moe_few_tokens: bad size");
+    if (tokens > FEW_MAX_TOKENS) return refuse(ARISTOS_ERR_CONFIG, "moe_few_tokens: %d tokens, at most %d", tokens, FEW_MAX_TOKENS);
     const int unit = weights_dtype == ARISTOS_DTYPE_FP8_E4M3 ? 128 : 64;
-    if (H % unit != 0 || I % unit != 0) {
-        set_last_error("moe_few_tokens: the feature sizes must be multiples of %d", unit);
-        return ARISTOS_ERR_CONFIG;
-    }
-    if (k > E || k > MAX_TOPK || E > FEW_MAX_EXPERTS) {
-        set_last_error("moe_few_tokens: need k <= min(E, %d), E <= %d", MAX_TOPK, FEW_MAX_EXPERTS);
-        return ARISTOS_ERR_CONFIG;
-    }
+    if (H % unit != 0 || I % unit != 0)
+        return refuse(ARISTOS_ERR_CONFIG, "moe_few_tokens: the feature sizes must be multiples of %d", unit);
+    if (k > E || k > MAX_TOPK || E > FEW_MAX_EXPERTS)
+        return refuse(ARISTOS_ERR_CONFIG, "moe_few_tokens: need k <= min(E, %d), E <= %d", MAX_TOPK, FEW_MAX_EXPERTS);
     // items are numbered in 31 bits
-    if ((int64_t)E * ((int64_t)H * few_parts(H, I) + I) >= (int64_t)1 << 30) { set_last_error("moe_few_tokens: too many weight rows"); return ARISTOS_ERR_CONFIG; }
+    if ((int64_t)E * ((int64_t)H * few_parts(H, I) + I) >= (int64_t)1 << 30)
+        return refuse(ARISTOS_ERR_CONFIG, "moe_few_tokens: too many weight rows");
     return ARISTOS_OK;
 }
 
 }  // namespace
+
+size_t few_layer_workspace_bytes(int H, int I, int E, int k) {
+    if (few_check(FEW_MAX_TOKENS, H, I, E, k, ARISTOS_DTYPE_BF16, false) != ARISTOS_OK) return 0;
+    return few_plan(FEW_MAX_TOKENS, H, I, E, k).total;
+}
+
 }  // namespace aristos
 
 using namespace aristos;

@@ -78,8 +78,9 @@ struct aristos_moe {
     int32_t *send_base = nullptr, *dense_count = nullptr, *src_off = nullptr;
     int32_t* ffn_done = nullptr;             // counters of the one-launch expert FFN (groups x row tiles)
     size_t ffn_done_ints = 0;
-    void* few_ws = nullptr;                  // decode (few tokens): workspace for ARISTOS_FEW_TOKENS_MAX tokens
+    void* few_ws = nullptr;                  // decode (few tokens): workspace of its own, for ARISTOS_FEW_TOKENS_MAX tokens
     size_t few_ws_bytes = 0;                 // 0: this layer has no decode
+    bool few_ws_owned = false;
     int64_t launches = 0;
     const void *b1 = nullptr, *b3 = nullptr, *b2 = nullptr;   // optional expert biases (caller-owned, device)
     // failure handling of the exchange: every wait for a forward's completion has a wall-clock limit; on expiry the
@@ -176,7 +177,6 @@ size_t plan_workspace(aristos_moe* L, char* base) {
         L->xr = L->xg;
         L->yg = L->yr;
     }
-    if (L->few_ws_bytes) CARVE(few_ws, void*, L->few_ws_bytes)
     for (int i = 0; i < aristos_moe::HOST_SLOTS; ++i) {
         CARVE(slots[i].x_dev, void*, S * H * elt)
         CARVE(slots[i].out_dev, void*, S * H * elt)
@@ -368,7 +368,7 @@ aristos_status_t aristos_moe_create(const aristos_config_t* cfg, int rank, int w
         }
     }
     if (world == 1 && (L->fp8 || cfg->torch_dtype == ARISTOS_DTYPE_BF16 || cfg->torch_dtype == ARISTOS_DTYPE_F16))
-        L->few_ws_bytes = aristos_moe_few_tokens_workspace_bytes(ARISTOS_FEW_TOKENS_MAX, L->H, L->I, L->E, L->k);
+        L->few_ws_bytes = few_layer_workspace_bytes(L->H, L->I, L->E, L->k);
     L->ws_bytes = plan_workspace(L, nullptr);
     *out = L;
     return ARISTOS_OK;
@@ -402,6 +402,22 @@ aristos_status_t aristos_moe_set_workspace(aristos_moe_t* L, void* workspace, si
     plan_workspace(L, static_cast<char*>(workspace));
     ARISTOS_CUDA_TRY(cudaMemset(L->dev_status, 0, 4));
     L->bias_ready = false;
+    return ARISTOS_OK;
+}
+
+size_t aristos_moe_decode_workspace_bytes(const aristos_moe_t* L) { return L ? L->few_ws_bytes : 0; }
+
+aristos_status_t aristos_moe_set_decode_workspace(aristos_moe_t* L, void* workspace, size_t bytes) {
+    if (!L || !workspace) { set_last_error("decode workspace: NULL pointer"); return ARISTOS_ERR_INVALID_ARG; }
+    if (L->few_ws_bytes == 0) { set_last_error("decode workspace: this layer has no decode"); return ARISTOS_ERR_UNSUPPORTED; }
+    if (bytes < L->few_ws_bytes) {
+        set_last_error("decode workspace: %zu bytes given, %zu needed", bytes, L->few_ws_bytes);
+        return ARISTOS_ERR_WORKSPACE;
+    }
+    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) { set_last_error("decode workspace must be 256-byte aligned"); return ARISTOS_ERR_INVALID_ARG; }
+    if (L->few_ws && L->few_ws_owned) cudaFree(L->few_ws);
+    L->few_ws = workspace;
+    L->few_ws_owned = false;
     return ARISTOS_OK;
 }
 
@@ -463,6 +479,16 @@ aristos_status_t aristos_moe_decode(aristos_moe_t* L, const void* x, int tokens,
     if (tokens == 0) return ARISTOS_OK;
     if (L->fp8 && !scales) { set_last_error("decode: fp8 needs the weight scales"); return ARISTOS_ERR_INVALID_ARG; }
     ARISTOS_TRY(ensure_workspace(L));
+    if (!L->few_ws) {
+        void* p = nullptr;
+        const cudaError_t e = cudaMalloc(&p, L->few_ws_bytes);
+        if (e != cudaSuccess) {
+            set_last_error("cudaMalloc of the %zu-byte decode workspace failed: %s", L->few_ws_bytes, cudaGetErrorString(e));
+            return ARISTOS_ERR_NOMEM;
+        }
+        L->few_ws = p;
+        L->few_ws_owned = true;
+    }
     const float* bias = nullptr;
     ARISTOS_TRY(gate_prior(L, gate_bias, static_cast<cudaStream_t>(stream), &bias));
     const bool swiglu = L->cfg.hidden_act == ARISTOS_ACT_SWIGLU;
@@ -1041,6 +1067,7 @@ aristos_status_t aristos_moe_destroy(aristos_moe_t* L) {
     if (L->p2p) ep_p2p_destroy(L->p2p);
     if (L->comm) ep_comm_destroy(L->comm);
     if (L->ws && L->ws_owned) cudaFree(L->ws);
+    if (L->few_ws && L->few_ws_owned) cudaFree(L->few_ws);
     delete L;
     return ARISTOS_OK;
 }

@@ -471,14 +471,15 @@ class MoELayer:
         self.E, self.k, self.cap = cfg.num_experts, cfg.expert_top_k, cfg.capacity
         self.E_local = self.E // world
         self.dtype = _TORCH_DTYPE[cfg.torch_dtype]
-        self._ws = None
+        self._ws = self._decode_ws = None
 
     @property
     def workspace_bytes(self) -> int:
         return int(self._lib.aristos_moe_workspace_bytes(self._h))
 
     def use_torch_workspace(self) -> None:
-        """Allocate the workspace from torch's caching allocator instead of cudaMalloc inside the library."""
+        """Allocate the workspace (and decode's own, when it first decodes) from torch's caching allocator instead of cudaMalloc
+        inside the library."""
         self._ws = torch.empty(self.workspace_bytes + 1024, dtype=torch.uint8, device="cuda")
         base = (self._ws.data_ptr() + 1023) // 1024 * 1024
         _lib.check(self._lib.aristos_moe_set_workspace(self._h, C.c_void_p(base), self.workspace_bytes))
@@ -548,6 +549,12 @@ class MoELayer:
         with _Device(x, w_gate, w1, w3, w2, gate_bias, scales, out, *bias) as on:
             if on.index != self.device or (stream is not None and stream.device.index != self.device):
                 raise ValueError(f"the layer, its tensors and the stream must be on one device, the layer is on cuda:{self.device}")
+            if self._ws is not None and self._decode_ws is None:
+                nbytes = int(self._lib.aristos_moe_decode_workspace_bytes(self._h))
+                if nbytes:                               # 0: the library refuses
+                    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+                    _lib.check(self._lib.aristos_moe_set_decode_workspace(self._h, _addr(ws), nbytes))
+                    self._decode_ws = ws
             with torch.cuda.stream(stream):              # outputs belong to the stream that writes them
                 out = torch.empty_like(x) if out is None else out
                 idx = x.new_empty((n, self.k), dtype=torch.int32)

@@ -70,6 +70,9 @@ public:
 
     size_t workspace_bytes() const { return aristos_moe_workspace_bytes(h_); }
     void set_workspace(void* device_ptr, size_t bytes) { check(aristos_moe_set_workspace(h_, device_ptr, bytes)); }
+    // decode's own workspace (0 bytes: this layer has no decode)
+    size_t decode_workspace_bytes() const { return aristos_moe_decode_workspace_bytes(h_); }
+    void set_decode_workspace(void* device_ptr, size_t bytes) { check(aristos_moe_set_decode_workspace(h_, device_ptr, bytes)); }
 
     // Device tensors: x (S,H), w_gate (E,H), w1/w3 (E_local,I,H), w2 (E_local,H,I), out (S,H). Asynchronous on stream.
     void forward(const void* x, const void* w_gate, const void* w1, const void* w3, const void* w2, void* out,

@@ -182,13 +182,17 @@ ARISTOS_API aristos_status_t aristos_moe_wait_host(aristos_moe_t* layer);
  * activation and biases and the arguments of aristos_moe_forward. x, out (tokens, H). No token is dropped, fp8 layers do
  * not quantise the activations, and nothing that aristos_moe_routing or aristos_moe_training_state returns changes;
  * topk_idx / topk_w (tokens, k) receive this call's routing, or NULL. One rank, torch_dtype 2, 3 or 4, E <= 512, else
- * ARISTOS_ERR_UNSUPPORTED. Uses the layer's workspace (which the first forward or decode allocates: outside a capture):
- * calls of one handle are ordered by the caller, as forwards are.
+ * ARISTOS_ERR_UNSUPPORTED. Uses the layer's workspace and one of its own, both allocated by the first call that needs them
+ * (outside a capture) unless the caller hands them over: calls of one handle are ordered by the caller, as forwards are.
  */
 ARISTOS_API aristos_status_t aristos_moe_decode(aristos_moe_t* layer, const void* x, int tokens, const void* w_gate,
                                                 const float* gate_bias, const void* w1, const void* w3, const void* w2,
                                                 const void* scales, void* out, int32_t* topk_idx, float* topk_w,
                                                 void* stream);
+/* Optional: decode's own workspace as a caller-owned one (>= aristos_moe_decode_workspace_bytes, which is 0 for a layer that
+ * has no decode; 256-byte aligned). A layer that never decodes needs none. */
+ARISTOS_API size_t aristos_moe_decode_workspace_bytes(const aristos_moe_t* layer);
+ARISTOS_API aristos_status_t aristos_moe_set_decode_workspace(aristos_moe_t* layer, void* workspace, size_t bytes);
 ARISTOS_API aristos_status_t aristos_moe_routing(const aristos_moe_t* layer, aristos_routing_t* out);
 /* Copies the routing tensors of the last forward into host buffers sized as in aristos_routing_t (any pointer may
  * be NULL); synchronises the device first. */
