@@ -84,6 +84,12 @@ int device_sm_count();
 
 // Workspace of the few-token layer for as many tokens as it takes; 0 (and no error text): sizes that it refuses.
 size_t few_layer_workspace_bytes(int H, int I, int E, int k);
+// aristos_moe_few_tokens. report_nan: a token whose gate logits are all NaN raises DEV_FAULT_NONFINITE in dev_status.
+aristos_status_t run_few_tokens(const void* x, const void* w_gate, const float* gate_bias, const void* w1, const void* w3,
+                                const void* w2, const void* s1, const void* s3, const void* s2, const void* b1, const void* b3,
+                                const void* b2, int tokens, int H, int I, int E, int k, int gate_fn, int renorm, int hidden_act,
+                                int dtype, int weights_dtype, void* out, int32_t* topk_idx, float* topk_w, void* workspace,
+                                size_t workspace_bytes, int32_t* dev_status, bool report_nan, void* stream);
 
 // Per-thread launch counter, read by the layer to report how many kernels it launched.
 int64_t& launch_counter();

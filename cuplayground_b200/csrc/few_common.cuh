@@ -35,6 +35,7 @@ struct FewParams {
     int gate_fn, renorm, act;
     int parts;                     // K of the down projection is cut into so many items
     int f16;                       // dtype of out and of the biases: fp16, else bf16
+    int report_nan;                // a token whose logits are all NaN raises DEV_FAULT_NONFINITE
 };
 
 struct FewWeights { const void *w1, *w3, *w2; };
@@ -71,6 +72,12 @@ __device__ __forceinline__ void few_topk(const float* __restrict__ l, const FewP
     float v[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) v[i] = i * 32 + lane < p.E ? __ldcg(l + i * 32 + lane) : 0.0f;
+    if (p.report_nan && blockIdx.x == 0) {
+        bool number = false;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) number |= i * 32 + lane < p.E && v[i] == v[i];
+        if (!__any_sync(0xffffffffu, number) && lane == 0 && p.dev_status) atomicOr(p.dev_status, DEV_FAULT_NONFINITE);
+    }
     uint32_t taken = 0;
     float my_l = 0.0f;
 #pragma unroll 1

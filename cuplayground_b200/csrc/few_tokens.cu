@@ -910,22 +910,11 @@ size_t few_layer_workspace_bytes(int H, int I, int E, int k) {
     return few_plan(FEW_MAX_TOKENS, H, I, E, k).total;
 }
 
-}  // namespace aristos
-
-using namespace aristos;
-
-extern "C" size_t aristos_moe_few_tokens_workspace_bytes(int tokens, int H, int I, int E, int k) {
-    if (few_check(tokens, H, I, E, k, ARISTOS_DTYPE_BF16) != ARISTOS_OK) return 0;
-    return few_plan(tokens, H, I, E, k).total;
-}
-
-extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_gate, const float* gate_bias,
-                                                   const void* w1, const void* w3, const void* w2, const void* s1,
-                                                   const void* s3, const void* s2, const void* b1, const void* b3,
-                                                   const void* b2, int tokens, int H, int I, int E, int k, int gate_fn,
-                                                   int renorm, int hidden_act, int dtype, int weights_dtype, void* out,
-                                                   int32_t* topk_idx, float* topk_w, void* workspace,
-                                                   size_t workspace_bytes, int32_t* dev_status, void* stream) {
+aristos_status_t run_few_tokens(const void* x, const void* w_gate, const float* gate_bias, const void* w1, const void* w3,
+                                const void* w2, const void* s1, const void* s3, const void* s2, const void* b1, const void* b3,
+                                const void* b2, int tokens, int H, int I, int E, int k, int gate_fn, int renorm, int hidden_act,
+                                int dtype, int weights_dtype, void* out, int32_t* topk_idx, float* topk_w, void* workspace,
+                                size_t workspace_bytes, int32_t* dev_status, bool report_nan, void* stream) {
     if (dtype != ARISTOS_DTYPE_BF16 && dtype != ARISTOS_DTYPE_F16) {
         set_last_error("moe_few_tokens: activations must be bf16 or fp16");
         return ARISTOS_ERR_UNSUPPORTED;
@@ -991,6 +980,7 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
     p.gate_fn = gate_fn; p.renorm = renorm; p.act = hidden_act;
     p.parts = few_parts(H, I);
     p.f16 = f16 ? 1 : 0;
+    p.report_nan = report_nan ? 1 : 0;
 
     // A warp per (expert, token) while that does not ask for more warps than run at once, else four tokens per warp.
     const int tok = (int64_t)E * tokens <= 2048 ? 1 : 4;
@@ -1019,4 +1009,24 @@ extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_
     if (fp4) return launch_few_fp4(p, w, st);
     if (fp8) return launch_few_tokens<FEW_FP8>(p, w, st);
     return f16 ? launch_few_tokens<FEW_F16>(p, w, st) : launch_few_tokens<FEW_BF16>(p, w, st);
+}
+
+}  // namespace aristos
+
+using namespace aristos;
+
+extern "C" size_t aristos_moe_few_tokens_workspace_bytes(int tokens, int H, int I, int E, int k) {
+    if (few_check(tokens, H, I, E, k, ARISTOS_DTYPE_BF16) != ARISTOS_OK) return 0;
+    return few_plan(tokens, H, I, E, k).total;
+}
+
+extern "C" aristos_status_t aristos_moe_few_tokens(const void* x, const void* w_gate, const float* gate_bias,
+                                                   const void* w1, const void* w3, const void* w2, const void* s1,
+                                                   const void* s3, const void* s2, const void* b1, const void* b3,
+                                                   const void* b2, int tokens, int H, int I, int E, int k, int gate_fn,
+                                                   int renorm, int hidden_act, int dtype, int weights_dtype, void* out,
+                                                   int32_t* topk_idx, float* topk_w, void* workspace,
+                                                   size_t workspace_bytes, int32_t* dev_status, void* stream) {
+    return run_few_tokens(x, w_gate, gate_bias, w1, w3, w2, s1, s3, s2, b1, b3, b2, tokens, H, I, E, k, gate_fn, renorm, hidden_act, dtype,
+                          weights_dtype, out, topk_idx, topk_w, workspace, workspace_bytes, dev_status, false, stream);
 }

@@ -495,11 +495,12 @@ aristos_status_t aristos_moe_decode(aristos_moe_t* L, const void* x, int tokens,
     const float* s1 = L->fp8 ? static_cast<const float*>(scales) : nullptr;
     const size_t nb = (size_t)L->E * (L->I / 128) * (L->H / 128);
     const int64_t launches0 = launch_counter();
-    const aristos_status_t s = aristos_moe_few_tokens(
+    // NaN logits are reported where a forward of this layer reports them: by the screened gate
+    const aristos_status_t s = run_few_tokens(
         x, w_gate, bias, w1, w3, w2, s1, L->fp8 && swiglu ? s1 + nb : nullptr, L->fp8 ? s1 + nb * (swiglu ? 2 : 1) : nullptr,
         L->b1, L->b3, L->b2, tokens, L->H, L->I, L->E, L->k, L->cfg.gate_fn, L->cfg.renorm_topk, L->cfg.hidden_act,
         L->fp8 ? ARISTOS_DTYPE_BF16 : L->cfg.torch_dtype, L->cfg.torch_dtype, out, topk_idx, topk_w, L->few_ws,
-        L->few_ws_bytes, L->dev_status, stream);
+        L->few_ws_bytes, L->dev_status, L->gate_scratch_bytes > 0, stream);
     L->launches += launch_counter() - launches0;
     return s;
 }

@@ -180,7 +180,9 @@ ARISTOS_API aristos_status_t aristos_moe_wait_host(aristos_moe_t* layer);
  * The layer's forward for a few tokens (a serving step; 0 <= tokens <= ARISTOS_FEW_TOKENS_MAX, whatever the layer's own
  * token count is): two kernels that read the chosen experts' weights once (aristos_moe_few_tokens), with the layer's gate,
  * activation and biases and the arguments of aristos_moe_forward. x, out (tokens, H). No token is dropped, fp8 layers do
- * not quantise the activations, and nothing that aristos_moe_routing or aristos_moe_training_state returns changes;
+ * not quantise the activations, and nothing that aristos_moe_routing or aristos_moe_training_state returns changes. A
+ * token whose gate logits are NaN is reported by aristos_moe_status as a forward's is (layers with the screened gate: 16-bit
+ * activations, 64 to 256 experts, at least 8 per choice). A ReLU of decode keeps a NaN, one of forward turns it into 0.
  * topk_idx / topk_w (tokens, k) receive this call's routing, or NULL. One rank, torch_dtype 2, 3 or 4, E <= 512, else
  * ARISTOS_ERR_UNSUPPORTED. Uses the layer's workspace and one of its own, both allocated by the first call that needs them
  * (outside a capture) unless the caller hands them over: calls of one handle are ordered by the caller, as forwards are.
