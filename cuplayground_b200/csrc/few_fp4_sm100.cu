@@ -58,31 +58,6 @@ struct Few4Shared : FewRouting {
 };
 static_assert(T4_SMEM_BYTES + sizeof(Few4Shared) <= 227 * 1024, "few tokens, fp4: shared memory");
 
-// D[tmem] (+)= A[smem] * B[smem]^T with block scales from TMEM; K = 64 elements, issued by ONE thread.
-__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                          uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-        "}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
-        : "memory");
-}
-// e2m1 x e2m1 -> fp32, ue8m0 scales, both operands K-major, tile M x N; sf: which 16-bit half of the scale words.
-__host__ __device__ constexpr uint32_t umma_idesc_mxf4(int M, int N, uint32_t sf) {
-    return (sf << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
-           (static_cast<uint32_t>(M >> 7) << 27) | (sf << 29);
-}
-// 32 rows x 16 bytes of shared memory (512 contiguous bytes) to 4 TMEM columns of every lane quarter.
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>(128 >> 4) << 32;          // 8-row groups are 128 bytes apart, no swizzle
-    d |= static_cast<uint64_t>(1) << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
 __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -92,11 +67,6 @@ __device__ __forceinline__ uint32_t load_word_l2(const void* p) {      // writte
     asm volatile("ld.global.cg.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
     return v;
 }
-__device__ __forceinline__ void wait_drained(uint32_t bar, uint32_t parity) {
-    const uint64_t t0 = ptx::globaltimer_ns();
-    while (!ptx::mbar_try_wait(bar, parity) && ptx::globaltimer_ns() - t0 < ptx::WAIT_LIMIT_NS) {}
-}
-
 // Waits until all hidden activations of chosen expert `a` have been written (`per_pass` counts for every pass over its
 // weights); the whole warp. The next experts' counters are read along with it: by now most of them are complete, and a
 // fence is paid once for all. ready: experts below it are known to be there.
@@ -246,7 +216,7 @@ few_ffn_fp4_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constan
                 if (!ok) break;
             }
             if (!ok)                                     // the copies in flight still write to this CTA's shared memory
-                for (int i = max(issued - T4_STAGES, 0); i < issued; ++i) wait_drained(bar_b + 8 * (i % T4_STAGES), (i / T4_STAGES) & 1);
+                for (int i = max(issued - T4_STAGES, 0); i < issued; ++i) ptx::mbar_wait_drained(bar_b + 8 * (i % T4_STAGES), (i / T4_STAGES) & 1);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -271,15 +241,15 @@ few_ffn_fp4_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constan
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
                         if (2 * h < steps) {
-                            tmem_copy_scales(tsf + 4 * h, sfa + h * FP4_TILE_BYTES);
-                            tmem_copy_scales(tsf + 8 + 8 * h, sfb + h * FP4_TILE_BYTES);
-                            tmem_copy_scales(tsf + 12 + 8 * h, sfb + (2 + h) * FP4_TILE_BYTES);
+                            ptx::tmem_copy_scales<1>(tsf + 4 * h, sfa + h * FP4_TILE_BYTES);
+                            ptx::tmem_copy_scales<1>(tsf + 8 + 8 * h, sfb + h * FP4_TILE_BYTES);
+                            ptx::tmem_copy_scales<1>(tsf + 12 + 8 * h, sfb + (2 + h) * FP4_TILE_BYTES);
                         }
                     const uint64_t da = ptx::umma_desc_k_sw128(sa), db = ptx::umma_desc_k_sw128(sa + T4_A_BYTES);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)          // K = 64 elements = 32 bytes per instruction
                         if (k < steps)
-                            umma_mxf4(tmem, da + 2 * k, db + 2 * k, umma_idesc_mxf4(T4_BM, T4_BN, (k & 1) * 2), tsf + 4 * (k >> 1),
+                            ptx::umma_mxf4<1>(tmem, da + 2 * k, db + 2 * k, ptx::umma_idesc_mxf4(T4_BM, T4_BN, (k & 1) * 2), tsf + 4 * (k >> 1),
                                       tsf + 8 + 8 * (k >> 1), (kb > begin || k > 0) ? 1u : 0u);
                     ptx::umma_commit(bar_empty + 8 * stage);
                     advance();
@@ -339,7 +309,7 @@ few_ffn_fp4_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constan
             if (!ok) break;
         }
         if (!ok)
-            for (int i = max(issued - T4_STAGES, 0); i < issued; ++i) wait_drained(bar_a + 8 * (i % T4_STAGES), (i / T4_STAGES) & 1);
+            for (int i = max(issued - T4_STAGES, 0); i < issued; ++i) ptx::mbar_wait_drained(bar_a + 8 * (i % T4_STAGES), (i / T4_STAGES) & 1);
     } else if (warp == 3) {
         // ------------------------------------------------------------------ counts finished tiles
         for (int t = 1; more && ok; more = forward(item), ++t) {
@@ -433,7 +403,7 @@ few_ffn_fp4_kernel(const __grid_constant__ CUtensorMap tm1, const __grid_constan
 
     if (warp == 1 && __any_sync(0xffffffffu, *abort_flag) && ptx::elect_one()) {   // MMAs in flight still read shared memory and write TMEM
         ptx::umma_commit(bar_drained);
-        wait_drained(bar_drained, 0);
+        ptx::mbar_wait_drained(bar_drained, 0);
     }
     ptx::tcgen05_fence_before();
     __syncthreads();

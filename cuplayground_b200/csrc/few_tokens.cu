@@ -11,7 +11,7 @@
 //  * few_gate_kernel: a warp per expert and one or four tokens computes the logits; it also clears the counters.
 //  * few_ffn_kernel: one CTA per SM, launched while the gate still runs. Every CTA does the (small) top-k and the
 //    expert lists for itself, so no further kernel or grid barrier is needed. The work is a list of items (chosen expert,
-//    8 * RG weight rows, part of K): all of the up projection, then all of the down projection, dealt out in turn to
+//    32 weight rows, part of K): all of the up projection, then all of the down projection, dealt out in turn to
 //    groups of W warps. The warps of a group cut K among themselves (128-byte pieces of all rows in turn, so together they
 //    read a row's bytes in order) and leave their sums in shared memory; a helper warp adds them in a fixed order and does
 //    the epilogue and the stores, another one the counting, so that the streaming warps never wait for any of it (a
@@ -279,23 +279,19 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t w, uint32_t& lo, uint32_t& 
     hi = half_bits(*reinterpret_cast<const __half2*>(&b));
 }
 
-template <int WF> struct FewFormat;                    // elements per byte of weights, doubled
-template <> struct FewFormat<FEW_BF16> { static constexpr int PACK = 1; };
-template <> struct FewFormat<FEW_F16> { static constexpr int PACK = 1; };
-template <> struct FewFormat<FEW_FP8> { static constexpr int PACK = 2; };
+template <int WF> struct FewFormat { static constexpr int PACK = WF == FEW_FP8 ? 2 : 1; };     // weights per two bytes
 
-// NT: token tiles of 8 per pass; RG: groups of 8 weight rows per item; D: steps in the ring; BUFS: buffers for
-// the sums of an item.
-template <int WF, int NT, int RG_, int D_, int BUFS_>
+// NT: token tiles of 8 per pass; D: steps in the ring; BUFS: buffers for the sums of an item.
+template <int WF, int NT, int D_, int BUFS_>
 struct FewShape {
-    static constexpr int RG = RG_, D = D_, BUFS = BUFS_;
+    static constexpr int RG = 4;                        // groups of 8 weight rows per item
+    static constexpr int D = D_, BUFS = BUFS_;
     static constexpr int STEP_K = 64 * FewFormat<WF>::PACK;     // elements of K per step: 128 bytes of a row
     static constexpr int TILES = RG / 2;                // m16 tiles: row groups (2 t, 2 t + 1)
     static constexpr int SLOT = RG * 1024;              // 8 rows x 128 bytes per row group
-    static constexpr int SCALES = WF == FEW_FP8 ? 16 : 0;       // bytes of scales per step
+    static constexpr int SCALES = WF == FEW_FP8 ? RG * 4 : 0;   // bytes of scales per step
     static constexpr int RED = TILES * NT * 128;        // floats per warp of one buffer
     static constexpr size_t SMEM = 1024 + (size_t)FEW_STREAM_WARPS * (D * (SLOT + SCALES) + BUFS * RED * 4);
-    static_assert(RG == 2 || RG == 4, "at most one 16-byte group of scales per step");
     static_assert(D <= FEW_MAX_DEPTH && D >= 2, "ring depth");
 };
 
@@ -879,9 +875,9 @@ aristos_status_t launch_few_tokens(const FewParams& p, const FewWeights& w, cuda
     // Two token tiles and three steps of ring leave room for the sums of one item only. 16-bit weights do well with that; with
     // fp8 ones the streaming warps then wait for the helper, and two steps with two buffers are faster where an item is long
     // (12 tokens, 4 of 16 experts, 2048 x 4096: 114 us against 126; 32 tokens, 4 of 32, 4096 x 128, the other way round: 103, 101).
-    if (p.n <= 8) return launch_few<WF, 1, FewShape<WF, 1, 4, 3, 2>>(p, w, st);
-    if constexpr (WF == FEW_FP8) return launch_few<WF, 2, FewShape<WF, 2, 4, 2, 2>>(p, w, st);
-    else return launch_few<WF, 2, FewShape<WF, 2, 4, 3, 1>>(p, w, st);
+    if (p.n <= 8) return launch_few<WF, 1, FewShape<WF, 1, 3, 2>>(p, w, st);
+    if constexpr (WF == FEW_FP8) return launch_few<WF, 2, FewShape<WF, 2, 2, 2>>(p, w, st);
+    else return launch_few<WF, 2, FewShape<WF, 2, 3, 1>>(p, w, st);
 }
 
 // say: whether a refusal becomes the thread's error text.

@@ -82,54 +82,16 @@ struct Fp4GemmParams {
     const int32_t* count;
     int groups, experts, rows_per_group;
     int N, K;
-    int gated, act;
-    const uint8_t* sa;       // scale tiles of A: [groups][row tiles][K tiles][512] (host side: they come by TMA)
-    const uint8_t* sb0;      // of B: [experts][N tiles][K tiles][512]
-    const uint8_t* sb1;      // SwiGLU: of the up projection's weights
+    int act;
     void* out;               // [groups * rows_per_group][N], bf16 / fp16 / fp32; or (quantised) codes, two per byte
     uint8_t* out_scales;     // quantised: scale tiles of the output
     int32_t* dev_status;
 };
 
-// D[tmem of both CTAs] (+)= A[smem] * B[smem]^T with block scales from TMEM; K = 64 elements, issued by ONE thread.
-__device__ __forceinline__ void umma_mxf4_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                          uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-        "}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
-        : "memory");
-}
-
-// e2m1 x e2m1 -> fp32, ue8m0 scales, both operands K-major, tile M x N; sf: which 16-bit half of the scale words.
-__host__ __device__ constexpr uint32_t umma_idesc_mxf4(int M, int N, uint32_t sf) {
-    return (sf << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
-           (static_cast<uint32_t>(M >> 7) << 27) | (sf << 29);
-}
-
-// 32 rows x 16 bytes of shared memory (512 contiguous bytes) to 4 TMEM columns of every lane quarter, in both CTAs from
-// their own shared memory.
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>(128 >> 4) << 32;          // 8-row groups are 128 bytes apart, no swizzle
-    d |= static_cast<uint64_t>(1) << 46;
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
-
 // Arrive on the barrier at this offset in both CTAs of the pair when the MMAs issued so far have completed.
 __device__ __forceinline__ void umma_commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
-}
-
-// After a wait that gave up: the copies and MMAs in flight still use shared memory and TMEM. Waits for them, with a limit.
-__device__ __forceinline__ void wait_drained(uint32_t bar, uint32_t parity) {
-    const uint64_t t0 = ptx::globaltimer_ns();
-    while (!ptx::mbar_try_wait(bar, parity) && ptx::globaltimer_ns() - t0 < ptx::WAIT_LIMIT_NS) {}
 }
 
 // Reciprocal and power of two in one instruction each (subnormal arguments and results count as zero: the arguments here are
@@ -380,7 +342,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             }
             // both CTAs' copies are counted in CTA 0; CTA 1 waits for it below
             for (int i = max(issued - F4_STAGES, 0); !ok && cta == 0 && i < issued; ++i)
-                wait_drained(bar_full + 8 * (i % F4_STAGES), (i / F4_STAGES) & 1);
+                ptx::mbar_wait_drained(bar_full + 8 * (i % F4_STAGES), (i / F4_STAGES) & 1);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -411,7 +373,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
 #pragma unroll
                     for (int k = 0; k < 4; ++k)            // K = 64 elements = 32 bytes per instruction
                         if (k < steps)
-                            umma_mxf4_pair(tmem_d, da + 2 * k, db + 2 * k, umma_idesc_mxf4(F4_PM, F4_BN, (k & 1) * 2),
+                            ptx::umma_mxf4<2>(tmem_d, da + 2 * k, db + 2 * k, ptx::umma_idesc_mxf4(F4_PM, F4_BN, (k & 1) * 2),
                                            tsf + 4 * (k >> 1), tsf + 8 + 8 * (k >> 1), (kb | k) != 0 ? 1u : 0u);
                     umma_commit_both(bar_empty + 8 * stage);   // release the stage in both CTAs
                 }
@@ -456,7 +418,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
                 }
             }
             for (int i = max(issued - F4_SF_STAGES, 0); !ok && cta == 0 && i < issued; ++i)
-                wait_drained(bar_sfull + 8 * (i % F4_SF_STAGES), (i / F4_SF_STAGES) & 1);
+                ptx::mbar_wait_drained(bar_sfull + 8 * (i % F4_SF_STAGES), (i / F4_SF_STAGES) & 1);
         }
         __syncwarp();
     } else if (warp == F4_SF_COPY_WARP) {
@@ -483,9 +445,9 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (2 * h < steps) {
-                            tmem_copy_scales(tsf + 4 * h, sf + h * FP4_TILE_BYTES);
-                            tmem_copy_scales(tsf + 8 + 8 * h, sf + F4_SF_BYTES + h * FP4_TILE_BYTES);
-                            tmem_copy_scales(tsf + 8 + 8 * h + 4, sf + 2 * F4_SF_BYTES + h * FP4_TILE_BYTES);
+                            ptx::tmem_copy_scales<2>(tsf + 4 * h, sf + h * FP4_TILE_BYTES);
+                            ptx::tmem_copy_scales<2>(tsf + 8 + 8 * h, sf + F4_SF_BYTES + h * FP4_TILE_BYTES);
+                            ptx::tmem_copy_scales<2>(tsf + 8 + 8 * h + 4, sf + 2 * F4_SF_BYTES + h * FP4_TILE_BYTES);
                         }
                     }
                     ptx::umma_commit_pair(bar_scales + 8 * buf);
@@ -555,7 +517,7 @@ ffn_fp4_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     if (cta == 0 && (warp == 1 || warp == F4_SF_COPY_WARP) && __any_sync(0xffffffffu, *abort_flag) && ptx::elect_one()) {
         const uint32_t bar = bar_drained + (warp == 1 ? 0 : 8);
         ptx::umma_commit_pair(bar);
-        wait_drained(bar, 0);
+        ptx::mbar_wait_drained(bar, 0);
     }
     ptx::tcgen05_fence_before();
     __syncthreads();
@@ -586,20 +548,22 @@ aristos_status_t encode_scale_map(CUtensorMap* tm, const void* base, int K, int 
     return ARISTOS_OK;
 }
 
+// Codes and scale tiles: A [groups][row tiles][K tiles][512], B [experts][N tiles][K tiles][512]; SwiGLU: B1 is the up projection's.
+struct Fp4Operands { const void *A, *SA, *B0, *SB0, *B1, *SB1; };
+
 // follows: the launch before this one on the stream is this kernel, too, with the same p.count (which is read before the wait).
-aristos_status_t launch_fp4_gemm(const void* A, const void* B0, const void* B1, const Fp4GemmParams& p, int out,
-                                 cudaStream_t st, bool follows = false) {
+aristos_status_t launch_fp4_gemm(const Fp4Operands& o, const Fp4GemmParams& p, int out, cudaStream_t st, bool follows = false) {
     CUtensorMap tmA, tmB0, tmB1;
-    ARISTOS_TRY(encode_map_3d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A, p.K / 2, p.rows_per_group, p.groups, 128));
-    ARISTOS_TRY(encode_map_3d(&tmB0, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B0, p.K / 2, p.N, p.experts, 128));
-    ARISTOS_TRY(encode_map_3d(&tmB1, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, B1, p.K / 2, p.N, p.experts, 128));
+    ARISTOS_TRY(encode_map_3d(&tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.A, p.K / 2, p.rows_per_group, p.groups, 128));
+    ARISTOS_TRY(encode_map_3d(&tmB0, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.B0, p.K / 2, p.N, p.experts, 128));
+    ARISTOS_TRY(encode_map_3d(&tmB1, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, o.B1, p.K / 2, p.N, p.experts, 128));
     CUtensorMap tmSA, tmSB0, tmSB1;
-    ARISTOS_TRY(encode_scale_map(&tmSA, p.sa, p.K, p.rows_per_group, p.groups));
-    ARISTOS_TRY(encode_scale_map(&tmSB0, p.sb0, p.K, p.N, p.experts));
-    ARISTOS_TRY(encode_scale_map(&tmSB1, p.sb1, p.K, p.N, p.experts));
+    ARISTOS_TRY(encode_scale_map(&tmSA, o.SA, p.K, p.rows_per_group, p.groups));
+    ARISTOS_TRY(encode_scale_map(&tmSB0, o.SB0, p.K, p.N, p.experts));
+    ARISTOS_TRY(encode_scale_map(&tmSB1, o.SB1, p.K, p.N, p.experts));
     const int sms = device_sm_count();
     if (sms <= 0) { set_last_error("no CUDA device"); return ARISTOS_ERR_CUDA; }
-    const int64_t bound = (int64_t)p.groups * ceil_div(p.rows_per_group, F4_PM) * ceil_div(p.N, p.gated ? 128 : 256);
+    const int64_t bound = (int64_t)p.groups * ceil_div(p.rows_per_group, F4_PM) * ceil_div(p.N, p.act == ARISTOS_ACT_SWIGLU ? 128 : 256);
     auto run = [&](auto output, auto activation) -> aristos_status_t {
         const auto kernel = ffn_fp4_grouped_gemm_kernel<decltype(output)::value, decltype(activation)::value>;
         ARISTOS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F4_SMEM_BYTES));
@@ -707,11 +671,9 @@ extern "C" aristos_status_t aristos_expert_product_fp4(const void* aq, const voi
     p.rows_per_group = rows_per_group;
     p.N = N; p.K = K;
     p.act = ARISTOS_ACT_IDENTITY;
-    p.sa = static_cast<const uint8_t*>(sa);
-    p.sb0 = p.sb1 = static_cast<const uint8_t*>(sb);
     p.out = y;
     p.dev_status = dev_status;
-    return launch_fp4_gemm(aq, bq, bq, p, out_dtype, static_cast<cudaStream_t>(stream));
+    return launch_fp4_gemm({aq, sa, bq, sb, bq, sb}, p, out_dtype, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" aristos_status_t aristos_expert_ffn_fp4(const void* xq, const void* sx, const int32_t* count, int groups,
@@ -744,20 +706,13 @@ extern "C" aristos_status_t aristos_expert_ffn_fp4(const void* xq, const void* s
     p.rows_per_group = rows_per_group;
     p.dev_status = dev_status;
     p.N = I; p.K = H;
-    p.gated = gated ? 1 : 0;
     p.act = hidden_act;
-    p.sa = static_cast<const uint8_t*>(sx);
-    p.sb0 = static_cast<const uint8_t*>(s1);
-    p.sb1 = static_cast<const uint8_t*>(gated ? s3 : s1);
     p.out = hq_scratch;
     p.out_scales = static_cast<uint8_t*>(sh_scratch);
-    ARISTOS_TRY(launch_fp4_gemm(xq, w1q, gated ? w3q : w1q, p, OUT_FP4, st));
+    ARISTOS_TRY(launch_fp4_gemm({xq, sx, w1q, s1, gated ? w3q : w1q, gated ? s3 : s1}, p, OUT_FP4, st));
     p.N = H; p.K = I;
-    p.gated = 0;
     p.act = ARISTOS_ACT_IDENTITY;
-    p.sa = static_cast<const uint8_t*>(sh_scratch);
-    p.sb0 = p.sb1 = static_cast<const uint8_t*>(s2);
     p.out = y;
     p.out_scales = nullptr;
-    return launch_fp4_gemm(hq_scratch, w2q, w2q, p, out_dtype, st, true);
+    return launch_fp4_gemm({hq_scratch, sh_scratch, w2q, s2, w2q, s2}, p, out_dtype, st, true);
 }

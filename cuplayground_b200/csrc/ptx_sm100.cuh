@@ -86,6 +86,13 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
     }
 }
 
+// After a wait that gave up: copies and MMAs in flight still use shared memory and TMEM. Waits for the phase that they
+// complete, with the same limit.
+__device__ __forceinline__ void mbar_wait_drained(uint32_t bar, uint32_t parity) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 < WAIT_LIMIT_NS) {}
+}
+
 // Wait until a 32-bit flag word in global memory, stored by another GPU (or an earlier kernel) with system scope, has
 // reached `epoch` (cyclic comparison, like the stream memory operation CU_STREAM_WAIT_VALUE_GEQ). The acquire load
 // orders the later reads of the data that the flag publishes; the proxy fence extends that to TMA loads. Bounded like
@@ -322,6 +329,38 @@ __device__ __forceinline__ uint64_t umma_desc_k_sw128(uint32_t smem_addr) {
 __host__ __device__ constexpr uint32_t umma_idesc_f32acc(int M, int N, uint32_t ab_format) {
     return (1u << 4) | (ab_format << 7) | (ab_format << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
            (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+
+// ---- block-scaled 4-bit operands (kind::mxf4): e2m1 elements, ue8m0 scales per 32 of K taken from TMEM ----------------------
+// CTAS = 2: a pair's instruction, as umma_f16_pair.
+// Instruction descriptor: both operands K-major, tile M x N -> fp32; sf: which 16-bit half of the scale words.
+__host__ __device__ constexpr uint32_t umma_idesc_mxf4(int M, int N, uint32_t sf) {
+    return (sf << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
+           (static_cast<uint32_t>(M >> 7) << 27) | (sf << 29);
+}
+// D[tmem] (+)= A[smem] * B[smem]^T; K = 64 elements, issued by ONE thread.
+template <int CTAS>
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t tmem_sa,
+                                          uint32_t tmem_sb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::%7.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+        "}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate), "n"(CTAS)
+        : "memory");
+}
+// 32 rows x 16 bytes of shared memory (512 contiguous bytes) to 4 TMEM columns of every lane quarter; a pair: in both CTAs,
+// each from its own shared memory.
+template <int CTAS>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(128 >> 4) << 32;          // 8-row groups are 128 bytes apart, no swizzle
+    d |= static_cast<uint64_t>(1) << 46;
+    asm volatile("tcgen05.cp.cta_group::%2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d), "n"(CTAS) : "memory");
 }
 
 }  // namespace ptx
