@@ -549,13 +549,13 @@ class MoELayer:
         with _Device(x, w_gate, w1, w3, w2, gate_bias, scales, out, *bias) as on:
             if on.index != self.device or (stream is not None and stream.device.index != self.device):
                 raise ValueError(f"the layer, its tensors and the stream must be on one device, the layer is on cuda:{self.device}")
-            if self._ws is not None and self._decode_ws is None:
-                nbytes = int(self._lib.aristos_moe_decode_workspace_bytes(self._h))
-                if nbytes:                               # 0: the library refuses
-                    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-                    _lib.check(self._lib.aristos_moe_set_decode_workspace(self._h, _addr(ws), nbytes))
-                    self._decode_ws = ws
-            with torch.cuda.stream(stream):              # outputs belong to the stream that writes them
+            with torch.cuda.stream(stream):              # workspace and outputs belong to the stream that writes them
+                if self._ws is not None and self._decode_ws is None:
+                    nbytes = int(self._lib.aristos_moe_decode_workspace_bytes(self._h))
+                    if nbytes:                           # 0: the library refuses
+                        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+                        _lib.check(self._lib.aristos_moe_set_decode_workspace(self._h, _addr(ws), nbytes))
+                        self._decode_ws = ws
                 out = torch.empty_like(x) if out is None else out
                 idx = x.new_empty((n, self.k), dtype=torch.int32)
                 w = x.new_empty((n, self.k), dtype=torch.float32)

@@ -85,3 +85,23 @@ def test_the_first_decode_may_be_captured_where_torch_has_the_workspaces():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, ref.decode(x, *w)))
     L.close(), ref.close()
+
+
+def test_a_torch_workspace_belongs_to_the_stream_of_the_first_decode():
+    """A block that the current stream has just given back may still be in use there: the workspace of a decode on another stream
+    must not be that block."""
+    torch, cp, layer = _mods()
+    w = _weights(torch)
+    x = torch.randn(7, 128, device="cuda").bfloat16()
+    L = _layer(cp, layer)
+    L.use_torch_workspace()
+    n = int(cp._lib.load().aristos_moe_decode_workspace_bytes(L._h))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    given_back = torch.empty(n, dtype=torch.uint8, device="cuda")
+    at = given_back.data_ptr()
+    del given_back
+    L.decode(x, *w, stream=side)
+    assert L._decode_ws.data_ptr() != at
+    torch.cuda.synchronize()
+    L.close()
