@@ -10,9 +10,9 @@
 //
 // A tile has 128 rows, of which a token takes eight: 16 tokens to a pass over an expert's weights. The tensor core computes
 // all of it whether there are 16 tokens or one, which does not matter here: it is busy for a quarter of the time. That case
-// takes 440 us with the gate, 418 us of it this kernel (5.9 TB/s). The smallest calls pay for the larger tiles (1 token, 256 x
-// 512: 31 us instead of 26 us with 16-bit instructions and items of 32 rows); from some 10 MB of chosen weights on this kernel
-// is the faster one.
+// takes 431 to 491 us with the gate, 418 us of it this kernel (5.9 TB/s). Few tiles fill few CTAs: one token, 2 of 8 experts, 4096
+// x 14336, takes 65 us where its bytes take 29. The smallest calls pay for the larger tiles (1 token, 256 x 512: 31 us instead of
+// 26 us with 16-bit instructions and items of 32 rows); from some 10 MB of chosen weights on this kernel is the faster one.
 //
 // Tile: 16 tokens x 256 weight rows (SwiGLU: 128 gate and 128 up rows), K in stages of 256 columns (one 128-byte row):
 // 32 KB of weights, their scales, the tokens' terms (1 KB each, only those that are there) and their scales, four

@@ -30,8 +30,8 @@
 //    in the order of j.
 //
 // Measured on a B200 whose copies run at 6.47 TB/s, L2 cold, both kernels: one token, 2 of 8 experts, 4096 x 14336 SwiGLU,
-// bf16 127 us (0.70 GB of weights, 5.5 TB/s); 64 tokens, 2 of 64, 2048 x 2048 GELU, bf16 178 us (0.93 GB); 5 tokens, 8 of 256,
-// 7168 x 2048 SwiGLU, e4m3 328 us (1.66 GB; here the conversions of the codes to fp16 count, too).
+// bf16 128 us (0.70 GB of weights, 5.5 TB/s); 64 tokens, 2 of 64, 2048 x 2048 GELU, bf16 178 to 189 us (0.93 GB); 5 tokens, 8
+// of 256, 7168 x 2048 SwiGLU, e4m3 314 to 328 us (1.66 GB; here the conversions of the codes to fp16 count, too).
 //
 // Operand types. The instruction multiplies 16-bit numbers. bf16 weights meet tokens in bf16 (as they are); fp16 and e4m3
 // weights meet fp16 numbers, in which both are exact, bf16 tokens being brought into fp16's range by a power of two per

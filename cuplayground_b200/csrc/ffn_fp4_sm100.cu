@@ -31,10 +31,11 @@
 // The up projection of the FFN writes its output as MXFP4 again: a thread holds 32 adjacent columns of its row, i.e. a
 // whole block, so scale and codes come out of its registers, rounded once from fp32. Only valid rows are written.
 //
-// Measured (B200, bf16 matrix products of the library reach 1.67 PFLOP/s in bursts): 20969 rows of 7 experts, 14336 x 4096,
-// bf16 output 490 us = 5.0 PFLOP/s for some milliseconds, 560 us on and on: then the 1000 W cap holds the SM clock at 1470 of
-// 1965 MHz. The FFN of 24896 rows of 31 experts, 7168 x 2048, SwiGLU 531 us = 4.1 PFLOP/s (4.8 counting what fills up tiles);
-// 15163 rows of 63 experts, 2048 x 2048, GELU 124 us (1.45 times as many rows in tiles, 8 stages each). Tiles of 128 x 256 in
+// Measured (B200, bf16 matrix products of the library reach 1.67 PFLOP/s in bursts), calls on and on: some 21000 rows of 7
+// experts, 14336 x 4096, bf16 output 547 to 650 us by box = 3.8 to 4.5 PFLOP/s, the 1000 W cap holding the SM clock at 1470 of
+// 1965 MHz (490 us = 5.0 PFLOP/s in a loop of some milliseconds). The FFN of 24896 rows of 31 experts, 7168 x 2048, SwiGLU 617 to
+// 668 us (527 in a short loop); 15163 rows of 63 experts, 2048 x 2048, GELU 139 to 142 us (124), with 1.45 times as many rows in
+// tiles, 8 stages each. Tiles of 128 x 256 in
 // single CTAs, with the epilogue of that time, took 680 us where pairs took 615 us on the first, and 6 to 11 % less than pairs
 // on the two others.
 #include <cuda.h>
