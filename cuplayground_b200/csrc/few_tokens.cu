@@ -869,9 +869,10 @@ template <int WF>
 aristos_status_t launch_few_tokens(const FewParams& p, const FewWeights& w, cudaStream_t st) {
     // Up to 16 tokens of an expert in one pass over its weights; more (few experts, many tokens) take further passes,
     // whose weights come from L2. Wider passes would cost every small one registers and shared memory. Up to 8 tokens a
-    // pass needs one token tile: the registers that this saves are worth 3 % with fp8 weights (345 us against 357 us for 5
-    // tokens of 256 experts, 7168 x 2048), nothing with 16-bit ones. Items of 32 rows: with 16 rows (and rings twice as
-    // deep) the same cases take 1.1 to 1.4 times as long, the tokens are read once per item.
+    // pass needs one token tile: the registers and the second sum buffer that this saves are worth 9 % with fp8 weights (328 us
+    // against 360 for 5 tokens, 8 of 256 experts, 7168 x 2048), 2 % with bf16 ones (one token, 4096 x 14336), nothing in a small
+    // layer. Items of 32 rows: with 16 rows (and rings twice as deep) the same cases took 1.1 to 1.4 times as long, the tokens are
+    // read once per item.
     // Two token tiles and three steps of ring leave room for the sums of one item only. 16-bit weights do well with that; with
     // fp8 ones the streaming warps then wait for the helper, and two steps with two buffers are faster where an item is long
     // (12 tokens, 4 of 16 experts, 2048 x 4096: 114 us against 126; 32 tokens, 4 of 32, 4096 x 128, the other way round: 103, 101).

@@ -407,8 +407,8 @@ ARISTOS_API aristos_status_t aristos_expert_ffn_fp4(const void* xq, const void* 
  * scales and workspace 16-byte aligned.
  * Activations are not quantised. The hidden ones are computed in fp32 and meet the weights as sums of 16-bit numbers (bf16
  * weights: three, all 24 bits; fp16 and fp8 weights: two, off by 2^-24 of the value or 2^-38 of the largest of the row) or of
- * eight 4-bit numbers (4-bit weights: 24 bits of the largest of 32). A token's results do not depend on the other tokens of the
- * call. The routing is aristos_gate_topk's, bit for bit; no token is dropped. topk_idx / topk_w (tokens, k) receive it, or NULL. workspace:
+ * eight 4-bit numbers (4-bit weights: 24 bits of the largest of 32), so that an infinite weight of w2 gives NaN. A token's
+ * results do not depend on the other tokens of the call. The routing is aristos_gate_topk's, bit for bit; no token is dropped. topk_idx / topk_w (tokens, k) receive it, or NULL. workspace:
  * aristos_moe_few_tokens_workspace_bytes (0: sizes out of range) on the device, owned by the caller; it needs no
  * initialisation, and calls that may overlap on the GPU need one each.
  */

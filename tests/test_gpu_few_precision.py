@@ -93,3 +93,20 @@ def test_e4m3_scales_that_are_parts_of_one_tensor():
     packed = torch.cat([c.s[m].reshape(-1) for m in ("1", "3", "2")])
     c.s = {m: packed[3 * i:3 * i + 3].view(3, 1, 1) for i, m in enumerate(("1", "3", "2"))}
     assert all(torch.equal(a, b) for a, b in zip(c.run(), want))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("n", [3, 8, 24])
+def test_an_infinite_weight_reaches_its_own_outputs_only(dtype, n):
+    """An infinity in w2 meets all terms of a hidden activation, zeros among them: its column is not finite for the tokens of its
+    expert, nothing else changes."""
+    import math
+    import torch
+    c = Case(n, 4, 2, 256, 384, 2, "16", dtype, seed=n)
+    clean, idx, _ = c.run()
+    c.w["2"][1, 77, 5] = math.inf
+    out = c.run()[0]
+    mine = (idx == 1).any(1)
+    rest = torch.arange(256, device="cuda") != 77
+    assert mine.any() and not torch.isfinite(out[mine][:, 77]).any()
+    assert torch.equal(out[:, rest], clean[:, rest]) and torch.equal(out[~mine], clean[~mine])
