@@ -45,7 +45,7 @@
 // bring the terms from the one scale to the other (a power of two: exact, down to 2^-24).
 // Three bf16 terms are three instructions. The two fp16 terms of up to 4 tokens are columns of one, the first in columns 0-3
 // and the second in 4-7 (most experts have no more tokens, and the columns would be empty otherwise): 5 tokens, 8 of 64
-// experts, 2048 x 2048, e4m3, 117 us against 126 with two instructions. More tokens take two (folded into tiles of four they
+// experts, 2048 x 2048, e4m3, 113 us against 126 with two instructions. More tokens take two (folded into tiles of four they
 // take longer, 8 tokens per expert 122 us against 101: their loads are not ahead of the wait). Either way the terms have sums of
 // their own, which are added when the item is done: the bits of a token do not depend on who else chose its experts.
 #include <cuda_fp8.h>
@@ -459,10 +459,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) few_ffn_kernel(const __grid_co
                     if constexpr (F16) {
                         uint32_t mag = __float_as_uint(v) & 0x7FFFFFFFu;
                         for (int d = rows >> 1; d >= 1; d >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, d));
-                        const int e = few_exponent(mag);
-                        v *= few_power(e);
+                        const int exponent = few_exponent(mag);
+                        v *= few_power(exponent);
                         if (in && j == 0) atomicMax(p.h_max + slot, mag);
-                        if (in && (j & 15) == 0) p.h_exp[(size_t)slot * (p.I / 16) + (row0 + j) / 16] = (int8_t)e;
+                        if (in && (j & 15) == 0) p.h_exp[(size_t)slot * (p.I / 16) + (row0 + j) / 16] = (int8_t)exponent;
                     }
                     if (in) {
                         uint16_t t[TERMS];
